@@ -10,6 +10,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "noel_logits.h"
+#include "noel_lora.h"
 #include "sampler.h"
 
 #ifdef __cplusplus
@@ -35,6 +37,22 @@ int noel_lmhead_sample(const noel_sampler_config_t *cfg, const void *d_weight, i
                        const float *d_hidden, size_t ldh, int batch, int hidden_dim, int vocab,
                        const int32_t *d_history, int history_len, size_t hld, uint64_t *d_rng, int32_t *d_ids,
                        float *d_probs, float *d_logits, void *stream);
+
+/*
+ * noel_lmhead_sample with what differs from request to request: after the
+ * projection, token t's adapter adds its part to the logits (lora and
+ * d_adapter [batch], noel_lora_apply; the adapters' rows are the vocabulary
+ * and their cols hidden_dim), then process is applied to them
+ * (noel_logits_process), then the batch is sampled; all in the same stream.
+ * lora or process may be NULL, and with both NULL this is
+ * noel_lmhead_sample.  d_work (work_bytes) is noel_lora_apply's scratch and
+ * may be NULL without lora.  d_logits receives the logits that were sampled.
+ */
+int noel_lmhead_sample_ex(const noel_sampler_config_t *cfg, const void *d_weight, int weight_type, size_t ldw,
+                          const float *d_hidden, size_t ldh, int batch, int hidden_dim, int vocab,
+                          const noel_lora_t *lora, const int32_t *d_adapter, const noel_logits_params_t *process,
+                          const int32_t *d_history, int history_len, size_t hld, uint64_t *d_rng, int32_t *d_ids,
+                          float *d_probs, float *d_logits, void *d_work, size_t work_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -23,10 +23,14 @@
 #include <vector>
 
 #include "noel_lmhead.h"
+#include "noel_logits.h"
+#include "noel_lora.h"
 #include "noel_postreq.h"
 #include "noel_router.h"
 #include "noel_sampler_cuda.h"
 #include "lmhead.cuh"
+#include "logits.cuh"
+#include "lora.cuh"
 #include "postreq.cuh"
 #include "router.cuh"
 #include "sampler_stream.cuh"
@@ -978,6 +982,189 @@ extern "C" int32_t noel_postreq_sample(float *logits, int vocab_size, const noel
     return *st.h_id;
 }
 
+/* ------------------------------------- per-request processing of logits */
+namespace {
+/* the checks of noel_logits_process that need no device, and its arguments */
+int logits_args(const noel_logits_params_t *p, void *logits, int dtype, int B, int V, size_t ld, LogitsArgs *out) {
+    if (!p) return fail(NOEL_ERR_INVALID_ARG, "params is NULL");
+    if (B < 0 || V <= 0) return fail(NOEL_ERR_INVALID_ARG, "batch %d / vocab %d", B, V);
+    if (dtype != NOEL_DTYPE_F32 && dtype != NOEL_DTYPE_BF16) return fail(NOEL_ERR_INVALID_ARG, "dtype %d", dtype);
+    if (ld < (size_t)V) return fail(NOEL_ERR_INVALID_ARG, "ld %zu < vocab %d", ld, V);
+    if (p->v_begin < 0 || p->v_begin > 0x7FFFFFFF - V)
+        return fail(NOEL_ERR_INVALID_ARG, "v_begin %d with %d columns", p->v_begin, V);
+    if (p->d_history) {
+        if (p->history_len < 0 || p->hld < (size_t)p->history_len)
+            return fail(NOEL_ERR_INVALID_ARG, "history_len %d / hld %zu", p->history_len, p->hld);
+        if (p->history_len >= kLogitsMaxHistory)
+            return fail(NOEL_ERR_TOO_LARGE, "history_len %d (below %d)", p->history_len, kLogitsMaxHistory);
+    }
+    if (!p->d_bias_ids != !p->d_bias) return fail(NOEL_ERR_INVALID_ARG, "bias ids and values come together");
+    if (p->d_bias_ids) {
+        if (p->bias_len < 0 || p->bld < (size_t)p->bias_len)
+            return fail(NOEL_ERR_INVALID_ARG, "bias_len %d / bld %zu", p->bias_len, p->bld);
+        if (p->bias_len > kLogitsMaxBias)
+            return fail(NOEL_ERR_TOO_LARGE, "bias_len %d (up to %d)", p->bias_len, kLogitsMaxBias);
+    }
+    if (p->d_mask) {
+        const size_t words = ((size_t)p->v_begin + (size_t)V + 31) / 32;
+        if (p->mld < words)
+            return fail(NOEL_ERR_INVALID_ARG, "mld %zu: ids up to %zu need %zu words", p->mld,
+                        (size_t)p->v_begin + V - 1, words);
+        if (p->mask_rows < 0 || (!p->d_mask_rows && p->mask_rows < B))
+            return fail(NOEL_ERR_INVALID_ARG, "mask_rows %d for %d rows", p->mask_rows, B);
+    }
+    if (B > 0 && !logits) return fail(NOEL_ERR_INVALID_ARG, "logits are required");
+    const uintptr_t es = dtype == NOEL_DTYPE_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(logits) % es)
+        return fail(NOEL_ERR_INVALID_ARG, "logits not %d-byte aligned", (int)es);
+    const void *arrays[] = {p->d_history, p->d_history_lens, p->d_prompt_lens, p->d_repetition, p->d_frequency,
+                            p->d_presence, p->d_bias_ids, p->d_bias, p->d_mask, p->d_mask_rows};
+    for (const void *q : arrays)
+        if (reinterpret_cast<uintptr_t>(q) & 3) return fail(NOEL_ERR_INVALID_ARG, "arrays must be 4-byte aligned");
+    LogitsArgs a{};
+    a.logits = logits;
+    a.ld = (int64_t)ld;
+    a.batch = B;
+    a.vocab = V;
+    a.v_begin = p->v_begin;
+    if (p->d_history && p->history_len > 0) {
+        a.hist = p->d_history;
+        a.hld = (int64_t)p->hld;
+        a.hist_len = p->history_len;
+        a.hist_lens = p->d_history_lens;
+        a.prompt_lens = p->d_prompt_lens;
+        a.rep = p->d_repetition;
+        a.freq = p->d_frequency;
+        a.pres = p->d_presence;
+    }
+    if (p->d_bias_ids && p->bias_len > 0) {
+        a.bias_ids = p->d_bias_ids;
+        a.bias = p->d_bias;
+        a.bld = (int64_t)p->bld;
+        a.bias_len = p->bias_len;
+    }
+    a.mask = p->d_mask;
+    a.mld = (int64_t)p->mld;
+    a.mask_rows = p->mask_rows;
+    a.mask_row = p->d_mask_rows;
+    a.slices = (V + kLogitsSlice - 1) / kLogitsSlice;
+    if ((int64_t)B * a.slices > 0x7FFFFFFF) return fail(NOEL_ERR_TOO_LARGE, "%d rows x %d columns", B, V);
+    *out = a;
+    return NOEL_OK;
+}
+
+int logits_launch(const LogitsArgs &a, int dtype, cudaStream_t s) {
+    if (a.batch == 0 || (!a.hist && !a.bias_ids && !a.mask)) return NOEL_OK;
+    const int grid = a.batch * a.slices;
+    if (dtype == NOEL_DTYPE_F32) logits_process_kernel<float><<<grid, kLogitsThreads, 0, s>>>(a);
+    else logits_process_kernel<uint16_t><<<grid, kLogitsThreads, 0, s>>>(a);
+    CUDA_TRY(cudaGetLastError());
+    return NOEL_OK;
+}
+}  // namespace
+
+extern "C" int noel_logits_process(const noel_logits_params_t *params, void *d_logits, int dtype, int batch, int vocab,
+                                   size_t ld, void *stream) {
+    LogitsArgs a{};
+    int r = logits_args(params, d_logits, dtype, batch, vocab, ld, &a);
+    if (r) return r;
+    if (batch == 0) return ok();
+    DeviceCtx *c = nullptr;
+    r = device_ctx(&c);
+    if (r) return r;
+    r = logits_launch(a, dtype, static_cast<cudaStream_t>(stream));
+    return r ? r : ok();
+}
+
+/* ------------------------------------------------ low-rank adapters */
+namespace {
+int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size_t ldx, int B, int cols, int rows,
+              float *y, size_t ldy, void *work, size_t work_bytes, LoraArgs *out) {
+    if (!l) return fail(NOEL_ERR_INVALID_ARG, "lora is NULL");
+    if (l->type != NOEL_HEAD_F32 && l->type != NOEL_HEAD_F16 && l->type != NOEL_HEAD_BF16)
+        return fail(NOEL_ERR_UNSUPPORTED, "adapter type %d (F32 0, F16 1, BF16 30)", l->type);
+    if (l->rank < 1 || l->rank > kLoraMaxRank) return fail(NOEL_ERR_TOO_LARGE, "rank %d (1..%d)", l->rank, kLoraMaxRank);
+    if (B < 0 || cols <= 0 || rows <= 0 || l->n_adapters < 0)
+        return fail(NOEL_ERR_INVALID_ARG, "batch %d / cols %d / rows %d / n_adapters %d", B, cols, rows, l->n_adapters);
+    if (ldx < (size_t)cols || ldy < (size_t)rows)
+        return fail(NOEL_ERR_INVALID_ARG, "ldx %zu < cols %d or ldy %zu < rows %d", ldx, cols, ldy, rows);
+    if (l->lda < (size_t)cols || l->ldb < (size_t)l->rank)
+        return fail(NOEL_ERR_INVALID_ARG, "lda %zu < cols %d or ldb %zu < rank %d", l->lda, cols, l->ldb, l->rank);
+    const uintptr_t es = l->type == NOEL_HEAD_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(l->d_a) % es || reinterpret_cast<uintptr_t>(l->d_b) % es)
+        return fail(NOEL_ERR_INVALID_ARG, "adapters not %d-byte aligned", (int)es);
+    const void *arrays[] = {l->d_scale, l->d_ranks, adapter, x, y};
+    for (const void *q : arrays)
+        if (reinterpret_cast<uintptr_t>(q) & 3) return fail(NOEL_ERR_INVALID_ARG, "arrays must be 4-byte aligned");
+    if (B > 0 && l->n_adapters > 0) {
+        if (!l->d_a || !l->d_b || !adapter || !x || !y)
+            return fail(NOEL_ERR_INVALID_ARG, "adapters, their ids, x and y are required");
+        const size_t need = noel_lora_workspace_bytes(B, l->rank);
+        if (!work || work_bytes < need || (reinterpret_cast<uintptr_t>(work) & 15))
+            return fail(NOEL_ERR_INVALID_ARG, "%zu bytes of 16-byte aligned scratch are needed (got %zu)", need,
+                        work ? work_bytes : (size_t)0);
+    }
+    LoraArgs a{};
+    a.a = l->d_a;
+    a.b = l->d_b;
+    a.lda = (int64_t)l->lda;
+    a.stride_a = (int64_t)l->stride_a;
+    a.ldb = (int64_t)l->ldb;
+    a.stride_b = (int64_t)l->stride_b;
+    a.scale = l->d_scale;
+    a.ranks = l->d_ranks;
+    a.n = l->n_adapters;
+    a.rank = l->rank;
+    a.adapter = adapter;
+    a.x = x;
+    a.ldx = (int64_t)ldx;
+    a.batch = B;
+    a.cols = cols;
+    a.rows = rows;
+    a.y = y;
+    a.ldy = (int64_t)ldy;
+    a.low = static_cast<float *>(work);
+    *out = a;
+    return NOEL_OK;
+}
+
+template <int WT>
+int lora_launch_t(const LoraArgs &a, cudaStream_t s) {
+    const int64_t warps = (int64_t)a.batch * a.rank;
+    lora_shrink_kernel<WT><<<(unsigned)((warps + kLoraThreads / 32 - 1) / (kLoraThreads / 32)), kLoraThreads, 0, s>>>(a);
+    CUDA_TRY(cudaGetLastError());
+    const dim3 grid((a.rows + kLoraThreads - 1) / kLoraThreads, a.batch < 65535 ? a.batch : 65535);
+    lora_expand_kernel<WT><<<grid, kLoraThreads, 0, s>>>(a);
+    CUDA_TRY(cudaGetLastError());
+    return NOEL_OK;
+}
+
+int lora_launch(const LoraArgs &a, int type, cudaStream_t s) {
+    if (a.batch == 0 || a.n == 0) return NOEL_OK;
+    return type == NOEL_HEAD_F32   ? lora_launch_t<kHeadF32>(a, s)
+           : type == NOEL_HEAD_F16 ? lora_launch_t<kHeadF16>(a, s)
+                                   : lora_launch_t<kHeadBF16>(a, s);
+}
+}  // namespace
+
+extern "C" size_t noel_lora_workspace_bytes(int batch, int rank) {
+    return batch > 0 && rank > 0 ? (size_t)batch * (size_t)rank * sizeof(float) : 0;
+}
+
+extern "C" int noel_lora_apply(const noel_lora_t *lora, const int32_t *d_adapter, const float *d_x, size_t ldx,
+                               int batch, int cols, int rows, float *d_y, size_t ldy, void *d_work, size_t work_bytes,
+                               void *stream) {
+    LoraArgs a{};
+    int r = lora_args(lora, d_adapter, d_x, ldx, batch, cols, rows, d_y, ldy, d_work, work_bytes, &a);
+    if (r) return r;
+    if (batch == 0 || a.n == 0) return ok();
+    DeviceCtx *c = nullptr;
+    r = device_ctx(&c);
+    if (r) return r;
+    r = lora_launch(a, lora->type, static_cast<cudaStream_t>(stream));
+    return r ? r : ok();
+}
+
 /* ------------------------------------------------ LM head -> sampler */
 namespace {
 template <int WT, int NB>
@@ -1004,6 +1191,17 @@ extern "C" int noel_lmhead_sample(const noel_sampler_config_t *cfg, const void *
                                   size_t ldw, const float *d_hidden, size_t ldh, int batch, int hidden_dim, int vocab,
                                   const int32_t *d_history, int history_len, size_t hld, uint64_t *d_rng,
                                   int32_t *d_ids, float *d_probs, float *d_logits, void *stream) {
+    return noel_lmhead_sample_ex(cfg, d_weight, weight_type, ldw, d_hidden, ldh, batch, hidden_dim, vocab, nullptr,
+                                 nullptr, nullptr, d_history, history_len, hld, d_rng, d_ids, d_probs, d_logits,
+                                 nullptr, 0, stream);
+}
+
+extern "C" int noel_lmhead_sample_ex(const noel_sampler_config_t *cfg, const void *d_weight, int weight_type,
+                                     size_t ldw, const float *d_hidden, size_t ldh, int batch, int hidden_dim,
+                                     int vocab, const noel_lora_t *lora, const int32_t *d_adapter,
+                                     const noel_logits_params_t *process, const int32_t *d_history, int history_len,
+                                     size_t hld, uint64_t *d_rng, int32_t *d_ids, float *d_probs, float *d_logits,
+                                     void *d_work, size_t work_bytes, void *stream) {
     if (!cfg || !d_weight || !d_hidden || !d_logits) return fail(NOEL_ERR_INVALID_ARG, "cfg, weight, hidden and logits are required");
     if (weight_type != NOEL_HEAD_F32 && weight_type != NOEL_HEAD_F16 && weight_type != NOEL_HEAD_BF16)
         return fail(NOEL_ERR_UNSUPPORTED, "weight type %d (F32 0, F16 1, BF16 30)", weight_type);
@@ -1014,9 +1212,16 @@ extern "C" int noel_lmhead_sample(const noel_sampler_config_t *cfg, const void *
     if ((reinterpret_cast<uintptr_t>(d_weight) & 15) || (reinterpret_cast<uintptr_t>(d_hidden) & 15) ||
         (reinterpret_cast<uintptr_t>(d_logits) & 3))
         return fail(NOEL_ERR_INVALID_ARG, "weight and hidden must be 16-byte aligned");
+    int r;
+    LoraArgs la{};
+    LogitsArgs pa{};
+    if (lora && (r = lora_args(lora, d_adapter, d_hidden, ldh, batch, hidden_dim, vocab, d_logits, (size_t)vocab, d_work,
+                               work_bytes, &la)))
+        return r;
+    if (process && (r = logits_args(process, d_logits, NOEL_DTYPE_F32, batch, vocab, (size_t)vocab, &pa))) return r;
     if (batch == 0) return ok();
     DeviceCtx *c = nullptr;
-    int r = device_ctx(&c);
+    r = device_ctx(&c);
     if (r) return r;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     for (int t0 = 0; t0 < batch;) {
@@ -1037,6 +1242,8 @@ extern "C" int noel_lmhead_sample(const noel_sampler_config_t *cfg, const void *
         if (r) return r;
         t0 += nb;
     }
+    if (lora && (r = lora_launch(la, lora->type, s))) return r;
+    if (process && (r = logits_launch(pa, NOEL_DTYPE_F32, s))) return r;
     noel_sample_extras_t ex{};
     ex.d_probs = d_probs;
     return sample_batch(cfg, d_logits, NOEL_DTYPE_F32, batch, vocab, (size_t)vocab, d_history, history_len, hld,

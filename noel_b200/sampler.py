@@ -16,6 +16,8 @@ import numpy as np
 from .build import LIB
 
 F32, BF16 = 0, 1
+HEAD_F32, HEAD_F16, HEAD_BF16 = 0, 1, 30
+ERR_INVALID_ARG = -1
 
 STAT_NUM_CANDS, STAT_N_TOPK, STAT_N_FINAL, STAT_FLAGS = range(4)
 ROW_GREEDY, ROW_EXACT_PASS, ROW_FALLBACK = 1, 2, 4
@@ -130,6 +132,18 @@ def lib() -> C.CDLL:
     L.noel_lmhead_sample.argtypes = [C.POINTER(SamplerConfig), C.c_void_p, C.c_int, C.c_size_t, C.c_void_p,
                                      C.c_size_t, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_size_t,
                                      C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    L.noel_lmhead_sample_ex.restype = C.c_int
+    L.noel_lmhead_sample_ex.argtypes = [C.POINTER(SamplerConfig), C.c_void_p, C.c_int, C.c_size_t, C.c_void_p,
+                                        C.c_size_t, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                        C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+    L.noel_logits_process.restype = C.c_int
+    L.noel_logits_process.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_size_t, C.c_void_p]
+    L.noel_lora_workspace_bytes.restype = C.c_size_t
+    L.noel_lora_workspace_bytes.argtypes = [C.c_int, C.c_int]
+    L.noel_lora_apply.restype = C.c_int
+    L.noel_lora_apply.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_int,
+                                  C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p]
     L.noel_moe_route_top_k.restype = C.c_int
     L.noel_moe_route_top_k.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p]
     L.noel_sampler_cuda_last_error.restype = C.c_int
@@ -414,14 +428,225 @@ def postreq_sample(logits, params: PostreqParams) -> int:
     return int(r)
 
 
-HEAD_F32, HEAD_F16, HEAD_BF16 = 0, 1, 30
+def _refuse(message: str):
+    raise NoelSamplerError(ERR_INVALID_ARG, message)
 
 
-def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: bool = False):
+def _on(tensor, dtype, shape, name: str, device):
+    """tensor's address after the checks every argument gets: on device, of
+    dtype, of shape (None: any extent), its last axis of unit stride."""
+    if tensor is None:
+        return None
+    if tensor.dtype != dtype:
+        _refuse(f"{name}: {dtype} wanted, got {tensor.dtype}")
+    if tensor.device != device or not tensor.is_cuda:
+        _refuse(f"{name} is on {tensor.device}, {device} wanted" if tensor.is_cuda else f"{name} is not on a GPU")
+    have = tensor.shape
+    if len(have) != len(shape) or any(w is not None and w != h for w, h in zip(shape, have)):
+        _refuse(f"{name}: shape {tuple(shape)} wanted, got {tuple(have)}")
+    if have[-1] > 1 and tensor.stride(-1) != 1:
+        _refuse(f"{name}: its last axis must be contiguous")
+    return tensor.data_ptr()
+
+
+def _pitch(tensor, axis: int = 0) -> int:
+    """Elements from one index of axis to the next; where there is only one
+    (its stride may be anything), the last axis's extent."""
+    return tensor.stride(axis) if tensor.shape[axis] > 1 else tensor.shape[-1]
+
+
+def _row_values(tensor, dtype, batch, name: str, device):
+    """The address of one value a row (or adapter)."""
+    return _on(tensor, dtype, (batch,), name, device)
+
+
+class _Device:
+    """Makes a tensor's device the current one for a call, where it is not."""
+
+    def __init__(self, device):
+        import torch
+
+        self.torch, self.index = torch, device.index
+        self.before = torch.cuda.current_device()
+
+    def __enter__(self):
+        if self.before != self.index:
+            self.torch.cuda.set_device(self.index)
+
+    def __exit__(self, *_):
+        if self.before != self.index:
+            self.torch.cuda.set_device(self.before)
+
+
+class LogitsParamsStruct(C.Structure):
+    """noel_logits_params_t (include/noel_logits.h)."""
+
+    _fields_ = [("d_history", C.c_void_p), ("hld", C.c_size_t), ("history_len", C.c_int),
+                ("d_history_lens", C.c_void_p), ("d_prompt_lens", C.c_void_p), ("d_repetition", C.c_void_p),
+                ("d_frequency", C.c_void_p), ("d_presence", C.c_void_p), ("d_bias_ids", C.c_void_p),
+                ("d_bias", C.c_void_p), ("bld", C.c_size_t), ("bias_len", C.c_int), ("d_mask", C.c_void_p),
+                ("mld", C.c_size_t), ("mask_rows", C.c_int), ("d_mask_rows", C.c_void_p), ("v_begin", C.c_int)]
+
+
+class LogitsParams:
+    """What ``logits_process`` applies to each row of a batch of B rows
+    (include/noel_logits.h); every part may be left out.
+
+    history [B, H] int32 token ids, its first history_lens [B] int32 used and
+    the first prompt_lens [B] int32 of them the prompt; repetition, frequency,
+    presence [B] float32; bias_ids [B, N] int32 with bias [B, N] float32; mask
+    [M, words] int32, bit v % 32 of word v // 32 set where id v is allowed, and
+    mask_rows [B] int32 the mask of each row (outside 0 .. M - 1: none; left
+    out: mask b for row b); v_begin the id of the logits' first column.
+
+    The object holds the tensors themselves: a serving loop makes it once over
+    its buffers and writes the next step's values into them.
+    """
+
+    def __init__(self, history=None, history_lens=None, prompt_lens=None, repetition=None, frequency=None,
+                 presence=None, bias_ids=None, bias=None, mask=None, mask_rows=None, v_begin: int = 0):
+        import torch
+
+        self.tensors = [t for t in (history, history_lens, prompt_lens, repetition, frequency, presence, bias_ids,
+                                    bias, mask, mask_rows) if t is not None]
+        self.device = self.tensors[0].device if self.tensors else None
+        dev = self.device
+        if (bias_ids is None) != (bias is None):
+            _refuse("bias_ids and bias come together")
+        if history is None and any(t is not None for t in (history_lens, prompt_lens)):
+            _refuse("history_lens and prompt_lens need a history")
+        if mask is None and mask_rows is not None:
+            _refuse("mask_rows needs a mask")
+        per_row = [t for t in (history, history_lens, prompt_lens, repetition, frequency, presence, bias_ids, bias,
+                               mask_rows) if t is not None]
+        self.batch = per_row[0].shape[0] if per_row and per_row[0].dim() else None
+        B, i32, f32 = self.batch, torch.int32, torch.float32
+        s = self.s = LogitsParamsStruct()
+        s.d_history = _on(history, i32, (B, None), "history", dev)
+        s.d_history_lens = _row_values(history_lens, i32, B, "history_lens", dev)
+        s.d_prompt_lens = _row_values(prompt_lens, i32, B, "prompt_lens", dev)
+        s.d_repetition = _row_values(repetition, f32, B, "repetition", dev)
+        s.d_frequency = _row_values(frequency, f32, B, "frequency", dev)
+        s.d_presence = _row_values(presence, f32, B, "presence", dev)
+        if history is not None:
+            s.hld, s.history_len = _pitch(history), history.shape[1]
+        if bias_ids is not None:
+            s.d_bias_ids = _on(bias_ids, i32, (B, None), "bias_ids", dev)
+            s.d_bias = _on(bias, f32, tuple(bias_ids.shape), "bias", dev)
+            s.bld, s.bias_len = _pitch(bias_ids), bias_ids.shape[1]
+            if _pitch(bias) != s.bld:
+                _refuse("bias and bias_ids need rows of the same pitch")
+        if mask is not None:
+            s.d_mask = _on(mask, i32, (None, None), "mask", dev)
+            s.mld, s.mask_rows = _pitch(mask), mask.shape[0]
+            s.d_mask_rows = _row_values(mask_rows, i32, B, "mask_rows", dev)
+            self.words = mask.shape[1]
+        s.v_begin = v_begin
+
+    def check(self, logits, vocab: int) -> None:
+        """Whether these parameters fit rows of logits of vocab columns."""
+        if self.tensors and self.device != logits.device:
+            _refuse(f"parameters on {self.device}, logits on {logits.device}")
+        if self.batch is not None and self.batch != logits.shape[0]:
+            _refuse(f"parameters for {self.batch} rows, logits of {logits.shape[0]}")
+        if self.s.d_mask and self.words * 32 < self.s.v_begin + vocab:
+            _refuse(f"masks of {self.words} words for ids up to {self.s.v_begin + vocab - 1}")
+
+
+def logits_process(logits, params: LogitsParams, vocab: int | None = None, stream=None):
+    """Penalties, biases and masks on every row of logits, in place
+    (include/noel_logits.h): logits [B, ld] CUDA float32 or bfloat16 with unit
+    column stride, of which the first vocab columns (default: all) hold the
+    ids from params.v_begin on.  Returns logits."""
+    import torch
+
+    dtype = {torch.float32: F32, torch.bfloat16: BF16}.get(logits.dtype)
+    if dtype is None:
+        _refuse(f"logits: float32 or bfloat16 wanted, got {logits.dtype}")
+    dev = logits.device
+    ptr = _on(logits, logits.dtype, (None, None), "logits", dev)
+    B, cols = logits.shape
+    V = cols if vocab is None else vocab
+    if V > cols:
+        _refuse(f"vocab {V} of {cols} columns")
+    params.check(logits, V)
+    with _Device(dev):
+        s = stream if stream is not None else torch.cuda.current_stream(dev)
+        _check(lib().noel_logits_process(C.byref(params.s), ptr, dtype, B, V, _pitch(logits), C.c_void_p(s.cuda_stream)))
+    return logits
+
+
+class LoraStruct(C.Structure):
+    """noel_lora_t (include/noel_lora.h)."""
+
+    _fields_ = [("d_a", C.c_void_p), ("lda", C.c_size_t), ("stride_a", C.c_size_t), ("d_b", C.c_void_p),
+                ("ldb", C.c_size_t), ("stride_b", C.c_size_t), ("d_scale", C.c_void_p), ("d_ranks", C.c_void_p),
+                ("type", C.c_int), ("n_adapters", C.c_int), ("rank", C.c_int)]
+
+
+class Adapters:
+    """n low-rank adapters of one weight [V, D] (include/noel_lora.h): adapter
+    i is scale[i] * b[i] @ a[i] with a [n, r, D] and b [n, V, r], both float32,
+    float16 or bfloat16; scale [n] float32 (default 1) and ranks [n] int32
+    (adapters of a smaller rank than r).  Holds the tensors themselves."""
+
+    def __init__(self, a, b, scale=None, ranks=None):
+        import torch
+
+        kind = {torch.float32: HEAD_F32, torch.float16: HEAD_F16, torch.bfloat16: HEAD_BF16}.get(a.dtype)
+        if kind is None:
+            _refuse(f"a: float32, float16 or bfloat16 wanted, got {a.dtype}")
+        self.device, self.tensors = a.device, (a, b, scale, ranks)
+        s = self.s = LoraStruct()
+        s.d_a = _on(a, a.dtype, (None, None, None), "a", a.device)
+        self.n, self.rank, self.cols = a.shape
+        s.d_b = _on(b, a.dtype, (self.n, None, self.rank), "b", a.device)
+        self.rows = b.shape[1]
+        s.lda, s.stride_a, s.ldb, s.stride_b = _pitch(a, 1), _pitch(a), _pitch(b, 1), _pitch(b)
+        s.d_scale = _row_values(scale, torch.float32, self.n, "scale", a.device)
+        s.d_ranks = _row_values(ranks, torch.int32, self.n, "ranks", a.device)
+        s.type, s.n_adapters, s.rank = kind, self.n, self.rank
+
+    def scratch(self, batch: int):
+        """Scratch of one call over batch tokens, or None when it needs none."""
+        import torch
+
+        need = lib().noel_lora_workspace_bytes(batch, self.rank)
+        return torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+
+
+def lora_apply(y, x, adapters: Adapters, adapter_ids, stream=None):
+    """y[t] += scale[i] * b[i] @ (a[i] @ x[t]) in place, i = adapter_ids[t]
+    (outside 0 .. n - 1: y[t] is left as it is): y [B, V] and x [B, D] CUDA
+    float32 with unit column stride, adapter_ids [B] int32.  Returns y."""
+    import torch
+
+    dev = adapters.device
+    yp = _on(y, torch.float32, (None, adapters.rows), "y", dev)
+    B = y.shape[0]
+    xp = _on(x, torch.float32, (B, adapters.cols), "x", dev)
+    ip = _row_values(adapter_ids, torch.int32, B, "adapter_ids", dev)
+    with _Device(dev):
+        s = stream if stream is not None else torch.cuda.current_stream(dev)
+        if stream is None:
+            work = adapters.scratch(B)
+        else:
+            with torch.cuda.stream(stream):
+                work = adapters.scratch(B)
+        _check(lib().noel_lora_apply(C.byref(adapters.s), ip, xp, _pitch(x), B, adapters.cols, adapters.rows, yp,
+                                     _pitch(y), work.data_ptr() if work is not None else None,
+                                     work.numel() if work is not None else 0, C.c_void_p(s.cuda_stream)))
+    return y
+
+
+def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: bool = False,
+                  adapters: Adapters | None = None, adapter_ids=None, process: LogitsParams | None = None):
     """The LM head then the sampler (include/noel_lmhead.h): weight [V, D]
     CUDA float32 / float16 / bfloat16 (unit column stride), hidden [B, D]
     CUDA float32, rng [B, 2] int64 advanced in place, history [B, H] int32 or
-    None.  Returns (ids [B] int32, logits [B, V] float32, probs or None)."""
+    None.  adapters with adapter_ids [B] int32 add each token's low-rank part
+    to its logits, and process is applied to them before sampling.  Returns
+    (ids [B] int32, logits [B, V] float32, probs or None)."""
     import torch
 
     wt = {torch.float32: HEAD_F32, torch.float16: HEAD_F16, torch.bfloat16: HEAD_BF16}[weight.dtype]
@@ -429,6 +654,8 @@ def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: 
     V, D = weight.shape
     B = hidden.shape[0]
     dev = weight.device
+    if (adapters is None) != (adapter_ids is None):
+        _refuse("adapters and adapter_ids come together")
     logits = torch.empty(B, V, dtype=torch.float32, device=dev)
     ids = torch.empty(B, dtype=torch.int32, device=dev)
     pr = torch.empty(B, dtype=torch.float32, device=dev) if probs else None
@@ -436,9 +663,20 @@ def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: 
         hp, H, hld = history.data_ptr(), history.shape[1], history.stride(0)
     else:
         hp, H, hld = None, 0, 0
+    lora = ip = work = None
+    if adapters is not None:
+        if adapters.device != dev or (adapters.rows, adapters.cols) != (V, D):
+            _refuse(f"adapters of a [{adapters.rows}, {adapters.cols}] weight on {adapters.device}, "
+                    f"the head is [{V}, {D}] on {dev}")
+        lora, ip = C.byref(adapters.s), _row_values(adapter_ids, torch.int32, B, "adapter_ids", dev)
+        work = adapters.scratch(B)
+    if process is not None:
+        process.check(logits, V)
     s = torch.cuda.current_stream(dev)
-    _check(lib().noel_lmhead_sample(C.byref(cfg), weight.data_ptr(), wt, weight.stride(0), hidden.data_ptr(),
-                                    hidden.stride(0), B, D, V, hp, H, hld, rng.data_ptr(), ids.data_ptr(),
-                                    pr.data_ptr() if pr is not None else None, logits.data_ptr(),
-                                    C.c_void_p(s.cuda_stream)))
+    _check(lib().noel_lmhead_sample_ex(C.byref(cfg), weight.data_ptr(), wt, weight.stride(0), hidden.data_ptr(),
+                                       hidden.stride(0), B, D, V, lora, ip,
+                                       C.byref(process.s) if process is not None else None, hp, H, hld,
+                                       rng.data_ptr(), ids.data_ptr(), pr.data_ptr() if pr is not None else None,
+                                       logits.data_ptr(), work.data_ptr() if work is not None else None,
+                                       work.numel() if work is not None else 0, C.c_void_p(s.cuda_stream)))
     return ids, logits, pr
