@@ -7,10 +7,18 @@
  *   x = x > 0 ? x / rep : x * rep (seen);  x -= freq n, x -= pres (n > 0);
  *   x += biases on v;  x = -inf (masked)
  * in fp32 with one rounding to bf16 at the end.
+ *
+ * Nothing here reads the row as a whole.  A row's history and bias list name
+ * the few logits that the penalties and biases change, and a mask only writes;
+ * what has to move is the history, the mask's bits, the touched logits and the
+ * masked ones.  The two halves of the work touch different logits (a mask
+ * wins, so the penalties leave masked ids alone, and the mask writes nothing
+ * else): they need no order between them and run as CTAs of one launch.
  */
 #pragma once
 
-#include "sampler_device.cuh"
+#include "sampler_kernels.cuh"
+#include "sampler_warp.cuh"
 
 #include <cuda_bf16.h>
 
@@ -33,12 +41,21 @@ struct LogitsArgs {
     int64_t mld;
     int mask_rows;
     const int32_t *mask_row;
-    int slices;
+    int ranges, range;  // CTAs per row and their columns; 0: no such launch
+    int cap;            // entries of a CTA's table; 0: none
+    int slices, slice;  // CTAs per row of the slice kernel and the words each counts in
 };
 
 constexpr int kLogitsThreads = 256;
-constexpr int kLogitsSlice = 8192;       // columns of a CTA: one 32-bit word of shared memory each
-constexpr int kLogitsMaxBias = 64 * kLogitsThreads;
+constexpr int kRowsCtas = 6;         // CTAs per SM the rows kernel is compiled for
+constexpr int kLogitsSms = 148;
+constexpr int kMaskPiece = 1024;     // columns of a warp's turn: 32 words of the mask
+constexpr int kMaskRange = 131072;   // bytes of a row that a CTA masks, at most
+constexpr int kTableMax = 2048;      // history plus biases a row's table may take
+constexpr int kTableBatch = 8;       // loads in flight per thread of the table half
+constexpr int kSliceThreads = 512;
+constexpr int kSliceMax = 24576;     // columns of a slice: one 32-bit word of shared memory each
+constexpr int kLogitsMaxBias = 16384;
 constexpr int kLogitsMaxHistory = 1 << 29;
 
 /* a column's word: the occurrences among the generated ids, and three marks */
@@ -80,63 +97,421 @@ __device__ __forceinline__ bool allowed(const uint32_t *mask, int id) {
     return !mask || (mask[id >> 5] >> (id & 31) & 1u);
 }
 
-/* One CTA per row and slice of kLogitsSlice columns: the slice's words are
- * counted in shared memory from the whole history, then the slice's columns
- * are gone through. */
+/* the ids of a row's history that count, and how many of them are prompt */
+struct RowHistory {
+    const int32_t *ids;
+    int len, prompt;
+};
+
+__device__ __forceinline__ RowHistory row_history(const LogitsArgs &a, int row) {
+    if (!a.hist) return {nullptr, 0, 0};
+    return {a.hist + (size_t)row * (size_t)a.hld,
+            a.hist_lens ? min(max(a.hist_lens[row], 0), a.hist_len) : a.hist_len,
+            a.prompt_lens ? a.prompt_lens[row] : 0};
+}
+
+/* the sum of a row's biases on one id, in list order, by a whole warp */
+__device__ __forceinline__ float bias_sum(const int32_t *bi, const float *bv, int nb, int id) {
+    const int lane = threadIdx.x & 31;
+    float s = 0.0f;
+    for (int j0 = 0; j0 < nb; j0 += 32) {
+        const int j = j0 + lane;
+        const bool hit = j < nb && bi[j] == id;
+        const float v = hit ? bv[j] : 0.0f;
+        for (uint32_t m = __ballot_sync(kFull, hit); m; m &= m - 1)
+            s = __fadd_rn(s, __shfl_sync(kFull, v, __ffs(m) - 1));
+    }
+    return s;
+}
+
+/* The table of a CTA's columns [lo, hi) of a row: open addressing in shared
+ * memory, entry = (column + 1, word, bias). */
+struct Table {
+    uint32_t *key, *word;
+    float *sum;
+    int cap;  // a power of two, a multiple of the CTA's threads, at least 3/2 of what can come in
+};
+
+__device__ __forceinline__ uint32_t table_slot(const Table &t, uint32_t k) {
+    uint32_t p = hs_hash(k) >> (33 - __ffs(t.cap));
+    for (int probe = 0; probe < t.cap; ++probe) {
+        uint32_t prev = *(volatile uint32_t *)&t.key[p];  // a repeated id needs no compare-and-swap
+        if (prev == 0u) prev = atomicCAS(&t.key[p], 0u, k);
+        if (prev == 0u || prev == k) break;
+        p = (p + 1) & (uint32_t)(t.cap - 1);
+    }
+    return p;
+}
+
+/* The row's history and bias ids of columns [lo, hi) into the table.  Loads go
+ * out kTableBatch at a time: with few CTAs per SM the time of this is the
+ * number of load latencies in a row. */
+template <int N>  // by the CTA's first N threads
+__device__ __forceinline__ void table_fill(const LogitsArgs &a, int row, const Table &t, int lo, int hi) {
+    const int tid = threadIdx.x;
+    const RowHistory h = row_history(a, row);
+    for (int i = tid; i < t.cap / 2; i += N)  // keys and words
+        reinterpret_cast<uint4 *>(t.key)[i] = make_uint4(0, 0, 0, 0);
+    if (N == 32) __syncwarp();
+    else __syncthreads();
+    for (int i0 = tid; i0 < h.len; i0 += kTableBatch * N) {
+        int id[kTableBatch];
+#pragma unroll
+        for (int u = 0; u < kTableBatch; ++u) {
+            const int i = i0 + u * N;
+            id[u] = i < h.len ? h.ids[i] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kTableBatch; ++u) {
+            const int64_t c = (int64_t)id[u] - a.v_begin;
+            if (id[u] < 0 || c < lo || c >= hi) continue;
+            const uint32_t p = table_slot(t, (uint32_t)c + 1u);
+            if (i0 + u * N < h.prompt) atomicOr(&t.word[p], kSeenPrompt);
+            else atomicAdd(&t.word[p], 1u);
+        }
+    }
+    const int nb = a.bias_len;
+    const int32_t *bi = nb ? a.bias_ids + (size_t)row * (size_t)a.bld : nullptr;
+    const float *bv = nb ? a.bias + (size_t)row * (size_t)a.bld : nullptr;
+    for (int i0 = tid; i0 < nb; i0 += 2 * N) {
+        int id[2];
+        float v[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int i = i0 + u * N;
+            id[u] = i < nb ? bi[i] : -1;
+            v[u] = i < nb ? bv[i] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int64_t c = (int64_t)id[u] - a.v_begin;
+            if (id[u] < 0 || c < lo || c >= hi) continue;
+            const uint32_t p = table_slot(t, (uint32_t)c + 1u);
+            if (atomicOr(&t.word[p], kHasBias) & kHasBias) atomicOr(&t.word[p], kManyBiases);
+            else t.sum[p] = v[u];  // the entry's only writer
+        }
+    }
+}
+
+/* Each entry's logit read, changed and written once, masked ones left alone. */
 template <typename T>
-__global__ void __launch_bounds__(kLogitsThreads) logits_process_kernel(const __grid_constant__ LogitsArgs a) {
-    __shared__ uint32_t word[kLogitsSlice];
+__device__ __forceinline__ void table_apply(const LogitsArgs &a, int row, const Table &t, const uint32_t *mask) {
+    const int tid = threadIdx.x, nb = a.bias_len;
+    const RowRules rules = row_rules(a, row);
+    const int32_t *bi = nb ? a.bias_ids + (size_t)row * (size_t)a.bld : nullptr;
+    const float *bv = nb ? a.bias + (size_t)row * (size_t)a.bld : nullptr;
+    T *x = static_cast<T *>(a.logits) + (size_t)row * (size_t)a.ld;
+    for (int s0 = tid; s0 < t.cap; s0 += kTableBatch * kLogitsThreads) {  // whole warps
+        uint32_t k[kTableBatch], m[kTableBatch];
+        float v[kTableBatch];
+#pragma unroll
+        for (int u = 0; u < kTableBatch; ++u) {
+            const int s = s0 + u * kLogitsThreads;
+            k[u] = s < t.cap ? t.key[s] : 0u;
+            v[u] = k[u] ? logit_load(x + (k[u] - 1u)) : 0.0f;
+            const uint32_t id = (uint32_t)a.v_begin + k[u] - 1u;
+            m[u] = k[u] && mask ? mask[id >> 5] >> (id & 31u) : 1u;
+        }
+#pragma unroll
+        for (int u = 0; u < kTableBatch; ++u) {
+            const int s = s0 + u * kLogitsThreads;
+            const bool on = k[u] && (m[u] & 1u);
+            const uint32_t w = on ? t.word[s] : 0u;
+            float b = on && (w & kHasBias) ? t.sum[s] : 0.0f;
+            if (nb) {
+                for (uint32_t q = __ballot_sync(kFull, (w & kManyBiases) != 0u); q; q &= q - 1) {
+                    const int l = __ffs(q) - 1;
+                    const float all = bias_sum(bi, bv, nb, a.v_begin + (int)(__shfl_sync(kFull, k[u], l) - 1u));
+                    if ((tid & 31) == l) b = all;
+                }
+            }
+            if (!on) continue;
+            float y = penalised(v[u], w, rules);
+            if (w & kHasBias) y = __fadd_rn(y, b);
+            logit_store(x + (k[u] - 1u), y);
+        }
+    }
+}
+
+/* 32 bytes of logits, the unit in which memory is written whole */
+struct Sector {
+    uint32_t u[8];
+};
+__device__ __forceinline__ Sector sector_load(const void *p) {
+    Sector s;
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(s.u[0]), "=r"(s.u[1]), "=r"(s.u[2]), "=r"(s.u[3]), "=r"(s.u[4]), "=r"(s.u[5]), "=r"(s.u[6]),
+                   "=r"(s.u[7])
+                 : "l"(p));
+    return s;
+}
+__device__ __forceinline__ void sector_store(void *p, const Sector &s) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(s.u[0]), "r"(s.u[1]),
+                 "r"(s.u[2]), "r"(s.u[3]), "r"(s.u[4]), "r"(s.u[5]), "r"(s.u[6]), "r"(s.u[7])
+                 : "memory");
+}
+__device__ __forceinline__ Sector sector_all(float) {
+    const uint32_t m = 0xFF800000u;
+    return {{m, m, m, m, m, m, m, m}};
+}
+__device__ __forceinline__ Sector sector_all(uint16_t) {
+    const uint32_t m = 0xFF80FF80u;
+    return {{m, m, m, m, m, m, m, m}};
+}
+/* -infinity for the elements whose bit in gone is set */
+__device__ __forceinline__ void sector_mask(Sector &s, uint32_t gone, float) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s.u[e] = gone >> e & 1u ? 0xFF800000u : s.u[e];
+}
+__device__ __forceinline__ void sector_mask(Sector &s, uint32_t gone, uint16_t) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t keep = (gone >> (2 * e) & 1u ? 0u : 0xFFFFu) | (gone >> (2 * e + 1) & 1u ? 0u : 0xFFFF0000u);
+        s.u[e] = (s.u[e] & keep) | (0xFF80FF80u & ~keep);
+    }
+}
+
+/* The 32 mask bits of columns c .. c + 31, those outside the row as allowed. */
+__device__ __forceinline__ uint32_t mask_bits(const LogitsArgs &a, const uint32_t *mask, int64_t c) {
+    if (c >= a.vocab) return 0xFFFFFFFFu;
+    const int64_t bit = a.v_begin + c, wi = bit >> 5, nw = ((int64_t)a.v_begin + a.vocab + 31) >> 5;
+    const uint32_t lo = wi >= 0 ? __ldg(mask + wi) : 0xFFFFFFFFu;
+    const uint32_t hi = (bit & 31) && wi + 1 < nw ? __ldg(mask + wi + 1) : 0xFFFFFFFFu;
+    uint32_t ok = __funnelshift_r(lo, hi, (uint32_t)bit & 31u);
+    if (c < 0) ok |= (1u << -c) - 1u;
+    if (c + 32 > a.vocab) ok |= 0xFFFFFFFFu << (a.vocab - c);
+    return ok;
+}
+
+/* One warp masks the 1024 columns from c0 on, whose mask bits lane l holds 32
+ * at a time; c0 lies on 32 bytes of memory and may lie before the row.
+ *
+ * Memory takes 1024 bytes of a warp's store fastest when none of them has to
+ * be filled in from what is there already: 584 MB of masked logits take 90 us
+ * where rows are masked throughout, but a single allowed logit left out of a
+ * line costs that line's read besides.  So where at least half of the warp's
+ * 32-byte sectors have something masked, the others and the partly masked
+ * ones are read and all of it is written in one store; where fewer have, the
+ * masked logits are written one by one. */
+template <typename T>
+__device__ __forceinline__ void mask_piece(const LogitsArgs &a, T *x, int64_t c0, uint32_t ok) {
+    constexpr int VE = 32 / sizeof(T);  // elements a lane takes at a time
+    constexpr int STEPS = kMaskPiece / (32 * VE), BATCH = 2;
+    constexpr uint32_t ALL = VE == 32 ? 0xFFFFFFFFu : (1u << VE) - 1u;
+    const int lane = threadIdx.x & 31;
+    if (!__any_sync(kFull, ok != 0xFFFFFFFFu)) return;
+    T *at = x + c0 + VE * lane;  // may lie outside the row; nothing there is touched
+    /* the steps whose columns all lie inside the row */
+    const int first = c0 < 0 ? 1 : 0;
+    const int last = (int)min((a.vocab - c0) / (32 * VE), (int64_t)STEPS);
+#pragma unroll
+    for (int q0 = 0; q0 < STEPS; q0 += BATCH) {
+        Sector s[BATCH];
+        uint32_t gone[BATCH];
+        bool whole[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {  // VE words of the mask cover 32 lanes x VE columns
+            const int q = q0 + j;
+            const uint32_t w = __shfl_sync(kFull, ok, q * VE + lane * VE / 32);
+            gone[j] = ~(w >> (lane * VE % 32)) & ALL;
+            whole[j] = __popc(__ballot_sync(kFull, gone[j] != 0u)) >= 16 && q >= first && q < last;
+            if (whole[j] && gone[j] != ALL) s[j] = sector_load(at + q * 32 * VE);
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            T *to = at + (q0 + j) * 32 * VE;
+            if (whole[j]) {
+                sector_mask(s[j], gone[j], T{});
+                sector_store(to, s[j]);
+            } else {
+                for (uint32_t g = gone[j]; g; g &= g - 1) logit_store(to + (__ffs(g) - 1), -INFINITY);
+            }
+        }
+    }
+}
+
+/* One CTA per row and range of its columns: the table of the range is filled,
+ * the range is masked, and then the table's logits are changed.  The mask
+ * never changes an allowed logit's value but may write it back as it read it,
+ * so the table's own writes come after the mask's, a CTA's barrier between
+ * them.  In a masked row one warp fills the table while the others mask; it
+ * takes its turns at the mask when it has done that. */
+template <typename T>
+__global__ void __launch_bounds__(kLogitsThreads, kRowsCtas) logits_rows_kernel(const __grid_constant__ LogitsArgs a) {
+    extern __shared__ __align__(16) uint32_t logits_smem[];
+    __shared__ int turn;
+    constexpr int VE = 32 / sizeof(T);
+    const int row = blockIdx.x / a.ranges, range = blockIdx.x % a.ranges;
+    const uint32_t *mask = row_mask(a, row);
+    T *x = static_cast<T *>(a.logits) + (size_t)row * (size_t)a.ld;
+    /* ranges begin on 32 bytes of memory, the first one up to VE - 1 columns before the row */
+    const int64_t begin = (int64_t)range * a.range - (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % VE);
+    const int64_t end = min(begin + a.range, (int64_t)a.vocab);
+    const Table t{logits_smem, logits_smem + a.cap, reinterpret_cast<float *>(logits_smem + 2 * a.cap), a.cap};
+    const int lo = (int)max(begin, (int64_t)0), hi = (int)max(end, (int64_t)lo);
+    if (mask) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        if (threadIdx.x == 0) turn = kLogitsThreads / 32;  // every warp's first turn is its own number
+        __syncthreads();
+        if (a.cap && warp == 0) table_fill<32>(a, row, t, lo, hi);
+        int k = warp;
+        uint32_t next = mask_bits(a, mask, begin + (int64_t)k * kMaskPiece + 32 * lane);
+        while (begin + (int64_t)k * kMaskPiece < end) {
+            const uint32_t ok = next;
+            const int64_t c = begin + (int64_t)k * kMaskPiece;
+            if (lane == 0) k = atomicAdd(&turn, 1);
+            k = __shfl_sync(kFull, k, 0);
+            next = mask_bits(a, mask, begin + (int64_t)k * kMaskPiece + 32 * lane);  // on its way meanwhile
+            mask_piece(a, x, c, ok);
+        }
+    } else if (a.cap) {
+        table_fill<kLogitsThreads>(a, row, t, lo, hi);
+    }
+    if (a.cap) {
+        __syncthreads();
+        table_apply<T>(a, row, t, mask);
+    }
+}
+
+/* the penalties of a sector's words on its logits, biased and masked ones left alone */
+template <typename T>
+__device__ __forceinline__ void sector_penalise(const LogitsArgs &a, Sector &s, const uint32_t (&w)[32 / sizeof(T)],
+                                                const RowRules &rules, const uint32_t *mask, int c) {
+    constexpr int VE = 32 / sizeof(T);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+        if (!w[e] || (w[e] & kHasBias) || !allowed(mask, a.v_begin + c + e)) continue;
+        if (sizeof(T) == 4) {
+            s.u[e] = __float_as_uint(penalised(__uint_as_float(s.u[e]), w[e], rules));
+        } else {
+            const int h = 16 * (e & 1);
+            const float v = penalised(__uint_as_float(s.u[e / 2] >> h << 16), w[e], rules);
+            const uint32_t r = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+            s.u[e / 2] = (s.u[e / 2] & ~(0xFFFFu << h)) | r << h;
+        }
+    }
+}
+
+/* Histories too long for a table: one CTA per row and slice of columns counts
+ * the whole history's ids of its slice, one word of shared memory per column,
+ * and then goes through the slice.  Slice s of S (a power of two) has every
+ * S-th line of 128 bytes: frequent tokens have low ids, and slices of
+ * consecutive columns leave the first one nearly all the counting; a line
+ * belongs to one CTA, which reads and writes it whole if the history touches
+ * any of it (a long history touches most of the low ids' lines, and single
+ * logits cost memory what whole lines cost). */
+template <typename T>
+__global__ void __launch_bounds__(kSliceThreads) logits_slice_kernel(const __grid_constant__ LogitsArgs a) {
+    extern __shared__ __align__(16) uint32_t logits_smem[];
+    uint32_t *word = logits_smem;
     const int tid = threadIdx.x;
     const int row = blockIdx.x / a.slices;
-    const int c0 = (blockIdx.x % a.slices) * kLogitsSlice;
-    const int width = min(kLogitsSlice, a.vocab - c0);
-    const int id0 = a.v_begin + c0;
-    T *x = static_cast<T *>(a.logits) + (size_t)row * (size_t)a.ld + c0;
-    const uint32_t *mask = row_mask(a, row);
+    const uint32_t mine_c = blockIdx.x % a.slices;
+    const int sh = __ffs(a.slices) - 1;
+    constexpr int VE = 32 / sizeof(T), BLK = 4 * VE;  // columns of a sector and of a line
+    const int width = a.slice;  // words of this slice (those past the vocabulary stay 0)
+    const RowHistory h = row_history(a, row);
     const RowRules rules = row_rules(a, row);
-    for (int i = tid; i < width; i += kLogitsThreads) word[i] = 0u;
+    const uint32_t *mask = row_mask(a, row);
+    for (int i = tid; i < (width + 3) / 4; i += kSliceThreads)
+        reinterpret_cast<uint4 *>(word)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (a.hist) {
-        const int32_t *h = a.hist + (size_t)row * (size_t)a.hld;
-        const int len = a.hist_lens ? min(max(a.hist_lens[row], 0), a.hist_len) : a.hist_len;
-        const int prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
-        for (int i = tid; i < len; i += kLogitsThreads) {
-            const int64_t c = (int64_t)h[i] - id0;
-            if (c < 0 || c >= width) continue;
-            if (i < prompt) atomicOr(&word[c], kSeenPrompt);
-            else atomicAdd(&word[c], 1u);
+    /* an id's column if it is one of the slice's, as its index in the slice */
+    auto index_of = [&](int id, uint32_t &c) {
+        c = (uint32_t)id - (uint32_t)a.v_begin;
+        const bool in = id >= a.v_begin && c < (uint32_t)a.vocab && (c / BLK & (uint32_t)(a.slices - 1)) == mine_c;
+        c = (c / BLK >> sh) * BLK + c % BLK;  // its word
+        return in;
+    };
+    /* the history 16 bytes at a time from its first aligned id on: the prompt
+     * only marks, the rest counts */
+    auto through = [&](const int32_t *ids, int n, auto take) {
+        const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(ids) & 15)) / 4 % 4));
+        const int vecs = (n - head) / 4;
+        if (tid < head) take(ids[tid]);
+        const int4 *v = reinterpret_cast<const int4 *>(ids + head);
+#pragma unroll 4
+        for (int i = tid; i < vecs; i += kSliceThreads) {
+            const int4 q = __ldg(v + i);
+            take(q.x);
+            take(q.y);
+            take(q.z);
+            take(q.w);
         }
-    }
-    __syncthreads();  // counts are whole before the marks above them are set
-    unsigned long long mine = 0ull;  // the biases whose column this thread marked first
-    const int32_t *bi = a.bias_ids ? a.bias_ids + (size_t)row * (size_t)a.bld : nullptr;
-    const float *bv = a.bias_ids ? a.bias + (size_t)row * (size_t)a.bld : nullptr;
-    const int nb = a.bias_ids ? a.bias_len : 0;
-    for (int i = tid, k = 0; i < nb; i += kLogitsThreads, ++k) {
-        const int64_t c = (int64_t)bi[i] - id0;
-        if (c < 0 || c >= width) continue;
-        if (atomicOr(&word[c], kHasBias) & kHasBias) atomicOr(&word[c], kManyBiases);
-        else mine |= 1ull << k;
-    }
+        const int tail = head + 4 * vecs + tid;
+        if (tail < n) take(ids[tail]);
+    };
+    const int prompt = min(max(h.prompt, 0), h.len);
+    through(h.ids, prompt, [&](int id) {
+        uint32_t c;
+        if (index_of(id, c)) word[c] = kSeenPrompt;  // every writer writes the same
+    });
     __syncthreads();
-    for (int i = tid, k = 0; i < nb; i += kLogitsThreads, ++k) {
-        if (!(mine >> k & 1ull)) continue;
+    through(h.ids + prompt, h.len - prompt, [&](int id) {
+        uint32_t c;
+        if (index_of(id, c)) atomicAdd(&word[c], 1u);
+    });
+    const int nb = a.bias_len;
+    const int32_t *bi = nb ? a.bias_ids + (size_t)row * (size_t)a.bld : nullptr;
+    const float *bv = nb ? a.bias + (size_t)row * (size_t)a.bld : nullptr;
+    uint32_t mine = 0u;  // the biases whose column this thread marked first
+    static_assert(kLogitsMaxBias <= 32 * kSliceThreads, "one bit of `mine` per bias of a thread");
+    for (int i = tid, k = 0; i < nb; i += kSliceThreads, ++k) {
         const int id = bi[i];
-        const uint32_t w = word[id - id0];
-        if (!allowed(mask, id)) continue;
-        float b = bv[i];
-        if (w & kManyBiases) {  // which thread came first is chance; the sum goes by the list's order
-            b = 0.0f;
-            for (int j = 0; j < nb; ++j)
-                if (bi[j] == id) b = __fadd_rn(b, bv[j]);
-        }
-        T *p = x + (id - id0);
-        logit_store(p, __fadd_rn(penalised(logit_load(p), w, rules), b));
+        uint32_t c;
+        if (!index_of(id, c)) continue;
+        if (atomicOr(&word[c], kHasBias) & kHasBias) atomicOr(&word[c], kManyBiases);
+        else mine |= 1u << k;
     }
-    for (int i = tid; i < width; i += kLogitsThreads) {
-        const uint32_t w = word[i];
-        if (!allowed(mask, id0 + i)) logit_store(x + i, -INFINITY);
-        else if (w && !(w & kHasBias)) logit_store(x + i, penalised(logit_load(x + i), w, rules));
+    __syncthreads();
+    T *x = static_cast<T *>(a.logits) + (size_t)row * (size_t)a.ld;
+    /* a lane takes a sector, four lanes a line, and a line with anything in it
+     * is read and written whole; rows that do not start on 32 bytes, and the
+     * row's last line, go by element */
+    const bool lines = (reinterpret_cast<uintptr_t>(x) & 31) == 0;
+    for (int s0 = tid; s0 * VE < width; s0 += kSliceThreads) {  // width / VE is a multiple of 32: whole warps
+        uint32_t w[VE];
+        uint32_t any = 0u;
+#pragma unroll
+        for (int e = 0; e < VE; e += 4) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(word + s0 * VE + e);
+            w[e] = q.x;
+            w[e + 1] = q.y;
+            w[e + 2] = q.z;
+            w[e + 3] = q.w;
+            any |= q.x | q.y | q.z | q.w;
+        }
+        const int c = ((((s0 * VE) / BLK) << sh) + (int)mine_c) * BLK + (s0 * VE) % BLK;
+        const uint32_t touched = __ballot_sync(kFull, any != 0u);
+        if (!(touched >> (tid & 28) & 15u)) continue;
+        if (lines && (int64_t)(c - c % BLK) + BLK <= a.vocab) {
+            Sector s = sector_load(x + c);
+            if (any) sector_penalise<T>(a, s, w, rules, mask, c);
+            sector_store(x + c, s);
+        } else if (any) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (w[e] && !(w[e] & kHasBias) && allowed(mask, a.v_begin + c + e))
+                    logit_store(x + c + e, penalised(logit_load(x + c + e), w[e], rules));
+        }
+    }
+    if (nb) __syncthreads();  // the lines are written; biased logits were written as they were read
+    for (int i0 = 0, k = 0; i0 < nb; i0 += kSliceThreads, ++k) {  // whole warps
+        const int i = i0 + tid;
+        const int id = i < nb ? bi[i] : 0;
+        const bool on = (mine >> k & 1u) && allowed(mask, id);
+        uint32_t c = 0u;
+        const uint32_t w = on && index_of(id, c) ? word[c] : 0u;
+        float b = on ? bv[i] : 0.0f;
+        for (uint32_t m = __ballot_sync(kFull, on && (w & kManyBiases)); m; m &= m - 1) {
+            const int l = __ffs(m) - 1;
+            const float all = bias_sum(bi, bv, nb, __shfl_sync(kFull, id, l));
+            if ((tid & 31) == l) b = all;
+        }
+        if (on) {
+            T *p = x + (id - a.v_begin);
+            logit_store(p, __fadd_rn(penalised(logit_load(p), w, rules), b));
+        }
     }
 }
 

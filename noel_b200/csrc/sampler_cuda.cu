@@ -1047,19 +1047,56 @@ int logits_args(const noel_logits_params_t *p, void *logits, int dtype, int B, i
     a.mld = (int64_t)p->mld;
     a.mask_rows = p->mask_rows;
     a.mask_row = p->d_mask_rows;
-    a.slices = (V + kLogitsSlice - 1) / kLogitsSlice;
-    if ((int64_t)B * a.slices > 0x7FFFFFFF) return fail(NOEL_ERR_TOO_LARGE, "%d rows x %d columns", B, V);
+    /* a row's history and biases in a table where they fit one, else counted
+     * over slices of its columns; the mask by ranges of the row */
+    const int n = a.hist_len + a.bias_len;
+    if (n > 0 && n <= kTableMax) a.cap = pow2_at_least(n + n / 2 > kLogitsThreads ? n + n / 2 : kLogitsThreads);
+    if (a.mask) {
+        /* ranges that give each of the GPU's CTA slots two, in whole turns of a CTA's warps: a large batch
+         * runs fastest at 128 KB (1024 x 152,064 fp32 under strict masks: 145, 125, 120 and 121 us at 32, 64,
+         * 128 and 256 KB), a small one with a turn per warp */
+        const int64_t turn = (int64_t)kMaskPiece * (kLogitsThreads / 32), most = kMaskRange / (int64_t)es;
+        int64_t want = (int64_t)B * V / (2 * kRowsCtas * kLogitsSms) / turn * turn;
+        want = want < turn ? turn : want;
+        a.range = (int)(want < most ? want : most);
+        a.ranges = (int)(((int64_t)V + 15 + a.range - 1) / a.range);
+    } else if (a.cap) {
+        a.range = 0x7FFFFFFF;  // the row whole
+        a.ranges = 1;
+    }
+    if (n > kTableMax) {
+        a.slices = pow2_at_least((V + kSliceMax - 1) / kSliceMax);
+        const int line = 64 * a.slices;  // 128 bytes of bf16 from every slice
+        a.slice = (V + line - 1) / line * 64;
+        a.slice = (a.slice + 511) / 512 * 512;  // whole warps of sectors of either type
+    }
+    if (B > 1 << 30 || (int64_t)B * a.slices > 0x7FFFFFFF || (int64_t)B * a.ranges > 0x7FFFFFFF) return fail(NOEL_ERR_TOO_LARGE, "%d rows x %d columns", B, V);
     *out = a;
     return NOEL_OK;
 }
 
-int logits_launch(const LogitsArgs &a, int dtype, cudaStream_t s) {
-    if (a.batch == 0 || (!a.hist && !a.bias_ids && !a.mask)) return NOEL_OK;
-    const int grid = a.batch * a.slices;
-    if (dtype == NOEL_DTYPE_F32) logits_process_kernel<float><<<grid, kLogitsThreads, 0, s>>>(a);
-    else logits_process_kernel<uint16_t><<<grid, kLogitsThreads, 0, s>>>(a);
-    CUDA_TRY(cudaGetLastError());
+template <typename T>
+int logits_launch_t(DeviceCtx *c, const LogitsArgs &a, cudaStream_t s) {
+    if (a.ranges) {
+        const size_t smem = (size_t)a.cap * 12;
+        const int r = set_smem(c, (const void *)logits_rows_kernel<T>, smem);
+        if (r) return r;
+        logits_rows_kernel<T><<<a.batch * a.ranges, kLogitsThreads, smem, s>>>(a);
+        CUDA_TRY(cudaGetLastError());
+    }
+    if (a.slices) {
+        const size_t smem = (size_t)a.slice * 4;
+        const int r = set_smem(c, (const void *)logits_slice_kernel<T>, smem);
+        if (r) return r;
+        logits_slice_kernel<T><<<a.batch * a.slices, kSliceThreads, smem, s>>>(a);
+        CUDA_TRY(cudaGetLastError());
+    }
     return NOEL_OK;
+}
+
+int logits_launch(DeviceCtx *c, const LogitsArgs &a, int dtype, cudaStream_t s) {
+    return a.batch == 0 ? NOEL_OK
+           : dtype == NOEL_DTYPE_F32 ? logits_launch_t<float>(c, a, s) : logits_launch_t<uint16_t>(c, a, s);
 }
 }  // namespace
 
@@ -1072,7 +1109,7 @@ extern "C" int noel_logits_process(const noel_logits_params_t *params, void *d_l
     DeviceCtx *c = nullptr;
     r = device_ctx(&c);
     if (r) return r;
-    r = logits_launch(a, dtype, static_cast<cudaStream_t>(stream));
+    r = logits_launch(c, a, dtype, static_cast<cudaStream_t>(stream));
     return r ? r : ok();
 }
 
@@ -1243,7 +1280,7 @@ extern "C" int noel_lmhead_sample_ex(const noel_sampler_config_t *cfg, const voi
         t0 += nb;
     }
     if (lora && (r = lora_launch(la, lora->type, s))) return r;
-    if (process && (r = logits_launch(pa, NOEL_DTYPE_F32, s))) return r;
+    if (process && (r = logits_launch(c, pa, NOEL_DTYPE_F32, s))) return r;
     noel_sample_extras_t ex{};
     ex.d_probs = d_probs;
     return sample_batch(cfg, d_logits, NOEL_DTYPE_F32, batch, vocab, (size_t)vocab, d_history, history_len, hld,
