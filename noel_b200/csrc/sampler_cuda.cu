@@ -1115,6 +1115,13 @@ extern "C" int noel_logits_process(const noel_logits_params_t *params, void *d_l
 
 /* ------------------------------------------------ low-rank adapters */
 namespace {
+int lora_rank_pad(int rank) { return rank <= 16 ? 16 : (rank + 31) / 32 * 32; }
+
+/* the low-rank numbers of one pass: three bf16 parts per token and rank */
+size_t lora_low_bytes(int batch, int rank) {
+    return (size_t)(batch < kLoraBatch ? batch : kLoraBatch) * 3 * lora_rank_pad(rank) * sizeof(uint16_t);
+}
+
 int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size_t ldx, int B, int cols, int rows,
               float *y, size_t ldy, void *work, size_t work_bytes, LoraArgs *out) {
     if (!l) return fail(NOEL_ERR_INVALID_ARG, "lora is NULL");
@@ -1160,32 +1167,75 @@ int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size
     a.rows = rows;
     a.y = y;
     a.ldy = (int64_t)ldy;
-    a.low = static_cast<float *>(work);
+    a.low = static_cast<uint16_t *>(work);
+    a.rank_pad = lora_rank_pad(l->rank);
+    a.plan = B > kLoraWarpBatch ? reinterpret_cast<LoraPlan *>(static_cast<char *>(work) + lora_low_bytes(B, l->rank))
+                                : nullptr;
+    auto rows_on = [](const void *p, size_t pitch, size_t stride, size_t bytes) {
+        return reinterpret_cast<uintptr_t>(p) % bytes == 0 && pitch % bytes == 0 && stride % bytes == 0;
+    };
+    const size_t lane_b = a.rank_pad == 16 && es == 2 ? 8 : 16;  // bytes of a lane's ranks, at most 16
+    a.vec_x = rows_on(x, ldx * 4, 0, 16);
+    a.vec_y = rows_on(y, ldy * 4, 0, 16);
+    a.vec_a = rows_on(l->d_a, l->lda * es, l->stride_a * es, 16);
+    a.vec_b = rows_on(l->d_b, l->ldb * es, l->stride_b * es, lane_b);
     *out = a;
     return NOEL_OK;
 }
 
+/* a kernel that may start while the one before it in the stream still runs
+ * (it waits for it with griddepcontrol.wait) */
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*k)(P...), dim3 grid, int threads, cudaStream_t s, bool dependent, A... args) {
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = grid;
+    lc.blockDim = dim3(threads);
+    lc.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at;
+    lc.numAttrs = dependent ? 1 : 0;
+    return cudaLaunchKernelEx(&lc, k, args...);
+}
+
 template <int WT>
-int lora_launch_t(const LoraArgs &a, cudaStream_t s) {
-    const int64_t warps = (int64_t)a.batch * a.rank;
-    lora_shrink_kernel<WT><<<(unsigned)((warps + kLoraThreads / 32 - 1) / (kLoraThreads / 32)), kLoraThreads, 0, s>>>(a);
-    CUDA_TRY(cudaGetLastError());
-    const dim3 grid((a.rows + kLoraThreads - 1) / kLoraThreads, a.batch < 65535 ? a.batch : 65535);
-    lora_expand_kernel<WT><<<grid, kLoraThreads, 0, s>>>(a);
-    CUDA_TRY(cudaGetLastError());
+int lora_launch_t(DeviceCtx *c, const LoraArgs &all, cudaStream_t s) {
+    for (int t0 = 0; t0 < all.batch; t0 += kLoraBatch) {
+        LoraArgs a = all;
+        a.adapter += t0;
+        a.x += (size_t)t0 * (size_t)a.ldx;
+        a.y += (size_t)t0 * (size_t)a.ldy;
+        a.batch = all.batch - t0 < kLoraBatch ? all.batch - t0 : kLoraBatch;
+        if (a.plan) {
+            lora_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
+            CUDA_TRY(cudaGetLastError());
+        }
+        /* an adapter's last item may be short: at most n + batch / 16 items */
+        const int64_t bound = (int64_t)a.n + a.batch / kLoraItem;
+        const int items = bound < a.batch ? (int)bound : a.batch;
+        CUDA_TRY(launch_dependent(lora_shrink_kernel<WT>, dim3(items, a.rank_pad / 16), kShrinkThreads, s,
+                                  a.plan != nullptr, a));
+        const int64_t turns = (int64_t)items * ((a.rows + kExpandRows - 1) / kExpandRows);
+        const int64_t ctas = (turns + kExpandThreads / 32 - 1) / (kExpandThreads / 32), most = 2 * c->sms;
+        const dim3 grid((unsigned)(ctas < most ? ctas : most));
+        CUDA_TRY(a.rank_pad == 16 ? launch_dependent(lora_expand_kernel<WT, 4>, grid, kExpandThreads, s, true, a)
+                                  : launch_dependent(lora_expand_kernel<WT, 8>, grid, kExpandThreads, s, true, a));
+    }
     return NOEL_OK;
 }
 
-int lora_launch(const LoraArgs &a, int type, cudaStream_t s) {
+int lora_launch(DeviceCtx *c, const LoraArgs &a, int type, cudaStream_t s) {
     if (a.batch == 0 || a.n == 0) return NOEL_OK;
-    return type == NOEL_HEAD_F32   ? lora_launch_t<kHeadF32>(a, s)
-           : type == NOEL_HEAD_F16 ? lora_launch_t<kHeadF16>(a, s)
-                                   : lora_launch_t<kHeadBF16>(a, s);
+    return type == NOEL_HEAD_F32   ? lora_launch_t<kHeadF32>(c, a, s)
+           : type == NOEL_HEAD_F16 ? lora_launch_t<kHeadF16>(c, a, s)
+                                   : lora_launch_t<kHeadBF16>(c, a, s);
 }
 }  // namespace
 
 extern "C" size_t noel_lora_workspace_bytes(int batch, int rank) {
-    return batch > 0 && rank > 0 ? (size_t)batch * (size_t)rank * sizeof(float) : 0;
+    if (batch <= 0 || rank <= 0 || rank > kLoraMaxRank) return 0;
+    return lora_low_bytes(batch, rank) + (batch > kLoraWarpBatch ? sizeof(LoraPlan) : 0);
 }
 
 extern "C" int noel_lora_apply(const noel_lora_t *lora, const int32_t *d_adapter, const float *d_x, size_t ldx,
@@ -1198,7 +1248,7 @@ extern "C" int noel_lora_apply(const noel_lora_t *lora, const int32_t *d_adapter
     DeviceCtx *c = nullptr;
     r = device_ctx(&c);
     if (r) return r;
-    r = lora_launch(a, lora->type, static_cast<cudaStream_t>(stream));
+    r = lora_launch(c, a, lora->type, static_cast<cudaStream_t>(stream));
     return r ? r : ok();
 }
 
@@ -1279,7 +1329,7 @@ extern "C" int noel_lmhead_sample_ex(const noel_sampler_config_t *cfg, const voi
         if (r) return r;
         t0 += nb;
     }
-    if (lora && (r = lora_launch(la, lora->type, s))) return r;
+    if (lora && (r = lora_launch(c, la, lora->type, s))) return r;
     if (process && (r = logits_launch(c, pa, NOEL_DTYPE_F32, s))) return r;
     noel_sample_extras_t ex{};
     ex.d_probs = d_probs;
