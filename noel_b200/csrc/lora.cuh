@@ -21,6 +21,10 @@
 
 #include "lmhead.cuh"
 
+#include <cooperative_groups.h>
+
+#include <utility>
+
 namespace noel {
 
 constexpr int kLoraMaxRank = 256;
@@ -28,10 +32,9 @@ constexpr int kLoraBatch = 2048;    // tokens of one pass over the adapters
 constexpr int kLoraItem = 16;       // tokens of an item
 constexpr int kLoraWarpBatch = 32;  // tokens up to which every warp finds the items by itself
 constexpr int kShrinkThreads = 512;
+constexpr int kShrinkSplit = 8;     // CTAs of a cluster that share an item's columns, at most
 constexpr int kExpandThreads = 256;
-constexpr int kExpandRows = 64;     // rows of B_i of a warp's turn
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanSlots = 4096;
+constexpr int kExpandWaves = 16;    // CTAs of the second kernel per SM, at most
 
 /* the items of a batch above kLoraWarpBatch, in the scratch */
 struct LoraPlan {
@@ -86,7 +89,9 @@ __device__ __forceinline__ int warp_item(const LoraArgs &a, int k, uint32_t &tok
 /* One CTA: tokens of one adapter counted and numbered in a table of adapters,
  * adapters numbered in the table's order, every 16 tokens an item.  Which
  * token of an adapter gets which number is chance; no result depends on it. */
+template <int kPlanThreads, int PER>  // for up to kPlanThreads x PER tokens
 __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const __grid_constant__ LoraArgs a) {
+    constexpr int kPlanSlots = 2 * kPlanThreads * PER;  // a power of two
     __shared__ int key[kPlanSlots], count[kPlanSlots];
     __shared__ int wsum[kPlanThreads / 32], wtok[kPlanThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -96,7 +101,6 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const __grid_co
         count[s] = 0;
     }
     __syncthreads();
-    constexpr int PER = kLoraBatch / kPlanThreads;
     int slot[PER], number[PER];
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
@@ -104,7 +108,7 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const __grid_co
         const int i = t < a.batch ? a.adapter[t] : -1;
         slot[u] = -1;
         if (i < 0 || i >= a.n) continue;
-        uint32_t p = ((uint32_t)i * 0x9E3779B1u) >> 20;  // the top 12 bits: kPlanSlots
+        uint32_t p = (uint32_t)i * 0x9E3779B1u / (0xFFFFFFFFu / kPlanSlots + 1u);
         for (int probe = 0; probe < kPlanSlots; ++probe) {  // at most half of the slots are taken
             const int prev = atomicCAS(&key[p], 0, i + 1);
             if (prev == 0 || prev == i + 1) break;
@@ -114,7 +118,7 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const __grid_co
         number[u] = atomicAdd(&count[p], 1);
     }
     __syncthreads();
-    /* prefix sums over the slots, four to a thread: items and tokens */
+    /* prefix sums over the slots: items and tokens */
     constexpr int SPT = kPlanSlots / kPlanThreads;
     int items = 0, toks = 0;
 #pragma unroll
@@ -182,6 +186,31 @@ __device__ __forceinline__ uint32_t take_part(float &v) {
 /* the next parts of two numbers as a bf16 pair */
 __device__ __forceinline__ uint32_t take_parts(float &lo, float &hi) {
     return __byte_perm(take_part(lo), take_part(hi), 0x7632);
+}
+/* N numbers in P parts, as bf16 pairs */
+template <int N, int P>
+__device__ __forceinline__ void split(float (&f)[N], uint32_t (&x)[P][N / 2]) {
+    float odd = 0.0f;  // stays 0 unless a number is infinite or NaN
+#pragma unroll
+    for (int e = 0; e < N; ++e) odd = __fmaf_rn(f[e], 0.0f, odd);
+    if (odd == 0.0f) {
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                const uint32_t u = __float_as_uint(f[e]), v = __float_as_uint(f[e + 1]);
+                x[i][e / 2] = __byte_perm(u, v, 0x7632);
+                if (i + 1 < P) {
+                    f[e] = __fsub_rn(f[e], __uint_as_float(u & 0xFFFF0000u));
+                    f[e + 1] = __fsub_rn(f[e + 1], __uint_as_float(v & 0xFFFF0000u));
+                }
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int e = 0; e < N; e += 2) x[i][e / 2] = take_parts(f[e], f[e + 1]);
+    }
 }
 
 template <int WT>
@@ -255,10 +284,7 @@ __device__ __forceinline__ Weights<WT, N> load_weights(const void *p, int valid,
                 for (int e = 0; e < N; ++e) f[e] = e < used ? s[e] : 0.0f;
             }
         }
-#pragma unroll
-        for (int j = 0; j < kWeightParts<WT>; ++j)
-#pragma unroll
-            for (int e = 0; e < N; e += 2) w.p[j][e / 2] = take_parts(f[e], f[e + 1]);
+        split<N, kWeightParts<WT>>(f, w.p);
     }
     return w;
 }
@@ -313,64 +339,83 @@ __device__ __forceinline__ void load_x(const float *p, int valid, bool vec, uint
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = e < valid ? __ldg(p + e) : 0.0f;
     }
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) x[i][e / 2] = take_parts(f[e], f[e + 1]);
+    split<8, 3>(f, x);
 }
 
 /* ------------------------------------------------------------ the kernels */
-/* One CTA per item (blockIdx.x) and 16 ranks (blockIdx.y): the warps take the
- * columns in turns of 32, each turn's products are added up from 0 by the
- * matrix instructions and then to the warp's sums in fp32 (the instructions cut
- * what they add to), and the warps' sums are added in their order. */
+/* An item: its adapter (-1: none), its number of tokens, and the tokens of a
+ * lane's two rows of the instructions (g and g + 8; -1: none). */
+struct LoraItem {
+    int adapter, m, t0, t1;
+};
+__device__ __forceinline__ LoraItem lora_item(const LoraArgs &a, int k) {
+    const int g = (threadIdx.x & 31) >> 2;
+    LoraItem it{-1, 0, -1, -1};
+    if (a.plan) {
+        if (k >= a.plan->n) return it;
+        const int first = a.plan->first[k];
+        it.adapter = a.plan->adapter[k];
+        it.m = min(a.plan->first[k + 1] - first, kLoraItem);
+        if (g < it.m) it.t0 = a.plan->order[first + g];
+        if (g + 8 < it.m) it.t1 = a.plan->order[first + g + 8];
+    } else {
+        uint32_t tokens;
+        int items;
+        it.adapter = warp_item(a, k, tokens, items);
+        it.m = __popc(tokens);
+        if (g < it.m) it.t0 = (int)__fns(tokens, 0, g + 1);
+        if (g + 8 < it.m) it.t1 = (int)__fns(tokens, 0, g + 9);
+    }
+    return it;
+}
+
+/* One cluster per item (blockIdx.y) and 16 ranks (blockIdx.z): its CTAs' warps
+ * take the columns in turns of 32, each turn's products are added up from 0 by
+ * the matrix instructions and then to the warp's sums in fp32 (the
+ * instructions cut what they add to), the warps' sums are added in their order
+ * and the CTAs' in theirs.  An item's weights are 128 KB at rank 16 and 4096
+ * columns; one CTA takes them in no faster than 6 us, so few items are spread
+ * over clusters of up to eight. */
 template <int WT>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __grid_constant__ LoraArgs a) {
     constexpr int WARPS = kShrinkThreads / 32;
     constexpr int ES = WT == kHeadF32 ? 4 : 2;
     __shared__ float part[WARPS][kLoraItem][16];
-    __shared__ int tok[kLoraItem];
+    __shared__ float2 gather[kShrinkSplit][kLoraItem][8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    asm volatile("griddepcontrol.wait;" ::: "memory");               // the plan is there
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan is there
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    int i, m;
-    if (a.plan) {
-        if ((int)blockIdx.x >= a.plan->n) return;
-        i = a.plan->adapter[blockIdx.x];
-        const int first = a.plan->first[blockIdx.x];
-        m = min(a.plan->first[blockIdx.x + 1] - first, kLoraItem);
-        if (threadIdx.x < kLoraItem) tok[threadIdx.x] = (int)threadIdx.x < m ? a.plan->order[first + threadIdx.x] : -1;
-    } else {
-        uint32_t tokens;
-        int items;
-        i = warp_item(a, blockIdx.x, tokens, items);
-        if (i < 0) return;
-        m = __popc(tokens);
-        if (threadIdx.x < kLoraItem) tok[threadIdx.x] = (int)threadIdx.x < m ? (int)__fns(tokens, 0, threadIdx.x + 1) : -1;
-    }
-    __syncthreads();
-    const int n = lora_rank(a, i), r0 = blockIdx.y * 16;
+    const LoraItem it = lora_item(a, blockIdx.y);
+    if (it.adapter < 0) return;  // the whole cluster
+    const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    auto begun = cluster.barrier_arrive();  // a CTA's shared memory is written by others once it has begun
+    const int i = it.adapter, n = lora_rank(a, i), r0 = blockIdx.z * 16;
     float acc[2][4] = {};
     if (r0 < n) {
-        const int t0 = tok[g], t1 = tok[g + 8];
-        const float *x0 = a.x + (size_t)max(t0, 0) * (size_t)a.ldx, *x1 = a.x + (size_t)max(t1, 0) * (size_t)a.ldx;
-        const char *w = static_cast<const char *>(a.a) + (size_t)i * (size_t)a.stride_a * ES;
+        const float *x0 = a.x + (size_t)max(it.t0, 0) * (size_t)a.ldx, *x1 = a.x + (size_t)max(it.t1, 0) * (size_t)a.ldx;
         const int ra = r0 + g, rb = ra + 8;
+        const char *w = static_cast<const char *>(a.a) + (size_t)i * (size_t)a.stride_a * ES;
+        const char *wa = w + (size_t)min(ra, n - 1) * (size_t)a.lda * ES, *wb = w + (size_t)min(rb, n - 1) * (size_t)a.lda * ES;
+        const bool vec = a.vec_x && a.vec_a;
 #pragma unroll 2
-        for (int k0 = warp * 32; k0 < a.cols; k0 += 32 * WARPS) {
+        for (int k0 = (blockIdx.x * WARPS + warp) * 32; k0 < a.cols; k0 += 32 * WARPS * gridDim.x) {
             const int k = k0 + 8 * q, left = a.cols - k;
             uint32_t p0[3][4] = {}, p1[3][4] = {};
-            if (t0 >= 0 && left > 0) load_x(x0 + k, left, a.vec_x, p0);
-            if (t1 >= 0 && left > 0) load_x(x1 + k, left, a.vec_x, p1);
-            const Weights<WT, 8> wa = ra < n && left > 0
-                ? load_weights<WT, 8>(w + ((size_t)ra * (size_t)a.lda + k) * ES, left, min(left, 8), a.vec_a)
-                : no_weights<WT, 8>();
-            const Weights<WT, 8> wb = rb < n && left > 0
-                ? load_weights<WT, 8>(w + ((size_t)rb * (size_t)a.lda + k) * ES, left, min(left, 8), a.vec_a)
-                : no_weights<WT, 8>();
+            Weights<WT, 8> ba = no_weights<WT, 8>(), bb = no_weights<WT, 8>();
+            if (vec && k0 + 32 <= a.cols) {
+                if (ra < n) ba = load_weights<WT, 8>(wa + (size_t)k * ES, 8, 8, true);
+                if (rb < n) bb = load_weights<WT, 8>(wb + (size_t)k * ES, 8, 8, true);
+                if (it.t0 >= 0) load_x(x0 + k, 8, true, p0);
+                if (it.t1 >= 0) load_x(x1 + k, 8, true, p1);
+            } else if (left > 0) {
+                if (ra < n) ba = load_weights<WT, 8>(wa + (size_t)k * ES, left, min(left, 8), false);
+                if (rb < n) bb = load_weights<WT, 8>(wb + (size_t)k * ES, left, min(left, 8), false);
+                if (it.t0 >= 0) load_x(x0 + k, left, false, p0);
+                if (it.t1 >= 0) load_x(x1 + k, left, false, p1);
+            }
             float c[2][4] = {};
-            multiply<WT, 8>(c[0], p0, p1, wa);
-            multiply<WT, 8>(c[1], p0, p1, wb);
+            multiply<WT, 8>(c[0], p0, p1, ba);
+            multiply<WT, 8>(c[1], p0, p1, bb);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 acc[0][e] = __fadd_rn(acc[0][e], c[0][e]);
@@ -380,34 +425,51 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __gri
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        part[warp][g][8 * h + 2 * q] = acc[h][0];
-        part[warp][g][8 * h + 2 * q + 1] = acc[h][1];
-        part[warp][g + 8][8 * h + 2 * q] = acc[h][2];
-        part[warp][g + 8][8 * h + 2 * q + 1] = acc[h][3];
+        *reinterpret_cast<float2 *>(&part[warp][g][8 * h + 2 * q]) = make_float2(acc[h][0], acc[h][1]);
+        *reinterpret_cast<float2 *>(&part[warp][g + 8][8 * h + 2 * q]) = make_float2(acc[h][2], acc[h][3]);
     }
     __syncthreads();
-    /* two ranks of one token per thread */
+    /* two ranks of one token per thread; warp w has tokens 4 w .. 4 w + 3 */
+    const int row = threadIdx.x >> 3, r = 2 * (threadIdx.x & 7);
+    float u = 0.0f, v = 0.0f;
     if (threadIdx.x < kLoraItem * 8) {
-        const int row = threadIdx.x >> 3, r = 2 * (threadIdx.x & 7), t = tok[row];
-        if (t >= 0) {
-            float u = 0.0f, v = 0.0f;
 #pragma unroll
-            for (int k = 0; k < WARPS; ++k) {
-                u = __fadd_rn(u, part[k][row][r]);
-                v = __fadd_rn(v, part[k][row][r + 1]);
-            }
-            if (a.scale) {
-                const float s = a.scale[i];
-                u = __fmul_rn(u, s);
-                v = __fmul_rn(v, s);
-            }
-            if (r0 + r >= n) u = 0.0f;  // not even an infinite scale gives an unused rank a value
-            if (r0 + r + 1 >= n) v = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 3; ++k)
-                *reinterpret_cast<uint32_t *>(a.low + ((size_t)t * 3 + k) * a.rank_pad + r0 + r) = take_parts(u, v);
+        for (int k = 0; k < WARPS; ++k) {
+            const float2 s = *reinterpret_cast<const float2 *>(&part[k][row][r]);
+            u = __fadd_rn(u, s.x);
+            v = __fadd_rn(v, s.y);
         }
     }
+    cluster.barrier_wait(std::move(begun));
+    if (gridDim.x > 1) {
+        if (threadIdx.x < kLoraItem * 8)
+            *cluster.map_shared_rank(&gather[blockIdx.x][row][r / 2], 0) = make_float2(u, v);
+        cluster.sync();
+        if (blockIdx.x) return;
+        if (threadIdx.x < kLoraItem * 8) {
+            u = v = 0.0f;
+            for (int k = 0; k < (int)gridDim.x; ++k) {
+                const float2 s = gather[k][row][r / 2];
+                u = __fadd_rn(u, s.x);
+                v = __fadd_rn(v, s.y);
+            }
+        }
+    }
+    if (threadIdx.x >= kLoraItem * 8) return;
+    /* token `row` of the item is what lanes 4 (row % 8) hold as t0 or t1 */
+    const int ta = __shfl_sync(kFull, it.t0, 4 * (row & 7)), tb = __shfl_sync(kFull, it.t1, 4 * (row & 7));
+    const int t = row < 8 ? ta : tb;
+    if (t < 0) return;
+    if (a.scale) {
+        const float s = a.scale[i];
+        u = __fmul_rn(u, s);
+        v = __fmul_rn(v, s);
+    }
+    if (r0 + r >= n) u = 0.0f;  // not even an infinite scale gives an unused rank a value
+    if (r0 + r + 1 >= n) v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+        *reinterpret_cast<uint32_t *>(a.low + ((size_t)t * 3 + k) * a.rank_pad + r0 + r) = take_parts(u, v);
 }
 
 /* N parts (8 or 4) of a token's low-rank numbers */
@@ -426,82 +488,90 @@ __device__ __forceinline__ void load_low(const LoraArgs &a, int t, int r, uint32
     }
 }
 
-/* A warp's turn: 64 rows of B_i for one item.  N is the number of ranks a lane
- * holds: 4 for ranks up to 16, else 8 (a group of 32 ranks at a time). */
-template <int WT, int N>
+/* One item per blockIdx.y; the warps of its CTAs take 16 PAIRS rows of B_i at
+ * a time.  N is the number of ranks a lane holds: 4 for ranks up to 16, else 8
+ * (a group of 32 ranks at a time).  Column h of instruction j of a pair stands
+ * for row 4 (h / 2) + 2 j + h % 2 of its 16, which gives lane q the four rows
+ * 4 q .. 4 q + 3 of the result: 16 bytes of y. */
+template <int WT, int N, int PAIRS>
 __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
-    constexpr int ES = WT == kHeadF32 ? 4 : 2, PAIRS = 2;  // 16 rows to a pair of instructions' columns
+    constexpr int ES = WT == kHeadF32 ? 4 : 2, ROWS = 16 * PAIRS;
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the low-rank numbers are there
-    int items;
-    uint32_t tokens = 0u;
-    if (a.plan) items = a.plan->n;
-    else warp_item(a, 32, tokens, items);
-    const int tiles = (a.rows + kExpandRows - 1) / kExpandRows;
-    const int64_t turns = (int64_t)items * tiles, step = (int64_t)gridDim.x * (kExpandThreads / 32);
-    for (int64_t u = ((int64_t)blockIdx.x * kExpandThreads + threadIdx.x) >> 5; u < turns; u += step) {
-        const int item = (int)(u % items), v0 = (int)(u / items) * kExpandRows;
-        int i, t0, t1;
-        if (a.plan) {
-            i = a.plan->adapter[item];
-            const int first = a.plan->first[item], m = min(a.plan->first[item + 1] - first, kLoraItem);
-            t0 = g < m ? a.plan->order[first + g] : -1;
-            t1 = g + 8 < m ? a.plan->order[first + g + 8] : -1;
-        } else {
-            int all;
-            i = warp_item(a, item, tokens, all);
-            const int m = __popc(tokens);
-            t0 = g < m ? (int)__fns(tokens, 0, g + 1) : -1;
-            t1 = g + 8 < m ? (int)__fns(tokens, 0, g + 9) : -1;
-        }
-        const int n = lora_rank(a, i);
-        const char *w = static_cast<const char *>(a.b) + (size_t)i * (size_t)a.stride_b * ES;
-        float *y0 = a.y + (size_t)max(t0, 0) * (size_t)a.ldy, *y1 = a.y + (size_t)max(t1, 0) * (size_t)a.ldy;
-#pragma unroll 1
-        for (int b0 = v0; b0 < v0 + kExpandRows && b0 < a.rows; b0 += 16 * PAIRS) {
-            float c[PAIRS][2][4] = {};
-            for (int r0 = 0; r0 < n; r0 += 4 * N) {
-                const int r = r0 + N * q;
-                uint32_t x0[3][N / 2] = {}, x1[3][N / 2] = {};
-                if (t0 >= 0) load_low<N>(a, t0, r, x0);
-                if (t1 >= 0) load_low<N>(a, t1, r, x1);
-#pragma unroll
-                for (int p = 0; p < PAIRS; ++p)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        /* column h of instruction j stands for row 4 (h / 2) + 2 j + h % 2 of the 16, which
-                         * gives lane q the four rows 4 q .. 4 q + 3 */
-                        const int v = b0 + 16 * p + 4 * (g >> 1) + 2 * j + (g & 1);
-                        const Weights<WT, N> b = v < a.rows && r < n
-                            ? load_weights<WT, N>(w + ((size_t)v * (size_t)a.ldb + r) * ES, a.rank - r, min(n - r, N), a.vec_b)
-                            : no_weights<WT, N>();
-                        multiply<WT, N>(c[p][j], x0, x1, b);
-                    }
-            }
+    const LoraItem it = lora_item(a, blockIdx.y);  // the kernel before let this one begin when the plan was there
+    if (it.adapter < 0) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // no CTA ends before the kernel before
+        return;
+    }
+    const int n = lora_rank(a, it.adapter);
+    const bool full = a.vec_b && a.vec_y && n % N == 0;
+    /* this lane's first row of B_i and ranks, and its tokens' rows of y */
+    const char *w = static_cast<const char *>(a.b) +
+                    ((size_t)it.adapter * (size_t)a.stride_b + (size_t)(4 * (g >> 1) + (g & 1)) * (size_t)a.ldb + N * q) * ES;
+    float *y0 = a.y + (size_t)max(it.t0, 0) * (size_t)a.ldy + 4 * q, *y1 = a.y + (size_t)max(it.t1, 0) * (size_t)a.ldy + 4 * q;
+    uint32_t x0[3][N / 2] = {}, x1[3][N / 2] = {};
+    bool have = false;  // the low-rank numbers are there, and the first group of them in x0 and x1
+    const int64_t step = (int64_t)gridDim.x * (kExpandThreads / 32) * ROWS;
+    for (int64_t v0 = ((int64_t)blockIdx.x * (kExpandThreads / 32) + (threadIdx.x >> 5)) * ROWS; v0 < a.rows; v0 += step) {
+        const bool inside = full && v0 + ROWS <= a.rows;
+        const char *wv = w + (size_t)v0 * (size_t)a.ldb * ES;
+        float4 o0[PAIRS], o1[PAIRS];
+        if (inside) {
 #pragma unroll
             for (int p = 0; p < PAIRS; ++p) {
-                const int v = b0 + 16 * p + 4 * q;
+                if (it.t0 >= 0) o0[p] = *reinterpret_cast<const float4 *>(y0 + v0 + 16 * p);
+                if (it.t1 >= 0) o1[p] = *reinterpret_cast<const float4 *>(y1 + v0 + 16 * p);
+            }
+        }
+        float c[PAIRS][2][4] = {};
+        for (int r0 = 0; r0 < n; r0 += 4 * N) {
+            const int r = r0 + N * q;
+            Weights<WT, N> b[PAIRS][2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if ((h ? t1 : t0) < 0) continue;
-                    float *y = (h ? y1 : y0) + v;
-                    const float d[4] = {c[p][0][2 * h], c[p][0][2 * h + 1], c[p][1][2 * h], c[p][1][2 * h + 1]};
-                    if (a.vec_y && v + 4 <= a.rows) {
-                        float4 o = *reinterpret_cast<const float4 *>(y);
-                        o.x = __fadd_rn(o.x, d[0]);
-                        o.y = __fadd_rn(o.y, d[1]);
-                        o.z = __fadd_rn(o.z, d[2]);
-                        o.w = __fadd_rn(o.w, d[3]);
-                        *reinterpret_cast<float4 *>(y) = o;
-                    } else {
+            for (int p = 0; p < PAIRS; ++p)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (v + e < a.rows) y[e] = __fadd_rn(y[e], d[e]);
+                for (int j = 0; j < 2; ++j) {
+                    const char *at = wv + ((size_t)(16 * p + 2 * j) * (size_t)a.ldb + r0) * ES;
+                    b[p][j] = no_weights<WT, N>();
+                    if (inside) {
+                        if (r < n) b[p][j] = load_weights<WT, N>(at, N, N, true);
+                    } else if (v0 + 16 * p + 4 * (g >> 1) + 2 * j + (g & 1) < a.rows && r < n) {
+                        b[p][j] = load_weights<WT, N>(at, N, min(n - r, N), false);
                     }
+                }
+            if (!have) asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (!have || n > 4 * N) {
+                if (it.t0 >= 0) load_low<N>(a, it.t0, r, x0);
+                if (it.t1 >= 0) load_low<N>(a, it.t1, r, x1);
+                have = true;
+            }
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) multiply<WT, N>(c[p][j], x0, x1, b[p][j]);
+        }
+#pragma unroll
+        for (int p = 0; p < PAIRS; ++p) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if ((h ? it.t1 : it.t0) < 0) continue;
+                float *y = (h ? y1 : y0) + v0 + 16 * p;
+                const float d[4] = {c[p][0][2 * h], c[p][0][2 * h + 1], c[p][1][2 * h], c[p][1][2 * h + 1]};
+                if (inside) {
+                    float4 o = h ? o1[p] : o0[p];
+                    o.x = __fadd_rn(o.x, d[0]);
+                    o.y = __fadd_rn(o.y, d[1]);
+                    o.z = __fadd_rn(o.z, d[2]);
+                    o.w = __fadd_rn(o.w, d[3]);
+                    *reinterpret_cast<float4 *>(y) = o;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (v0 + 16 * p + 4 * q + e < a.rows) y[e] = __fadd_rn(y[e], d[e]);
                 }
             }
         }
     }
+    if (!have) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace noel

@@ -1183,20 +1183,32 @@ int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size
     return NOEL_OK;
 }
 
-/* a kernel that may start while the one before it in the stream still runs
- * (it waits for it with griddepcontrol.wait) */
+/* a kernel in clusters along x; dependent: it may start while the one before
+ * it in the stream still runs (it waits with griddepcontrol.wait) */
 template <typename... P, typename... A>
-cudaError_t launch_dependent(void (*k)(P...), dim3 grid, int threads, cudaStream_t s, bool dependent, A... args) {
+cudaError_t launch_cluster(void (*k)(P...), dim3 grid, int threads, int cluster, bool dependent, cudaStream_t s, A... args) {
     cudaLaunchConfig_t lc = {};
     lc.gridDim = grid;
     lc.blockDim = dim3(threads);
     lc.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
-    lc.numAttrs = dependent ? 1 : 0;
+    lc.numAttrs = dependent ? 2 : 1;
     return cudaLaunchKernelEx(&lc, k, args...);
+}
+
+template <int WT, int N, int PAIRS>
+cudaError_t expand_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
+    const int rows = 16 * PAIRS * (kExpandThreads / 32);
+    const int64_t all = ((int64_t)a.rows + rows - 1) / rows;
+    const int64_t want = ((int64_t)c->sms * kExpandWaves + items - 1) / items;
+    return launch_cluster(lora_expand_kernel<WT, N, PAIRS>, dim3((unsigned)(all < want ? all : want), items), kExpandThreads,
+                          1, true, s, a);
 }
 
 template <int WT>
@@ -1208,19 +1220,18 @@ int lora_launch_t(DeviceCtx *c, const LoraArgs &all, cudaStream_t s) {
         a.y += (size_t)t0 * (size_t)a.ldy;
         a.batch = all.batch - t0 < kLoraBatch ? all.batch - t0 : kLoraBatch;
         if (a.plan) {
-            lora_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
+            if (a.batch <= 256) lora_plan_kernel<256, 1><<<1, 256, 0, s>>>(a);
+            else lora_plan_kernel<1024, 2><<<1, 1024, 0, s>>>(a);
             CUDA_TRY(cudaGetLastError());
         }
         /* an adapter's last item may be short: at most n + batch / 16 items */
         const int64_t bound = (int64_t)a.n + a.batch / kLoraItem;
-        const int items = bound < a.batch ? (int)bound : a.batch;
-        CUDA_TRY(launch_dependent(lora_shrink_kernel<WT>, dim3(items, a.rank_pad / 16), kShrinkThreads, s,
-                                  a.plan != nullptr, a));
-        const int64_t turns = (int64_t)items * ((a.rows + kExpandRows - 1) / kExpandRows);
-        const int64_t ctas = (turns + kExpandThreads / 32 - 1) / (kExpandThreads / 32), most = 2 * c->sms;
-        const dim3 grid((unsigned)(ctas < most ? ctas : most));
-        CUDA_TRY(a.rank_pad == 16 ? launch_dependent(lora_expand_kernel<WT, 4>, grid, kExpandThreads, s, true, a)
-                                  : launch_dependent(lora_expand_kernel<WT, 8>, grid, kExpandThreads, s, true, a));
+        const int items = bound < a.batch ? (int)bound : a.batch, groups = a.rank_pad / 16;
+        int split = 1;
+        while (split < kShrinkSplit && 2 * split * items * groups <= c->sms && split * kShrinkThreads < a.cols) split *= 2;
+        CUDA_TRY(launch_cluster(lora_shrink_kernel<WT>, dim3(split, items, groups), kShrinkThreads, split,
+                                a.plan != nullptr, s, a));
+        CUDA_TRY((a.rank_pad == 16 ? expand_launch<WT, 4, 4>(c, a, items, s) : expand_launch<WT, 8, 2>(c, a, items, s)));
     }
     return NOEL_OK;
 }
