@@ -18,6 +18,7 @@
 #pragma once
 
 #include "sampler_kernels.cuh"
+#include "sector.cuh"
 #include "sampler_warp.cuh"
 
 #include <cuda_bf16.h>
@@ -233,31 +234,6 @@ __device__ __forceinline__ void table_apply(const LogitsArgs &a, int row, const 
     }
 }
 
-/* 32 bytes of logits, the unit in which memory is written whole */
-struct Sector {
-    uint32_t u[8];
-};
-__device__ __forceinline__ Sector sector_load(const void *p) {
-    Sector s;
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(s.u[0]), "=r"(s.u[1]), "=r"(s.u[2]), "=r"(s.u[3]), "=r"(s.u[4]), "=r"(s.u[5]), "=r"(s.u[6]),
-                   "=r"(s.u[7])
-                 : "l"(p));
-    return s;
-}
-__device__ __forceinline__ void sector_store(void *p, const Sector &s) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(s.u[0]), "r"(s.u[1]),
-                 "r"(s.u[2]), "r"(s.u[3]), "r"(s.u[4]), "r"(s.u[5]), "r"(s.u[6]), "r"(s.u[7])
-                 : "memory");
-}
-__device__ __forceinline__ Sector sector_all(float) {
-    const uint32_t m = 0xFF800000u;
-    return {{m, m, m, m, m, m, m, m}};
-}
-__device__ __forceinline__ Sector sector_all(uint16_t) {
-    const uint32_t m = 0xFF80FF80u;
-    return {{m, m, m, m, m, m, m, m}};
-}
 /* -infinity for the elements whose bit in gone is set */
 __device__ __forceinline__ void sector_mask(Sector &s, uint32_t gone, float) {
 #pragma unroll

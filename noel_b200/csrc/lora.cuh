@@ -20,6 +20,7 @@
 #pragma once
 
 #include "lmhead.cuh"
+#include "sector.cuh"
 
 #include <cooperative_groups.h>
 
@@ -31,10 +32,10 @@ constexpr int kLoraMaxRank = 256;
 constexpr int kLoraBatch = 2048;    // tokens of one pass over the adapters
 constexpr int kLoraItem = 16;       // tokens of an item
 constexpr int kLoraWarpBatch = 32;  // tokens up to which every warp finds the items by itself
-constexpr int kShrinkThreads = 512;
+constexpr int kShrinkThreads = 256;
 constexpr int kShrinkSplit = 8;     // CTAs of a cluster that share an item's columns, at most
 constexpr int kExpandThreads = 256;
-constexpr int kExpandWaves = 16;    // CTAs of the second kernel per SM, at most
+constexpr int kExpandWaves = 4;     // turns of the GPU's CTAs that the second kernel's work is cut into
 
 /* the items of a batch above kLoraWarpBatch, in the scratch */
 struct LoraPlan {
@@ -59,7 +60,8 @@ struct LoraArgs {
     uint16_t *low;   // [batch][3][rank_pad] bf16 parts of scale A x
     int rank_pad;    // 16, or the rank rounded up to 32
     LoraPlan *plan;  // NULL: every warp finds the items
-    int vec_x, vec_a, vec_b, vec_y;  // rows start on 16 bytes (B with rank_pad 16: on 4 elements)
+    int staged;                      // the second kernel's stages can be filled 16 bytes at a time
+    int vec_x, vec_a, vec_b, vec_y;  // rows start on 16 bytes (B with rank_pad 16: on 4 elements; y: 2 for 32 bytes)
 };
 
 __device__ __forceinline__ int lora_rank(const LoraArgs &a, int i) {
@@ -187,24 +189,30 @@ __device__ __forceinline__ uint32_t take_part(float &v) {
 __device__ __forceinline__ uint32_t take_parts(float &lo, float &hi) {
     return __byte_perm(take_part(lo), take_part(hi), 0x7632);
 }
-/* N numbers in P parts, as bf16 pairs */
+/* N numbers in P parts, as bf16 pairs; of an infinity or NaN the second part is
+ * a NaN */
+template <int N, int P>
+__device__ __forceinline__ void split_finite(float (&f)[N], uint32_t (&x)[P][N / 2]) {
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const uint32_t u = __float_as_uint(f[e]), v = __float_as_uint(f[e + 1]);
+            x[i][e / 2] = __byte_perm(u, v, 0x7632);
+            if (i + 1 < P) {
+                f[e] = __fsub_rn(f[e], __uint_as_float(u & 0xFFFF0000u));
+                f[e + 1] = __fsub_rn(f[e + 1], __uint_as_float(v & 0xFFFF0000u));
+            }
+        }
+}
+/* the same, an infinity or NaN whole in its first part */
 template <int N, int P>
 __device__ __forceinline__ void split(float (&f)[N], uint32_t (&x)[P][N / 2]) {
     float odd = 0.0f;  // stays 0 unless a number is infinite or NaN
 #pragma unroll
     for (int e = 0; e < N; ++e) odd = __fmaf_rn(f[e], 0.0f, odd);
     if (odd == 0.0f) {
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-#pragma unroll
-            for (int e = 0; e < N; e += 2) {
-                const uint32_t u = __float_as_uint(f[e]), v = __float_as_uint(f[e + 1]);
-                x[i][e / 2] = __byte_perm(u, v, 0x7632);
-                if (i + 1 < P) {
-                    f[e] = __fsub_rn(f[e], __uint_as_float(u & 0xFFFF0000u));
-                    f[e + 1] = __fsub_rn(f[e + 1], __uint_as_float(v & 0xFFFF0000u));
-                }
-            }
+        split_finite<N, P>(f, x);
     } else {
 #pragma unroll
         for (int i = 0; i < P; ++i)
@@ -215,107 +223,98 @@ __device__ __forceinline__ void split(float (&f)[N], uint32_t (&x)[P][N / 2]) {
 
 template <int WT>
 constexpr int kWeightParts = WT == kHeadBF16 ? 1 : WT == kHeadF16 ? 2 : 3;
+template <int WT>
+constexpr int kWeightBytes = WT == kHeadF32 ? 4 : 2;
 
-/* N consecutive weights as bf16 pairs, part by part */
+/* N consecutive weights: as they lie in memory, and as bf16 pairs part by part */
+template <int WT, int N>
+struct Raw {
+    uint32_t u[N * kWeightBytes<WT> / 4];
+};
 template <int WT, int N>
 struct Weights {
     uint32_t p[kWeightParts<WT>][N / 2];
 };
 
-/* weights at p; valid (<= N) of them exist and used (<= N) of them count, the
- * others are 0; vec: p is aligned to the N weights (16 bytes at most) */
 template <int WT, int N>
-__device__ __forceinline__ Weights<WT, N> load_weights(const void *p, int valid, int used, bool vec) {
+__device__ __forceinline__ Raw<WT, N> raw_zero() {
+    Raw<WT, N> r;
+#pragma unroll
+    for (int e = 0; e < N * kWeightBytes<WT> / 4; ++e) r.u[e] = 0u;
+    return r;
+}
+/* from 16-byte aligned memory (8 where there are 8 bytes) */
+template <int WT, int N>
+__device__ __forceinline__ Raw<WT, N> raw_load(const void *p) {
+    Raw<WT, N> r;
+    constexpr int WORDS = N * kWeightBytes<WT> / 4;
+    if (WORDS == 2) {
+        const uint2 q = __ldg(static_cast<const uint2 *>(p));
+        r.u[0] = q.x, r.u[1] = q.y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < WORDS; e += 4) {
+            const uint4 q = __ldg(static_cast<const uint4 *>(p) + e / 4);
+            r.u[e] = q.x, r.u[e + 1] = q.y, r.u[(e + 2) % WORDS] = q.z, r.u[(e + 3) % WORDS] = q.w;
+        }
+    }
+    return r;
+}
+/* the first used of them, one by one; the others are 0 */
+template <int WT, int N>
+__device__ __forceinline__ Raw<WT, N> raw_elements(const void *p, int used) {
+    Raw<WT, N> r;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        if (WT == kHeadF32) {
+            r.u[e % (N * kWeightBytes<WT> / 4)] = e < used ? static_cast<const uint32_t *>(p)[e] : 0u;
+        } else {
+            const uint32_t h = e < used ? (uint32_t)static_cast<const uint16_t *>(p)[e] : 0u;
+            r.u[e / 2] = e & 1 ? r.u[e / 2] | h << 16 : h;
+        }
+    }
+    return r;
+}
+template <int WT, int N>
+__device__ __forceinline__ Weights<WT, N> weights(const Raw<WT, N> &r) {
     Weights<WT, N> w;
     if (WT == kHeadBF16) {
-        uint32_t *u = w.p[0];
-        if (vec && valid >= N) {
-            if (N == 8) {
-                const uint4 q = __ldg(static_cast<const uint4 *>(p));
-                u[0] = q.x, u[1] = q.y, u[N / 2 - 2] = q.z, u[N / 2 - 1] = q.w;
-            } else {
-                const uint2 q = __ldg(static_cast<const uint2 *>(p));
-                u[0] = q.x, u[1] = q.y;
-            }
-            if (used < N) {
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (e >= used) u[e / 2] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-            }
-        } else {
-            const uint16_t *h = static_cast<const uint16_t *>(p);
-#pragma unroll
-            for (int e = 0; e < N; e += 2)
-                u[e / 2] = (e < used ? (uint32_t)h[e] : 0u) | (e + 1 < used ? (uint32_t)h[e + 1] << 16 : 0u);
-        }
+        for (int e = 0; e < N / 2; ++e) w.p[0][e] = r.u[e];
     } else {
         float f[N];
-        if (WT == kHeadF16) {
-            const __half *h = static_cast<const __half *>(p);
-            if (vec && valid >= N) {
-                uint32_t u[N / 2];
-                if (N == 8) {
-                    const uint4 q = __ldg(static_cast<const uint4 *>(p));
-                    u[0] = q.x, u[1] = q.y, u[N / 2 - 2] = q.z, u[N / 2 - 1] = q.w;
-                } else {
-                    const uint2 q = __ldg(static_cast<const uint2 *>(p));
-                    u[0] = q.x, u[1] = q.y;
-                }
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    f[e] = e < used ? __half2float(__ushort_as_half((uint16_t)(u[e / 2] >> (16 * (e & 1))))) : 0.0f;
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) f[e] = e < used ? __half2float(h[e]) : 0.0f;
-            }
-        } else {
-            const float *s = static_cast<const float *>(p);
-            if (vec && valid >= N) {
-#pragma unroll
-                for (int e = 0; e < N; e += 4) {
-                    const float4 q = __ldg(reinterpret_cast<const float4 *>(s + e));
-                    f[e] = q.x, f[e + 1] = q.y, f[e + 2] = q.z, f[e + 3] = q.w;
-                }
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (e >= used) f[e] = 0.0f;
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) f[e] = e < used ? s[e] : 0.0f;
-            }
-        }
-        split<N, kWeightParts<WT>>(f, w.p);
+        for (int e = 0; e < N; ++e)
+            f[e] = WT == kHeadF32 ? __uint_as_float(r.u[e % (N * kWeightBytes<WT> / 4)])
+                                  : __half2float(__ushort_as_half((uint16_t)(r.u[e / 2] >> (16 * (e & 1)))));
+        split_finite<N, kWeightParts<WT>>(f, w.p);  // an infinity comes out as a NaN
     }
     return w;
 }
 
-template <int WT, int N>
-__device__ __forceinline__ Weights<WT, N> no_weights() {
-    Weights<WT, N> w;
-#pragma unroll
-    for (int j = 0; j < kWeightParts<WT>; ++j)
-#pragma unroll
-        for (int e = 0; e < N / 2; ++e) w.p[j][e] = 0u;
-    return w;
+/* c = a b + c, or a b alone */
+__device__ __forceinline__ void mma_bf16(float (&c)[4], bool from_zero, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    if (from_zero)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-                 "{%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-/* c += x w over 4 N contracted numbers, of which lane 4 g + q holds N
+/* c (+)= x w over 4 N contracted numbers, of which lane 4 g + q holds N
  * consecutive ones of tokens g (x0) and g + 8 (x1) and of weight row g: the
  * order of a contraction is free, so lane q's numbers 4 s .. 4 s + 3 stand in
  * the places that instruction s gives to lane q.  x?[part][pair]. */
 template <int WT, int N>
-__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&x0)[3][N / 2], const uint32_t (&x1)[3][N / 2],
-                                         const Weights<WT, N> &w) {
+__device__ __forceinline__ void multiply(float (&c)[4], bool from_zero, const uint32_t (&x0)[3][N / 2],
+                                         const uint32_t (&x1)[3][N / 2], const Weights<WT, N> &w) {
     constexpr int P = kWeightParts<WT>;
-    __syncwarp();  // lanes may have loaded by different ways
 #pragma unroll
     for (int sum = P + 1; sum >= 0; --sum)  // the smallest products first
 #pragma unroll
@@ -323,23 +322,27 @@ __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&x0)[3][
             const int i = sum - j;
             if (i < 0 || i > 2 || (P == 3 && i == 2 && j == 2)) continue;
 #pragma unroll
-            for (int s = 0; s < N / 4; ++s)
-                mma_bf16(c, x0[i][2 * s], x1[i][2 * s], x0[i][2 * s + 1], x1[i][2 * s + 1], w.p[j][2 * s],
-                         w.p[j][2 * s + 1]);
+            for (int s = 0; s < N / 4; ++s) {
+                const bool first = s == 0 && (P == 3 ? sum == 3 && j == 2 : sum == P + 1);
+                mma_bf16(c, from_zero && first, x0[i][2 * s], x1[i][2 * s], x0[i][2 * s + 1], x1[i][2 * s + 1],
+                         w.p[j][2 * s], w.p[j][2 * s + 1]);
+            }
         }
 }
 
-/* 8 numbers of x at p (valid of them exist) in three parts */
-__device__ __forceinline__ void load_x(const float *p, int valid, bool vec, uint32_t (&x)[3][4]) {
+/* 8 numbers of x */
+struct RawX {
     float f[8];
-    if (vec && valid >= 8) {
-        const float4 q0 = __ldg(reinterpret_cast<const float4 *>(p)), q1 = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-        f[0] = q0.x, f[1] = q0.y, f[2] = q0.z, f[3] = q0.w, f[4] = q1.x, f[5] = q1.y, f[6] = q1.z, f[7] = q1.w;
-    } else {
+};
+__device__ __forceinline__ RawX x_load(const float *p) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+__device__ __forceinline__ RawX x_elements(const float *p, int used) {
+    RawX r;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = e < valid ? __ldg(p + e) : 0.0f;
-    }
-    split<8, 3>(f, x);
+    for (int e = 0; e < 8; ++e) r.f[e] = e < used ? __ldg(p + e) : 0.0f;
+    return r;
 }
 
 /* ------------------------------------------------------------ the kernels */
@@ -369,19 +372,19 @@ __device__ __forceinline__ LoraItem lora_item(const LoraArgs &a, int k) {
     return it;
 }
 
-/* One cluster per item (blockIdx.y) and 16 ranks (blockIdx.z): its CTAs' warps
- * take the columns in turns of 32, each turn's products are added up from 0 by
- * the matrix instructions and then to the warp's sums in fp32 (the
+/* One cluster per item (blockIdx.y) and 8 TILES ranks (blockIdx.z): its CTAs'
+ * warps take the columns in turns of 32, each turn's products are added up
+ * from 0 by the matrix instructions and then to the warp's sums in fp32 (the
  * instructions cut what they add to), the warps' sums are added in their order
  * and the CTAs' in theirs.  An item's weights are 128 KB at rank 16 and 4096
  * columns; one CTA takes them in no faster than 6 us, so few items are spread
  * over clusters of up to eight. */
-template <int WT>
+template <int WT, int TILES>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __grid_constant__ LoraArgs a) {
-    constexpr int WARPS = kShrinkThreads / 32;
-    constexpr int ES = WT == kHeadF32 ? 4 : 2;
-    __shared__ float part[WARPS][kLoraItem][16];
-    __shared__ float2 gather[kShrinkSplit][kLoraItem][8];
+    constexpr int WARPS = kShrinkThreads / 32, RANKS = 8 * TILES;
+    constexpr int ES = kWeightBytes<WT>;
+    __shared__ float part[WARPS][kLoraItem][RANKS];
+    __shared__ float2 gather[kShrinkSplit][kLoraItem][RANKS / 2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan is there
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -389,50 +392,70 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __gri
     if (it.adapter < 0) return;  // the whole cluster
     const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     auto begun = cluster.barrier_arrive();  // a CTA's shared memory is written by others once it has begun
-    const int i = it.adapter, n = lora_rank(a, i), r0 = blockIdx.z * 16;
-    float acc[2][4] = {};
+    const int i = it.adapter, n = lora_rank(a, i), r0 = blockIdx.z * RANKS;
+    float acc[TILES][4] = {};
     if (r0 < n) {
         const float *x0 = a.x + (size_t)max(it.t0, 0) * (size_t)a.ldx, *x1 = a.x + (size_t)max(it.t1, 0) * (size_t)a.ldx;
-        const int ra = r0 + g, rb = ra + 8;
         const char *w = static_cast<const char *>(a.a) + (size_t)i * (size_t)a.stride_a * ES;
-        const char *wa = w + (size_t)min(ra, n - 1) * (size_t)a.lda * ES, *wb = w + (size_t)min(rb, n - 1) * (size_t)a.lda * ES;
-        const bool vec = a.vec_x && a.vec_a;
-#pragma unroll 2
-        for (int k0 = (blockIdx.x * WARPS + warp) * 32; k0 < a.cols; k0 += 32 * WARPS * gridDim.x) {
-            const int k = k0 + 8 * q, left = a.cols - k;
-            uint32_t p0[3][4] = {}, p1[3][4] = {};
-            Weights<WT, 8> ba = no_weights<WT, 8>(), bb = no_weights<WT, 8>();
-            if (vec && k0 + 32 <= a.cols) {
-                if (ra < n) ba = load_weights<WT, 8>(wa + (size_t)k * ES, 8, 8, true);
-                if (rb < n) bb = load_weights<WT, 8>(wb + (size_t)k * ES, 8, 8, true);
-                if (it.t0 >= 0) load_x(x0 + k, 8, true, p0);
-                if (it.t1 >= 0) load_x(x1 + k, 8, true, p1);
-            } else if (left > 0) {
-                if (ra < n) ba = load_weights<WT, 8>(wa + (size_t)k * ES, left, min(left, 8), false);
-                if (rb < n) bb = load_weights<WT, 8>(wb + (size_t)k * ES, left, min(left, 8), false);
-                if (it.t0 >= 0) load_x(x0 + k, left, false, p0);
-                if (it.t1 >= 0) load_x(x1 + k, left, false, p1);
-            }
-            float c[2][4] = {};
-            multiply<WT, 8>(c[0], p0, p1, ba);
-            multiply<WT, 8>(c[1], p0, p1, bb);
+        const char *wr[TILES];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                acc[0][e] = __fadd_rn(acc[0][e], c[0][e]);
-                acc[1][e] = __fadd_rn(acc[1][e], c[1][e]);
+        for (int h = 0; h < TILES; ++h) wr[h] = w + (size_t)min(r0 + 8 * h + g, n - 1) * (size_t)a.lda * ES;
+        const bool both = it.m > 8;
+        const int stride = WARPS * gridDim.x, whole = a.vec_x && a.vec_a ? a.cols / 32 : 0;
+        uint32_t p0[3][4] = {}, p1[3][4] = {};
+        Raw<WT, 8> b[TILES];
+        RawX f0, f1;
+        auto load = [&](int k0) {
+            const int k = 32 * k0 + 8 * q;
+#pragma unroll
+            for (int h = 0; h < TILES; ++h)
+                if (r0 + 8 * h + g < n) b[h] = raw_load<WT, 8>(wr[h] + (size_t)k * ES);
+            if (it.t0 >= 0) f0 = x_load(x0 + k);
+            if (both && it.t1 >= 0) f1 = x_load(x1 + k);
+        };
+        auto load_ragged = [&](int k0) {
+            const int k = 32 * k0 + 8 * q, left = a.cols - k;
+#pragma unroll
+            for (int h = 0; h < TILES; ++h)
+                if (r0 + 8 * h + g < n) b[h] = raw_elements<WT, 8>(wr[h] + (size_t)k * ES, left);
+            if (it.t0 >= 0) f0 = x_elements(x0 + k, left);
+            if (it.t1 >= 0) f1 = x_elements(x1 + k, left);
+        };
+#pragma unroll
+        for (int h = 0; h < TILES; ++h) b[h] = raw_zero<WT, 8>();
+        const int blocks = (a.cols + 31) / 32;
+        int k0 = blockIdx.x * WARPS + warp;
+        if (k0 < whole) load(k0);
+        for (; k0 < blocks; k0 += stride) {  // the next turn's numbers are on their way while this one's are multiplied
+            if (k0 >= whole) load_ragged(k0);
+            Weights<WT, 8> w8[TILES];
+#pragma unroll
+            for (int h = 0; h < TILES; ++h) w8[h] = weights<WT, 8>(b[h]);
+            if (it.t0 >= 0) split<8, 3>(f0.f, p0);
+            if (it.t1 >= 0) split<8, 3>(f1.f, p1);
+            if (k0 + stride < whole) load(k0 + stride);
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < TILES; ++h) {
+                float c[4];
+                multiply<WT, 8>(c, true, p0, p1, w8[h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[h][e] = __fadd_rn(acc[h][e], c[e]);
             }
         }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < TILES; ++h) {
         *reinterpret_cast<float2 *>(&part[warp][g][8 * h + 2 * q]) = make_float2(acc[h][0], acc[h][1]);
         *reinterpret_cast<float2 *>(&part[warp][g + 8][8 * h + 2 * q]) = make_float2(acc[h][2], acc[h][3]);
     }
     __syncthreads();
-    /* two ranks of one token per thread; warp w has tokens 4 w .. 4 w + 3 */
-    const int row = threadIdx.x >> 3, r = 2 * (threadIdx.x & 7);
+    /* two ranks of one token per thread: token `row` of the item */
+    constexpr int PER_ROW = RANKS / 2, USED = kLoraItem * PER_ROW;
+    static_assert(USED <= kShrinkThreads, "a thread for every two ranks");
+    const int row = threadIdx.x / PER_ROW, r = 2 * (threadIdx.x % PER_ROW);
     float u = 0.0f, v = 0.0f;
-    if (threadIdx.x < kLoraItem * 8) {
+    if (threadIdx.x < USED) {
 #pragma unroll
         for (int k = 0; k < WARPS; ++k) {
             const float2 s = *reinterpret_cast<const float2 *>(&part[k][row][r]);
@@ -442,11 +465,10 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __gri
     }
     cluster.barrier_wait(std::move(begun));
     if (gridDim.x > 1) {
-        if (threadIdx.x < kLoraItem * 8)
-            *cluster.map_shared_rank(&gather[blockIdx.x][row][r / 2], 0) = make_float2(u, v);
+        if (threadIdx.x < USED) *cluster.map_shared_rank(&gather[blockIdx.x][row][r / 2], 0) = make_float2(u, v);
         cluster.sync();
         if (blockIdx.x) return;
-        if (threadIdx.x < kLoraItem * 8) {
+        if (threadIdx.x < USED) {
             u = v = 0.0f;
             for (int k = 0; k < (int)gridDim.x; ++k) {
                 const float2 s = gather[k][row][r / 2];
@@ -455,8 +477,8 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __gri
             }
         }
     }
-    if (threadIdx.x >= kLoraItem * 8) return;
-    /* token `row` of the item is what lanes 4 (row % 8) hold as t0 or t1 */
+    if (threadIdx.x >= USED) return;  // whole warps
+    /* the token is what lanes 4 (row % 8) hold as t0 or t1 */
     const int ta = __shfl_sync(kFull, it.t0, 4 * (row & 7)), tb = __shfl_sync(kFull, it.t1, 4 * (row & 7));
     const int t = row < 8 ? ta : tb;
     if (t < 0) return;
@@ -488,90 +510,238 @@ __device__ __forceinline__ void load_low(const LoraArgs &a, int t, int r, uint32
     }
 }
 
-/* One item per blockIdx.y; the warps of its CTAs take 16 PAIRS rows of B_i at
- * a time.  N is the number of ranks a lane holds: 4 for ranks up to 16, else 8
- * (a group of 32 ranks at a time).  Column h of instruction j of a pair stands
- * for row 4 (h / 2) + 2 j + h % 2 of its 16, which gives lane q the four rows
- * 4 q .. 4 q + 3 of the result: 16 bytes of y. */
-template <int WT, int N, int PAIRS>
-__global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
-    constexpr int ES = WT == kHeadF32 ? 4 : 2, ROWS = 16 * PAIRS;
+/* What a warp of the second kernel knows: its item, and for this lane the first
+ * weights of the row that it holds in instruction 0, the bytes from there to
+ * its row in instruction 1, and its tokens' rows of y.
+ *
+ * A warp takes 32 rows of B_i at a time, four instructions wide.  Column h of
+ * instruction j stands for row 8 (h / 2) + 2 j + h % 2 of the 32, which gives
+ * lane q the eight rows 8 q .. 8 q + 7 of the result: 32 bytes of y, a line for
+ * the four lanes of a token.  Where rows of y do not start on 16 bytes it
+ * stands for row 8 j + h instead, and y goes by element. */
+template <int WT>
+struct ExpandLane {
+    LoraItem it;
+    int n;  // the adapter's rank
+    bool wide;
+    const char *b, *w;
+    size_t pitch, next;
+    float *y0, *y1;
+    __device__ __forceinline__ ExpandLane(const LoraArgs &a, const LoraItem &item, int N) : it(item) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+        constexpr int ES = kWeightBytes<WT>;
+        n = lora_rank(a, it.adapter);
+        wide = a.vec_y != 0;
+        b = static_cast<const char *>(a.b) + (size_t)it.adapter * (size_t)a.stride_b * ES;
+        pitch = (size_t)a.ldb * ES;
+        w = b + (size_t)(wide ? 8 * (g >> 1) + (g & 1) : g) * pitch + (size_t)(N * q) * ES;
+        next = (wide ? 2 : 8) * pitch;
+        y0 = a.y + (size_t)max(it.t0, 0) * (size_t)a.ldy;
+        y1 = a.y + (size_t)max(it.t1, 0) * (size_t)a.ldy;
+    }
+};
+
+/* 32 rows from v0 on, any alignment, sizes and end */
+template <int WT, int N>
+__device__ __forceinline__ void expand_any(const LoraArgs &a, const ExpandLane<WT> &l, int64_t v0) {
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    float c[4][4] = {};
+    uint32_t x0[3][N / 2] = {}, x1[3][N / 2] = {};
+    for (int r0 = 0; r0 < l.n; r0 += 4 * N) {
+        const int r = r0 + N * q;
+        if (l.it.t0 >= 0) load_low<N>(a, l.it.t0, r, x0);
+        if (l.it.t1 >= 0) load_low<N>(a, l.it.t1, r, x1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t v = v0 + (l.wide ? 8 * (g >> 1) + 2 * j + (g & 1) : 8 * j + g);
+            Raw<WT, N> b = raw_zero<WT, N>();
+            if (v < a.rows && r < l.n) {
+                const char *p = l.w + (size_t)v0 * l.pitch + j * l.next + (size_t)r0 * kWeightBytes<WT>;
+                if (a.vec_b && r + N <= l.n) b = raw_load<WT, N>(p);
+                else b = raw_elements<WT, N>(p, l.n - r);
+            }
+            const Weights<WT, N> wb = weights<WT, N>(b);
+            __syncwarp();
+            multiply<WT, N>(c[j], false, x0, x1, wb);
+        }
+    }
+    if (l.n == 0) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if ((h ? l.it.t1 : l.it.t0) < 0) continue;
+        float *y = h ? l.y1 : l.y0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int64_t v = v0 + (l.wide ? 8 * q + e : 8 * (e / 2) + 2 * q + (e & 1));
+            if (v < a.rows) y[v] = __fadd_rn(y[v], c[e / 2][2 * h + (e & 1)]);
+        }
+    }
+}
+
+/* The second kernel for arrays that the one below cannot take: one item per
+ * blockIdx.y, a warp its 32 rows at a time. */
+template <int WT, int N>
+__global__ void __launch_bounds__(kExpandThreads) lora_expand_any_kernel(const __grid_constant__ LoraArgs a) {
     const LoraItem it = lora_item(a, blockIdx.y);  // the kernel before let this one begin when the plan was there
-    if (it.adapter < 0) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");  // no CTA ends before the kernel before
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (it.adapter < 0) return;
+    const ExpandLane<WT> l(a, it, N);
+    const int64_t step = (int64_t)gridDim.x * (kExpandThreads / 32) * 32;
+    for (int64_t v0 = ((int64_t)blockIdx.x * (kExpandThreads / 32) + (threadIdx.x >> 5)) * 32; v0 < a.rows; v0 += step)
+        expand_any<WT, N>(a, l, v0);
+}
+
+/* bytes (at most 16) of src and zeros up to 16 */
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+/* Bytes of a row of B_i in shared memory and of one of a warp's stages: 32 such
+ * rows (64 bytes more after every eight where a row is 32 bytes), then a line
+ * of y for each of 16 tokens. */
+__host__ __device__ constexpr int expand_row_bytes(int rank_pad, int es) { return rank_pad * es; }
+__host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es) {
+    return 32 * rank_pad * es + (rank_pad * es == 32 ? 256 : 0) + kLoraItem * 128;
+}
+
+/* The second kernel: one item per blockIdx.y.  Every warp has D stages of
+ * shared memory, which cp.async fills with the 32 rows of B_i and the lines of
+ * y of its turns to come: D - 1 turns are on their way while one is
+ * multiplied, and none needs a barrier of the CTA.  The kernel begins while
+ * the one before still runs, and its first stages are on their way until that
+ * is done.  Rows lie in shared memory with their 16-byte pieces exchanged so
+ * that the eight lanes of a quarter warp read eight different ones.
+ *
+ * N is the number of ranks a lane holds: 4 for ranks up to 16, else 8 (a group
+ * of 32 ranks at a time).  G groups of low-rank numbers stay in registers
+ * (0: they are read again for every turn). */
+template <int WT, int N, int G, int D>
+__global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
+    extern __shared__ __align__(128) unsigned char lora_smem[];
+    constexpr int ES = kWeightBytes<WT>, ROWS = 32, WARPS = kExpandThreads / 32, GR = G ? G : 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const LoraItem it = lora_item(a, blockIdx.y);  // the kernel before let this one begin when the plan was there
+    const int64_t first = ((int64_t)blockIdx.x * WARPS + warp) * ROWS, step = (int64_t)gridDim.x * WARPS * ROWS;
+    if (it.adapter < 0 || first >= a.rows) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // no warp ends before the kernel before
         return;
     }
-    const int n = lora_rank(a, it.adapter);
-    const bool full = a.vec_b && a.vec_y && n % N == 0;
-    /* this lane's first row of B_i and ranks, and its tokens' rows of y */
-    const char *w = static_cast<const char *>(a.b) +
-                    ((size_t)it.adapter * (size_t)a.stride_b + (size_t)(4 * (g >> 1) + (g & 1)) * (size_t)a.ldb + N * q) * ES;
-    float *y0 = a.y + (size_t)max(it.t0, 0) * (size_t)a.ldy + 4 * q, *y1 = a.y + (size_t)max(it.t1, 0) * (size_t)a.ldy + 4 * q;
-    uint32_t x0[3][N / 2] = {}, x1[3][N / 2] = {};
-    bool have = false;  // the low-rank numbers are there, and the first group of them in x0 and x1
-    const int64_t step = (int64_t)gridDim.x * (kExpandThreads / 32) * ROWS;
-    for (int64_t v0 = ((int64_t)blockIdx.x * (kExpandThreads / 32) + (threadIdx.x >> 5)) * ROWS; v0 < a.rows; v0 += step) {
-        const bool inside = full && v0 + ROWS <= a.rows;
-        const char *wv = w + (size_t)v0 * (size_t)a.ldb * ES;
-        float4 o0[PAIRS], o1[PAIRS];
-        if (inside) {
+    const ExpandLane<WT> l(a, it, N);
+    const int rank_pad = G ? 4 * N * G : a.rank_pad;  // known to the compiler but for the largest ranks
+    const int row_bytes = expand_row_bytes(rank_pad, ES), stage_bytes = expand_stage_bytes(rank_pad, ES);
+    const int pad8 = row_bytes == 32 ? 64 : 0, y_at = 32 * row_bytes + 4 * pad8;
+    const int swap = ES == 2 ? (row_bytes % 128 == 0 ? 4 : 0) : (N == 8 ? 1 : 0);  // of odd rows' pieces
+    unsigned char *mem = lora_smem + warp * D * stage_bytes;
+    /* how the lanes share a copy of 32 rows: `share` of them a row, in as many rounds; what lies past the adapter's
+     * rank is filled with zeros */
+    const int share = G ? 4 * N * G * ES / 16 : 16;
+    const int c_row = lane / share, c_piece = lane % share, c_rows = 32 / share;
+    const bool c_on = c_piece * 16 < row_bytes;
+    const uint32_t c_bytes = (uint32_t)min(max(l.n * ES - c_piece * 16, 0), 16);
+    const char *b_from = l.b + (size_t)(first + c_row) * l.pitch + (c_bytes ? c_piece << 4 : 0);
+    const size_t b_round = (size_t)c_rows * l.pitch, b_step = (size_t)step * l.pitch;
+    const uint32_t mem_s = (uint32_t)__cvta_generic_to_shared(mem);
+    const uint32_t b_to = c_row * row_bytes + (c_row >> 3) * pad8 + ((c_piece ^ (c_row & 1 ? swap : 0)) << 4);
+    const uint32_t b_to_round = c_rows * row_bytes + (c_rows >> 3) * pad8;  // c_rows is even: rows keep their oddness
+    const float *y_from[kLoraItem / 4];  // this lane's piece of a token's line, four tokens at a time
 #pragma unroll
-            for (int p = 0; p < PAIRS; ++p) {
-                if (it.t0 >= 0) o0[p] = *reinterpret_cast<const float4 *>(y0 + v0 + 16 * p);
-                if (it.t1 >= 0) o1[p] = *reinterpret_cast<const float4 *>(y1 + v0 + 16 * p);
+    for (int p = 0; p < kLoraItem / 4; ++p) {
+        const int tk = 4 * p + (lane >> 3);
+        const int ta = __shfl_sync(kFull, it.t0, 4 * (tk & 7)), tb = __shfl_sync(kFull, it.t1, 4 * (tk & 7));
+        const int t = tk < 8 ? ta : tb;
+        y_from[p] = a.y + (size_t)max(t, 0) * (size_t)a.ldy + first + 4 * (lane & 7);
+    }
+    const uint32_t y_to = y_at + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3 & 1)) << 4);
+    const int turns = (int)((a.rows - ROWS - first + step) / step);  // whole ones
+    int ahead = 0;  // the next turn to bring
+    auto issue = [&](int stage) {
+        if (ahead < turns) {
+            const uint32_t to = mem_s + stage * stage_bytes;
+            if (c_on) {
+                const char *src = b_from;
+#pragma unroll
+                for (int r = 0; r < share; ++r, src += b_round) cp_async16_at(to + b_to + r * b_to_round, src, c_bytes);
             }
+#pragma unroll
+            for (int p = 0; p < kLoraItem / 4; ++p) {
+                if (4 * p >= it.m) break;
+                if (4 * p + (lane >> 3) < it.m) cp_async16_at(to + y_to + 512 * p, y_from[p], 16u);
+                y_from[p] += step;
+            }
+            b_from += b_step;
+            ++ahead;
         }
-        float c[PAIRS][2][4] = {};
-        for (int r0 = 0; r0 < n; r0 += 4 * N) {
-            const int r = r0 + N * q;
-            Weights<WT, N> b[PAIRS][2];
+        cp_async_commit();
+    };
 #pragma unroll
-            for (int p = 0; p < PAIRS; ++p)
+    for (int s = 0; s < D - 1; ++s) issue(s);
+    uint32_t x0[GR][3][N / 2] = {}, x1[GR][3][N / 2] = {};
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the low-rank numbers are there
+    if (G) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const char *at = wv + ((size_t)(16 * p + 2 * j) * (size_t)a.ldb + r0) * ES;
-                    b[p][j] = no_weights<WT, N>();
-                    if (inside) {
-                        if (r < n) b[p][j] = load_weights<WT, N>(at, N, N, true);
-                    } else if (v0 + 16 * p + 4 * (g >> 1) + 2 * j + (g & 1) < a.rows && r < n) {
-                        b[p][j] = load_weights<WT, N>(at, N, min(n - r, N), false);
-                    }
-                }
-            if (!have) asm volatile("griddepcontrol.wait;" ::: "memory");
-            if (!have || n > 4 * N) {
-                if (it.t0 >= 0) load_low<N>(a, it.t0, r, x0);
-                if (it.t1 >= 0) load_low<N>(a, it.t1, r, x1);
-                have = true;
-            }
-#pragma unroll
-            for (int p = 0; p < PAIRS; ++p)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) multiply<WT, N>(c[p][j], x0, x1, b[p][j]);
-        }
-#pragma unroll
-        for (int p = 0; p < PAIRS; ++p) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if ((h ? it.t1 : it.t0) < 0) continue;
-                float *y = (h ? y1 : y0) + v0 + 16 * p;
-                const float d[4] = {c[p][0][2 * h], c[p][0][2 * h + 1], c[p][1][2 * h], c[p][1][2 * h + 1]};
-                if (inside) {
-                    float4 o = h ? o1[p] : o0[p];
-                    o.x = __fadd_rn(o.x, d[0]);
-                    o.y = __fadd_rn(o.y, d[1]);
-                    o.z = __fadd_rn(o.z, d[2]);
-                    o.w = __fadd_rn(o.w, d[3]);
-                    *reinterpret_cast<float4 *>(y) = o;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (v0 + 16 * p + 4 * q + e < a.rows) y[e] = __fadd_rn(y[e], d[e]);
-                }
-            }
+        for (int k = 0; k < GR; ++k) {
+            if (it.t0 >= 0) load_low<N>(a, it.t0, k * 4 * N + N * q, x0[k]);
+            if (it.t1 >= 0) load_low<N>(a, it.t1, k * 4 * N + N * q, x1[k]);
         }
     }
-    if (!have) asm volatile("griddepcontrol.wait;" ::: "memory");
+    /* where this lane's row of instruction 0 lies in a stage, its piece there, and its lines of y */
+    const int w_at = (8 * (g >> 1) + (g & 1)) * row_bytes + (g >> 1) * pad8, w_swap = g & 1 ? swap : 0;
+    const int line0 = y_at + g * 128 + ((2 * q ^ (g & 1)) << 4), line1 = y_at + g * 128 + ((2 * q + 1 ^ (g & 1)) << 4);
+    float *y0 = l.y0 + first + 8 * q, *y1 = l.y1 + first + 8 * q;
+    const bool both = it.m > 8, line = a.vec_y == 2;
+    int st = 0;
+    for (int turn = 0; turn < turns; ++turn, y0 += step, y1 += step, st = st + 1 == D ? 0 : st + 1) {
+        cp_async_wait<D - 2>();
+        __syncwarp();  // stage st has landed for every lane, and no lane still reads the one before it
+        issue(st == 0 ? D - 1 : st - 1);
+        const unsigned char *from = mem + st * stage_bytes;
+        float c[4][4];
+        auto group = [&](int k, bool from_zero, const uint32_t (&u0)[3][N / 2], const uint32_t (&u1)[3][N / 2]) {
+            const int r = k * 4 * N + N * q;
+            const unsigned char *row = from + w_at;
+#pragma unroll
+            for (int j = 0; j < 4; ++j, row += 2 * row_bytes) {
+                Raw<WT, N> b;
+                if (N * ES == 8) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(row + r * ES);
+                    b.u[0] = v.x, b.u[1] = v.y;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N * ES / 16; ++e) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(row + ((((r * ES >> 4) + e) ^ w_swap) << 4));
+                        constexpr int WORDS = N * ES / 4;
+                        b.u[4 * e] = v.x, b.u[4 * e + 1] = v.y, b.u[(4 * e + 2) % WORDS] = v.z, b.u[(4 * e + 3) % WORDS] = v.w;
+                    }
+                }
+                multiply<WT, N>(c[j], from_zero, u0, u1, weights<WT, N>(b));
+            }
+        };
+        if (l.n == 0) continue;
+        if (G) {
+            group(0, true, x0[0], x1[0]);
+            if (GR > 1 && 4 * N < l.n) group(1, false, x0[GR - 1], x1[GR - 1]);
+        } else {
+            for (int k = 0; k * 4 * N < l.n; ++k) {
+                if (it.t0 >= 0) load_low<N>(a, it.t0, k * 4 * N + N * q, x0[0]);
+                if (it.t1 >= 0) load_low<N>(a, it.t1, k * 4 * N + N * q, x1[0]);
+                __syncwarp();
+                group(k, k == 0, x0[0], x1[0]);
+            }
+        }
+        auto add = [&](int h, float *y) {
+            const float4 o = *reinterpret_cast<const float4 *>(from + line0 + 1024 * h);
+            const float4 p = *reinterpret_cast<const float4 *>(from + line1 + 1024 * h);
+            const float f[8] = {o.x, o.y, o.z, o.w, p.x, p.y, p.z, p.w};
+            Sector s;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s.u[e] = __float_as_uint(__fadd_rn(f[e], c[e / 2][2 * h + (e & 1)]));
+            if (line) sector_store(y, s);
+            else sector_store16(y, s);
+        };
+        if (it.t0 >= 0) add(0, y0);
+        if (both && it.t1 >= 0) add(1, y1);
+    }
+    if (first + turns * step < a.rows) expand_any<WT, N>(a, l, first + turns * step);  // the last rows
 }
 
 }  // namespace noel

@@ -1176,9 +1176,11 @@ int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size
     };
     const size_t lane_b = a.rank_pad == 16 && es == 2 ? 8 : 16;  // bytes of a lane's ranks, at most 16
     a.vec_x = rows_on(x, ldx * 4, 0, 16);
-    a.vec_y = rows_on(y, ldy * 4, 0, 16);
+    a.vec_y = rows_on(y, ldy * 4, 0, 32) ? 2 : rows_on(y, ldy * 4, 0, 16) ? 1 : 0;
     a.vec_a = rows_on(l->d_a, l->lda * es, l->stride_a * es, 16);
     a.vec_b = rows_on(l->d_b, l->ldb * es, l->stride_b * es, lane_b);
+    a.staged = rows_on(l->d_b, l->ldb * es, l->stride_b * es, 16) && a.vec_y && (size_t)l->rank * es % 16 == 0 &&
+               a.rank_pad * es <= 256;
     *out = a;
     return NOEL_OK;
 }
@@ -1186,10 +1188,12 @@ int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size
 /* a kernel in clusters along x; dependent: it may start while the one before
  * it in the stream still runs (it waits with griddepcontrol.wait) */
 template <typename... P, typename... A>
-cudaError_t launch_cluster(void (*k)(P...), dim3 grid, int threads, int cluster, bool dependent, cudaStream_t s, A... args) {
+cudaError_t launch_cluster(void (*k)(P...), dim3 grid, int threads, size_t smem, int cluster, bool dependent, cudaStream_t s,
+                           A... args) {
     cudaLaunchConfig_t lc = {};
     lc.gridDim = grid;
     lc.blockDim = dim3(threads);
+    lc.dynamicSmemBytes = smem;
     lc.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1202,13 +1206,52 @@ cudaError_t launch_cluster(void (*k)(P...), dim3 grid, int threads, int cluster,
     return cudaLaunchKernelEx(&lc, k, args...);
 }
 
-template <int WT, int N, int PAIRS>
-cudaError_t expand_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
-    const int rows = 16 * PAIRS * (kExpandThreads / 32);
-    const int64_t all = ((int64_t)a.rows + rows - 1) / rows;
-    const int64_t want = ((int64_t)c->sms * kExpandWaves + items - 1) / items;
-    return launch_cluster(lora_expand_kernel<WT, N, PAIRS>, dim3((unsigned)(all < want ? all : want), items), kExpandThreads,
-                          1, true, s, a);
+template <int WT, int TILES>
+cudaError_t shrink_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
+    const int groups = a.rank_pad / (8 * TILES);
+    int split = 1;
+    while (split < kShrinkSplit && split * items * groups <= c->sms && split * kShrinkThreads < a.cols) split *= 2;
+    return launch_cluster(lora_shrink_kernel<WT, TILES>, dim3(split, items, groups), kShrinkThreads, 0, split,
+                          a.plan != nullptr, s, a);
+}
+
+/* CTAs per item of the second kernel: one turn of the GPU's CTA slots where
+ * that is enough work for them, else kExpandWaves, so that items of unlike size
+ * even out */
+dim3 expand_grid(DeviceCtx *c, const LoraArgs &a, int items, int per_sm) {
+    const int rows = 32 * (kExpandThreads / 32);
+    const int64_t all = ((int64_t)a.rows + rows - 1) / rows, slots = (int64_t)c->sms * per_sm;
+    const int64_t waves = all * items <= kExpandWaves * slots ? 1 : kExpandWaves;
+    const int64_t want = (waves * slots + items - 1) / items;
+    return dim3((unsigned)(all < want ? all : want), items);
+}
+
+template <int WT, int N, int G, int D>
+int expand_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
+    const size_t smem = (size_t)(kExpandThreads / 32) * D * expand_stage_bytes(a.rank_pad, kWeightBytes<WT>);
+    const int r = set_smem(c, (const void *)lora_expand_kernel<WT, N, G, D>, smem);
+    if (r) return r;
+    CUDA_TRY((launch_cluster(lora_expand_kernel<WT, N, G, D>, expand_grid(c, a, items, smem <= 112 * 1024 ? 2 : 1),
+                             kExpandThreads, smem, 1, true, s, a)));
+    return NOEL_OK;
+}
+
+template <int WT, int N>
+int expand_any_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
+    CUDA_TRY((launch_cluster(lora_expand_any_kernel<WT, N>, expand_grid(c, a, items, 2), kExpandThreads, 0, 1, true, s, a)));
+    return NOEL_OK;
+}
+
+/* The second kernel: through shared memory where rows of B and of y start on
+ * 16 bytes and two stages of a warp fit (ranks up to 128, fp32 64). */
+template <int WT>
+int expand(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
+    constexpr bool kF32 = WT == kHeadF32;
+    if (!a.staged) return a.rank_pad == 16 ? expand_any_launch<WT, 4>(c, a, items, s) : expand_any_launch<WT, 8>(c, a, items, s);
+    if (a.rank_pad == 16) return expand_launch<WT, 4, 1, kF32 ? 3 : 4>(c, a, items, s);
+    if (a.rank_pad == 32) return expand_launch<WT, 8, 1, kF32 ? 2 : 3>(c, a, items, s);
+    if (a.rank_pad == 64 && !kF32) return expand_launch<WT, 8, kF32 ? 0 : 2, 2>(c, a, items, s);
+    return expand_launch<WT, 8, 0, 2>(c, a, items, s);
 }
 
 template <int WT>
@@ -1226,12 +1269,10 @@ int lora_launch_t(DeviceCtx *c, const LoraArgs &all, cudaStream_t s) {
         }
         /* an adapter's last item may be short: at most n + batch / 16 items */
         const int64_t bound = (int64_t)a.n + a.batch / kLoraItem;
-        const int items = bound < a.batch ? (int)bound : a.batch, groups = a.rank_pad / 16;
-        int split = 1;
-        while (split < kShrinkSplit && 2 * split * items * groups <= c->sms && split * kShrinkThreads < a.cols) split *= 2;
-        CUDA_TRY(launch_cluster(lora_shrink_kernel<WT>, dim3(split, items, groups), kShrinkThreads, split,
-                                a.plan != nullptr, s, a));
-        CUDA_TRY((a.rank_pad == 16 ? expand_launch<WT, 4, 4>(c, a, items, s) : expand_launch<WT, 8, 2>(c, a, items, s)));
+        const int items = bound < a.batch ? (int)bound : a.batch;
+        CUDA_TRY((a.rank_pad == 16 ? shrink_launch<WT, 2>(c, a, items, s) : shrink_launch<WT, 4>(c, a, items, s)));
+        const int r = expand<WT>(c, a, items, s);
+        if (r) return r;
     }
     return NOEL_OK;
 }
