@@ -35,6 +35,7 @@ constexpr int kLoraWarpBatch = 32;  // tokens up to which every warp finds the i
 constexpr int kShrinkThreads = 256;
 constexpr int kShrinkSplit = 8;     // CTAs of a cluster that share an item's columns, at most
 constexpr int kExpandThreads = 256;
+constexpr int kExpandFetch = 1;    // turns between asking the L2 for a line of y and copying it
 constexpr int kExpandWaves = 4;     // turns of the GPU's CTAs that the second kernel's work is cut into
 
 /* the items of a batch above kLoraWarpBatch, in the scratch */
@@ -260,16 +261,16 @@ __device__ __forceinline__ Raw<WT, N> raw_load(const void *p) {
     }
     return r;
 }
-/* the first used of them, one by one; the others are 0 */
-template <int WT, int N>
+/* every STRIDE-th from p on, one by one; those from the used-th on (counting all) are 0 */
+template <int WT, int N, int STRIDE = 1>
 __device__ __forceinline__ Raw<WT, N> raw_elements(const void *p, int used) {
     Raw<WT, N> r;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         if (WT == kHeadF32) {
-            r.u[e % (N * kWeightBytes<WT> / 4)] = e < used ? static_cast<const uint32_t *>(p)[e] : 0u;
+            r.u[e % (N * kWeightBytes<WT> / 4)] = e * STRIDE < used ? __ldg(static_cast<const uint32_t *>(p) + e * STRIDE) : 0u;
         } else {
-            const uint32_t h = e < used ? (uint32_t)static_cast<const uint16_t *>(p)[e] : 0u;
+            const uint32_t h = e * STRIDE < used ? (uint32_t)__ldg(static_cast<const uint16_t *>(p) + e * STRIDE) : 0u;
             r.u[e / 2] = e & 1 ? r.u[e / 2] | h << 16 : h;
         }
     }
@@ -338,10 +339,11 @@ __device__ __forceinline__ RawX x_load(const float *p) {
     const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
     return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
+template <int STRIDE>
 __device__ __forceinline__ RawX x_elements(const float *p, int used) {
     RawX r;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r.f[e] = e < used ? __ldg(p + e) : 0.0f;
+    for (int e = 0; e < 8; ++e) r.f[e] = e * STRIDE < used ? __ldg(p + e * STRIDE) : 0.0f;
     return r;
 }
 
@@ -405,35 +407,37 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __gri
         uint32_t p0[3][4] = {}, p1[3][4] = {};
         Raw<WT, 8> b[TILES];
         RawX f0, f1;
+        /* a lane's eight of the 32 columns: consecutive ones where rows start on 16 bytes, else every fourth, so
+         * that the lanes of a row read side by side */
         auto load = [&](int k0) {
-            const int k = 32 * k0 + 8 * q;
+            if (k0 < whole) {
+                const int k = 32 * k0 + 8 * q;
 #pragma unroll
-            for (int h = 0; h < TILES; ++h)
-                if (r0 + 8 * h + g < n) b[h] = raw_load<WT, 8>(wr[h] + (size_t)k * ES);
-            if (it.t0 >= 0) f0 = x_load(x0 + k);
-            if (both && it.t1 >= 0) f1 = x_load(x1 + k);
-        };
-        auto load_ragged = [&](int k0) {
-            const int k = 32 * k0 + 8 * q, left = a.cols - k;
+                for (int h = 0; h < TILES; ++h)
+                    if (r0 + 8 * h + g < n) b[h] = raw_load<WT, 8>(wr[h] + (size_t)k * ES);
+                if (it.t0 >= 0) f0 = x_load(x0 + k);
+                if (both && it.t1 >= 0) f1 = x_load(x1 + k);
+            } else {
+                const int k = 32 * k0 + q, left = a.cols - k;
 #pragma unroll
-            for (int h = 0; h < TILES; ++h)
-                if (r0 + 8 * h + g < n) b[h] = raw_elements<WT, 8>(wr[h] + (size_t)k * ES, left);
-            if (it.t0 >= 0) f0 = x_elements(x0 + k, left);
-            if (it.t1 >= 0) f1 = x_elements(x1 + k, left);
+                for (int h = 0; h < TILES; ++h)
+                    if (r0 + 8 * h + g < n) b[h] = raw_elements<WT, 8, 4>(wr[h] + (size_t)k * ES, left);
+                if (it.t0 >= 0) f0 = x_elements<4>(x0 + k, left);
+                if (both && it.t1 >= 0) f1 = x_elements<4>(x1 + k, left);
+            }
         };
 #pragma unroll
         for (int h = 0; h < TILES; ++h) b[h] = raw_zero<WT, 8>();
         const int blocks = (a.cols + 31) / 32;
         int k0 = blockIdx.x * WARPS + warp;
-        if (k0 < whole) load(k0);
+        if (k0 < blocks) load(k0);
         for (; k0 < blocks; k0 += stride) {  // the next turn's numbers are on their way while this one's are multiplied
-            if (k0 >= whole) load_ragged(k0);
             Weights<WT, 8> w8[TILES];
 #pragma unroll
             for (int h = 0; h < TILES; ++h) w8[h] = weights<WT, 8>(b[h]);
             if (it.t0 >= 0) split<8, 3>(f0.f, p0);
             if (it.t1 >= 0) split<8, 3>(f1.f, p1);
-            if (k0 + stride < whole) load(k0 + stride);
+            if (k0 + stride < blocks) load(k0 + stride);
             __syncwarp();
 #pragma unroll
             for (int h = 0; h < TILES; ++h) {
@@ -591,6 +595,7 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_any_kernel(const _
         expand_any<WT, N>(a, l, v0);
 }
 
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 /* bytes (at most 16) of src and zeros up to 16 */
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -600,8 +605,8 @@ __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src, uin
  * rows (64 bytes more after every eight where a row is 32 bytes), then a line
  * of y for each of 16 tokens. */
 __host__ __device__ constexpr int expand_row_bytes(int rank_pad, int es) { return rank_pad * es; }
-__host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es) {
-    return 32 * rank_pad * es + (rank_pad * es == 32 ? 256 : 0) + kLoraItem * 128;
+__host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es, bool wide) {
+    return 32 * rank_pad * es + (rank_pad * es == 32 ? 256 : 0) + (wide ? kLoraItem * 128 : 0);
 }
 
 /* The second kernel: one item per blockIdx.y.  Every warp has D stages of
@@ -614,8 +619,9 @@ __host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es) {
  *
  * N is the number of ranks a lane holds: 4 for ranks up to 16, else 8 (a group
  * of 32 ranks at a time).  G groups of low-rank numbers stay in registers
- * (0: they are read again for every turn). */
-template <int WT, int N, int G, int D>
+ * (0: they are read again for every turn).  Without WIDE, rows of y start
+ * anywhere: y is not staged but read and written by element. */
+template <int WT, int N, int G, int D, bool WIDE>
 __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
     extern __shared__ __align__(128) unsigned char lora_smem[];
     constexpr int ES = kWeightBytes<WT>, ROWS = 32, WARPS = kExpandThreads / 32, GR = G ? G : 1;
@@ -628,7 +634,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
     }
     const ExpandLane<WT> l(a, it, N);
     const int rank_pad = G ? 4 * N * G : a.rank_pad;  // known to the compiler but for the largest ranks
-    const int row_bytes = expand_row_bytes(rank_pad, ES), stage_bytes = expand_stage_bytes(rank_pad, ES);
+    const int row_bytes = expand_row_bytes(rank_pad, ES), stage_bytes = expand_stage_bytes(rank_pad, ES, WIDE);
     const int pad8 = row_bytes == 32 ? 64 : 0, y_at = 32 * row_bytes + 4 * pad8;
     const int swap = ES == 2 ? (row_bytes % 128 == 0 ? 4 : 0) : (N == 8 ? 1 : 0);  // of odd rows' pieces
     unsigned char *mem = lora_smem + warp * D * stage_bytes;
@@ -654,6 +660,13 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
     const uint32_t y_to = y_at + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3 & 1)) << 4);
     const int turns = (int)((a.rows - ROWS - first + step) / step);  // whole ones
     int ahead = 0;  // the next turn to bring
+    /* one lane per token asks the L2 for that token's line kExpandFetch turns before it is copied from there */
+    const float *y_fetch;
+    {
+        const int ta = __shfl_sync(kFull, it.t0, 4 * (lane & 7)), tb = __shfl_sync(kFull, it.t1, 4 * (lane & 7));
+        const int t = lane < 8 ? ta : tb;
+        y_fetch = a.y + (size_t)max(t, 0) * (size_t)a.ldy + first + kExpandFetch * step;
+    }
     auto issue = [&](int stage) {
         if (ahead < turns) {
             const uint32_t to = mem_s + stage * stage_bytes;
@@ -664,10 +677,12 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
             }
 #pragma unroll
             for (int p = 0; p < kLoraItem / 4; ++p) {
-                if (4 * p >= it.m) break;
+                if (!WIDE || 4 * p >= it.m) break;
                 if (4 * p + (lane >> 3) < it.m) cp_async16_at(to + y_to + 512 * p, y_from[p], 16u);
                 y_from[p] += step;
             }
+            if (lane < it.m && ahead + kExpandFetch < turns) prefetch_l2(y_fetch);
+            y_fetch += step;
             b_from += b_step;
             ++ahead;
         }
@@ -684,10 +699,12 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
             if (it.t1 >= 0) load_low<N>(a, it.t1, k * 4 * N + N * q, x1[k]);
         }
     }
-    /* where this lane's row of instruction 0 lies in a stage, its piece there, and its lines of y */
-    const int w_at = (8 * (g >> 1) + (g & 1)) * row_bytes + (g >> 1) * pad8, w_swap = g & 1 ? swap : 0;
+    /* where this lane's row of instruction 0 lies in a stage and what instruction j adds, its piece there, and its
+     * lines of y */
+    const int w_at = WIDE ? (8 * (g >> 1) + (g & 1)) * row_bytes + (g >> 1) * pad8 : g * row_bytes;
+    const int w_next = WIDE ? 2 * row_bytes : 8 * row_bytes + pad8, w_swap = g & 1 ? swap : 0;
     const int line0 = y_at + g * 128 + ((2 * q ^ (g & 1)) << 4), line1 = y_at + g * 128 + ((2 * q + 1 ^ (g & 1)) << 4);
-    float *y0 = l.y0 + first + 8 * q, *y1 = l.y1 + first + 8 * q;
+    float *y0 = l.y0 + first + (WIDE ? 8 : 2) * q, *y1 = l.y1 + first + (WIDE ? 8 : 2) * q;
     const bool both = it.m > 8, line = a.vec_y == 2;
     int st = 0;
     for (int turn = 0; turn < turns; ++turn, y0 += step, y1 += step, st = st + 1 == D ? 0 : st + 1) {
@@ -700,7 +717,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
             const int r = k * 4 * N + N * q;
             const unsigned char *row = from + w_at;
 #pragma unroll
-            for (int j = 0; j < 4; ++j, row += 2 * row_bytes) {
+            for (int j = 0; j < 4; ++j, row += w_next) {
                 Raw<WT, N> b;
                 if (N * ES == 8) {
                     const uint2 v = *reinterpret_cast<const uint2 *>(row + r * ES);
@@ -717,6 +734,14 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
             }
         };
         if (l.n == 0) continue;
+        float e0[8], e1[8];
+        if (!WIDE) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (it.t0 >= 0) e0[e] = y0[8 * (e / 2) + (e & 1)];
+                if (both && it.t1 >= 0) e1[e] = y1[8 * (e / 2) + (e & 1)];
+            }
+        }
         if (G) {
             group(0, true, x0[0], x1[0]);
             if (GR > 1 && 4 * N < l.n) group(1, false, x0[GR - 1], x1[GR - 1]);
@@ -738,8 +763,16 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
             if (line) sector_store(y, s);
             else sector_store16(y, s);
         };
-        if (it.t0 >= 0) add(0, y0);
-        if (both && it.t1 >= 0) add(1, y1);
+        if (WIDE) {
+            if (it.t0 >= 0) add(0, y0);
+            if (both && it.t1 >= 0) add(1, y1);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (it.t0 >= 0) y0[8 * (e / 2) + (e & 1)] = __fadd_rn(e0[e], c[e / 2][e & 1]);
+                if (both && it.t1 >= 0) y1[8 * (e / 2) + (e & 1)] = __fadd_rn(e1[e], c[e / 2][2 + (e & 1)]);
+            }
+        }
     }
     if (first + turns * step < a.rows) expand_any<WT, N>(a, l, first + turns * step);  // the last rows
 }

@@ -1179,7 +1179,7 @@ int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size
     a.vec_y = rows_on(y, ldy * 4, 0, 32) ? 2 : rows_on(y, ldy * 4, 0, 16) ? 1 : 0;
     a.vec_a = rows_on(l->d_a, l->lda * es, l->stride_a * es, 16);
     a.vec_b = rows_on(l->d_b, l->ldb * es, l->stride_b * es, lane_b);
-    a.staged = rows_on(l->d_b, l->ldb * es, l->stride_b * es, 16) && a.vec_y && (size_t)l->rank * es % 16 == 0 &&
+    a.staged = rows_on(l->d_b, l->ldb * es, l->stride_b * es, 16) && (size_t)l->rank * es % 16 == 0 &&
                a.rank_pad * es <= 256;
     *out = a;
     return NOEL_OK;
@@ -1196,13 +1196,18 @@ cudaError_t launch_cluster(void (*k)(P...), dim3 grid, int threads, size_t smem,
     lc.dynamicSmemBytes = smem;
     lc.stream = s;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
-    lc.numAttrs = dependent ? 2 : 1;
+    if (cluster > 1) {
+        at[lc.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[lc.numAttrs].val.clusterDim.x = cluster;
+        at[lc.numAttrs].val.clusterDim.y = at[lc.numAttrs].val.clusterDim.z = 1;
+        ++lc.numAttrs;
+    }
+    if (dependent) {
+        at[lc.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[lc.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++lc.numAttrs;
+    }
     return cudaLaunchKernelEx(&lc, k, args...);
 }
 
@@ -1226,14 +1231,18 @@ dim3 expand_grid(DeviceCtx *c, const LoraArgs &a, int items, int per_sm) {
     return dim3((unsigned)(all < want ? all : want), items);
 }
 
-template <int WT, int N, int G, int D>
-int expand_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
-    const size_t smem = (size_t)(kExpandThreads / 32) * D * expand_stage_bytes(a.rank_pad, kWeightBytes<WT>);
-    const int r = set_smem(c, (const void *)lora_expand_kernel<WT, N, G, D>, smem);
+template <int WT, int N, int G, int D, bool WIDE>
+int expand_launch_y(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
+    const size_t smem = (size_t)(kExpandThreads / 32) * D * expand_stage_bytes(a.rank_pad, kWeightBytes<WT>, WIDE);
+    const int r = set_smem(c, (const void *)lora_expand_kernel<WT, N, G, D, WIDE>, smem);
     if (r) return r;
-    CUDA_TRY((launch_cluster(lora_expand_kernel<WT, N, G, D>, expand_grid(c, a, items, smem <= 112 * 1024 ? 2 : 1),
+    CUDA_TRY((launch_cluster(lora_expand_kernel<WT, N, G, D, WIDE>, expand_grid(c, a, items, smem <= 112 * 1024 ? 2 : 1),
                              kExpandThreads, smem, 1, true, s, a)));
     return NOEL_OK;
+}
+template <int WT, int N, int G, int D>
+int expand_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
+    return a.vec_y ? expand_launch_y<WT, N, G, D, true>(c, a, items, s) : expand_launch_y<WT, N, G, D, false>(c, a, items, s);
 }
 
 template <int WT, int N>
@@ -1242,8 +1251,8 @@ int expand_any_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s
     return NOEL_OK;
 }
 
-/* The second kernel: through shared memory where rows of B and of y start on
- * 16 bytes and two stages of a warp fit (ranks up to 128, fp32 64). */
+/* The second kernel: through shared memory where rows of B start on 16 bytes
+ * and end there, and two stages of a warp fit (ranks up to 128, fp32 64). */
 template <int WT>
 int expand(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
     constexpr bool kF32 = WT == kHeadF32;

@@ -437,13 +437,18 @@ def _on(tensor, dtype, shape, name: str, device):
     dtype, of shape (None: any extent), its last axis of unit stride."""
     if tensor is None:
         return None
-    if tensor.dtype != dtype:
+    if tensor.dtype is not dtype:
         _refuse(f"{name}: {dtype} wanted, got {tensor.dtype}")
-    if tensor.device != device or not tensor.is_cuda:
-        _refuse(f"{name} is on {tensor.device}, {device} wanted" if tensor.is_cuda else f"{name} is not on a GPU")
+    if not tensor.is_cuda:
+        _refuse(f"{name} is not on a GPU")
+    if tensor.get_device() != device.index:
+        _refuse(f"{name} is on {tensor.device}, {device} wanted")
     have = tensor.shape
-    if len(have) != len(shape) or any(w is not None and w != h for w, h in zip(shape, have)):
+    if len(have) != len(shape):
         _refuse(f"{name}: shape {tuple(shape)} wanted, got {tuple(have)}")
+    for w, h in zip(shape, have):
+        if w is not None and w != h:
+            _refuse(f"{name}: shape {tuple(shape)} wanted, got {tuple(have)}")
     if have[-1] > 1 and tensor.stride(-1) != 1:
         _refuse(f"{name}: its last axis must be contiguous")
     return tensor.data_ptr()
@@ -460,22 +465,22 @@ def _row_values(tensor, dtype, batch, name: str, device):
     return _on(tensor, dtype, (batch,), name, device)
 
 
-class _Device:
-    """Makes a tensor's device the current one for a call, where it is not."""
+def _call(device, stream, run) -> None:
+    """run(stream address) with device the current one, on stream or on the
+    device's current stream; raises on a status that is not 0."""
+    import torch
 
-    def __init__(self, device):
-        import torch
-
-        self.torch, self.index = torch, device.index
-        self.before = torch.cuda.current_device()
-
-    def __enter__(self):
-        if self.before != self.index:
-            self.torch.cuda.set_device(self.index)
-
-    def __exit__(self, *_):
-        if self.before != self.index:
-            self.torch.cuda.set_device(self.before)
+    index = device.index
+    before = torch._C._cuda_getDevice()
+    if before != index:
+        torch.cuda.set_device(index)
+    try:
+        status = run(stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index))
+    finally:
+        if before != index:
+            torch.cuda.set_device(before)
+    if status != 0:
+        _check(status)
 
 
 class LogitsParamsStruct(C.Structure):
@@ -542,6 +547,7 @@ class LogitsParams:
             s.d_mask_rows = _row_values(mask_rows, i32, B, "mask_rows", dev)
             self.words = mask.shape[1]
         s.v_begin = v_begin
+        self.ref = C.byref(s)
 
     def check(self, logits, vocab: int) -> None:
         """Whether these parameters fit rows of logits of vocab columns."""
@@ -570,9 +576,7 @@ def logits_process(logits, params: LogitsParams, vocab: int | None = None, strea
     if V > cols:
         _refuse(f"vocab {V} of {cols} columns")
     params.check(logits, V)
-    with _Device(dev):
-        s = stream if stream is not None else torch.cuda.current_stream(dev)
-        _check(lib().noel_logits_process(C.byref(params.s), ptr, dtype, B, V, _pitch(logits), C.c_void_p(s.cuda_stream)))
+    _call(dev, stream, lambda s: lib().noel_logits_process(params.ref, ptr, dtype, B, V, _pitch(logits), s))
     return logits
 
 
@@ -606,13 +610,16 @@ class Adapters:
         s.d_scale = _row_values(scale, torch.float32, self.n, "scale", a.device)
         s.d_ranks = _row_values(ranks, torch.int32, self.n, "ranks", a.device)
         s.type, s.n_adapters, s.rank = kind, self.n, self.rank
+        self.ref, self.sizes = C.byref(s), {}
 
     def scratch(self, batch: int):
-        """Scratch of one call over batch tokens, or None when it needs none."""
+        """Scratch of one call over batch tokens (None where it needs none) and its bytes."""
         import torch
 
-        need = lib().noel_lora_workspace_bytes(batch, self.rank)
-        return torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        size = self.sizes.get(batch)
+        if size is None:
+            size = self.sizes[batch] = lib().noel_lora_workspace_bytes(batch, self.rank)
+        return (torch.empty(size, dtype=torch.uint8, device=self.device) if size else None), size
 
 
 def lora_apply(y, x, adapters: Adapters, adapter_ids, stream=None):
@@ -626,16 +633,13 @@ def lora_apply(y, x, adapters: Adapters, adapter_ids, stream=None):
     B = y.shape[0]
     xp = _on(x, torch.float32, (B, adapters.cols), "x", dev)
     ip = _row_values(adapter_ids, torch.int32, B, "adapter_ids", dev)
-    with _Device(dev):
-        s = stream if stream is not None else torch.cuda.current_stream(dev)
-        if stream is None:
-            work = adapters.scratch(B)
-        else:
-            with torch.cuda.stream(stream):
-                work = adapters.scratch(B)
-        _check(lib().noel_lora_apply(C.byref(adapters.s), ip, xp, _pitch(x), B, adapters.cols, adapters.rows, yp,
-                                     _pitch(y), work.data_ptr() if work is not None else None,
-                                     work.numel() if work is not None else 0, C.c_void_p(s.cuda_stream)))
+    if stream is None:
+        work, size = adapters.scratch(B)
+    else:
+        with torch.cuda.stream(stream):
+            work, size = adapters.scratch(B)
+    _call(dev, stream, lambda s: lib().noel_lora_apply(adapters.ref, ip, xp, _pitch(x), B, adapters.cols, adapters.rows,
+                                                       yp, _pitch(y), work.data_ptr() if size else None, size, s))
     return y
 
 
@@ -664,19 +668,20 @@ def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: 
     else:
         hp, H, hld = None, 0, 0
     lora = ip = work = None
+    size = 0
     if adapters is not None:
         if adapters.device != dev or (adapters.rows, adapters.cols) != (V, D):
             _refuse(f"adapters of a [{adapters.rows}, {adapters.cols}] weight on {adapters.device}, "
                     f"the head is [{V}, {D}] on {dev}")
-        lora, ip = C.byref(adapters.s), _row_values(adapter_ids, torch.int32, B, "adapter_ids", dev)
-        work = adapters.scratch(B)
+        lora, ip = adapters.ref, _row_values(adapter_ids, torch.int32, B, "adapter_ids", dev)
+        work, size = adapters.scratch(B)
     if process is not None:
         process.check(logits, V)
     s = torch.cuda.current_stream(dev)
     _check(lib().noel_lmhead_sample_ex(C.byref(cfg), weight.data_ptr(), wt, weight.stride(0), hidden.data_ptr(),
                                        hidden.stride(0), B, D, V, lora, ip,
-                                       C.byref(process.s) if process is not None else None, hp, H, hld,
+                                       process.ref if process is not None else None, hp, H, hld,
                                        rng.data_ptr(), ids.data_ptr(), pr.data_ptr() if pr is not None else None,
-                                       logits.data_ptr(), work.data_ptr() if work is not None else None,
-                                       work.numel() if work is not None else 0, C.c_void_p(s.cuda_stream)))
+                                       logits.data_ptr(), work.data_ptr() if size else None, size,
+                                       C.c_void_p(s.cuda_stream)))
     return ids, logits, pr
