@@ -44,6 +44,7 @@ struct LogitsArgs {
     const int32_t *mask_row;
     int ranges, range;  // CTAs per row and their columns; 0: no such launch
     int cap;            // entries of a CTA's table; 0: none
+    bool together;      // all warps of a masked row's CTA fill the table
     int slices, slice;  // CTAs per row of the slice kernel and the words each counts in
 };
 
@@ -74,15 +75,28 @@ __device__ __forceinline__ void logit_store(uint16_t *p, float x) {
 
 struct RowRules {
     float rep, freq, pres;
+    float inv;  // 1 / rep, or 0 where quotients by rep are left to the division
 };
 
 __device__ __forceinline__ RowRules row_rules(const LogitsArgs &a, int row) {
-    return {a.rep ? a.rep[row] : 1.0f, a.freq ? a.freq[row] : 0.0f, a.pres ? a.pres[row] : 0.0f};
+    const float rep = a.rep ? a.rep[row] : 1.0f;
+    return {rep, a.freq ? a.freq[row] : 0.0f, a.pres ? a.pres[row] : 0.0f,
+            rep > 0.0009765625f && rep < 1024.0f ? __fdiv_rn(1.0f, rep) : 0.0f};
+}
+
+/* x / rep: a quotient from the reciprocal, corrected by its remainder
+ * (Markstein 1990), which is the rounded quotient where nothing on the way
+ * over- or underflows; |x| and rep are kept well inside that. */
+__device__ __forceinline__ float quotient(float x, const RowRules &r) {
+    const uint32_t e = __float_as_uint(x) & 0x7F800000u;
+    if (r.inv == 0.0f || e < 0x0D000000u || e > 0x70000000u) return __fdiv_rn(x, r.rep);
+    const float q = __fmul_rn(x, r.inv);
+    return __fmaf_rn(__fmaf_rn(-q, r.rep, x), r.inv, q);
 }
 
 __device__ __forceinline__ float penalised(float x, uint32_t w, const RowRules &r) {
     const uint32_t n = w & kCount;
-    if (w & (kSeenPrompt | kCount)) x = x > 0.0f ? __fdiv_rn(x, r.rep) : __fmul_rn(x, r.rep);
+    if (w & (kSeenPrompt | kCount)) x = x > 0.0f ? quotient(x, r) : __fmul_rn(x, r.rep);
     if (n) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.freq, (float)n)), r.pres);
     return x;
 }
@@ -310,8 +324,10 @@ __device__ __forceinline__ void mask_piece(const LogitsArgs &a, T *x, int64_t c0
  * the range is masked, and then the table's logits are changed.  The mask
  * never changes an allowed logit's value but may write it back as it read it,
  * so the table's own writes come after the mask's, a CTA's barrier between
- * them.  In a masked row one warp fills the table while the others mask; it
- * takes its turns at the mask when it has done that. */
+ * them.  In a masked row of a large batch one warp fills the table while the
+ * others mask, and takes its turns at the mask when it has done that; where
+ * the CTAs all run at once, their time is that of the longest warp, and all
+ * warps fill it first. */
 template <typename T>
 __global__ void __launch_bounds__(kLogitsThreads, kRowsCtas) logits_rows_kernel(const __grid_constant__ LogitsArgs a) {
     extern __shared__ __align__(16) uint32_t logits_smem[];
@@ -329,7 +345,8 @@ __global__ void __launch_bounds__(kLogitsThreads, kRowsCtas) logits_rows_kernel(
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         if (threadIdx.x == 0) turn = kLogitsThreads / 32;  // every warp's first turn is its own number
         __syncthreads();
-        if (a.cap && warp == 0) table_fill<32>(a, row, t, lo, hi);
+        if (a.cap && a.together) table_fill<kLogitsThreads>(a, row, t, lo, hi);
+        else if (a.cap && warp == 0) table_fill<32>(a, row, t, lo, hi);
         int k = warp;
         uint32_t next = mask_bits(a, mask, begin + (int64_t)k * kMaskPiece + 32 * lane);
         while (begin + (int64_t)k * kMaskPiece < end) {
@@ -349,21 +366,41 @@ __global__ void __launch_bounds__(kLogitsThreads, kRowsCtas) logits_rows_kernel(
     }
 }
 
-/* the penalties of a sector's words on its logits, biased and masked ones left alone */
+/* The penalties of a sector's words on its logits: on those whose bit of
+ * `change` is set.  All of them are computed, and the odd quotients (see
+ * quotient()) again by division. */
 template <typename T>
-__device__ __forceinline__ void sector_penalise(const LogitsArgs &a, Sector &s, const uint32_t (&w)[32 / sizeof(T)],
-                                                const RowRules &rules, const uint32_t *mask, int c) {
+__device__ __forceinline__ void sector_penalise(Sector &s, const uint32_t (&w)[32 / sizeof(T)], uint32_t change,
+                                                const RowRules &r) {
     constexpr int VE = 32 / sizeof(T);
+    float v[VE];
+    uint32_t odd = 0u;
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-        if (!w[e] || (w[e] & kHasBias) || !allowed(mask, a.v_begin + c + e)) continue;
+        const float x = sizeof(T) == 4 ? __uint_as_float(s.u[e % 8])
+                                       : __uint_as_float(e & 1 ? s.u[e / 2 % 8] & 0xFFFF0000u : s.u[e / 2 % 8] << 16);
+        const uint32_t exponent = __float_as_uint(x) & 0x7F800000u, n = w[e] & kCount;
+        if (x > 0.0f && (r.inv == 0.0f || exponent < 0x0D000000u || exponent > 0x70000000u)) odd |= 1u << e;
+        const float q = __fmul_rn(x, r.inv);
+        float y = x > 0.0f ? __fmaf_rn(__fmaf_rn(-q, r.rep, x), r.inv, q) : __fmul_rn(x, r.rep);
+        if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(r.freq, (float)n)), r.pres);
+        v[e] = y;
+    }
+    if (odd & change) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+            if (odd & change & 1u << e)
+                v[e] = penalised(sizeof(T) == 4 ? __uint_as_float(s.u[e % 8])
+                                                : __uint_as_float(e & 1 ? s.u[e / 2 % 8] & 0xFFFF0000u : s.u[e / 2 % 8] << 16),
+                                 w[e], r);
+    }
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
         if (sizeof(T) == 4) {
-            s.u[e] = __float_as_uint(penalised(__uint_as_float(s.u[e]), w[e], rules));
-        } else {
-            const int h = 16 * (e & 1);
-            const float v = penalised(__uint_as_float(s.u[e / 2] >> h << 16), w[e], rules);
-            const uint32_t r = __bfloat16_as_ushort(__float2bfloat16_rn(v));
-            s.u[e / 2] = (s.u[e / 2] & ~(0xFFFFu << h)) | r << h;
+            if (change >> e & 1u) s.u[e % 8] = __float_as_uint(v[e]);
+        } else if (change >> e & 1u) {
+            const uint32_t b = __bfloat16_as_ushort(__float2bfloat16_rn(v[e]));
+            s.u[e / 2 % 8] = e & 1 ? (s.u[e / 2 % 8] & 0x0000FFFFu) | b << 16 : (s.u[e / 2 % 8] & 0xFFFF0000u) | b;
         }
     }
 }
@@ -377,7 +414,7 @@ __device__ __forceinline__ void sector_penalise(const LogitsArgs &a, Sector &s, 
  * any of it (a long history touches most of the low ids' lines, and single
  * logits cost memory what whole lines cost). */
 template <typename T>
-__global__ void __launch_bounds__(kSliceThreads) logits_slice_kernel(const __grid_constant__ LogitsArgs a) {
+__global__ void __launch_bounds__(kSliceThreads, 2) logits_slice_kernel(const __grid_constant__ LogitsArgs a) {
     extern __shared__ __align__(16) uint32_t logits_smem[];
     uint32_t *word = logits_smem;
     const int tid = threadIdx.x;
@@ -389,8 +426,7 @@ __global__ void __launch_bounds__(kSliceThreads) logits_slice_kernel(const __gri
     const RowHistory h = row_history(a, row);
     const RowRules rules = row_rules(a, row);
     const uint32_t *mask = row_mask(a, row);
-    for (int i = tid; i < (width + 3) / 4; i += kSliceThreads)
-        reinterpret_cast<uint4 *>(word)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < width / 4; i += kSliceThreads) reinterpret_cast<uint4 *>(word)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     /* an id's column if it is one of the slice's, as its index in the slice */
     auto index_of = [&](int id, uint32_t &c) {
@@ -445,30 +481,43 @@ __global__ void __launch_bounds__(kSliceThreads) logits_slice_kernel(const __gri
      * is read and written whole; rows that do not start on 32 bytes, and the
      * row's last line, go by element */
     const bool lines = (reinterpret_cast<uintptr_t>(x) & 31) == 0;
-    for (int s0 = tid; s0 * VE < width; s0 += kSliceThreads) {  // width / VE is a multiple of 32: whole warps
-        uint32_t w[VE];
-        uint32_t any = 0u;
+    constexpr int BATCH = 1;  // sectors of a lane that are on their way at a time
+    for (int s0 = tid; s0 * VE < width; s0 += BATCH * kSliceThreads) {  // width / VE is a multiple of 32: whole warps
+        Sector s[BATCH];
+        uint32_t w[BATCH][VE], change[BATCH];
+        int col[BATCH];
+        bool whole[BATCH];
 #pragma unroll
-        for (int e = 0; e < VE; e += 4) {
-            const uint4 q = *reinterpret_cast<const uint4 *>(word + s0 * VE + e);
-            w[e] = q.x;
-            w[e + 1] = q.y;
-            w[e + 2] = q.z;
-            w[e + 3] = q.w;
-            any |= q.x | q.y | q.z | q.w;
-        }
-        const int c = ((((s0 * VE) / BLK) << sh) + (int)mine_c) * BLK + (s0 * VE) % BLK;
-        const uint32_t touched = __ballot_sync(kFull, any != 0u);
-        if (!(touched >> (tid & 28) & 15u)) continue;
-        if (lines && (int64_t)(c - c % BLK) + BLK <= a.vocab) {
-            Sector s = sector_load(x + c);
-            if (any) sector_penalise<T>(a, s, w, rules, mask, c);
-            sector_store(x + c, s);
-        } else if (any) {
+        for (int b = 0; b < BATCH; ++b) {
+            const int at = (s0 + b * kSliceThreads) * VE;
+            change[b] = 0u;
+            whole[b] = false;
+            if (at >= width) continue;
+#pragma unroll
+            for (int e = 0; e < VE; e += 4) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(word + at + e);
+                w[b][e] = q.x, w[b][e + 1] = q.y, w[b][e + 2] = q.z, w[b][e + 3] = q.w;
+            }
 #pragma unroll
             for (int e = 0; e < VE; ++e)
-                if (w[e] && !(w[e] & kHasBias) && allowed(mask, a.v_begin + c + e))
-                    logit_store(x + c + e, penalised(logit_load(x + c + e), w[e], rules));
+                if (w[b][e] && !(w[b][e] & kHasBias)) change[b] |= 1u << e;
+            const int c = col[b] = ((at / BLK << sh) + (int)mine_c) * BLK + at % BLK;
+            if (mask && change[b]) change[b] &= mask_bits(a, mask, c);
+            const uint32_t touched = __ballot_sync(kFull, change[b] != 0u);
+            whole[b] = (touched >> (tid & 28) & 15u) && lines && (int64_t)(c - c % BLK) + BLK <= a.vocab;
+            if (whole[b]) s[b] = sector_load(x + c);
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            T *p = x + col[b];
+            if (whole[b]) {
+                if (change[b]) sector_penalise<T>(s[b], w[b], change[b], rules);
+                sector_store(p, s[b]);
+            } else if (change[b]) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                    if (change[b] >> e & 1u) logit_store(p + e, penalised(logit_load(p + e), w[b][e], rules));
+            }
         }
     }
     if (nb) __syncthreads();  // the lines are written; biased logits were written as they were read

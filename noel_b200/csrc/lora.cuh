@@ -596,6 +596,9 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_any_kernel(const _
 }
 
 __device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+__device__ __forceinline__ void cp_async4_at(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 /* bytes (at most 16) of src and zeros up to 16 */
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -605,8 +608,8 @@ __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src, uin
  * rows (64 bytes more after every eight where a row is 32 bytes), then a line
  * of y for each of 16 tokens. */
 __host__ __device__ constexpr int expand_row_bytes(int rank_pad, int es) { return rank_pad * es; }
-__host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es, bool wide) {
-    return 32 * rank_pad * es + (rank_pad * es == 32 ? 256 : 0) + (wide ? kLoraItem * 128 : 0);
+__host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es) {
+    return 32 * rank_pad * es + (rank_pad * es == 32 ? 256 : 0) + kLoraItem * 128;
 }
 
 /* The second kernel: one item per blockIdx.y.  Every warp has D stages of
@@ -620,7 +623,8 @@ __host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es, bool 
  * N is the number of ranks a lane holds: 4 for ranks up to 16, else 8 (a group
  * of 32 ranks at a time).  G groups of low-rank numbers stay in registers
  * (0: they are read again for every turn).  Without WIDE, rows of y start
- * anywhere: y is not staged but read and written by element. */
+ * anywhere: their 32 numbers are copied 4 bytes at a time, and go back through
+ * the stage so that a store writes a token's 32 numbers side by side. */
 template <int WT, int N, int G, int D, bool WIDE>
 __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
     extern __shared__ __align__(128) unsigned char lora_smem[];
@@ -634,7 +638,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
     }
     const ExpandLane<WT> l(a, it, N);
     const int rank_pad = G ? 4 * N * G : a.rank_pad;  // known to the compiler but for the largest ranks
-    const int row_bytes = expand_row_bytes(rank_pad, ES), stage_bytes = expand_stage_bytes(rank_pad, ES, WIDE);
+    const int row_bytes = expand_row_bytes(rank_pad, ES), stage_bytes = expand_stage_bytes(rank_pad, ES);
     const int pad8 = row_bytes == 32 ? 64 : 0, y_at = 32 * row_bytes + 4 * pad8;
     const int swap = ES == 2 ? (row_bytes % 128 == 0 ? 4 : 0) : (N == 8 ? 1 : 0);  // of odd rows' pieces
     unsigned char *mem = lora_smem + warp * D * stage_bytes;
@@ -657,6 +661,16 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
         const int t = tk < 8 ? ta : tb;
         y_from[p] = a.y + (size_t)max(t, 0) * (size_t)a.ldy + first + 4 * (lane & 7);
     }
+    /* without WIDE: the lane's number of the tokens' lines, their rows' places in y, and where number `lane` of
+     * token k lies in a stage */
+    const float *y_lane = a.y + first + lane;
+    __shared__ int64_t y_off[WIDE ? 1 : WARPS][kLoraItem];
+    auto line_of = [&](int k) { return y_at + k * 128 + (((lane >> 2) ^ (k & 1)) << 4) + ((lane & 3) << 2); };
+    if (!WIDE) {
+        const int ta = __shfl_sync(kFull, it.t0, 4 * (lane & 7)), tb = __shfl_sync(kFull, it.t1, 4 * (lane & 7));
+        if (lane < kLoraItem) y_off[warp][lane] = (int64_t)max(lane < 8 ? ta : tb, 0) * a.ldy;
+        __syncwarp();
+    }
     const uint32_t y_to = y_at + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3 & 1)) << 4);
     const int turns = (int)((a.rows - ROWS - first + step) / step);  // whole ones
     int ahead = 0;  // the next turn to bring
@@ -674,6 +688,11 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
                 const char *src = b_from;
 #pragma unroll
                 for (int r = 0; r < share; ++r, src += b_round) cp_async16_at(to + b_to + r * b_to_round, src, c_bytes);
+            }
+            if (!WIDE) {
+                for (int k = 0; k < it.m; ++k)
+                    cp_async4_at(to + line_of(k), y_lane + y_off[warp][k]);
+                y_lane += step;
             }
 #pragma unroll
             for (int p = 0; p < kLoraItem / 4; ++p) {
@@ -701,17 +720,17 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
     }
     /* where this lane's row of instruction 0 lies in a stage and what instruction j adds, its piece there, and its
      * lines of y */
-    const int w_at = WIDE ? (8 * (g >> 1) + (g & 1)) * row_bytes + (g >> 1) * pad8 : g * row_bytes;
-    const int w_next = WIDE ? 2 * row_bytes : 8 * row_bytes + pad8, w_swap = g & 1 ? swap : 0;
+    const int w_at = (8 * (g >> 1) + (g & 1)) * row_bytes + (g >> 1) * pad8, w_next = 2 * row_bytes;
+    const int w_swap = g & 1 ? swap : 0;
     const int line0 = y_at + g * 128 + ((2 * q ^ (g & 1)) << 4), line1 = y_at + g * 128 + ((2 * q + 1 ^ (g & 1)) << 4);
-    float *y0 = l.y0 + first + (WIDE ? 8 : 2) * q, *y1 = l.y1 + first + (WIDE ? 8 : 2) * q;
+    float *y0 = l.y0 + first + 8 * q, *y1 = l.y1 + first + 8 * q, *y_back = a.y + first + lane;
     const bool both = it.m > 8, line = a.vec_y == 2;
     int st = 0;
-    for (int turn = 0; turn < turns; ++turn, y0 += step, y1 += step, st = st + 1 == D ? 0 : st + 1) {
+    for (int turn = 0; turn < turns; ++turn, y0 += step, y1 += step, y_back += step, st = st + 1 == D ? 0 : st + 1) {
         cp_async_wait<D - 2>();
         __syncwarp();  // stage st has landed for every lane, and no lane still reads the one before it
         issue(st == 0 ? D - 1 : st - 1);
-        const unsigned char *from = mem + st * stage_bytes;
+        unsigned char *from = mem + st * stage_bytes;
         float c[4][4];
         auto group = [&](int k, bool from_zero, const uint32_t (&u0)[3][N / 2], const uint32_t (&u1)[3][N / 2]) {
             const int r = k * 4 * N + N * q;
@@ -734,14 +753,6 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
             }
         };
         if (l.n == 0) continue;
-        float e0[8], e1[8];
-        if (!WIDE) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (it.t0 >= 0) e0[e] = y0[8 * (e / 2) + (e & 1)];
-                if (both && it.t1 >= 0) e1[e] = y1[8 * (e / 2) + (e & 1)];
-            }
-        }
         if (G) {
             group(0, true, x0[0], x1[0]);
             if (GR > 1 && 4 * N < l.n) group(1, false, x0[GR - 1], x1[GR - 1]);
@@ -754,24 +765,29 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
             }
         }
         auto add = [&](int h, float *y) {
-            const float4 o = *reinterpret_cast<const float4 *>(from + line0 + 1024 * h);
-            const float4 p = *reinterpret_cast<const float4 *>(from + line1 + 1024 * h);
+            float4 *at0 = reinterpret_cast<float4 *>(from + line0 + 1024 * h);
+            float4 *at1 = reinterpret_cast<float4 *>(from + line1 + 1024 * h);
+            const float4 o = *at0, p = *at1;
             const float f[8] = {o.x, o.y, o.z, o.w, p.x, p.y, p.z, p.w};
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(f[e], c[e / 2][2 * h + (e & 1)]);
+            if (!WIDE) {
+                *at0 = make_float4(v[0], v[1], v[2], v[3]);
+                *at1 = make_float4(v[4], v[5], v[6], v[7]);
+                return;
+            }
             Sector s;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s.u[e] = __float_as_uint(__fadd_rn(f[e], c[e / 2][2 * h + (e & 1)]));
+            for (int e = 0; e < 8; ++e) s.u[e] = __float_as_uint(v[e]);
             if (line) sector_store(y, s);
             else sector_store16(y, s);
         };
-        if (WIDE) {
-            if (it.t0 >= 0) add(0, y0);
-            if (both && it.t1 >= 0) add(1, y1);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (it.t0 >= 0) y0[8 * (e / 2) + (e & 1)] = __fadd_rn(e0[e], c[e / 2][e & 1]);
-                if (both && it.t1 >= 0) y1[8 * (e / 2) + (e & 1)] = __fadd_rn(e1[e], c[e / 2][2 + (e & 1)]);
-            }
+        if (it.t0 >= 0) add(0, y0);
+        if (both && it.t1 >= 0) add(1, y1);
+        if (!WIDE) {
+            __syncwarp();
+            for (int k = 0; k < it.m; ++k) y_back[y_off[warp][k]] = *reinterpret_cast<const float *>(from + line_of(k));
         }
     }
     if (first + turns * step < a.rows) expand_any<WT, N>(a, l, first + turns * step);  // the last rows

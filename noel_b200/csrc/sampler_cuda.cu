@@ -1060,6 +1060,7 @@ int logits_args(const noel_logits_params_t *p, void *logits, int dtype, int B, i
         want = want < turn ? turn : want;
         a.range = (int)(want < most ? want : most);
         a.ranges = (int)(((int64_t)V + 15 + a.range - 1) / a.range);
+        a.together = a.range < most;
     } else if (a.cap) {
         a.range = 0x7FFFFFFF;  // the row whole
         a.ranges = 1;
@@ -1233,7 +1234,7 @@ dim3 expand_grid(DeviceCtx *c, const LoraArgs &a, int items, int per_sm) {
 
 template <int WT, int N, int G, int D, bool WIDE>
 int expand_launch_y(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
-    const size_t smem = (size_t)(kExpandThreads / 32) * D * expand_stage_bytes(a.rank_pad, kWeightBytes<WT>, WIDE);
+    const size_t smem = (size_t)(kExpandThreads / 32) * D * expand_stage_bytes(a.rank_pad, kWeightBytes<WT>);
     const int r = set_smem(c, (const void *)lora_expand_kernel<WT, N, G, D, WIDE>, smem);
     if (r) return r;
     CUDA_TRY((launch_cluster(lora_expand_kernel<WT, N, G, D, WIDE>, expand_grid(c, a, items, smem <= 112 * 1024 ? 2 : 1),
