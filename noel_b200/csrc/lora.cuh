@@ -61,7 +61,7 @@ struct LoraArgs {
     uint16_t *low;   // [batch][3][rank_pad] bf16 parts of scale A x
     int rank_pad;    // 16, or the rank rounded up to 32
     LoraPlan *plan;  // NULL: every warp finds the items
-    int staged;                      // the second kernel's stages can be filled 16 bytes at a time
+    int staged;                      // bytes at a time that fill the second kernel's stages: 16, 4, or 0: not staged
     int vec_x, vec_a, vec_b, vec_y;  // rows start on 16 bytes (B with rank_pad 16: on 4 elements; y: 2 for 32 bytes)
 };
 
@@ -596,10 +596,10 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_any_kernel(const _
 }
 
 __device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-__device__ __forceinline__ void cp_async4_at(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+/* bytes of src and zeros up to 4 or 16 */
+__device__ __forceinline__ void cp_async4_at(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-/* bytes (at most 16) of src and zeros up to 16 */
 __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -622,9 +622,11 @@ __host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es) {
  *
  * N is the number of ranks a lane holds: 4 for ranks up to 16, else 8 (a group
  * of 32 ranks at a time).  G groups of low-rank numbers stay in registers
- * (0: they are read again for every turn).  Without WIDE, rows of y start
- * anywhere: their 32 numbers are copied 4 bytes at a time, and go back through
- * the stage so that a store writes a token's 32 numbers side by side. */
+ * (0: they are read again for every turn).  WIDE: rows of y and of B_i start on
+ * 16 bytes.  Without it rows of y start anywhere: their 32 numbers are copied
+ * 4 bytes at a time, and go back through the stage so that a store writes a
+ * token's 32 numbers side by side; and so are rows of B_i that do not start on
+ * 16 bytes but on 4. */
 template <int WT, int N, int G, int D, bool WIDE>
 __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
     extern __shared__ __align__(128) unsigned char lora_smem[];
@@ -649,6 +651,8 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
     const bool c_on = c_piece * 16 < row_bytes;
     const uint32_t c_bytes = (uint32_t)min(max(l.n * ES - c_piece * 16, 0), 16);
     const char *b_from = l.b + (size_t)(first + c_row) * l.pitch + (c_bytes ? c_piece << 4 : 0);
+    constexpr int W4 = G ? 4 * N * G * ES / 4 : 1;
+    const char *b_from4 = l.b + (size_t)(first + lane / W4) * l.pitch + (4 * (lane % W4) < l.n * ES ? 4 * (lane % W4) : 0);
     const size_t b_round = (size_t)c_rows * l.pitch, b_step = (size_t)step * l.pitch;
     const uint32_t mem_s = (uint32_t)__cvta_generic_to_shared(mem);
     const uint32_t b_to = c_row * row_bytes + (c_row >> 3) * pad8 + ((c_piece ^ (c_row & 1 ? swap : 0)) << 4);
@@ -684,14 +688,23 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
     auto issue = [&](int stage) {
         if (ahead < turns) {
             const uint32_t to = mem_s + stage * stage_bytes;
-            if (c_on) {
+            if (!WIDE && G && a.staged == 4) {  // rows of B_i that start on 4 bytes only
+                constexpr int PER = W4 < 32 ? 32 / W4 : 1;  // rows a round
+                const int word = lane % W4;
+                const char *src = b_from4;
+                const uint32_t bytes = (uint32_t)min(max(l.n * ES - 4 * word, 0), 4);
+                for (int r = lane / W4; r < ROWS; r += PER, src += PER * l.pitch)
+                    cp_async4_at(to + r * row_bytes + (r >> 3) * pad8 + ((word >> 2 ^ (r & 1 ? swap : 0)) << 4) + (word & 3) * 4,
+                                 src, bytes);
+                b_from4 += b_step;
+            } else if (c_on) {
                 const char *src = b_from;
 #pragma unroll
                 for (int r = 0; r < share; ++r, src += b_round) cp_async16_at(to + b_to + r * b_to_round, src, c_bytes);
             }
             if (!WIDE) {
                 for (int k = 0; k < it.m; ++k)
-                    cp_async4_at(to + line_of(k), y_lane + y_off[warp][k]);
+                    cp_async4_at(to + line_of(k), y_lane + y_off[warp][k], 4u);
                 y_lane += step;
             }
 #pragma unroll

@@ -1180,8 +1180,10 @@ int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size
     a.vec_y = rows_on(y, ldy * 4, 0, 32) ? 2 : rows_on(y, ldy * 4, 0, 16) ? 1 : 0;
     a.vec_a = rows_on(l->d_a, l->lda * es, l->stride_a * es, 16);
     a.vec_b = rows_on(l->d_b, l->ldb * es, l->stride_b * es, lane_b);
-    a.staged = rows_on(l->d_b, l->ldb * es, l->stride_b * es, 16) && (size_t)l->rank * es % 16 == 0 &&
-               a.rank_pad * es <= 256;
+    a.staged = a.rank_pad * es > 256 ? 0
+               : rows_on(l->d_b, l->ldb * es, l->stride_b * es, 16) && (size_t)l->rank * es % 16 == 0 ? 16
+               : rows_on(l->d_b, l->ldb * es, l->stride_b * es, 4) && (a.rank_pad <= 32 || (a.rank_pad == 64 && es == 2)) ? 4
+                                                                                                                        : 0;
     *out = a;
     return NOEL_OK;
 }
@@ -1243,7 +1245,8 @@ int expand_launch_y(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) 
 }
 template <int WT, int N, int G, int D>
 int expand_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
-    return a.vec_y ? expand_launch_y<WT, N, G, D, true>(c, a, items, s) : expand_launch_y<WT, N, G, D, false>(c, a, items, s);
+    return a.vec_y && a.staged == 16 ? expand_launch_y<WT, N, G, D, true>(c, a, items, s)
+                                     : expand_launch_y<WT, N, G, D, false>(c, a, items, s);
 }
 
 template <int WT, int N>
@@ -1252,8 +1255,9 @@ int expand_any_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s
     return NOEL_OK;
 }
 
-/* The second kernel: through shared memory where rows of B start on 16 bytes
- * and end there, and two stages of a warp fit (ranks up to 128, fp32 64). */
+/* The second kernel: through shared memory where two stages of a warp fit
+ * (ranks up to 128, fp32 64) and rows of B start on 16 bytes and end there, or
+ * start on 4 bytes (ranks up to 64, fp32 32). */
 template <int WT>
 int expand(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
     constexpr bool kF32 = WT == kHeadF32;
