@@ -43,8 +43,10 @@ size_t noel_lora_workspace_bytes(int batch, int rank);
  * d_y[t] += scale[i] * B_i (A_i d_x[t]), i = d_adapter[t], for t < batch:
  * d_x [batch][ldx] (cols used) and d_y [batch][ldy] (rows used) fp32, 4-byte
  * aligned.  A token whose d_adapter is outside 0 .. n_adapters - 1 has no
- * adapter and its row of d_y is left as it was.  Sums are in fp32; a token's
- * result does not depend on which other tokens are in the batch.  d_work
+ * adapter and its row of d_y is left as it was.  Sums are in fp32 (every product
+ * of fp16 and bf16 weights enters them exactly, of fp32 weights to 2^-30); a
+ * token's result does not depend on which other tokens are in the batch.  Where
+ * a sum in fp32 is infinite or NaN the result is one of the two.  d_work
  * (16-byte aligned, work_bytes >= noel_lora_workspace_bytes(batch, rank)) is
  * scratch of this call until it has run.  Returns NOEL_OK or a negative
  * status (noel_sampler_cuda_last_error_message() says why).  Asynchronous on

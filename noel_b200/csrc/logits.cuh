@@ -11,15 +11,21 @@
  * Nothing here reads the row as a whole.  A row's history and bias list name
  * the few logits that the penalties and biases change, and a mask only writes;
  * what has to move is the history, the mask's bits, the touched logits and the
- * masked ones.  The two halves of the work touch different logits (a mask
- * wins, so the penalties leave masked ids alone, and the mask writes nothing
- * else): they need no order between them and run as CTAs of one launch.
+ * masked ones.  What bounds it is memory's rate for single sectors: 200,000
+ * touched logits (256 rows, histories of 1024 ids, 300 biases) take 16 us and
+ * as many random 4-byte reads and writes of a bare loop 17 us, at a fiftieth
+ * of the bandwidth; strict masks write whole rows at 6.2 TB/s.
+ *
+ * Measured on 1024 x 152,064 fp32 under masks that allow 0.5 % of the ids:
+ * 119 us for 582 MB (a bare fill of the rows takes 88 us); 1024 x 256,000 bf16
+ * under masks that allow 98 %: 110 us; 64 rows with histories of 65,536 ids:
+ * 52 us; one row: 5 us.
  */
 #pragma once
 
 #include "sampler_kernels.cuh"
-#include "sector.cuh"
 #include "sampler_warp.cuh"
+#include "sector.cuh"
 
 #include <cuda_bf16.h>
 
@@ -42,9 +48,9 @@ struct LogitsArgs {
     int64_t mld;
     int mask_rows;
     const int32_t *mask_row;
-    int ranges, range;  // CTAs per row and their columns; 0: no such launch
+    int ranges, range;  // CTAs per row of the rows kernel and their columns
     int cap;            // entries of a CTA's table; 0: none
-    bool together;      // all warps of a masked row's CTA fill the table
+    bool write_mask;    // the rows kernel writes the masked logits
     int slices, slice;  // CTAs per row of the slice kernel and the words each counts in
 };
 
@@ -53,8 +59,10 @@ constexpr int kRowsCtas = 6;         // CTAs per SM the rows kernel is compiled 
 constexpr int kLogitsSms = 148;
 constexpr int kMaskPiece = 1024;     // columns of a warp's turn: 32 words of the mask
 constexpr int kMaskRange = 131072;   // bytes of a row that a CTA masks, at most
-constexpr int kTableMax = 2048;      // history plus biases a row's table may take
-constexpr int kTableBatch = 8;       // loads in flight per thread of the table half
+constexpr int kMaskWhole = 22;       // touched sectors of 32 from which on they are written whole
+constexpr int kTableMax = 8192;      // history plus biases a row's table may take
+constexpr int kTableMaskMax = 2048;  // and where the same CTA masks
+constexpr int kTableBatch = 8;       // loads in flight per thread of the table
 constexpr int kSliceThreads = 512;
 constexpr int kSliceMax = 24576;     // columns of a slice: one 32-bit word of shared memory each
 constexpr int kLogitsMaxBias = 16384;
@@ -161,19 +169,17 @@ __device__ __forceinline__ uint32_t table_slot(const Table &t, uint32_t k) {
 /* The row's history and bias ids of columns [lo, hi) into the table.  Loads go
  * out kTableBatch at a time: with few CTAs per SM the time of this is the
  * number of load latencies in a row. */
-template <int N>  // by the CTA's first N threads
 __device__ __forceinline__ void table_fill(const LogitsArgs &a, int row, const Table &t, int lo, int hi) {
     const int tid = threadIdx.x;
     const RowHistory h = row_history(a, row);
-    for (int i = tid; i < t.cap / 2; i += N)  // keys and words
+    for (int i = tid; i < t.cap / 2; i += kLogitsThreads)  // keys and words
         reinterpret_cast<uint4 *>(t.key)[i] = make_uint4(0, 0, 0, 0);
-    if (N == 32) __syncwarp();
-    else __syncthreads();
-    for (int i0 = tid; i0 < h.len; i0 += kTableBatch * N) {
+    __syncthreads();
+    for (int i0 = tid; i0 < h.len; i0 += kTableBatch * kLogitsThreads) {
         int id[kTableBatch];
 #pragma unroll
         for (int u = 0; u < kTableBatch; ++u) {
-            const int i = i0 + u * N;
+            const int i = i0 + u * kLogitsThreads;
             id[u] = i < h.len ? h.ids[i] : -1;
         }
 #pragma unroll
@@ -181,19 +187,19 @@ __device__ __forceinline__ void table_fill(const LogitsArgs &a, int row, const T
             const int64_t c = (int64_t)id[u] - a.v_begin;
             if (id[u] < 0 || c < lo || c >= hi) continue;
             const uint32_t p = table_slot(t, (uint32_t)c + 1u);
-            if (i0 + u * N < h.prompt) atomicOr(&t.word[p], kSeenPrompt);
+            if (i0 + u * kLogitsThreads < h.prompt) atomicOr(&t.word[p], kSeenPrompt);
             else atomicAdd(&t.word[p], 1u);
         }
     }
     const int nb = a.bias_len;
     const int32_t *bi = nb ? a.bias_ids + (size_t)row * (size_t)a.bld : nullptr;
     const float *bv = nb ? a.bias + (size_t)row * (size_t)a.bld : nullptr;
-    for (int i0 = tid; i0 < nb; i0 += 2 * N) {
+    for (int i0 = tid; i0 < nb; i0 += 2 * kLogitsThreads) {
         int id[2];
         float v[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int i = i0 + u * N;
+            const int i = i0 + u * kLogitsThreads;
             id[u] = i < nb ? bi[i] : -1;
             v[u] = i < nb ? bv[i] : 0.0f;
         }
@@ -276,13 +282,14 @@ __device__ __forceinline__ uint32_t mask_bits(const LogitsArgs &a, const uint32_
 /* One warp masks the 1024 columns from c0 on, whose mask bits lane l holds 32
  * at a time; c0 lies on 32 bytes of memory and may lie before the row.
  *
- * Memory takes 1024 bytes of a warp's store fastest when none of them has to
- * be filled in from what is there already: 584 MB of masked logits take 90 us
- * where rows are masked throughout, but a single allowed logit left out of a
- * line costs that line's read besides.  So where at least half of the warp's
- * 32-byte sectors have something masked, the others and the partly masked
- * ones are read and all of it is written in one store; where fewer have, the
- * masked logits are written one by one. */
+ * A line of which some bytes are written and others left costs its read as
+ * well, when the L2 gets to it.  So where kMaskWhole of the warp's 32 sectors
+ * have something masked, the others and the partly masked ones are read and
+ * all 1024 bytes are written in one store; where fewer have, the masked logits
+ * are written one by one.  Measured on 512 x 152,064 under masks that allow
+ * 50, 90, 95 and 98 % of the ids (fp32: 100, 57, 34, 15 % of the sectors
+ * touched; bf16: 100, 81, 56, 28 %): always whole 99, 99, 99, 99 us (bf16 55,
+ * 55, 55, 55), always one by one 232, 79, 57, 43 (bf16 235, 74, 45, 31). */
 template <typename T>
 __device__ __forceinline__ void mask_piece(const LogitsArgs &a, T *x, int64_t c0, uint32_t ok) {
     constexpr int VE = 32 / sizeof(T);  // elements a lane takes at a time
@@ -304,7 +311,7 @@ __device__ __forceinline__ void mask_piece(const LogitsArgs &a, T *x, int64_t c0
             const int q = q0 + j;
             const uint32_t w = __shfl_sync(kFull, ok, q * VE + lane * VE / 32);
             gone[j] = ~(w >> (lane * VE % 32)) & ALL;
-            whole[j] = __popc(__ballot_sync(kFull, gone[j] != 0u)) >= 16 && q >= first && q < last;
+            whole[j] = __popc(__ballot_sync(kFull, gone[j] != 0u)) >= kMaskWhole && q >= first && q < last;
             if (whole[j] && gone[j] != ALL) s[j] = sector_load(at + q * 32 * VE);
         }
 #pragma unroll
@@ -324,10 +331,8 @@ __device__ __forceinline__ void mask_piece(const LogitsArgs &a, T *x, int64_t c0
  * the range is masked, and then the table's logits are changed.  The mask
  * never changes an allowed logit's value but may write it back as it read it,
  * so the table's own writes come after the mask's, a CTA's barrier between
- * them.  In a masked row of a large batch one warp fills the table while the
- * others mask, and takes its turns at the mask when it has done that; where
- * the CTAs all run at once, their time is that of the longest warp, and all
- * warps fill it first. */
+ * them.  (One warp filling the table while the others mask was slower in small
+ * batches, 27 against 18 us at 64 rows, and no faster in large ones.) */
 template <typename T>
 __global__ void __launch_bounds__(kLogitsThreads, kRowsCtas) logits_rows_kernel(const __grid_constant__ LogitsArgs a) {
     extern __shared__ __align__(16) uint32_t logits_smem[];
@@ -341,13 +346,12 @@ __global__ void __launch_bounds__(kLogitsThreads, kRowsCtas) logits_rows_kernel(
     const int64_t end = min(begin + a.range, (int64_t)a.vocab);
     const Table t{logits_smem, logits_smem + a.cap, reinterpret_cast<float *>(logits_smem + 2 * a.cap), a.cap};
     const int lo = (int)max(begin, (int64_t)0), hi = (int)max(end, (int64_t)lo);
-    if (mask) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        if (threadIdx.x == 0) turn = kLogitsThreads / 32;  // every warp's first turn is its own number
-        __syncthreads();
-        if (a.cap && a.together) table_fill<kLogitsThreads>(a, row, t, lo, hi);
-        else if (a.cap && warp == 0) table_fill<32>(a, row, t, lo, hi);
-        int k = warp;
+    if (threadIdx.x == 0) turn = kLogitsThreads / 32;  // every warp's first turn is its own number
+    if (a.cap) table_fill(a, row, t, lo, hi);
+    if (mask && a.write_mask) {
+        const int lane = threadIdx.x & 31;
+        if (!a.cap) __syncthreads();
+        int k = threadIdx.x >> 5;
         uint32_t next = mask_bits(a, mask, begin + (int64_t)k * kMaskPiece + 32 * lane);
         while (begin + (int64_t)k * kMaskPiece < end) {
             const uint32_t ok = next;
@@ -357,8 +361,6 @@ __global__ void __launch_bounds__(kLogitsThreads, kRowsCtas) logits_rows_kernel(
             next = mask_bits(a, mask, begin + (int64_t)k * kMaskPiece + 32 * lane);  // on its way meanwhile
             mask_piece(a, x, c, ok);
         }
-    } else if (a.cap) {
-        table_fill<kLogitsThreads>(a, row, t, lo, hi);
     }
     if (a.cap) {
         __syncthreads();

@@ -36,7 +36,7 @@ constexpr int kShrinkThreads = 256;
 constexpr int kShrinkSplit = 8;     // CTAs of a cluster that share an item's columns, at most
 constexpr int kExpandThreads = 256;
 constexpr int kExpandFetch = 1;    // turns between asking the L2 for a line of y and copying it
-constexpr int kExpandWaves = 4;     // turns of the GPU's CTAs that the second kernel's work is cut into
+constexpr int kExpandWaves = 4;         // turns of the GPU's CTAs that the second kernel's work is cut into
 
 /* the items of a batch above kLoraWarpBatch, in the scratch */
 struct LoraPlan {

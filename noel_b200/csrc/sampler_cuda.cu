@@ -1047,10 +1047,22 @@ int logits_args(const noel_logits_params_t *p, void *logits, int dtype, int B, i
     a.mld = (int64_t)p->mld;
     a.mask_rows = p->mask_rows;
     a.mask_row = p->d_mask_rows;
-    /* a row's history and biases in a table where they fit one, else counted
-     * over slices of its columns; the mask by ranges of the row */
+    /* A row's history and biases go into a table, or are counted over slices of its columns: the table up to
+     * kTableMax of them, but for a batch whose slices run all at once from 1024 on (16 rows of 152,064 with 1024,
+     * 2048, 4096 and 8192 ids: table 7.6, 11.4, 17.2, 33.1 us, slices 7.7, 8.4, 8.9, 10.2; 256 rows: table 9.6, 15.4,
+     * 27.2, 73.8, slices 56, 64, 78, 96). */
     const int n = a.hist_len + a.bias_len;
-    if (n > 0 && n <= kTableMax) a.cap = pow2_at_least(n + n / 2 > kLogitsThreads ? n + n / 2 : kLogitsThreads);
+    const int slices = pow2_at_least((int)(((int64_t)V + kSliceMax - 1) / kSliceMax));
+    const bool at_once = (int64_t)B * slices <= 2 * kLogitsSms;
+    if (n > 0 && n <= (at_once ? 1024 : kTableMax)) {
+        a.cap = pow2_at_least(n + n / 2 > kLogitsThreads ? n + n / 2 : kLogitsThreads);
+    } else if (n > 0) {
+        a.slices = slices;
+        const int64_t line = 64 * (int64_t)a.slices;  // 128 bytes of bf16 from every slice
+        a.slice = (int)((V + line - 1) / line * 64 + 511) / 512 * 512;  // and whole warps of sectors of either type
+    }
+    a.ranges = 1;
+    a.range = 0x7FFFFFFF;  // the row whole
     if (a.mask) {
         /* ranges that give each of the GPU's CTA slots two, in whole turns of a CTA's warps: a large batch
          * runs fastest at 128 KB (1024 x 152,064 fp32 under strict masks: 145, 125, 120 and 121 us at 32, 64,
@@ -1060,34 +1072,43 @@ int logits_args(const noel_logits_params_t *p, void *logits, int dtype, int B, i
         want = want < turn ? turn : want;
         a.range = (int)(want < most ? want : most);
         a.ranges = (int)(((int64_t)V + 15 + a.range - 1) / a.range);
-        a.together = a.range < most;
-    } else if (a.cap) {
-        a.range = 0x7FFFFFFF;  // the row whole
-        a.ranges = 1;
+        a.write_mask = true;
     }
-    if (n > kTableMax) {
-        a.slices = pow2_at_least((V + kSliceMax - 1) / kSliceMax);
-        const int line = 64 * a.slices;  // 128 bytes of bf16 from every slice
-        a.slice = (V + line - 1) / line * 64;
-        a.slice = (a.slice + 511) / 512 * 512;  // whole warps of sectors of either type
-    }
-    if (B > 1 << 30 || (int64_t)B * a.slices > 0x7FFFFFFF || (int64_t)B * a.ranges > 0x7FFFFFFF) return fail(NOEL_ERR_TOO_LARGE, "%d rows x %d columns", B, V);
+    if (B > 1 << 30 || (int64_t)B * a.slices > 0x7FFFFFFF || (int64_t)B * a.ranges > 0x7FFFFFFF)
+        return fail(NOEL_ERR_TOO_LARGE, "%d rows x %d columns", B, V);
     *out = a;
     return NOEL_OK;
 }
 
 template <typename T>
+int logits_rows_launch(DeviceCtx *c, const LogitsArgs &a, cudaStream_t s) {
+    const size_t smem = (size_t)a.cap * 12;
+    const int r = set_smem(c, (const void *)logits_rows_kernel<T>, smem);
+    if (r) return r;
+    logits_rows_kernel<T><<<a.batch * a.ranges, kLogitsThreads, smem, s>>>(a);
+    CUDA_TRY(cudaGetLastError());
+    return NOEL_OK;
+}
+
+template <typename T>
 int logits_launch_t(DeviceCtx *c, const LogitsArgs &a, cudaStream_t s) {
-    if (a.ranges) {
-        const size_t smem = (size_t)a.cap * 12;
-        const int r = set_smem(c, (const void *)logits_rows_kernel<T>, smem);
-        if (r) return r;
-        logits_rows_kernel<T><<<a.batch * a.ranges, kLogitsThreads, smem, s>>>(a);
-        CUDA_TRY(cudaGetLastError());
+    int r = NOEL_OK;
+    if (a.mask && a.cap && a.hist_len + a.bias_len > kTableMaskMax) {
+        /* a table of this size in every range's CTA would leave too few CTAs to mask */
+        LogitsArgs m = a, t = a;
+        m.cap = 0;
+        t.write_mask = false;
+        t.ranges = 1;
+        t.range = 0x7FFFFFFF;
+        r = logits_rows_launch<T>(c, m, s);
+        if (!r) r = logits_rows_launch<T>(c, t, s);
+    } else if (a.mask || a.cap) {
+        r = logits_rows_launch<T>(c, a, s);
     }
+    if (r) return r;
     if (a.slices) {
         const size_t smem = (size_t)a.slice * 4;
-        const int r = set_smem(c, (const void *)logits_slice_kernel<T>, smem);
+        r = set_smem(c, (const void *)logits_slice_kernel<T>, smem);
         if (r) return r;
         logits_slice_kernel<T><<<a.batch * a.slices, kSliceThreads, smem, s>>>(a);
         CUDA_TRY(cudaGetLastError());
@@ -1102,7 +1123,7 @@ int logits_launch(DeviceCtx *c, const LogitsArgs &a, int dtype, cudaStream_t s) 
 }  // namespace
 
 extern "C" int noel_logits_process(const noel_logits_params_t *params, void *d_logits, int dtype, int batch, int vocab,
-                                   size_t ld, void *stream) {
+                                   size_t ld, void *stream) try {
     LogitsArgs a{};
     int r = logits_args(params, d_logits, dtype, batch, vocab, ld, &a);
     if (r) return r;
@@ -1112,6 +1133,8 @@ extern "C" int noel_logits_process(const noel_logits_params_t *params, void *d_l
     if (r) return r;
     r = logits_launch(c, a, dtype, static_cast<cudaStream_t>(stream));
     return r ? r : ok();
+} catch (...) {  // the host's memory ran out in a table of kernels or devices
+    return fail(NOEL_ERR_CUDA, "host memory");
 }
 
 /* ------------------------------------------------ low-rank adapters */
@@ -1225,12 +1248,15 @@ cudaError_t shrink_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream
 
 /* CTAs per item of the second kernel: one turn of the GPU's CTA slots where
  * that is enough work for them, else kExpandWaves, so that items of unlike size
- * even out */
+ * even out.  Just under whole turns: items is a bound, and about batch / 16 or
+ * as many as there are adapters will come. */
 dim3 expand_grid(DeviceCtx *c, const LoraArgs &a, int items, int per_sm) {
     const int rows = 32 * (kExpandThreads / 32);
     const int64_t all = ((int64_t)a.rows + rows - 1) / rows, slots = (int64_t)c->sms * per_sm;
     const int64_t waves = all * items <= kExpandWaves * slots ? 1 : kExpandWaves;
-    const int64_t want = (waves * slots + items - 1) / items;
+    int64_t likely = a.batch / kLoraItem > a.n ? a.batch / kLoraItem : a.n;
+    likely = likely + 1 < items ? likely + 1 : items;
+    const int64_t want = waves * slots / likely > 1 ? waves * slots / likely : 1;
     return dim3((unsigned)(all < want ? all : want), items);
 }
 
@@ -1306,7 +1332,7 @@ extern "C" size_t noel_lora_workspace_bytes(int batch, int rank) {
 
 extern "C" int noel_lora_apply(const noel_lora_t *lora, const int32_t *d_adapter, const float *d_x, size_t ldx,
                                int batch, int cols, int rows, float *d_y, size_t ldy, void *d_work, size_t work_bytes,
-                               void *stream) {
+                               void *stream) try {
     LoraArgs a{};
     int r = lora_args(lora, d_adapter, d_x, ldx, batch, cols, rows, d_y, ldy, d_work, work_bytes, &a);
     if (r) return r;
@@ -1316,6 +1342,8 @@ extern "C" int noel_lora_apply(const noel_lora_t *lora, const int32_t *d_adapter
     if (r) return r;
     r = lora_launch(c, a, lora->type, static_cast<cudaStream_t>(stream));
     return r ? r : ok();
+} catch (...) {
+    return fail(NOEL_ERR_CUDA, "host memory");
 }
 
 /* ------------------------------------------------ LM head -> sampler */
@@ -1354,7 +1382,7 @@ extern "C" int noel_lmhead_sample_ex(const noel_sampler_config_t *cfg, const voi
                                      int vocab, const noel_lora_t *lora, const int32_t *d_adapter,
                                      const noel_logits_params_t *process, const int32_t *d_history, int history_len,
                                      size_t hld, uint64_t *d_rng, int32_t *d_ids, float *d_probs, float *d_logits,
-                                     void *d_work, size_t work_bytes, void *stream) {
+                                     void *d_work, size_t work_bytes, void *stream) try {
     if (!cfg || !d_weight || !d_hidden || !d_logits) return fail(NOEL_ERR_INVALID_ARG, "cfg, weight, hidden and logits are required");
     if (weight_type != NOEL_HEAD_F32 && weight_type != NOEL_HEAD_F16 && weight_type != NOEL_HEAD_BF16)
         return fail(NOEL_ERR_UNSUPPORTED, "weight type %d (F32 0, F16 1, BF16 30)", weight_type);
@@ -1401,6 +1429,8 @@ extern "C" int noel_lmhead_sample_ex(const noel_sampler_config_t *cfg, const voi
     ex.d_probs = d_probs;
     return sample_batch(cfg, d_logits, NOEL_DTYPE_F32, batch, vocab, (size_t)vocab, d_history, history_len, hld,
                         d_rng, d_ids, &ex, s);
+} catch (...) {
+    return fail(NOEL_ERR_CUDA, "host memory");
 }
 
 extern "C" int noel_moe_route_top_k(const float *d_gate_logits, int n_tokens, int n_experts, size_t ld, int top_k,

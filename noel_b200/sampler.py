@@ -677,11 +677,8 @@ def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: 
         work, size = adapters.scratch(B)
     if process is not None:
         process.check(logits, V)
-    s = torch.cuda.current_stream(dev)
-    _check(lib().noel_lmhead_sample_ex(C.byref(cfg), weight.data_ptr(), wt, weight.stride(0), hidden.data_ptr(),
-                                       hidden.stride(0), B, D, V, lora, ip,
-                                       process.ref if process is not None else None, hp, H, hld,
-                                       rng.data_ptr(), ids.data_ptr(), pr.data_ptr() if pr is not None else None,
-                                       logits.data_ptr(), work.data_ptr() if size else None, size,
-                                       C.c_void_p(s.cuda_stream)))
+    _call(dev, None, lambda s: lib().noel_lmhead_sample_ex(
+        C.byref(cfg), weight.data_ptr(), wt, weight.stride(0), hidden.data_ptr(), hidden.stride(0), B, D, V, lora, ip,
+        process.ref if process is not None else None, hp, H, hld, rng.data_ptr(), ids.data_ptr(),
+        pr.data_ptr() if pr is not None else None, logits.data_ptr(), work.data_ptr() if size else None, size, s))
     return ids, logits, pr

@@ -113,7 +113,7 @@ def test_process_parts_left_out_gpu(cuda, without):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("H", [1, 31, 1023, 1024, 1025, 2047, 2048, 2049, 5000, 20000])
+@pytest.mark.parametrize("H", [1, 31, 1023, 1024, 1025, 2047, 2048, 2049, 5000, 8192, 20000])
 @pytest.mark.parametrize("bias", [0, 300])
 def test_process_history_lengths_gpu(cuda, H, bias, dtype):
     t, p = build(4, 20011, dtype, seed=H, H=H, bias=bias, masks=2, density=0.9)
@@ -268,6 +268,60 @@ def test_process_on_two_streams_gpu(cuda):
     torch.cuda.synchronize()
     for d in rows:
         assert torch.equal(d, want)
+
+
+@pytest.mark.parametrize("H,V", [(1000, 4096), (60000, 4096)])
+def test_process_quotients_are_the_division_s_gpu(cuda, H, V):
+    """x / repetition has the bits of the division, over all exponents and on
+    both ways through (a table, and counted slices)"""
+    import torch
+
+    from noel_b200 import sampler as S
+
+    g = torch.Generator(device=cuda).manual_seed(H)
+    B = 64
+    raw = torch.randint(0, 0x7F800000, (B, V), generator=g, device=cuda, dtype=torch.int32)  # every positive number
+    raw[:, :64] = torch.randint(0x3F800000, 0x40000000, (B, 64), generator=g, device=cuda, dtype=torch.int32)
+    x = raw.view(torch.float32)
+    rep = torch.cat([1.0 + torch.rand(48, generator=g, device=cuda),
+                     torch.tensor([1e-3, 2e-3, 0.3, 0.999, 1.0, 3.0, 1000.0, 1025.0, 1e9, 1e-9, 0.0, float("inf"), 1e38, 1e-38,
+                                   1.5, 7.0], device=cuda)])
+    h = torch.randint(0, V, (B, H), generator=g, device=cuda, dtype=torch.int32)
+    seen = torch.zeros(B, V, dtype=torch.bool, device=cuda).scatter_(1, h.long(), True)
+    want = torch.where(seen, x / rep[:, None], x)
+    got = S.logits_process(x.clone(), S.LogitsParams(history=h, repetition=rep))
+    same = (got.view(torch.int32) == want.view(torch.int32)) | (got.isnan() & want.isnan())
+    assert same.all(), (x[~same][:5], got[~same][:5], want[~same][:5])
+
+
+@pytest.mark.parametrize("H,bias", [(40, 8), (3000, 8), (9000, 0), (2000, 0)])
+def test_process_large_batch_equals_small_ones_gpu(cuda, H, bias):
+    """the ranges and kernels that a large batch takes give the bits that eight rows at a time give"""
+    import torch
+
+    from noel_b200 import sampler as S
+
+    B, V = 1200, 50021
+    g = torch.Generator(device=cuda).manual_seed(H)
+    r = lambda *s: torch.rand(*s, generator=g, device=cuda)  # noqa: E731
+    p = {"history": (torch.exp(r(B, H) * 10.8) - 1).to(torch.int32).clamp_(max=V - 1),
+         "history_lens": torch.randint(0, H + 1, (B,), generator=g, device=cuda, dtype=torch.int32),
+         "repetition": 1 + r(B), "frequency": r(B), "presence": r(B),
+         "mask": torch.randint(-2**31, 2**31 - 1, (40, 1564), generator=g, device=cuda, dtype=torch.int32),
+         "mask_rows": torch.randint(-1, 40, (B,), generator=g, device=cuda, dtype=torch.int32)}
+    p["mask"][:10] = 0
+    p["mask"][:10, 700] = 5
+    p["mask"][10:20] = -1
+    p["mask"][10:20, ::90] = -9
+    if bias:
+        p["bias_ids"] = torch.randint(0, V, (B, bias), generator=g, device=cuda, dtype=torch.int32)
+        p["bias"] = r(B, bias)
+    x = torch.randn(B, V, generator=g, device=cuda)
+    got = S.logits_process(x.clone(), S.LogitsParams(**p))
+    for b in range(0, B, 8):
+        part = {k: v if k == "mask" else v[b:b + 8].contiguous() for k, v in p.items()}
+        want = S.logits_process(x[b:b + 8].clone(), S.LogitsParams(**part))
+        assert torch.equal(got[b:b + 8], want), b
 
 
 def test_process_python_refusals_gpu(cuda):

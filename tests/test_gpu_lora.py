@@ -146,6 +146,20 @@ def test_lora_a_token_does_not_depend_on_the_others_gpu(cuda):
         assert torch.equal(part["y"], s["y"][at])
 
 
+@pytest.mark.parametrize("dtype,B,D,V,r,n", [("bf16", 300, 512, 40000, 64, 2), ("f16", 260, 1000, 30002, 16, 40),
+                                             ("f32", 150, 777, 20001, 18, 3), ("bf16", 200, 640, 20003, 33, 3)])
+def test_lora_large_equals_token_by_token_gpu(cuda, dtype, B, D, V, r, n):
+    import torch
+
+    s = build(cuda, B, D, V, r, n, dtype, seed=B, ragged=True)
+    y0 = s["y"].clone()
+    apply(s)
+    for t in range(0, B, 37):
+        part = {**s, "y": y0[t:t + 1].clone(), "x": s["x"][t:t + 1].contiguous(), "ids": s["ids"][t:t + 1].contiguous()}
+        apply(part)
+        assert torch.equal(part["y"].view(torch.int32), s["y"][t:t + 1].view(torch.int32)), t
+
+
 def test_lora_special_values_stay_in_their_token_gpu(cuda):
     """infinities and NaN in one token's x reach that token's row only, and
     reach it as they do in the plain form"""
