@@ -16,6 +16,13 @@
  * three.  All products of parts are added, smallest first, but for the last
  * parts' of two fp32 numbers (2^-30 of the product), so a sum is as exact as
  * in fp32.
+ *
+ * Measured at 152,064 rows x 4096 columns: one token at rank 16 in 7.5 us; 64
+ * tokens with 64 bf16 adapters of rank 16 in 77 us (399 MB, 5.2 TB/s); 256
+ * tokens over eight fp16 adapters of ranks up to 32 in 75 us (287 MB); 2048
+ * tokens over four bf16 adapters of rank 64 in 500 us (2.6 GB, 5.2 TB/s).  The
+ * second kernel's time: half of the issue slots and 40 % of the matrix pipe are
+ * busy at rank 16, so memory is not all that bounds it there.
  */
 #pragma once
 
@@ -31,12 +38,16 @@ namespace noel {
 constexpr int kLoraMaxRank = 256;
 constexpr int kLoraBatch = 2048;    // tokens of one pass over the adapters
 constexpr int kLoraItem = 16;       // tokens of an item
-constexpr int kLoraWarpBatch = 32;  // tokens up to which every warp finds the items by itself
+constexpr int kLoraWarpBatch = 32;  // tokens up to which every warp finds the items by itself (one token: 9.0 -> 7.5 us)
 constexpr int kShrinkThreads = 256;
 constexpr int kShrinkSplit = 8;     // CTAs of a cluster that share an item's columns, at most
 constexpr int kExpandThreads = 256;
-constexpr int kExpandFetch = 1;    // turns between asking the L2 for a line of y and copying it
-constexpr int kExpandWaves = 4;         // turns of the GPU's CTAs that the second kernel's work is cut into
+/* turns between asking the L2 for a line of y and copying it from there (2048 tokens at rank 64: 551 us without, 496,
+ * 521 and 535 us at 1, 2 and 4) */
+constexpr int kExpandFetch = 1;
+/* turns of the GPU's CTA slots that the second kernel's work is cut into (64 adapters, 256 and 2048 tokens: 73, 75, 582
+ * us at 2; 77, 75, 513 at 4; 81, 78, 560 at 6) */
+constexpr int kExpandWaves = 4;
 
 /* the items of a batch above kLoraWarpBatch, in the scratch */
 struct LoraPlan {
@@ -378,9 +389,10 @@ __device__ __forceinline__ LoraItem lora_item(const LoraArgs &a, int k) {
  * warps take the columns in turns of 32, each turn's products are added up
  * from 0 by the matrix instructions and then to the warp's sums in fp32 (the
  * instructions cut what they add to), the warps' sums are added in their order
- * and the CTAs' in theirs.  An item's weights are 128 KB at rank 16 and 4096
- * columns; one CTA takes them in no faster than 6 us, so few items are spread
- * over clusters of up to eight. */
+ * and the CTAs' in theirs.  Few items are spread over clusters of up to eight
+ * CTAs: one CTA alone takes an item's weights (128 KB at rank 16 and 4096
+ * columns) in at its own pace (the whole call: one token 12.3 us with one CTA,
+ * 7.5 with eight; 64 adapters 86 and 77). */
 template <int WT, int TILES>
 __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __grid_constant__ LoraArgs a) {
     constexpr int WARPS = kShrinkThreads / 32, RANKS = 8 * TILES;
@@ -582,8 +594,10 @@ __device__ __forceinline__ void expand_any(const LoraArgs &a, const ExpandLane<W
     }
 }
 
-/* The second kernel for arrays that the one below cannot take: one item per
- * blockIdx.y, a warp its 32 rows at a time. */
+/* The second kernel for arrays that the one below cannot take (rows of B_i that
+ * start on 2 bytes, the largest ranks): one item per blockIdx.y, a warp its 32
+ * rows at a time.  Where both could, it takes 11.3 us for one token and 207 for
+ * 64 adapters against 7.5 and 77. */
 template <int WT, int N>
 __global__ void __launch_bounds__(kExpandThreads) lora_expand_any_kernel(const __grid_constant__ LoraArgs a) {
     const LoraItem it = lora_item(a, blockIdx.y);  // the kernel before let this one begin when the plan was there
@@ -626,7 +640,9 @@ __host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es) {
  * 16 bytes.  Without it rows of y start anywhere: their 32 numbers are copied
  * 4 bytes at a time, and go back through the stage so that a store writes a
  * token's 32 numbers side by side; and so are rows of B_i that do not start on
- * 16 bytes but on 4. */
+ * 16 bytes but on 4 (aligned rows taken that way: 97 instead of 77 us for 64
+ * adapters; unaligned ones by plain loads: 324 instead of 191 us for 651 tokens
+ * x 138,974).  Ranks up to 16 held as if they were 32: 104 instead of 77 us. */
 template <int WT, int N, int G, int D, bool WIDE>
 __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
     extern __shared__ __align__(128) unsigned char lora_smem[];
