@@ -93,14 +93,31 @@ __device__ __forceinline__ RowRules row_rules(const LogitsArgs &a, int row) {
             rep > 0.0009765625f && rep < 1024.0f ? __fdiv_rn(1.0f, rep) : 0.0f};
 }
 
-/* x / rep: a quotient from the reciprocal, corrected by its remainder
- * (Markstein 1990), which is the rounded quotient where nothing on the way
- * over- or underflows; |x| and rep are kept well inside that. */
+/* x / rep for x > 0: a quotient from the reciprocal, corrected by its
+ * remainder (Markstein 1990), which is the rounded quotient where nothing on
+ * the way over- or underflows.  x below 2^-101 is taken times 2^100; of a
+ * quotient that is subnormal then, the last bit is made odd where a remainder
+ * is left (Boldo and Melquiond 2008), so that scaling it back rounds as if
+ * from the exact quotient (it has to lose two bits for that; one binade is
+ * left to the division, as are huge x and unlikely rep). */
 __device__ __forceinline__ float quotient(float x, const RowRules &r) {
     const uint32_t e = __float_as_uint(x) & 0x7F800000u;
-    if (r.inv == 0.0f || e < 0x0D000000u || e > 0x70000000u) return __fdiv_rn(x, r.rep);
-    const float q = __fmul_rn(x, r.inv);
-    return __fmaf_rn(__fmaf_rn(-q, r.rep, x), r.inv, q);
+    if (r.inv == 0.0f || e > 0x70000000u) return __fdiv_rn(x, r.rep);
+    if (e >= 0x0D000000u) {
+        const float q = __fmul_rn(x, r.inv);
+        return __fmaf_rn(__fmaf_rn(-q, r.rep, x), r.inv, q);
+    }
+    const float up = __uint_as_float((127u + 100u) << 23), down = __uint_as_float((127u - 100u) << 23);
+    const float X = __fmul_rn(x, up);
+    float q = __fmul_rn(X, r.inv);
+    q = __fmaf_rn(__fmaf_rn(-q, r.rep, X), r.inv, q);
+    const float rest = __fmaf_rn(-q, r.rep, X);
+    uint32_t b = __float_as_uint(q);
+    if (b < (127u - 26u) << 23) {           // subnormal
+        if (b >= (127u - 27u) << 23) return __fdiv_rn(x, r.rep);
+        if (rest != 0.0f) b = (rest > 0.0f ? b : b - 1u) | 1u;
+    }
+    return __fmul_rn(__uint_as_float(b), down);
 }
 
 __device__ __forceinline__ float penalised(float x, uint32_t w, const RowRules &r) {
