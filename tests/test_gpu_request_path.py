@@ -132,6 +132,64 @@ def test_processed_shards_through_the_sharded_sampler_gpu(cuda):
     assert torch.equal(got, want)
 
 
+def test_empty_batches_gpu(cuda):
+    import torch
+
+    from noel_b200 import sampler as S
+
+    z = torch.zeros(0, 500, device=cuda)
+    h = torch.zeros(0, 7, dtype=torch.int32, device=cuda)
+    assert S.logits_process(z, S.LogitsParams(history=h)).shape == (0, 500)
+    ad = S.Adapters(torch.zeros(2, 4, 16, device=cuda), torch.zeros(2, 500, 4, device=cuda))
+    ids = torch.zeros(0, dtype=torch.int32, device=cuda)
+    assert S.lora_apply(z, torch.zeros(0, 16, device=cuda), ad, ids).shape == (0, 500)
+    x = torch.randn(3, 500, device=cuda)
+    none = S.LogitsParams(history=torch.zeros(3, 0, dtype=torch.int32, device=cuda),
+                          bias_ids=torch.zeros(3, 0, dtype=torch.int32, device=cuda), bias=torch.zeros(3, 0, device=cuda))
+    assert torch.equal(S.logits_process(x.clone(), none), x)
+
+
+def test_a_row_that_allows_nothing_is_sampled_gpu(cuda, oracle):
+    """-infinity throughout goes through the sampler as it does through the reference's"""
+    import torch
+
+    from noel_b200 import sampler as S
+    from oracle.oracle import make_config as orc_config
+
+    x = torch.randn(4, 3000, device=cuda)
+    S.logits_process(x, S.LogitsParams(mask=torch.zeros(1, 94, dtype=torch.int32, device=cuda),
+                                       mask_rows=torch.tensor([-1, 0, 0, 1], dtype=torch.int32, device=cuda)))
+    assert torch.isneginf(x[1:3]).all() and torch.isfinite(x[[0, 3]]).all()
+    rng = np.arange(1, 9, dtype=np.uint64).reshape(4, 2)
+    rng_t = torch.from_numpy(rng.view(np.int64).copy()).to(cuda)
+    got = S.sample_batch(x, rng_t, S.make_config(**CFG))
+    want = oracle.sample_batch(orc_config(**CFG, repetition_window=0), x.cpu().numpy(), rng=rng)
+    np.testing.assert_array_equal(got["ids"].cpu().numpy(), want.ids)
+
+
+def test_requests_change_between_replays_gpu(cuda):
+    """one captured step, replayed while the histories, biases, masks and adapters in its buffers change"""
+    import torch
+
+    from noel_b200 import sampler as S
+
+    s = inputs(cuda, 9, seed=5)
+    ad, prm = S.Adapters(s["a"], s["b"]), params(S, cuda, s["process"])
+    x0, y = torch.randn(9, 9000, device=cuda), torch.empty(9, 9000, device=cuda)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y.copy_(x0)
+        S.logits_process(S.lora_apply(y, s["hidden"], ad, s["ids"]), prm)
+    for k in range(3):
+        for t in prm.tensors:  # the buffers that the parameters were made over
+            if t.dtype == torch.int32 and t.dim() == 2:
+                t.copy_(t.roll(k, 0))
+        s["ids"].copy_(s["ids"].roll(1))
+        g.replay()
+        want = S.logits_process(S.lora_apply(x0.clone(), s["hidden"], ad, s["ids"]), prm)
+        assert torch.equal(y, want)
+
+
 def test_path_refusals_gpu(cuda):
     import torch
 
