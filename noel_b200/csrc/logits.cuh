@@ -17,9 +17,9 @@
  * of the bandwidth; strict masks write whole rows at 6.2 TB/s.
  *
  * Measured on 1024 x 152,064 fp32 under masks that allow 0.5 % of the ids:
- * 119 us for 582 MB (a bare fill of the rows takes 88 us); 1024 x 256,000 bf16
- * under masks that allow 98 %: 110 us; 64 rows with histories of 65,536 ids:
- * 52 us; one row: 5 us.
+ * 123 us for 582 MB (a bare fill of the rows takes 88 us); 1024 x 256,000 bf16
+ * under masks that allow 98 %: 112 us; 64 rows with histories of 65,536 ids:
+ * 44 us; one row: 5 us.
  */
 #pragma once
 
@@ -455,12 +455,32 @@ __global__ void __launch_bounds__(kSliceThreads, 2) logits_slice_kernel(const __
     const uint32_t *mask = row_mask(a, row);
     for (int i = tid; i < width / 4; i += kSliceThreads) reinterpret_cast<uint4 *>(word)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    /* an id's column if it is one of the slice's, as its index in the slice */
+    /* An id's column is id - v_begin (an id below wraps round to more than vocab), a column's line its bits from
+     * LINE on, and its slice the lowest bits of the line; the slice's words hold its lines one after the other. */
+    constexpr int LINE = sizeof(T) == 4 ? 5 : 6;
+    static_assert(1 << LINE == BLK, "columns of a line");
+    const uint32_t of_slice = (uint32_t)(a.slices - 1) << LINE, want = mine_c << LINE;
     auto index_of = [&](int id, uint32_t &c) {
         c = (uint32_t)id - (uint32_t)a.v_begin;
-        const bool in = id >= a.v_begin && c < (uint32_t)a.vocab && (c / BLK & (uint32_t)(a.slices - 1)) == mine_c;
-        c = (c / BLK >> sh) * BLK + c % BLK;  // its word
+        const bool in = c < (uint32_t)a.vocab && (c & of_slice) == want;
+        c = (c >> (LINE + sh) << LINE) | (c & (BLK - 1));  // its word
         return in;
+    };
+    /* the same and the change of the word without a branch: seven ids of eight are another slice's */
+    const uint32_t word_s = (uint32_t)__cvta_generic_to_shared(word);
+    auto mark = [&](int id) {
+        const uint32_t c = (uint32_t)id - (uint32_t)a.v_begin;
+        const uint32_t at = word_s + ((c >> (LINE + sh) << (LINE + 2)) | (c & (BLK - 1)) << 2);
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .u32 s;\n\tand.b32 s, %0, %1;\n\tsetp.eq.u32 p, s, %2;\n\t"
+                     "setp.lt.and.u32 p, %0, %3, p;\n\t@p st.shared.u32 [%4], %5;\n\t}" ::"r"(c), "r"(of_slice), "r"(want),
+                     "r"(a.vocab), "r"(at), "r"(kSeenPrompt) : "memory");
+    };
+    auto count = [&](int id) {
+        const uint32_t c = (uint32_t)id - (uint32_t)a.v_begin;
+        const uint32_t at = word_s + ((c >> (LINE + sh) << (LINE + 2)) | (c & (BLK - 1)) << 2);
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .u32 s;\n\tand.b32 s, %0, %1;\n\tsetp.eq.u32 p, s, %2;\n\t"
+                     "setp.lt.and.u32 p, %0, %3, p;\n\t@p red.shared.add.u32 [%4], %5;\n\t}" ::"r"(c), "r"(of_slice),
+                     "r"(want), "r"(a.vocab), "r"(at), "r"(1) : "memory");
     };
     /* the history 16 bytes at a time from its first aligned id on: the prompt
      * only marks, the rest counts */
@@ -481,15 +501,9 @@ __global__ void __launch_bounds__(kSliceThreads, 2) logits_slice_kernel(const __
         if (tail < n) take(ids[tail]);
     };
     const int prompt = min(max(h.prompt, 0), h.len);
-    through(h.ids, prompt, [&](int id) {
-        uint32_t c;
-        if (index_of(id, c)) word[c] = kSeenPrompt;  // every writer writes the same
-    });
+    through(h.ids, prompt, mark);  // every writer of a word writes the same
     __syncthreads();
-    through(h.ids + prompt, h.len - prompt, [&](int id) {
-        uint32_t c;
-        if (index_of(id, c)) atomicAdd(&word[c], 1u);
-    });
+    through(h.ids + prompt, h.len - prompt, count);
     const int nb = a.bias_len;
     const int32_t *bi = nb ? a.bias_ids + (size_t)row * (size_t)a.bld : nullptr;
     const float *bv = nb ? a.bias + (size_t)row * (size_t)a.bld : nullptr;
