@@ -50,7 +50,6 @@ struct LogitsArgs {
     const int32_t *mask_row;
     int ranges, range;  // CTAs per row of the rows kernel and their columns
     int cap;            // entries of a CTA's table; 0: none
-    bool write_mask;    // the rows kernel writes the masked logits
     int slices, slice;  // CTAs per row of the slice kernel and the words each counts in
 };
 
@@ -353,13 +352,14 @@ __device__ __forceinline__ void mask_piece(const LogitsArgs &a, T *x, int64_t c0
 }
 
 /* One CTA per row and range of its columns: the table of the range is filled,
- * the range is masked, and then the table's logits are changed.  The mask
+ * the range is masked (WRITE; without it the kernel has 64 registers a thread
+ * instead of 40: 16.3 against 17.9 us for 256 rows with 1024 ids), and then the table's logits are changed.  The mask
  * never changes an allowed logit's value but may write it back as it read it,
  * so the table's own writes come after the mask's, a CTA's barrier between
  * them.  (One warp filling the table while the others mask was slower in small
  * batches, 27 against 18 us at 64 rows, and no faster in large ones.) */
-template <typename T>
-__global__ void __launch_bounds__(kLogitsThreads, kRowsCtas) logits_rows_kernel(const __grid_constant__ LogitsArgs a) {
+template <typename T, bool WRITE>
+__global__ void __launch_bounds__(kLogitsThreads, WRITE ? kRowsCtas : 4) logits_rows_kernel(const __grid_constant__ LogitsArgs a) {
     extern __shared__ __align__(16) uint32_t logits_smem[];
     __shared__ int turn;
     constexpr int VE = 32 / sizeof(T);
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kLogitsThreads, kRowsCtas) logits_rows_kernel(
     const int lo = (int)max(begin, (int64_t)0), hi = (int)max(end, (int64_t)lo);
     if (threadIdx.x == 0) turn = kLogitsThreads / 32;  // every warp's first turn is its own number
     if (a.cap) table_fill(a, row, t, lo, hi);
-    if (mask && a.write_mask) {
+    if (WRITE && mask) {
         const int lane = threadIdx.x & 31;
         if (!a.cap) __syncthreads();
         int k = threadIdx.x >> 5;

@@ -1072,7 +1072,6 @@ int logits_args(const noel_logits_params_t *p, void *logits, int dtype, int B, i
         want = want < turn ? turn : want;
         a.range = (int)(want < most ? want : most);
         a.ranges = (int)(((int64_t)V + 15 + a.range - 1) / a.range);
-        a.write_mask = true;
     }
     if (B > 1 << 30 || (int64_t)B * a.slices > 0x7FFFFFFF || (int64_t)B * a.ranges > 0x7FFFFFFF)
         return fail(NOEL_ERR_TOO_LARGE, "%d rows x %d columns", B, V);
@@ -1080,12 +1079,12 @@ int logits_args(const noel_logits_params_t *p, void *logits, int dtype, int B, i
     return NOEL_OK;
 }
 
-template <typename T>
+template <typename T, bool WRITE>
 int logits_rows_launch(DeviceCtx *c, const LogitsArgs &a, cudaStream_t s) {
     const size_t smem = (size_t)a.cap * 12;
-    const int r = set_smem(c, (const void *)logits_rows_kernel<T>, smem);
+    const int r = set_smem(c, (const void *)logits_rows_kernel<T, WRITE>, smem);
     if (r) return r;
-    logits_rows_kernel<T><<<a.batch * a.ranges, kLogitsThreads, smem, s>>>(a);
+    logits_rows_kernel<T, WRITE><<<a.batch * a.ranges, kLogitsThreads, smem, s>>>(a);
     CUDA_TRY(cudaGetLastError());
     return NOEL_OK;
 }
@@ -1097,13 +1096,14 @@ int logits_launch_t(DeviceCtx *c, const LogitsArgs &a, cudaStream_t s) {
         /* a table of this size in every range's CTA would leave too few CTAs to mask */
         LogitsArgs m = a, t = a;
         m.cap = 0;
-        t.write_mask = false;
         t.ranges = 1;
         t.range = 0x7FFFFFFF;
-        r = logits_rows_launch<T>(c, m, s);
-        if (!r) r = logits_rows_launch<T>(c, t, s);
-    } else if (a.mask || a.cap) {
-        r = logits_rows_launch<T>(c, a, s);
+        r = logits_rows_launch<T, true>(c, m, s);
+        if (!r) r = logits_rows_launch<T, false>(c, t, s);
+    } else if (a.mask) {
+        r = logits_rows_launch<T, true>(c, a, s);
+    } else if (a.cap) {
+        r = logits_rows_launch<T, false>(c, a, s);
     }
     if (r) return r;
     if (a.slices) {
