@@ -1204,7 +1204,7 @@ int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size
     a.vec_a = rows_on(l->d_a, l->lda * es, l->stride_a * es, 16);
     a.vec_b = rows_on(l->d_b, l->ldb * es, l->stride_b * es, lane_b);
     a.staged = a.rank_pad * es > 256 ? 0
-               : rows_on(l->d_b, l->ldb * es, l->stride_b * es, 16) && (size_t)l->rank * es % 16 == 0 ? 16
+               : rows_on(l->d_b, l->ldb * es, l->stride_b * es, 16) ? 16
                : rows_on(l->d_b, l->ldb * es, l->stride_b * es, 4) && (a.rank_pad <= 32 || (a.rank_pad == 64 && es == 2)) ? 4
                                                                                                                         : 0;
     *out = a;
@@ -1282,8 +1282,8 @@ int expand_any_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s
 }
 
 /* The second kernel: through shared memory where two stages of a warp fit
- * (ranks up to 128, fp32 64) and rows of B start on 16 bytes and end there, or
- * start on 4 bytes (ranks up to 64, fp32 32). */
+ * (ranks up to 128, fp32 64) and rows of B start on 16 bytes, or on 4 (ranks
+ * up to 64, fp32 32). */
 template <int WT>
 int expand(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
     constexpr bool kF32 = WT == kHeadF32;

@@ -90,6 +90,13 @@ def test_lora_wider_rows_gpu(cuda, r, pad, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("r,pad", [(3, 13), (13, 3), (21, 11), (50, 14), (57, 7), (100, 4)])
+def test_lora_odd_ranks_in_aligned_rows_gpu(cuda, r, pad, dtype):
+    """rows of B on 16 bytes that end between two of them, NaN behind the rank"""
+    check(build(cuda, 21, 256, 1060, r, 3, dtype, seed=r, pad=pad))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("r", [8, 16, 48, 64])
 def test_lora_ranks_of_their_own_gpu(cuda, r, dtype):
     check(build(cuda, 50, 200, 700, r, 6, dtype, seed=r, ragged=True))
