@@ -71,6 +71,7 @@ struct LoraArgs {
     int64_t ldy;
     uint16_t *low;   // [batch][3][rank_pad] bf16 parts of scale A x
     int rank_pad;    // 16, or the rank rounded up to 32
+    int r_begin, r_count;  // ranks that the second kernel takes: some of many, or all
     LoraPlan *plan;  // NULL: every warp finds the items
     int staged;                      // bytes at a time that fill the second kernel's stages: 16, 4, or 0: not staged
     int vec_x, vec_a, vec_b, vec_y;  // rows start on 16 bytes (B with rank_pad 16: on 4 elements; y: 2 for 32 bytes)
@@ -510,12 +511,12 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __gri
         *reinterpret_cast<uint32_t *>(a.low + ((size_t)t * 3 + k) * a.rank_pad + r0 + r) = take_parts(u, v);
 }
 
-/* N parts (8 or 4) of a token's low-rank numbers */
+/* N parts (8 or 4) of a token's low-rank numbers, of the ranks from r_begin on */
 template <int N>
 __device__ __forceinline__ void load_low(const LoraArgs &a, int t, int r, uint32_t (&x)[3][N / 2]) {
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        const uint16_t *p = a.low + ((size_t)t * 3 + k) * a.rank_pad + r;
+        const uint16_t *p = a.low + ((size_t)t * 3 + k) * a.rank_pad + a.r_begin + r;
         if (N == 8) {
             const uint4 v = *reinterpret_cast<const uint4 *>(p);
             x[k][0] = v.x, x[k][1] = v.y, x[k][N / 2 - 2] = v.z, x[k][N / 2 - 1] = v.w;
@@ -538,7 +539,7 @@ __device__ __forceinline__ void load_low(const LoraArgs &a, int t, int r, uint32
 template <int WT>
 struct ExpandLane {
     LoraItem it;
-    int n;  // the adapter's rank
+    int n;  // the adapter's ranks among those that are taken
     bool wide;
     const char *b, *w;
     size_t pitch, next;
@@ -546,9 +547,9 @@ struct ExpandLane {
     __device__ __forceinline__ ExpandLane(const LoraArgs &a, const LoraItem &item, int N) : it(item) {
         const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
         constexpr int ES = kWeightBytes<WT>;
-        n = lora_rank(a, it.adapter);
+        n = min(max(lora_rank(a, it.adapter) - a.r_begin, 0), a.r_count);
         wide = a.vec_y != 0;
-        b = static_cast<const char *>(a.b) + (size_t)it.adapter * (size_t)a.stride_b * ES;
+        b = static_cast<const char *>(a.b) + ((size_t)it.adapter * (size_t)a.stride_b + a.r_begin) * ES;
         pitch = (size_t)a.ldb * ES;
         w = b + (size_t)(wide ? 8 * (g >> 1) + (g & 1) : g) * pitch + (size_t)(N * q) * ES;
         next = (wide ? 2 : 8) * pitch;
@@ -595,7 +596,7 @@ __device__ __forceinline__ void expand_any(const LoraArgs &a, const ExpandLane<W
 }
 
 /* The second kernel for arrays that the one below cannot take (rows of B_i that
- * start on 2 bytes, the largest ranks): one item per blockIdx.y, a warp its 32
+ * start on 2 bytes): one item per blockIdx.y, a warp its 32
  * rows at a time.  Where both could, it takes 11.3 us for one token and 207 for
  * 64 adapters against 7.5 and 77. */
 template <int WT, int N>
@@ -618,12 +619,10 @@ __device__ __forceinline__ void cp_async16_at(uint32_t dst, const void *src, uin
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-/* Bytes of a row of B_i in shared memory and of one of a warp's stages: 32 such
- * rows (64 bytes more after every eight where a row is 32 bytes), then a line
+/* Bytes of one of a warp's stages: 32 rows of B_i (64 bytes more after every eight where a row is 32 bytes), then a line
  * of y for each of 16 tokens. */
-__host__ __device__ constexpr int expand_row_bytes(int rank_pad, int es) { return rank_pad * es; }
-__host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es) {
-    return 32 * rank_pad * es + (rank_pad * es == 32 ? 256 : 0) + kLoraItem * 128;
+__host__ __device__ constexpr int expand_stage_bytes(int ranks, int es) {
+    return 32 * ranks * es + (ranks * es == 32 ? 256 : 0) + kLoraItem * 128;
 }
 
 /* The second kernel: one item per blockIdx.y.  Every warp has D stages of
@@ -635,8 +634,10 @@ __host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es) {
  * that the eight lanes of a quarter warp read eight different ones.
  *
  * N is the number of ranks a lane holds: 4 for ranks up to 16, else 8 (a group
- * of 32 ranks at a time).  G groups of low-rank numbers stay in registers
- * (0: they are read again for every turn).  WIDE: rows of y and of B_i start on
+ * of 32 ranks at a time).  A launch takes up to 4 N G ranks, whose low-rank
+ * numbers stay in registers; adapters of more ranks take several launches.
+ * (All ranks in one launch, with two stages and their numbers read again every
+ * turn: 512 tokens at rank 128 522 us against 281, 16 adapters 180 against 124.)  WIDE: rows of y and of B_i start on
  * 16 bytes.  Without it rows of y start anywhere: their 32 numbers are copied
  * 4 bytes at a time, and go back through the stage so that a store writes a
  * token's 32 numbers side by side; and so are rows of B_i that do not start on
@@ -646,7 +647,7 @@ __host__ __device__ constexpr int expand_stage_bytes(int rank_pad, int es) {
 template <int WT, int N, int G, int D, bool WIDE>
 __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __grid_constant__ LoraArgs a) {
     extern __shared__ __align__(128) unsigned char lora_smem[];
-    constexpr int ES = kWeightBytes<WT>, ROWS = 32, WARPS = kExpandThreads / 32, GR = G ? G : 1;
+    constexpr int ES = kWeightBytes<WT>, ROWS = 32, WARPS = kExpandThreads / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const LoraItem it = lora_item(a, blockIdx.y);  // the kernel before let this one begin when the plan was there
     const int64_t first = ((int64_t)blockIdx.x * WARPS + warp) * ROWS, step = (int64_t)gridDim.x * WARPS * ROWS;
@@ -655,22 +656,24 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
         return;
     }
     const ExpandLane<WT> l(a, it, N);
-    const int rank_pad = G ? 4 * N * G : a.rank_pad;  // known to the compiler but for the largest ranks
-    const int row_bytes = expand_row_bytes(rank_pad, ES), stage_bytes = expand_stage_bytes(rank_pad, ES);
-    const int pad8 = row_bytes == 32 ? 64 : 0, y_at = 32 * row_bytes + 4 * pad8;
-    const int swap = ES == 2 ? (row_bytes % 128 == 0 ? 4 : 0) : (N == 8 ? 1 : 0);  // of odd rows' pieces
+    if (l.n == 0) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
+    constexpr int row_bytes = 4 * N * G * ES, stage_bytes = expand_stage_bytes(4 * N * G, ES);
+    constexpr int pad8 = row_bytes == 32 ? 64 : 0, y_at = 32 * row_bytes + 4 * pad8;
+    constexpr int swap = ES == 2 ? (row_bytes % 128 == 0 ? 4 : 0) : (N == 8 ? 1 : 0);  // of odd rows' pieces
     unsigned char *mem = lora_smem + warp * D * stage_bytes;
     /* how the lanes share a copy of 32 rows: `share` of them a row, in as many rounds; what lies past the adapter's
      * rank is filled with zeros */
-    const int share = G ? 4 * N * G * ES / 16 : 16;
-    const int c_row = lane / share, c_piece = lane % share, c_rows = 32 / share;
-    const bool c_on = c_piece * 16 < row_bytes;
+    constexpr int share = row_bytes / 16, c_rows = 32 / share;
+    const int c_row = lane / share, c_piece = lane % share;
     /* rows side by side: a turn's addresses differ by constants (2048 tokens at rank 64 without a pause: 586 -> 576 us;
      * no gain at rank 16, where a turn has two copies) */
-    const bool tight = G && N == 8 && l.pitch == (size_t)row_bytes;
+    const bool tight = N == 8 && l.pitch == (size_t)row_bytes;
     const uint32_t c_bytes = (uint32_t)min(max(l.n * ES - c_piece * 16, 0), 16);
     const char *b_from = l.b + (size_t)(first + c_row) * l.pitch + (c_bytes ? c_piece << 4 : 0);
-    constexpr int W4 = G ? 4 * N * G * ES / 4 : 1;
+    constexpr int W4 = row_bytes / 4;
     const char *b_from4 = l.b + (size_t)(first + lane / W4) * l.pitch + (4 * (lane % W4) < l.n * ES ? 4 * (lane % W4) : 0);
     const size_t b_round = (size_t)c_rows * l.pitch, b_step = (size_t)step * l.pitch;
     const uint32_t mem_s = (uint32_t)__cvta_generic_to_shared(mem);
@@ -707,7 +710,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
     auto issue = [&](int stage) {
         if (ahead < turns) {
             const uint32_t to = mem_s + stage * stage_bytes;
-            if (!WIDE && G && a.staged == 4) {  // rows of B_i that start on 4 bytes only
+            if (!WIDE && a.staged == 4) {  // rows of B_i that start on 4 bytes only
                 constexpr int PER = W4 < 32 ? 32 / W4 : 1;  // rows a round
                 const int word = lane % W4;
                 const char *src = b_from4;
@@ -720,7 +723,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
 #pragma unroll
                 for (int r = 0; r < share; ++r)
                     cp_async16_at(to + b_to + r * b_to_round, b_from + r * (c_rows * row_bytes), c_bytes);
-            } else if (c_on) {
+            } else {
                 const char *src = b_from;
 #pragma unroll
                 for (int r = 0; r < share; ++r, src += b_round) cp_async16_at(to + b_to + r * b_to_round, src, c_bytes);
@@ -745,14 +748,13 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
     };
 #pragma unroll
     for (int s = 0; s < D - 1; ++s) issue(s);
-    uint32_t x0[GR][3][N / 2] = {}, x1[GR][3][N / 2] = {};
+    uint32_t x0[G][3][N / 2] = {}, x1[G][3][N / 2] = {};
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the low-rank numbers are there
-    if (G) {
 #pragma unroll
-        for (int k = 0; k < GR; ++k) {
-            if (it.t0 >= 0) load_low<N>(a, it.t0, k * 4 * N + N * q, x0[k]);
-            if (it.t1 >= 0) load_low<N>(a, it.t1, k * 4 * N + N * q, x1[k]);
-        }
+    for (int k = 0; k < G; ++k) {
+        if (k * 4 * N >= l.n) break;
+        if (it.t0 >= 0) load_low<N>(a, it.t0, k * 4 * N + N * q, x0[k]);
+        if (it.t1 >= 0) load_low<N>(a, it.t1, k * 4 * N + N * q, x1[k]);
     }
     /* where this lane's row of instruction 0 lies in a stage and what instruction j adds, its piece there, and its
      * lines of y */
@@ -788,18 +790,8 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
                 multiply<WT, N>(c[j], from_zero, u0, u1, weights<WT, N>(b));
             }
         };
-        if (l.n == 0) continue;
-        if (G) {
-            group(0, true, x0[0], x1[0]);
-            if (GR > 1 && 4 * N < l.n) group(1, false, x0[GR - 1], x1[GR - 1]);
-        } else {
-            for (int k = 0; k * 4 * N < l.n; ++k) {
-                if (it.t0 >= 0) load_low<N>(a, it.t0, k * 4 * N + N * q, x0[0]);
-                if (it.t1 >= 0) load_low<N>(a, it.t1, k * 4 * N + N * q, x1[0]);
-                __syncwarp();
-                group(k, k == 0, x0[0], x1[0]);
-            }
-        }
+        group(0, true, x0[0], x1[0]);
+        if (G > 1 && 4 * N < l.n) group(1, false, x0[G - 1], x1[G - 1]);
         auto add = [&](int h, float *y) {
             float4 *at0 = reinterpret_cast<float4 *>(from + line0 + 1024 * h);
             float4 *at1 = reinterpret_cast<float4 *>(from + line1 + 1024 * h);

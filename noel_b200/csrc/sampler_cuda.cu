@@ -1203,10 +1203,8 @@ int lora_args(const noel_lora_t *l, const int32_t *adapter, const float *x, size
     a.vec_y = rows_on(y, ldy * 4, 0, 32) ? 2 : rows_on(y, ldy * 4, 0, 16) ? 1 : 0;
     a.vec_a = rows_on(l->d_a, l->lda * es, l->stride_a * es, 16);
     a.vec_b = rows_on(l->d_b, l->ldb * es, l->stride_b * es, lane_b);
-    a.staged = a.rank_pad * es > 256 ? 0
-               : rows_on(l->d_b, l->ldb * es, l->stride_b * es, 16) ? 16
-               : rows_on(l->d_b, l->ldb * es, l->stride_b * es, 4) && (a.rank_pad <= 32 || (a.rank_pad == 64 && es == 2)) ? 4
-                                                                                                                        : 0;
+    a.staged = rows_on(l->d_b, l->ldb * es, l->stride_b * es, 16) ? 16 : rows_on(l->d_b, l->ldb * es, l->stride_b * es, 4) ? 4 : 0;
+    a.r_count = l->rank;
     *out = a;
     return NOEL_OK;
 }
@@ -1260,13 +1258,19 @@ dim3 expand_grid(DeviceCtx *c, const LoraArgs &a, int items, int per_sm) {
     return dim3((unsigned)(all < want ? all : want), items);
 }
 
+/* The second kernel through shared memory, up to 4 N G ranks a launch.  The
+ * first launch may start while the kernel before it runs; the others read the
+ * y that the one before them wrote. */
 template <int WT, int N, int G, int D, bool WIDE>
-int expand_launch_y(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
-    const size_t smem = (size_t)(kExpandThreads / 32) * D * expand_stage_bytes(a.rank_pad, kWeightBytes<WT>);
+int expand_launch_y(DeviceCtx *c, const LoraArgs &all, int items, cudaStream_t s) {
+    const size_t smem = (size_t)(kExpandThreads / 32) * D * expand_stage_bytes(4 * N * G, kWeightBytes<WT>);
     const int r = set_smem(c, (const void *)lora_expand_kernel<WT, N, G, D, WIDE>, smem);
     if (r) return r;
-    CUDA_TRY((launch_cluster(lora_expand_kernel<WT, N, G, D, WIDE>, expand_grid(c, a, items, smem <= 112 * 1024 ? 2 : 1),
-                             kExpandThreads, smem, 1, true, s, a)));
+    LoraArgs a = all;
+    a.r_count = 4 * N * G;
+    for (a.r_begin = 0; a.r_begin < a.rank; a.r_begin += a.r_count)
+        CUDA_TRY((launch_cluster(lora_expand_kernel<WT, N, G, D, WIDE>, expand_grid(c, a, items, smem <= 112 * 1024 ? 2 : 1),
+                                 kExpandThreads, smem, 1, a.r_begin == 0, s, a)));
     return NOEL_OK;
 }
 template <int WT, int N, int G, int D>
@@ -1281,17 +1285,15 @@ int expand_any_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s
     return NOEL_OK;
 }
 
-/* The second kernel: through shared memory where two stages of a warp fit
- * (ranks up to 128, fp32 64) and rows of B start on 16 bytes, or on 4 (ranks
- * up to 64, fp32 32). */
+/* The second kernel: through shared memory where rows of B start on 16 bytes
+ * or on 4. */
 template <int WT>
 int expand(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
     constexpr bool kF32 = WT == kHeadF32;
     if (!a.staged) return a.rank_pad == 16 ? expand_any_launch<WT, 4>(c, a, items, s) : expand_any_launch<WT, 8>(c, a, items, s);
     if (a.rank_pad == 16) return expand_launch<WT, 4, 1, kF32 ? 3 : 4>(c, a, items, s);
-    if (a.rank_pad == 32) return expand_launch<WT, 8, 1, kF32 ? 2 : 3>(c, a, items, s);
-    if (a.rank_pad == 64 && !kF32) return expand_launch<WT, 8, kF32 ? 0 : 2, 2>(c, a, items, s);
-    return expand_launch<WT, 8, 0, 2>(c, a, items, s);
+    if (a.rank_pad == 32 || kF32) return expand_launch<WT, 8, 1, kF32 ? 2 : 3>(c, a, items, s);
+    return expand_launch<WT, 8, kF32 ? 1 : 2, 2>(c, a, items, s);
 }
 
 template <int WT>

@@ -77,7 +77,8 @@ def check(s):
 @pytest.mark.parametrize("B,D,V,r,n", [
     (1, 1, 1, 1, 1), (1, 64, 1000, 16, 3), (2, 5, 31, 3, 2), (7, 1000, 4099, 12, 3), (16, 2048, 513, 16, 1),
     (17, 256, 777, 8, 1), (33, 96, 2000, 32, 2), (33, 97, 2001, 33, 4), (100, 512, 999, 64, 7), (64, 128, 640, 17, 64),
-    (40, 72, 300, 128, 2), (9, 300, 1025, 256, 3), (130, 40, 130, 5, 2)])
+    (40, 72, 300, 128, 2), (9, 300, 1025, 256, 3), (130, 40, 130, 5, 2), (50, 128, 1000, 96, 2), (20, 64, 2052, 200, 2),
+    (70, 64, 1004, 130, 3)])
 def test_lora_gpu(cuda, B, D, V, r, n, dtype):
     check(build(cuda, B, D, V, r, n, dtype, seed=B + D + V))
 
@@ -97,7 +98,7 @@ def test_lora_odd_ranks_in_aligned_rows_gpu(cuda, r, pad, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("r", [8, 16, 48, 64])
+@pytest.mark.parametrize("r", [8, 16, 48, 64, 128, 224])
 def test_lora_ranks_of_their_own_gpu(cuda, r, dtype):
     check(build(cuda, 50, 200, 700, r, 6, dtype, seed=r, ragged=True))
 
