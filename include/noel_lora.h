@@ -44,8 +44,10 @@ size_t noel_lora_workspace_bytes(int batch, int rank);
  * d_x [batch][ldx] (cols used) and d_y [batch][ldy] (rows used) fp32, 4-byte
  * aligned.  A token whose d_adapter is outside 0 .. n_adapters - 1 has no
  * adapter and its row of d_y is left as it was.  Sums are in fp32 (every product
- * of fp16 and bf16 weights enters them exactly, of fp32 weights to 2^-30); a
- * token's result does not depend on which other tokens are in the batch.  Where
+ * of fp16 and bf16 weights enters them exactly, of fp32 weights to 2^-30), in an
+ * order that the sizes of the adapters give, and whether rows of d_x and A_i
+ * start on 16 bytes: a token's result does not depend on which and how many
+ * other tokens are in the batch, on its place there, or on n_adapters.  Where
  * a sum in fp32 is infinite or NaN the result is one of the two.  d_work
  * (16-byte aligned, work_bytes >= noel_lora_workspace_bytes(batch, rank)) is
  * scratch of this call until it has run.  Returns NOEL_OK or a negative

@@ -40,7 +40,6 @@ constexpr int kLoraBatch = 2048;    // tokens of one pass over the adapters
 constexpr int kLoraItem = 16;       // tokens of an item
 constexpr int kLoraWarpBatch = 32;  // tokens up to which every warp finds the items by itself (one token: 9.0 -> 7.5 us)
 constexpr int kShrinkThreads = 256;
-constexpr int kShrinkSplit = 8;     // CTAs of a cluster that share an item's columns, at most
 constexpr int kExpandThreads = 256;
 /* turns between asking the L2 for a line of y and copying it from there (2048 tokens at rank 64: 551 us without, 496,
  * 521 and 535 us at 1, 2 and 4) */
@@ -386,20 +385,30 @@ __device__ __forceinline__ LoraItem lora_item(const LoraArgs &a, int k) {
     return it;
 }
 
-/* One cluster per item (blockIdx.y) and 8 TILES ranks (blockIdx.z): its CTAs'
- * warps take the columns in turns of 32, each turn's products are added up
- * from 0 by the matrix instructions and then to the warp's sums in fp32 (the
- * instructions cut what they add to), the warps' sums are added in their order
- * and the CTAs' in theirs.  Few items are spread over clusters of up to eight
+/* One cluster per item (blockIdx.y) and 8 TILES ranks (blockIdx.z).  The
+ * columns are taken 32 at a time (a block), a block's products are added up
+ * from 0 by the matrix instructions and then to a sum in fp32 (the instructions
+ * cut what they add to).  Few items are spread over clusters of up to eight
  * CTAs: one CTA alone takes an item's weights (128 KB at rank 16 and 4096
- * columns) in at its own pace (the whole call: one token 12.3 us with one CTA,
- * 7.5 with eight; 64 adapters 86 and 77). */
-template <int WT, int TILES>
-__global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __grid_constant__ LoraArgs a) {
+ * columns) in at its own pace (the two kernels on the device: one token 12.3 us
+ * with one CTA, 7.6 with eight; 64 adapters 86 with one, 77 with four).
+ *
+ * The order of the additions does not depend on that split.  Block k belongs to
+ * sum k % 64, a number of the bits 5 .. 0.  The sums that differ in bits 5 and 4
+ * only are added in their order, the results that differ in bit 3 as a pair,
+ * those in bit 2, in bit 1 and in bit 0.  The CTA's number stands for the lowest
+ * bits, the warp's for the three above, and a warp makes the sums of all values
+ * of the rest in turn.  (Eight CTAs whatever the number of items: 2048 tokens at
+ * rank 64 534 against 509 us.  One CTA where two are taken: 75 adapters x 32,000
+ * rows 42.5 against 37.1.) */
+template <int WT, int TILES, int CTAS>
+__global__ void __launch_bounds__(kShrinkThreads, TILES == 2 || WT == kHeadBF16 ? 2 : 1) lora_shrink_kernel(const __grid_constant__ LoraArgs a) {
     constexpr int WARPS = kShrinkThreads / 32, RANKS = 8 * TILES;
     constexpr int ES = kWeightBytes<WT>;
-    __shared__ float part[WARPS][kLoraItem][RANKS];
-    __shared__ float2 gather[kShrinkSplit][kLoraItem][RANKS / 2];
+    constexpr int SUMS = 8 / CTAS, SETS = CTAS == 1 || CTAS == 4 ? 2 : 1;  // sums of a warp, and results it keeps apart
+    static_assert(WARPS == 8 && SUMS * CTAS == 8, "64 sums");
+    __shared__ float part[SETS][WARPS][kLoraItem][RANKS];
+    __shared__ float2 gather[CTAS][kLoraItem][RANKS / 2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan is there
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -408,7 +417,17 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __gri
     const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     auto begun = cluster.barrier_arrive();  // a CTA's shared memory is written by others once it has begun
     const int i = it.adapter, n = lora_rank(a, i), r0 = blockIdx.z * RANKS;
-    float acc[TILES][4] = {};
+    /* the warp's result in its place in part, or added to what is there */
+    auto keep = [&](int set, bool add, const float (&v)[TILES][4]) {
+#pragma unroll
+        for (int h = 0; h < TILES; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                float2 *to = reinterpret_cast<float2 *>(&part[set][warp][g + 4 * e][8 * h + 2 * q]);
+                const float2 o = add ? *to : make_float2(0.0f, 0.0f);
+                *to = make_float2(__fadd_rn(o.x, v[h][e]), __fadd_rn(o.y, v[h][e + 1]));
+            }
+    };
     if (r0 < n) {
         const float *x0 = a.x + (size_t)max(it.t0, 0) * (size_t)a.ldx, *x1 = a.x + (size_t)max(it.t1, 0) * (size_t)a.ldx;
         const char *w = static_cast<const char *>(a.a) + (size_t)i * (size_t)a.stride_a * ES;
@@ -416,7 +435,7 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __gri
 #pragma unroll
         for (int h = 0; h < TILES; ++h) wr[h] = w + (size_t)min(r0 + 8 * h + g, n - 1) * (size_t)a.lda * ES;
         const bool both = it.m > 8;
-        const int stride = WARPS * gridDim.x, whole = a.vec_x && a.vec_a ? a.cols / 32 : 0;
+        const int whole = a.vec_x && a.vec_a ? a.cols / 32 : 0;
         uint32_t p0[3][4] = {}, p1[3][4] = {};
         Raw<WT, 8> b[TILES];
         RawX f0, f1;
@@ -442,67 +461,94 @@ __global__ void __launch_bounds__(kShrinkThreads) lora_shrink_kernel(const __gri
 #pragma unroll
         for (int h = 0; h < TILES; ++h) b[h] = raw_zero<WT, 8>();
         const int blocks = (a.cols + 31) / 32;
-        int k0 = blockIdx.x * WARPS + warp;
-        if (k0 < blocks) load(k0);
-        for (; k0 < blocks; k0 += stride) {  // the next turn's numbers are on their way while this one's are multiplied
-            Weights<WT, 8> w8[TILES];
+        /* the block to load next, and which of this warp's sums it belongs to: alone, a CTA's warp makes the four
+         * sums of bit 3 clear before the others */
+        int at = 0, k0 = warp * CTAS + blockIdx.x;
+        const int first = k0;
+        auto skip = [&] {
+            while (k0 >= blocks && ++at < SUMS)
+                k0 = first + (CTAS == 1 ? 2 * (at & 3) + (at >> 2) : at) * (WARPS * CTAS);
+        };
+        skip();
+        if (at < SUMS) load(k0);
+#pragma unroll 1
+        for (int sum = 0; sum < SUMS; ++sum) {
+            float acc[TILES][4] = {};
+            while (at == sum) {  // the next block's numbers are on their way while this one's are multiplied
+                Weights<WT, 8> w8[TILES];
 #pragma unroll
-            for (int h = 0; h < TILES; ++h) w8[h] = weights<WT, 8>(b[h]);
-            if (it.t0 >= 0) split<8, 3>(f0.f, p0);
-            if (it.t1 >= 0) split<8, 3>(f1.f, p1);
-            if (k0 + stride < blocks) load(k0 + stride);
-            __syncwarp();
+                for (int h = 0; h < TILES; ++h) w8[h] = weights<WT, 8>(b[h]);
+                if (it.t0 >= 0) split<8, 3>(f0.f, p0);
+                if (it.t1 >= 0) split<8, 3>(f1.f, p1);
+                k0 += 8 * WARPS;
+                skip();
+                if (at < SUMS) load(k0);
+                __syncwarp();
 #pragma unroll
-            for (int h = 0; h < TILES; ++h) {
-                float c[4];
-                multiply<WT, 8>(c, true, p0, p1, w8[h]);
+                for (int h = 0; h < TILES; ++h) {
+                    float c[4];
+                    multiply<WT, 8>(c, true, p0, p1, w8[h]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[h][e] = __fadd_rn(acc[h][e], c[e]);
+                    for (int e = 0; e < 4; ++e) acc[h][e] = __fadd_rn(acc[h][e], c[e]);
+                }
             }
+            if (CTAS == 1) keep(sum >> 2, sum & 3, acc);
+            else if (CTAS == 4) keep(sum, false, acc);
+            else keep(0, sum > 0, acc);
         }
-    }
+    } else {
+        const float none[TILES][4] = {};
 #pragma unroll
-    for (int h = 0; h < TILES; ++h) {
-        *reinterpret_cast<float2 *>(&part[warp][g][8 * h + 2 * q]) = make_float2(acc[h][0], acc[h][1]);
-        *reinterpret_cast<float2 *>(&part[warp][g + 8][8 * h + 2 * q]) = make_float2(acc[h][2], acc[h][3]);
+        for (int k = 0; k < SETS; ++k) keep(k, false, none);
     }
     __syncthreads();
     /* two ranks of one token per thread: token `row` of the item */
     constexpr int PER_ROW = RANKS / 2, USED = kLoraItem * PER_ROW;
     static_assert(USED <= kShrinkThreads, "a thread for every two ranks");
     const int row = threadIdx.x / PER_ROW, r = 2 * (threadIdx.x % PER_ROW);
-    float u = 0.0f, v = 0.0f;
+    auto number = [&](int set, int k) { return *reinterpret_cast<const float2 *>(&part[set][k][row][r]); };
+    auto plus = [](float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); };
+    /* four in their order, from 0 as where a warp has added them */
+    auto row_of = [&](float2 a0, float2 a1, float2 a2, float2 a3) {
+        return plus(plus(plus(plus(make_float2(0.0f, 0.0f), a0), a1), a2), a3);
+    };
+    float2 s = make_float2(0.0f, 0.0f);
     if (threadIdx.x < USED) {
-#pragma unroll
-        for (int k = 0; k < WARPS; ++k) {
-            const float2 s = *reinterpret_cast<const float2 *>(&part[k][row][r]);
-            u = __fadd_rn(u, s.x);
-            v = __fadd_rn(v, s.y);
+        if (CTAS == 8) {  // the warp's number is bits 5 .. 3
+            s = plus(row_of(number(0, 0), number(0, 2), number(0, 4), number(0, 6)),
+                     row_of(number(0, 1), number(0, 3), number(0, 5), number(0, 7)));
+        } else if (CTAS == 4) {  // the set bit 5, the warp's number bits 4 .. 2
+            auto bit3 = [&](int w) {
+                return row_of(number(0, w), number(0, w + 4), number(1 % SETS, w), number(1 % SETS, w + 4));
+            };
+            s = plus(plus(bit3(0), bit3(2)), plus(bit3(1), bit3(3)));
+        } else {  // bits 3 .. 1; alone, the set bit 3 and the warp's number bits 2 .. 0
+            auto one = [&](int w) { return CTAS == 1 ? plus(number(0, w), number(1 % SETS, w)) : number(0, w); };
+            auto pair = [&](int w) { return plus(one(w), one(w + 4)); };
+            s = plus(plus(pair(0), pair(2)), plus(pair(1), pair(3)));
         }
     }
     cluster.barrier_wait(std::move(begun));
-    if (gridDim.x > 1) {
-        if (threadIdx.x < USED) *cluster.map_shared_rank(&gather[blockIdx.x][row][r / 2], 0) = make_float2(u, v);
+    if (CTAS > 1) {
+        if (threadIdx.x < USED) *cluster.map_shared_rank(&gather[blockIdx.x][row][r / 2], 0) = s;
         cluster.sync();
         if (blockIdx.x) return;
         if (threadIdx.x < USED) {
-            u = v = 0.0f;
-            for (int k = 0; k < (int)gridDim.x; ++k) {
-                const float2 s = gather[k][row][r / 2];
-                u = __fadd_rn(u, s.x);
-                v = __fadd_rn(v, s.y);
-            }
+            auto from = [&](int c) { return gather[c % CTAS][row][r / 2]; };
+            auto four = [&](int c) { return CTAS == 8 ? plus(from(c), from(c + 4)) : from(c); };
+            auto two = [&](int c) { return CTAS >= 4 ? plus(four(c), four(c + 2)) : from(c); };
+            s = plus(two(0), two(1));
         }
     }
+    float u = s.x, v = s.y;
     if (threadIdx.x >= USED) return;  // whole warps
     /* the token is what lanes 4 (row % 8) hold as t0 or t1 */
     const int ta = __shfl_sync(kFull, it.t0, 4 * (row & 7)), tb = __shfl_sync(kFull, it.t1, 4 * (row & 7));
     const int t = row < 8 ? ta : tb;
     if (t < 0) return;
     if (a.scale) {
-        const float s = a.scale[i];
-        u = __fmul_rn(u, s);
-        v = __fmul_rn(v, s);
+        u = __fmul_rn(u, a.scale[i]);
+        v = __fmul_rn(v, a.scale[i]);
     }
     if (r0 + r >= n) u = 0.0f;  // not even an infinite scale gives an unused rank a value
     if (r0 + r + 1 >= n) v = 0.0f;

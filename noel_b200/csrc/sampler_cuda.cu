@@ -1235,13 +1235,18 @@ cudaError_t launch_cluster(void (*k)(P...), dim3 grid, int threads, size_t smem,
     return cudaLaunchKernelEx(&lc, k, args...);
 }
 
+template <int WT, int TILES, int CTAS>
+cudaError_t shrink_launch_split(const LoraArgs &a, int items, int groups, cudaStream_t s) {
+    return launch_cluster(lora_shrink_kernel<WT, TILES, CTAS>, dim3(CTAS, items, groups), kShrinkThreads, 0, CTAS,
+                          a.plan != nullptr, s, a);
+}
 template <int WT, int TILES>
 cudaError_t shrink_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
-    const int groups = a.rank_pad / (8 * TILES);
-    int split = 1;
-    while (split < kShrinkSplit && split * items * groups <= c->sms && split * kShrinkThreads < a.cols) split *= 2;
-    return launch_cluster(lora_shrink_kernel<WT, TILES>, dim3(split, items, groups), kShrinkThreads, 0, split,
-                          a.plan != nullptr, s, a);
+    const int groups = a.rank_pad / (8 * TILES), ctas = items * groups;  // CTAs without a split
+    if (4 * ctas <= c->sms && a.cols > 4 * kShrinkThreads) return shrink_launch_split<WT, TILES, 8>(a, items, groups, s);
+    if (2 * ctas <= c->sms && a.cols > 2 * kShrinkThreads) return shrink_launch_split<WT, TILES, 4>(a, items, groups, s);
+    if (ctas <= c->sms && a.cols > kShrinkThreads) return shrink_launch_split<WT, TILES, 2>(a, items, groups, s);
+    return shrink_launch_split<WT, TILES, 1>(a, items, groups, s);
 }
 
 /* CTAs per item of the second kernel: one turn of the GPU's CTA slots where

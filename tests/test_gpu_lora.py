@@ -259,3 +259,35 @@ def test_lora_python_refusals_gpu(cuda):
             call()
     torch.cuda.synchronize()
     assert torch.equal(s["y"], y0)
+
+
+def alone(s, y0, t):
+    """token t's row of y where it is the whole batch"""
+    part = {**s, "y": y0[t:t + 1].clone(), "x": s["x"][t:t + 1].contiguous(), "ids": s["ids"][t:t + 1].contiguous()}
+    apply(part)
+    return part["y"]
+
+
+@pytest.mark.parametrize("dtype,B,D,V,r,n", [("bf16", 64, 4096, 300, 16, 64), ("bf16", 2048, 4096, 200, 64, 4),
+                                             ("f16", 256, 4096, 264, 32, 8), ("f32", 150, 8192, 130, 33, 40),
+                                             ("bf16", 2049, 2048, 130, 8, 2), ("f16", 2100, 5000, 77, 200, 3)])
+def test_lora_a_token_alone_has_the_batch_s_bits_gpu(cuda, dtype, B, D, V, r, n):
+    """columns enough for one token's to be shared by more CTAs than a batch's; the last tokens are a second pass's"""
+    import torch
+
+    s = build(cuda, B, D, V, r, n, dtype, seed=B + r, without=0.0)
+    y0 = s["y"].clone()
+    apply(s)
+    for t in [*range(0, B, B // 8 + 1), B - 1]:
+        assert torch.equal(alone(s, y0, t).view(torch.int32), s["y"][t:t + 1].view(torch.int32)), t
+
+
+def test_lora_resident_adapters_change_no_bit_gpu(cuda):
+    import torch
+
+    s = build(cuda, 64, 4096, 300, 16, 256, "bf16", seed=21, without=0.0)
+    s["ids"] %= 2
+    few = {**s, "y": s["y"].clone(), "a": s["a"][:2], "b": s["b"][:2], "scale": s["scale"][:2]}
+    apply(s)
+    apply(few)
+    assert torch.equal(few["y"].view(torch.int32), s["y"].view(torch.int32))
