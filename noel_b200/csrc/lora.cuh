@@ -604,14 +604,27 @@ struct ExpandLane {
     }
 };
 
-/* 32 rows from v0 on, any alignment, sizes and end */
-template <int WT, int N>
+/* 32 rows from v0 on, any alignment, sizes and end; the sums are those of the
+ * kernel below, bit for bit: up to 4 N G ranks by matrix instructions from 0 on,
+ * and each such sum added to y in fp32 */
+template <int WT, int N, int G>
 __device__ __forceinline__ void expand_any(const LoraArgs &a, const ExpandLane<WT> &l, int64_t v0) {
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    float c[4][4] = {};
+    if (l.n == 0) return;
+    float y[4][4] = {}, c[4][4] = {};
+    auto each = [&](auto what) {  // number k of instruction j's result and its place in y
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int j = k >> 2, h = k >> 1 & 1, b = k & 1;
+            const int64_t v = v0 + (l.wide ? 8 * q + 2 * j + b : 8 * j + 2 * q + b);
+            if ((h ? l.it.t1 : l.it.t0) >= 0 && v < a.rows) what(y[j][2 * h + b], (h ? l.y1 : l.y0) + v);
+        }
+    };
+    each([](float &f, float *p) { f = *p; });
     uint32_t x0[3][N / 2] = {}, x1[3][N / 2] = {};
     for (int r0 = 0; r0 < l.n; r0 += 4 * N) {
         const int r = r0 + N * q;
+        const bool last = r0 / (4 * N) % G == G - 1 || r0 + 4 * N >= l.n;  // of a sum
         if (l.it.t0 >= 0) load_low<N>(a, l.it.t0, r, x0);
         if (l.it.t1 >= 0) load_low<N>(a, l.it.t1, r, x1);
 #pragma unroll
@@ -626,26 +639,23 @@ __device__ __forceinline__ void expand_any(const LoraArgs &a, const ExpandLane<W
             const Weights<WT, N> wb = weights<WT, N>(b);
             __syncwarp();
             multiply<WT, N>(c[j], false, x0, x1, wb);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!last) continue;
+                y[j][e] = __fadd_rn(y[j][e], c[j][e]);
+                c[j][e] = 0.0f;
+            }
         }
     }
-    if (l.n == 0) return;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        if ((h ? l.it.t1 : l.it.t0) < 0) continue;
-        float *y = h ? l.y1 : l.y0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int64_t v = v0 + (l.wide ? 8 * q + e : 8 * (e / 2) + 2 * q + (e & 1));
-            if (v < a.rows) y[v] = __fadd_rn(y[v], c[e / 2][2 * h + (e & 1)]);
-        }
-    }
+    each([](float &f, float *p) { *p = f; });
 }
 
 /* The second kernel for arrays that the one below cannot take (rows of B_i that
  * start on 2 bytes): one item per blockIdx.y, a warp its 32
- * rows at a time.  Where both could, it takes 11.3 us for one token and 207 for
- * 64 adapters against 7.5 and 77. */
-template <int WT, int N>
+ * rows at a time, y on its way while the products are formed (100 tokens x 50,001
+ * rows at rank 33: 126 -> 55 us).  Where both could, without that, it took 11.3
+ * us for one token and 207 for 64 adapters against 7.5 and 77. */
+template <int WT, int N, int G>
 __global__ void __launch_bounds__(kExpandThreads) lora_expand_any_kernel(const __grid_constant__ LoraArgs a) {
     const LoraItem it = lora_item(a, blockIdx.y);  // the kernel before let this one begin when the plan was there
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -653,7 +663,7 @@ __global__ void __launch_bounds__(kExpandThreads) lora_expand_any_kernel(const _
     const ExpandLane<WT> l(a, it, N);
     const int64_t step = (int64_t)gridDim.x * (kExpandThreads / 32) * 32;
     for (int64_t v0 = ((int64_t)blockIdx.x * (kExpandThreads / 32) + (threadIdx.x >> 5)) * 32; v0 < a.rows; v0 += step)
-        expand_any<WT, N>(a, l, v0);
+        expand_any<WT, N, G>(a, l, v0);
 }
 
 __device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
@@ -681,7 +691,11 @@ __host__ __device__ constexpr int expand_stage_bytes(int ranks, int es) {
  *
  * N is the number of ranks a lane holds: 4 for ranks up to 16, else 8 (a group
  * of 32 ranks at a time).  A launch takes up to 4 N G ranks, whose low-rank
- * numbers stay in registers; adapters of more ranks take several launches.
+ * numbers stay in registers; adapters of more ranks take several launches.  The
+ * ranks of a launch are one chain of matrix instructions, which cut where fp32
+ * rounds: 12 steps (fp16 weights 24), less than the 63 roundings of a
+ * sum in fp32 may be off by.  (Each 32 ranks from 0 and added in fp32: 2048
+ * tokens at rank 64 531 -> 600 us.)
  * (All ranks in one launch, with two stages and their numbers read again every
  * turn: 512 tokens at rank 128 522 us against 281, 16 adapters 180 against 124.)  WIDE: rows of y and of B_i start on
  * 16 bytes.  Without it rows of y start anywhere: their 32 numbers are copied
@@ -864,7 +878,7 @@ __global__ void __launch_bounds__(kExpandThreads, 2) lora_expand_kernel(const __
             for (int k = 0; k < it.m; ++k) y_back[y_off[warp][k]] = *reinterpret_cast<const float *>(from + line_of(k));
         }
     }
-    if (first + turns * step < a.rows) expand_any<WT, N>(a, l, first + turns * step);  // the last rows
+    if (first + turns * step < a.rows) expand_any<WT, N, G>(a, l, first + turns * step);  // the last rows
 }
 
 }  // namespace noel

@@ -1284,9 +1284,9 @@ int expand_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
                                      : expand_launch_y<WT, N, G, D, false>(c, a, items, s);
 }
 
-template <int WT, int N>
+template <int WT, int N, int G>
 int expand_any_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
-    CUDA_TRY((launch_cluster(lora_expand_any_kernel<WT, N>, expand_grid(c, a, items, 2), kExpandThreads, 0, 1, true, s, a)));
+    CUDA_TRY((launch_cluster(lora_expand_any_kernel<WT, N, G>, expand_grid(c, a, items, 2), kExpandThreads, 0, 1, true, s, a)));
     return NOEL_OK;
 }
 
@@ -1295,7 +1295,9 @@ int expand_any_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s
 template <int WT>
 int expand(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
     constexpr bool kF32 = WT == kHeadF32;
-    if (!a.staged) return a.rank_pad == 16 ? expand_any_launch<WT, 4>(c, a, items, s) : expand_any_launch<WT, 8>(c, a, items, s);
+    if (!a.staged)
+        return a.rank_pad == 16 ? expand_any_launch<WT, 4, 1>(c, a, items, s)
+                                : expand_any_launch<WT, 8, kF32 ? 1 : 2>(c, a, items, s);
     if (a.rank_pad == 16) return expand_launch<WT, 4, 1, kF32 ? 3 : 4>(c, a, items, s);
     if (a.rank_pad == 32 || kF32) return expand_launch<WT, 8, 1, kF32 ? 2 : 3>(c, a, items, s);
     return expand_launch<WT, 8, kF32 ? 1 : 2, 2>(c, a, items, s);

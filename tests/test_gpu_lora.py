@@ -291,3 +291,43 @@ def test_lora_resident_adapters_change_no_bit_gpu(cuda):
     apply(s)
     apply(few)
     assert torch.equal(few["y"].view(torch.int32), s["y"].view(torch.int32))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("r", [16, 24, 40, 64, 100, 128, 256])
+def test_lora_the_layout_of_b_changes_no_bit_gpu(cuda, r, dtype):
+    """rows of B on 16 bytes and on 2: the same sums in the same order"""
+    import torch
+
+    s = build(cuda, 40, 256, 1100, r, 3, dtype, seed=r, without=0.0)
+    store = torch.zeros(3, 1100, r + 1 + r % 2, dtype=s["b"].dtype, device=cuda)
+    store[:, :, :r] = s["b"]
+    odd = {**s, "y": s["y"].clone(), "b": store[:, :, :r]}
+    apply(s)
+    apply(odd)
+    assert torch.equal(odd["y"].view(torch.int32), s["y"].view(torch.int32))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("r,far", [(128, 64), (128, 127), (200, 130), (256, 65), (256, 255)])
+def test_lora_sums_of_64_ranks_are_added_in_fp32_gpu(cuda, r, far, pad, dtype):
+    """Row v of B is 1 at rank 0 and c_v at a rank of another 64, A x is 1 at the one and 2^-23 at the other, y is 0: of the sum
+    1 + c_v 2^-23, whose two numbers are exact, the fp32 addition's rounding is all that is left.  No c_v is a tie."""
+    import torch
+
+    c = torch.tensor([0.25, 0.375, 0.5625, 0.625, 0.75, 0.875, 0.9375, 1.25, 1.625, -0.125, -0.375, -0.75], device=cuda)
+    V, tt = 12 * 31, {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    c = c.repeat(31)
+    a = torch.zeros(1, r, 8, dtype=tt, device=cuda)
+    a[0, 0, 0] = 1.0
+    a[0, far, 1] = 1.0
+    b = torch.zeros(1, V, r + pad, dtype=tt, device=cuda)
+    b[0, :, 0] = 1.0
+    b[0, :, far] = c
+    x = torch.zeros(3, 8, device=cuda)
+    x[:, 0], x[:, 1] = 1.0, 2.0 ** -23
+    s = {"y": torch.zeros(3, V, device=cuda), "x": x, "a": a, "b": b[:, :, :r], "scale": None, "ranks": None,
+         "ids": torch.zeros(3, dtype=torch.int32, device=cuda)}
+    apply(s)
+    assert torch.equal(s["y"], (1.0 + c.double() * 2.0 ** -23).float().expand(3, V))
