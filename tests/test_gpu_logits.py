@@ -347,3 +347,20 @@ def test_process_python_refusals_gpu(cuda):
             call()
     torch.cuda.synchronize()
     assert not x.any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V,H,bias,pad", [(60001, 9000, 0, 0), (60001, 9000, 300, 5), (152064, 9000, 300, 0),
+                                          (152064, 1500, 21, 64), (24577, 30000, 16384, 31)])
+@pytest.mark.parametrize("v_begin", [0, 45, 100000])
+def test_process_long_histories_over_slices_gpu(cuda, v_begin, V, H, bias, pad, dtype):
+    """several slices a row, rows on 32 bytes and off them, ids below and above a shard's columns"""
+    t, p = build(4, V, dtype, seed=V + H + v_begin, pad=pad, H=H, bias=bias, masks=3, density=0.7, v_begin=v_begin)
+    check(cuda, t, p, V, dtype, v_begin=v_begin)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_process_long_histories_uniform_and_whole_gpu(cuda, dtype):
+    """ids of every line of every slice, all of them generated, no mask"""
+    t, p = build(3, 100003, dtype, seed=8, pad=13, H=60000, lens=False, zipf=False)
+    check(cuda, t, p, 100003, dtype)
