@@ -55,7 +55,6 @@ struct LogitsArgs {
 
 constexpr int kLogitsThreads = 256;
 constexpr int kRowsCtas = 6;         // CTAs per SM the rows kernel is compiled for
-constexpr int kLogitsSms = 148;
 constexpr int kMaskPiece = 1024;     // columns of a warp's turn: 32 words of the mask
 constexpr int kMaskRange = 131072;   // bytes of a row that a CTA masks, at most
 constexpr int kMaskWhole = 22;       // touched sectors of 32 from which on they are written whole

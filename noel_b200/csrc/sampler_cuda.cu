@@ -1047,13 +1047,26 @@ int logits_args(const noel_logits_params_t *p, void *logits, int dtype, int B, i
     a.mld = (int64_t)p->mld;
     a.mask_rows = p->mask_rows;
     a.mask_row = p->d_mask_rows;
+    if (B > 1 << 30) return fail(NOEL_ERR_TOO_LARGE, "%d rows x %d columns", B, V);
+    *out = a;
+    return NOEL_OK;
+}
+
+/* how the work of those arguments is cut for this device */
+int logits_plan(const DeviceCtx *c, int dtype, LogitsArgs *out) {
+    LogitsArgs &a = *out;
+    const int B = a.batch, V = a.vocab;
+    const int64_t es = dtype == NOEL_DTYPE_F32 ? 4 : 2;
     /* A row's history and biases go into a table, or are counted over slices of its columns: the table up to
-     * kTableMax of them, but for a batch whose slices run all at once from 1024 on (16 rows of 152,064 with 1024,
-     * 2048, 4096 and 8192 ids: table 7.6, 11.4, 17.2, 33.1 us, slices 7.7, 8.4, 8.9, 10.2; 256 rows: table 9.6, 15.4,
-     * 27.2, 73.8, slices 56, 64, 78, 96). */
+     * kTableMax of them, but for a batch whose slices run all at once from 1024 on.  fp32 rows, Zipf, no biases, table
+     * against slices at 1024, 2048, 4096 and 8192 ids in us.  All at once: 16 x 152,064 7.7 10.1 16.6 31.4 against 7.5
+     * 7.9 8.5 9.4; 16 x 256,000 8.0 10.6 17.4 31.2 against 8.4 9.2 10.1 11.4; 64 x 32,000 7.3 9.9 16.0 27.1 against 7.7
+     * 7.9 8.0 8.7.  Not at once: 256 x 152,064 9.6 12.8 25.5 69.6 against 52 59 73 89; 256 x 256,000 9.1 13.8 27.7 72.4
+     * against 84 94 115 141; 256 x 32,000 8.2 11.8 19.3 51.0 against 18.8 20.1 21.5 26.1 (the one place where the rule
+     * is off: few slices and many ids). */
     const int n = a.hist_len + a.bias_len;
     const int slices = pow2_at_least((int)(((int64_t)V + kSliceMax - 1) / kSliceMax));
-    const bool at_once = (int64_t)B * slices <= 2 * kLogitsSms;
+    const bool at_once = (int64_t)B * slices <= 2 * c->sms;
     if (n > 0 && n <= (at_once ? 1024 : kTableMax)) {
         a.cap = pow2_at_least(n + n / 2 > kLogitsThreads ? n + n / 2 : kLogitsThreads);
     } else if (n > 0) {
@@ -1067,15 +1080,14 @@ int logits_args(const noel_logits_params_t *p, void *logits, int dtype, int B, i
         /* ranges that give each of the GPU's CTA slots two, in whole turns of a CTA's warps: a large batch
          * runs fastest at 128 KB (1024 x 152,064 fp32 under strict masks: 145, 125, 120 and 121 us at 32, 64,
          * 128 and 256 KB), a small one with a turn per warp */
-        const int64_t turn = (int64_t)kMaskPiece * (kLogitsThreads / 32), most = kMaskRange / (int64_t)es;
-        int64_t want = (int64_t)B * V / (2 * kRowsCtas * kLogitsSms) / turn * turn;
+        const int64_t turn = (int64_t)kMaskPiece * (kLogitsThreads / 32), most = kMaskRange / es;
+        int64_t want = (int64_t)B * V / (2 * kRowsCtas * c->sms) / turn * turn;
         want = want < turn ? turn : want;
         a.range = (int)(want < most ? want : most);
         a.ranges = (int)(((int64_t)V + 15 + a.range - 1) / a.range);
     }
-    if (B > 1 << 30 || (int64_t)B * a.slices > 0x7FFFFFFF || (int64_t)B * a.ranges > 0x7FFFFFFF)
+    if ((int64_t)B * a.slices > 0x7FFFFFFF || (int64_t)B * a.ranges > 0x7FFFFFFF)
         return fail(NOEL_ERR_TOO_LARGE, "%d rows x %d columns", B, V);
-    *out = a;
     return NOEL_OK;
 }
 
@@ -1130,6 +1142,7 @@ extern "C" int noel_logits_process(const noel_logits_params_t *params, void *d_l
     if (batch == 0) return ok();
     DeviceCtx *c = nullptr;
     r = device_ctx(&c);
+    if (!r) r = logits_plan(c, dtype, &a);
     if (r) return r;
     r = logits_launch(c, a, dtype, static_cast<cudaStream_t>(stream));
     return r ? r : ok();
@@ -1412,6 +1425,7 @@ extern "C" int noel_lmhead_sample_ex(const noel_sampler_config_t *cfg, const voi
     if (batch == 0) return ok();
     DeviceCtx *c = nullptr;
     r = device_ctx(&c);
+    if (!r && process) r = logits_plan(c, NOEL_DTYPE_F32, &pa);
     if (r) return r;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     for (int t0 = 0; t0 < batch;) {
