@@ -521,43 +521,29 @@ __global__ void __launch_bounds__(kSliceThreads, 2) logits_slice_kernel(const __
      * is read and written whole; rows that do not start on 32 bytes, and the
      * row's last line, go by element */
     const bool lines = (reinterpret_cast<uintptr_t>(x) & 31) == 0;
-    constexpr int BATCH = 1;  // sectors of a lane that are on their way at a time
-    for (int s0 = tid; s0 * VE < width; s0 += BATCH * kSliceThreads) {  // width / VE is a multiple of 32: whole warps
-        Sector s[BATCH];
-        uint32_t w[BATCH][VE], change[BATCH];
-        int col[BATCH];
-        bool whole[BATCH];
+    for (int s0 = tid; s0 * VE < width; s0 += kSliceThreads) {  // width / VE is a multiple of 32: whole warps
+        const int at = s0 * VE;
+        uint32_t w[VE], change = 0u;
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-            const int at = (s0 + b * kSliceThreads) * VE;
-            change[b] = 0u;
-            whole[b] = false;
-            if (at >= width) continue;
-#pragma unroll
-            for (int e = 0; e < VE; e += 4) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(word + at + e);
-                w[b][e] = q.x, w[b][e + 1] = q.y, w[b][e + 2] = q.z, w[b][e + 3] = q.w;
-            }
-#pragma unroll
-            for (int e = 0; e < VE; ++e)
-                if (w[b][e] && !(w[b][e] & kHasBias)) change[b] |= 1u << e;
-            const int c = col[b] = ((at / BLK << sh) + (int)mine_c) * BLK + at % BLK;
-            if (mask && change[b]) change[b] &= mask_bits(a, mask, c);
-            const uint32_t touched = __ballot_sync(kFull, change[b] != 0u);
-            whole[b] = (touched >> (tid & 28) & 15u) && lines && (int64_t)(c - c % BLK) + BLK <= a.vocab;
-            if (whole[b]) s[b] = sector_load(x + c);
+        for (int e = 0; e < VE; e += 4) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(word + at + e);
+            w[e] = q.x, w[e + 1] = q.y, w[e + 2] = q.z, w[e + 3] = q.w;
         }
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-            T *p = x + col[b];
-            if (whole[b]) {
-                if (change[b]) sector_penalise<T>(s[b], w[b], change[b], rules);
-                sector_store(p, s[b]);
-            } else if (change[b]) {
+        for (int e = 0; e < VE; ++e)
+            if (w[e] && !(w[e] & kHasBias)) change |= 1u << e;
+        const int c = ((at / BLK << sh) + (int)mine_c) * BLK + at % BLK;
+        if (mask && change) change &= mask_bits(a, mask, c);
+        const uint32_t touched = __ballot_sync(kFull, change != 0u);
+        T *p = x + c;
+        if ((touched >> (tid & 28) & 15u) && lines && (int64_t)(c - c % BLK) + BLK <= a.vocab) {
+            Sector s = sector_load(p);
+            if (change) sector_penalise<T>(s, w, change, rules);
+            sector_store(p, s);
+        } else if (change) {
 #pragma unroll
-                for (int e = 0; e < VE; ++e)
-                    if (change[b] >> e & 1u) logit_store(p + e, penalised(logit_load(p + e), w[b][e], rules));
-            }
+            for (int e = 0; e < VE; ++e)
+                if (change >> e & 1u) logit_store(p + e, penalised(logit_load(p + e), w[e], rules));
         }
     }
     if (nb) __syncthreads();  // the lines are written; biased logits were written as they were read

@@ -1308,9 +1308,9 @@ int expand_any_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s
 template <int WT>
 int expand(DeviceCtx *c, const LoraArgs &a, int items, cudaStream_t s) {
     constexpr bool kF32 = WT == kHeadF32;
-    if (!a.staged)
-        return a.rank_pad == 16 ? expand_any_launch<WT, 4, 1>(c, a, items, s)
-                                : expand_any_launch<WT, 8, kF32 ? 1 : 2>(c, a, items, s);
+    if constexpr (!kF32)  // fp32 rows always start on 4
+        if (!a.staged)
+            return a.rank_pad == 16 ? expand_any_launch<WT, 4, 1>(c, a, items, s) : expand_any_launch<WT, 8, 2>(c, a, items, s);
     if (a.rank_pad == 16) return expand_launch<WT, 4, 1, kF32 ? 3 : 4>(c, a, items, s);
     if (a.rank_pad == 32 || kF32) return expand_launch<WT, 8, 1, kF32 ? 2 : 3>(c, a, items, s);
     return expand_launch<WT, 8, kF32 ? 1 : 2, 2>(c, a, items, s);

@@ -26,10 +26,6 @@ __device__ __forceinline__ void sector_store(void *p, const Sector &s) {
                  : "memory");
 }
 /* the same on 16-byte aligned memory */
-__device__ __forceinline__ Sector sector_load16(const void *p) {
-    const uint4 a = static_cast<const uint4 *>(p)[0], b = static_cast<const uint4 *>(p)[1];
-    return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-}
 __device__ __forceinline__ void sector_store16(void *p, const Sector &s) {
     static_cast<uint4 *>(p)[0] = make_uint4(s.u[0], s.u[1], s.u[2], s.u[3]);
     static_cast<uint4 *>(p)[1] = make_uint4(s.u[4], s.u[5], s.u[6], s.u[7]);
