@@ -546,6 +546,8 @@ class LogitsParams:
             s.mld, s.mask_rows = _pitch(mask), mask.shape[0]
             s.d_mask_rows = _row_values(mask_rows, i32, B, "mask_rows", dev)
             self.words = mask.shape[1]
+        if not 0 <= v_begin < 2**31:  # ctypes would keep its lowest 32 bits
+            _refuse(f"v_begin {v_begin}")
         s.v_begin = v_begin
         self.ref = C.byref(s)
 
@@ -573,7 +575,7 @@ def logits_process(logits, params: LogitsParams, vocab: int | None = None, strea
     ptr = _on(logits, logits.dtype, (None, None), "logits", dev)
     B, cols = logits.shape
     V = cols if vocab is None else vocab
-    if V > cols:
+    if not 0 < V <= cols:
         _refuse(f"vocab {V} of {cols} columns")
     params.check(logits, V)
     _call(dev, stream, lambda s: lib().noel_logits_process(params.ref, ptr, dtype, B, V, _pitch(logits), s))

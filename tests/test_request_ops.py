@@ -209,3 +209,12 @@ def test_python_refusals_without_a_gpu():
         S.Adapters(torch.zeros(1, 2, 8), torch.zeros(1, 9, 2))
     with pytest.raises(S.NoelSamplerError):
         S.Adapters(torch.zeros(1, 2, 8, dtype=torch.int32), torch.zeros(1, 9, 2))
+
+
+@pytest.mark.parametrize("v_begin", [-1, 2**31, 2**32, 2**32 + 5, -2**32 + 5])
+def test_python_refuses_a_first_id_that_is_no_int(v_begin):
+    """not taken for its lowest 32 bits"""
+    from noel_b200 import sampler as S
+
+    with pytest.raises(S.NoelSamplerError):
+        S.LogitsParams(v_begin=v_begin)
