@@ -656,17 +656,21 @@ def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: 
     import torch
 
     wt = {torch.float32: HEAD_F32, torch.float16: HEAD_F16, torch.bfloat16: HEAD_BF16}[weight.dtype]
-    assert weight.is_cuda and hidden.is_cuda and hidden.dtype == torch.float32
-    V, D = weight.shape
-    B = hidden.shape[0]
     dev = weight.device
+    wp = _on(weight, weight.dtype, (None, None), "weight", dev)
+    V, D = weight.shape
+    xp = _on(hidden, torch.float32, (None, D), "hidden", dev)
+    B = hidden.shape[0]
+    gp = _on(rng, torch.int64, (B, 2), "rng", dev)
+    if not rng.is_contiguous():
+        _refuse("rng: rows side by side wanted")
     if (adapters is None) != (adapter_ids is None):
         _refuse("adapters and adapter_ids come together")
     logits = torch.empty(B, V, dtype=torch.float32, device=dev)
     ids = torch.empty(B, dtype=torch.int32, device=dev)
     pr = torch.empty(B, dtype=torch.float32, device=dev) if probs else None
     if history is not None:
-        hp, H, hld = history.data_ptr(), history.shape[1], history.stride(0)
+        hp, H, hld = _on(history, torch.int32, (B, None), "history", dev), history.shape[1], _pitch(history)
     else:
         hp, H, hld = None, 0, 0
     lora = ip = work = None
@@ -680,7 +684,7 @@ def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: 
     if process is not None:
         process.check(logits, V)
     _call(dev, None, lambda s: lib().noel_lmhead_sample_ex(
-        C.byref(cfg), weight.data_ptr(), wt, weight.stride(0), hidden.data_ptr(), hidden.stride(0), B, D, V, lora, ip,
-        process.ref if process is not None else None, hp, H, hld, rng.data_ptr(), ids.data_ptr(),
+        C.byref(cfg), wp, wt, _pitch(weight), xp, _pitch(hidden), B, D, V, lora, ip,
+        process.ref if process is not None else None, hp, H, hld, gp, ids.data_ptr(),
         pr.data_ptr() if pr is not None else None, logits.data_ptr(), work.data_ptr() if size else None, size, s))
     return ids, logits, pr

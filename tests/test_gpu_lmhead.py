@@ -57,3 +57,25 @@ def test_lmhead_rejects_ragged_width_gpu(cuda):
     rng = torch.ones(1, 2, dtype=torch.int64, device=cuda)
     with pytest.raises(S.NoelSamplerError):
         S.lmhead_sample(w, torch.zeros(1, 12, device=cuda), rng, S.make_config())
+
+
+def test_lmhead_python_refusals_gpu(cuda):
+    """tensors of fewer rows or columns than the call would read or write"""
+    import torch
+
+    from noel_b200 import sampler as S
+
+    w, x = torch.zeros(100, 16, device=cuda), torch.zeros(4, 16, device=cuda)
+    rng = torch.ones(4, 2, dtype=torch.int64, device=cuda)
+    h = torch.zeros(4, 5, dtype=torch.int32, device=cuda)
+    cfg = S.make_config()
+    for a in ((w, x[:, :8], rng), (w, x.half(), rng), (w, x[0], rng), (w.cpu(), x, rng), (w, x.cpu(), rng),
+              (w.T, x, rng), (w, x, rng[:3]), (w, x, rng[:, :1]), (w, x, rng.int()), (w, x, rng.cpu()),
+              (w, x, torch.ones(4, 3, dtype=torch.int64, device=cuda)[:, :2])):
+        with pytest.raises(S.NoelSamplerError):
+            S.lmhead_sample(*a, cfg)
+    for bad in (h[:3], h.long(), h.cpu(), h[0], h[:, ::2]):
+        with pytest.raises(S.NoelSamplerError):
+            S.lmhead_sample(w, x, rng, cfg, history=bad)
+    torch.cuda.synchronize()
+    assert bool((rng == 1).all())
