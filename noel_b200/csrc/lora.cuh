@@ -17,12 +17,14 @@
  * parts' of two fp32 numbers (2^-30 of the product), so a sum is as exact as
  * in fp32.
  *
- * Measured at 152,064 rows x 4096 columns: one token at rank 16 in 7.5 us; 64
- * tokens with 64 bf16 adapters of rank 16 in 77 us (399 MB, 5.2 TB/s); 256
- * tokens over eight fp16 adapters of ranks up to 32 in 75 us (287 MB); 2048
- * tokens over four bf16 adapters of rank 64 in 500 us (2.6 GB, 5.2 TB/s).  The
- * second kernel's time: half of the issue slots and 40 % of the matrix pipe are
- * busy at rank 16, so memory is not all that bounds it there.
+ * Measured on the device, in a CUDA graph, at 152,064 rows x 4096 columns (and
+ * as back-to-back calls from Python): one token at rank 16 in 7.4 us (14.5); 64
+ * tokens with 64 bf16 adapters of rank 16 in 77 us (84; 399 MB, 5.2 TB/s); 256
+ * tokens over eight fp16 adapters of ranks up to 32 in 73 us (78; 287 MB); 2048
+ * tokens over four bf16 adapters of rank 64 in 510 us (556; 2.6 GB, 5.1 TB/s).
+ * What bounds the second kernel: at rank 16 nothing alone, half of the issue
+ * slots, 41 % of the matrix pipe and 5.2 TB/s of memory are busy; at rank 64
+ * memory at 5.6 TB/s, with 36 % of the issue slots and 52 % of the matrix pipe.
  */
 #pragma once
 

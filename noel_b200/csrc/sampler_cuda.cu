@@ -1265,7 +1265,9 @@ cudaError_t shrink_launch(DeviceCtx *c, const LoraArgs &a, int items, cudaStream
 /* CTAs per item of the second kernel: one turn of the GPU's CTA slots where
  * that is enough work for them, else kExpandWaves, so that items of unlike size
  * even out.  Just under whole turns: items is a bound, and about batch / 16 or
- * as many as there are adapters will come. */
+ * as many as there are adapters will come.  That holds where the batch uses the
+ * resident adapters; where it does not, items get too few CTAs (256 tokens over
+ * two of 256 adapters 107 us, over two of two 60). */
 dim3 expand_grid(DeviceCtx *c, const LoraArgs &a, int items, int per_sm) {
     const int rows = 32 * (kExpandThreads / 32);
     const int64_t all = ((int64_t)a.rows + rows - 1) / rows, slots = (int64_t)c->sms * per_sm;
