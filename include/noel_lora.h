@@ -48,10 +48,10 @@ size_t noel_lora_workspace_bytes(int batch, int rank);
  * columns at a time, and of B_i times that, 64 ranks at a time (fp32 weights
  * 32), are added by matrix instructions of 16 products, which add in 32 bits and
  * cut where fp32 rounds; those sums are added in fp32, the latter to d_y one
- * after the other.  The order depends on the adapters' sizes and on whether rows
- * of d_x and A_i start on 16 bytes: a token's result does not depend on which
- * and how many other tokens are in the batch, on its place there, on n_adapters
- * or on where rows of B_i and d_y start.  Where a sum in fp32 is infinite or NaN
+ * after the other.  The order depends on the adapters' sizes and on whether d_x,
+ * ldx, d_a, lda and stride_a are all multiples of 16 bytes: a token's result does
+ * not depend on which and how many other tokens are in the batch, on its place
+ * there, on n_adapters or on the addresses and pitches of B_i and d_y.  Where a sum in fp32 is infinite or NaN
  * the result is one of the two.  d_work
  * (16-byte aligned, work_bytes >= noel_lora_workspace_bytes(batch, rank)) is
  * scratch of this call until it has run.  Returns NOEL_OK or a negative

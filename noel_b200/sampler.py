@@ -460,6 +460,13 @@ def _pitch(tensor, axis: int = 0) -> int:
     return tensor.stride(axis) if tensor.shape[axis] > 1 else tensor.shape[-1]
 
 
+def _own_pitch(tensor, axis: int = 0) -> int:
+    """_pitch, but a single one keeps its stride where rows may have it: the
+    adapters' kernels go by the alignment of pitches, and a view of one row is
+    taken as the row is among others."""
+    return max(tensor.stride(axis), tensor.shape[-1]) if tensor.shape[axis] == 1 else tensor.stride(axis)
+
+
 def _row_values(tensor, dtype, batch, name: str, device):
     """The address of one value a row (or adapter)."""
     return _on(tensor, dtype, (batch,), name, device)
@@ -608,7 +615,7 @@ class Adapters:
         self.n, self.rank, self.cols = a.shape
         s.d_b = _on(b, a.dtype, (self.n, None, self.rank), "b", a.device)
         self.rows = b.shape[1]
-        s.lda, s.stride_a, s.ldb, s.stride_b = _pitch(a, 1), _pitch(a), _pitch(b, 1), _pitch(b)
+        s.lda, s.stride_a, s.ldb, s.stride_b = _own_pitch(a, 1), _own_pitch(a), _own_pitch(b, 1), _own_pitch(b)
         s.d_scale = _row_values(scale, torch.float32, self.n, "scale", a.device)
         s.d_ranks = _row_values(ranks, torch.int32, self.n, "ranks", a.device)
         s.type, s.n_adapters, s.rank = kind, self.n, self.rank
@@ -640,8 +647,8 @@ def lora_apply(y, x, adapters: Adapters, adapter_ids, stream=None):
     else:
         with torch.cuda.stream(stream):
             work, size = adapters.scratch(B)
-    _call(dev, stream, lambda s: lib().noel_lora_apply(adapters.ref, ip, xp, _pitch(x), B, adapters.cols, adapters.rows,
-                                                       yp, _pitch(y), work.data_ptr() if size else None, size, s))
+    _call(dev, stream, lambda s: lib().noel_lora_apply(adapters.ref, ip, xp, _own_pitch(x), B, adapters.cols, adapters.rows,
+                                                       yp, _own_pitch(y), work.data_ptr() if size else None, size, s))
     return y
 
 
@@ -684,7 +691,7 @@ def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: 
     if process is not None:
         process.check(logits, V)
     _call(dev, None, lambda s: lib().noel_lmhead_sample_ex(
-        C.byref(cfg), wp, wt, _pitch(weight), xp, _pitch(hidden), B, D, V, lora, ip,
+        C.byref(cfg), wp, wt, _pitch(weight), xp, _own_pitch(hidden), B, D, V, lora, ip,
         process.ref if process is not None else None, hp, H, hld, gp, ids.data_ptr(),
         pr.data_ptr() if pr is not None else None, logits.data_ptr(), work.data_ptr() if size else None, size, s))
     return ids, logits, pr

@@ -331,3 +331,19 @@ def test_lora_sums_of_64_ranks_are_added_in_fp32_gpu(cuda, r, far, pad, dtype):
          "ids": torch.zeros(3, dtype=torch.int32, device=cuda)}
     apply(s)
     assert torch.equal(s["y"], (1.0 + c.double() * 2.0 ** -23).float().expand(3, V))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lora_one_token_and_one_adapter_of_wider_rows_gpu(cuda, dtype):
+    """a view of one token's row, and of one adapter, keeps the pitch that the rows have among others"""
+    import torch
+
+    s = build(cuda, 40, 1001, 301, 12, 3, dtype, seed=31, pad=7, without=0.0)
+    s["ids"].fill_(1)
+    y0 = s["y"].clone()
+    apply(s)
+    for t in (0, 7, 39):
+        part = {**s, "y": y0[t:t + 1].clone(), "x": s["x"][t:t + 1], "a": s["a"][1:2], "b": s["b"][1:2],
+                "scale": s["scale"][1:2], "ids": torch.zeros(1, dtype=torch.int32, device=cuda)}
+        apply(part)
+        assert torch.equal(part["y"].view(torch.int32), s["y"][t:t + 1].view(torch.int32)), t
