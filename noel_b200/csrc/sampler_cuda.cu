@@ -18,9 +18,9 @@
 #include <string.h>
 #include <time.h>
 
+#include <deque>
 #include <map>
 #include <mutex>
-#include <vector>
 
 #include "noel_lmhead.h"
 #include "noel_logits.h"
@@ -85,7 +85,7 @@ struct DeviceCtx {
 };
 
 std::mutex g_mu;
-std::vector<DeviceCtx> g_dev;
+std::deque<DeviceCtx> g_dev;  // grows without moving what other threads hold
 
 int device_ctx(DeviceCtx **out) {
     int dev = 0;
