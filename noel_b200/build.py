@@ -7,12 +7,12 @@ Steps:
    where the C library's expf differs from the correctly rounded exp, into
    ``csrc/_gen/expf_table.inc``.  It calls the C library's expf on this host,
    so the table matches the libm the reference sampler links against.
-2. nvcc compiles ``csrc/sampler_cuda.cu`` for sm_100a into
-   ``noel_b200/libnoel_sampler_cuda.so`` (C ABI of include/sampler.h and
-   include/noel_sampler_cuda.h).
+2. nvcc compiles the units of ``csrc`` for sm_100a side by side and links them
+   into ``noel_b200/libnoel_sampler_cuda.so`` (C ABI of include/).
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -25,12 +25,14 @@ GEN = os.path.join(CSRC, "_gen")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libnoel_sampler_cuda.so")
 
+ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a",
-    "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    *ARCH, "-O3", "-lineinfo", "-std=c++17",
+    "-Xcompiler", "-fPIC",
     "-Xptxas", "-warn-spills",
 ]
+# the library's translation units, and the headers of csrc that the smaller ones take
+UNITS = {"sampler_cuda": None, "int8": ("host.h", "int8.cuh")}
 
 
 def _nvcc() -> str:
@@ -69,17 +71,31 @@ def gen_table(force: bool = False) -> str:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     inc = gen_table(force)
-    srcs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".h"))]
-    srcs += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)]
-    if force or _stale(LIB, srcs + [inc]):
-        cmd = [_nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC,
-               os.path.join(CSRC, "sampler_cuda.cu"), "-o", LIB + ".tmp"]
-        if verbose:
-            cmd.insert(1, "-Xptxas=-v")
-        r = _run(cmd)
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".h"))]
+    deps += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)] + [inc]
+    if force or _stale(LIB, deps):
+        headers = [d for d in deps if not d.endswith(".cu")]
+
+        def compile(name):
+            src, obj = os.path.join(CSRC, name + ".cu"), os.path.join(GEN, name + ".o")
+            # a unit's own kernels and what it shares with others: the sampler's headers are not the other units'
+            own = headers if name == "sampler_cuda" else [h for h in headers if os.path.basename(h) in UNITS[name]
+                                                          or os.path.dirname(h) == INCLUDE]
+            if not force and not _stale(obj, [src, *own]):
+                return obj, ""
+            cmd = [_nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", src, "-o", obj + ".tmp"]
+            if verbose:
+                cmd.insert(1, "-Xptxas=-v")
+            r = _run(cmd)
+            os.replace(obj + ".tmp", obj)
+            return obj, r.stderr
+
+        with concurrent.futures.ThreadPoolExecutor() as pool:
+            done = list(pool.map(compile, UNITS))
+        _run([_nvcc(), *ARCH, "-shared", *[obj for obj, _ in done], "-o", LIB + ".tmp"])
         os.replace(LIB + ".tmp", LIB)
         if verbose:
-            print(r.stderr)
+            print("".join(err for _, err in done))
     return LIB
 
 

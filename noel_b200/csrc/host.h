@@ -1,0 +1,36 @@
+/*
+ * What the library's translation units share on the host: the calling
+ * thread's status and message, and the per-device context.
+ */
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <stddef.h>
+
+#include "noel_sampler_cuda.h"
+
+namespace noel {
+
+/* Keep code and the formatted message as the thread's last error; returns code. */
+__attribute__((visibility("hidden"), format(printf, 2, 3))) int fail(int code, const char *fmt, ...);
+/* Clear them; returns NOEL_OK. */
+__attribute__((visibility("hidden"))) int ok();
+/* The current device's number of SMs (an error where it is not sm_100). */
+__attribute__((visibility("hidden"))) int device_sms(int *sms);
+/* Let kernel take bytes of dynamic shared memory on the current device. */
+__attribute__((visibility("hidden"))) int dynamic_smem(const void *kernel, size_t bytes);
+/* Limit of the device-side waits of the calling thread's calls, in ns. */
+__attribute__((visibility("hidden"))) unsigned long long wait_limit_ns();
+/* Whether the thread asked that its next call load nothing (which ends the request). */
+__attribute__((visibility("hidden"))) bool take_stall();
+/* Whether a wait of the int8 product ran out on the current device since the last call (which clears it). */
+__attribute__((visibility("hidden"))) int i8_wait_failed(bool *failed);
+
+#define CUDA_TRY(call)                                                                     \
+    do {                                                                                   \
+        cudaError_t e_ = (call);                                                           \
+        if (e_ != cudaSuccess) return fail(NOEL_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); \
+    } while (0)
+
+}  // namespace noel

@@ -1,0 +1,460 @@
+/*
+ * Projections in 8-bit integers: the cast of tokens with a scale for each,
+ * and the product with weights that have a scale for each output channel,
+ *   y[t][v] = a_scale[t] * w_scale[v] * sum_d a[t][d] * w[v][d].
+ * Sums are exact 32-bit integers (tcgen05.mma kind::i8), so a result does
+ * not depend on tiles, on their order or on the rest of the batch.
+ */
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <stdint.h>
+
+namespace noel {
+
+/* ------------------------------------------------------------------ cast */
+
+enum I8Type { kI8F32 = 0, kI8F16 = 1, kI8BF16 = 30 };  // NOEL_HEAD_* of noel_lmhead.h
+
+struct I8CastArgs {
+    const void *x;  // [rows][ldx]
+    int64_t ldx;
+    int rows, cols;
+    bool vec;       // every row of x starts on 16 bytes
+    int8_t *q;      // [rows][ldq], 16-byte aligned rows
+    int64_t ldq;
+    float *scale;
+};
+
+constexpr int kI8CastThreads = 256;
+constexpr int kI8CastEach = 16;  // columns of a thread's turn
+
+template <int WT>
+struct I8In;
+template <>
+struct I8In<kI8F32> {
+    using T = float;
+    static __device__ __forceinline__ float get(float v) { return v; }
+};
+template <>
+struct I8In<kI8F16> {
+    using T = __half;
+    static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+};
+template <>
+struct I8In<kI8BF16> {
+    using T = __nv_bfloat16;
+    static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+};
+
+template <int WT>
+__device__ __forceinline__ void i8_load(const I8CastArgs &a, const typename I8In<WT>::T *row, int c, float (&v)[kI8CastEach]) {
+    using T = typename I8In<WT>::T;
+    if (a.vec && c + kI8CastEach <= a.cols) {
+        constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kI8CastEach; i += kPer) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(row + c + i);
+            const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) v[i + j] = I8In<WT>::get(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kI8CastEach; ++i) v[i] = c + i < a.cols ? I8In<WT>::get(row[c + i]) : 0.0f;
+    }
+}
+
+/* x / s to the nearest integer, ties to even, of the exact quotient: the
+ * candidate from the rounded reciprocal is off by one at most, and the
+ * remainder x - n s is a number of 24 bits, so fmaf gives it exactly. */
+__device__ __forceinline__ int i8_quotient(float x, float s, float inv) {
+    float n = rintf(x * inv);
+    const float twice = 2.0f * fmaf(-n, s, x);
+    const bool odd = (__float2int_rn(n) & 1) != 0;
+    if (twice > s || (twice == s && odd)) n += 1.0f;
+    else if (twice < -s || (twice == -s && odd)) n -= 1.0f;
+    return __float2int_rn(n);
+}
+
+/* One CTA a row: its largest magnitude, then the cast.  The row is read
+ * again for the cast, from the caches. */
+template <int WT>
+__global__ void __launch_bounds__(kI8CastThreads) i8_cast_kernel(const __grid_constant__ I8CastArgs a) {
+    __shared__ uint32_t s_top[kI8CastThreads / 32];
+    using T = typename I8In<WT>::T;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x;
+    const T *row = static_cast<const T *>(a.x) + (int64_t)blockIdx.x * a.ldx;
+    uint32_t top = 0;  // magnitudes as bits: NaN is above infinity
+    for (int c = tid * kI8CastEach; c < a.cols; c += kI8CastThreads * kI8CastEach) {
+        float v[kI8CastEach];
+        i8_load<WT>(a, row, c, v);
+#pragma unroll
+        for (int i = 0; i < kI8CastEach; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    }
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if ((tid & 31) == 0) s_top[tid >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kI8CastThreads / 32; ++w) top = max(top, s_top[w]);
+    const bool finite = top < 0x7F800000u;
+    const float s = finite ? fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 1.17549435e-38f) : 1.0f;
+    const float inv = __frcp_rn(s);
+    int8_t *q = a.q + (int64_t)blockIdx.x * a.ldq;
+    for (int c = tid * kI8CastEach; c < a.cols; c += kI8CastThreads * kI8CastEach) {
+        float v[kI8CastEach];
+        i8_load<WT>(a, row, c, v);
+        uint32_t word[kI8CastEach / 4];
+#pragma unroll
+        for (int i = 0; i < kI8CastEach; ++i) {
+            const uint32_t b = finite ? (uint32_t)i8_quotient(v[i], s, inv) & 0xFFu : 0u;
+            word[i / 4] = i % 4 ? word[i / 4] | b << (8 * (i % 4)) : b;
+        }
+        if (c + kI8CastEach <= a.cols) {
+            *reinterpret_cast<uint4 *>(q + c) = make_uint4(word[0], word[1], word[2], word[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kI8CastEach; ++i)
+                if (c + i < a.cols) q[c + i] = (int8_t)(word[i / 4] >> (8 * (i % 4)));
+        }
+    }
+    /* a row with an infinity or a NaN has no cast: its scale makes every result of it NaN */
+    if (tid == 0) a.scale[blockIdx.x] = finite ? s : __uint_as_float(0x7FC00000u);
+}
+
+/* --------------------------------------------------------------- product */
+
+struct I8Args {
+    const float *a_scale;  // [tokens]
+    const float *w_scale;  // [rows]
+    void *y;               // [tokens][ldy]
+    int64_t ldy;
+    int tokens, rows, cols;
+    bool ranges;           // every group one range of rows and all tokens (one tile of them)
+    unsigned long long wait_ns;
+    int stall;             // load nothing, so that waits run out
+    int *failed;
+};
+
+constexpr int kI8Threads = 192;  // a warp of loads, one of products, four of results
+constexpr int kI8RowsCta = 128;  // rows of w in a CTA's tile (lanes of the tensor memory)
+constexpr int kI8Chunk = 128;    // columns (bytes) of a stage: one swizzled line of each row
+constexpr int kI8Box = 32;       // rows of w in one copy
+constexpr int kI8MaxStages = 12;
+constexpr int kI8Ring = 229376;  // bytes of the ring at most
+
+__host__ __device__ constexpr int i8_stage_bytes(int nt, bool pair) {
+    return (kI8RowsCta + (pair ? nt / 2 : nt)) * kI8Chunk;
+}
+__host__ __device__ constexpr int i8_stages(int nt, bool pair) {
+    return kI8Ring / i8_stage_bytes(nt, pair) < kI8MaxStages ? kI8Ring / i8_stage_bytes(nt, pair) : kI8MaxStages;
+}
+__host__ __device__ constexpr int i8_smem(int nt, bool pair) {
+    return i8_stages(nt, pair) * i8_stage_bytes(nt, pair) + 1024;  // stages start on 1024 bytes
+}
+
+__device__ __forceinline__ uint32_t i8_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void i8_bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void i8_bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+/* arrive at a barrier of either CTA of the cluster */
+__device__ __forceinline__ void i8_bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+/* the address in shared::cluster of CTA rank's variable at this CTA's address */
+__device__ __forceinline__ uint32_t i8_peer(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ unsigned long long i8_now() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+/* Wait for the phase of that parity; false where the limit ran out. */
+__device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, unsigned long long limit) {
+    unsigned long long begin = 0;
+    for (int i = 0;; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (i == 0) begin = i8_now();
+        else if ((i & 15) == 0 && i8_now() - begin > limit) return false;
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void i8_copy(const CUtensorMap *map, uint32_t dst, uint32_t bar, int x, int y) {
+    if (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+/* Operand rows of 128 bytes in groups of eight, swizzled by 128 bytes: start / 16, stride between groups 1024 / 16,
+ * version 1, swizzle mode 2. */
+__device__ __forceinline__ uint64_t i8_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+template <bool PAIR>
+__device__ __forceinline__ void i8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+            "r"((uint32_t)add) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+            "r"((uint32_t)add) : "memory");
+}
+/* arrive at bar (of both CTAs of a pair) when the products issued so far are done */
+template <bool PAIR>
+__device__ __forceinline__ void i8_commit(uint32_t bar) {
+    if (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"((uint16_t)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void i8_store(float *p, float v) { *p = v; }
+__device__ __forceinline__ void i8_store(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+
+/* What a group (a CTA, or a pair of CTAs that share tiles of 256 rows) works through. */
+template <int NT, bool PAIR>
+struct I8Tiles {
+    static constexpr int kRows = PAIR ? 2 * kI8RowsCta : kI8RowsCta;
+    int row, row_end, t0;
+    int group, groups, last, token_tiles, rows;
+    bool ranges;
+    int64_t index;
+
+    __device__ __forceinline__ I8Tiles(const I8Args &a) {
+        group = blockIdx.x / (PAIR ? 2 : 1);
+        groups = gridDim.x / (PAIR ? 2 : 1);
+        rows = a.rows;
+        token_tiles = (a.tokens + NT - 1) / NT;
+        ranges = a.ranges;
+        last = (int)((int64_t)rows * (group + 1) / groups);
+        index = group;
+        row = (int)((int64_t)rows * group / groups);
+        t0 = 0;
+        if (!ranges) place();
+        else row_end = min(row + kRows, last);
+    }
+    __device__ __forceinline__ void place() {
+        const int64_t m = index / token_tiles;
+        t0 = (int)(index - m * token_tiles) * NT;
+        row = (int)min((int64_t)rows, m * kRows);
+        row_end = min(rows, row + kRows);
+    }
+    __device__ __forceinline__ bool more() const { return row < (ranges ? last : rows); }
+    __device__ __forceinline__ void next() {
+        if (ranges) {
+            row += kRows;
+            row_end = min(row + kRows, last);
+        } else {
+            index += groups;
+            place();
+        }
+    }
+};
+
+/*
+ * A tile is 128 rows of w (256 of a pair of CTAs) by NT tokens: rows are
+ * lanes of the tensor memory and tokens its columns, so that a warp's
+ * results for a token lie side by side in y, and the few tokens of a decode
+ * batch are columns of a narrow tile.  One lane copies stages of 128 columns
+ * by TMA, one lane issues their products, four warps scale and store a
+ * finished tile while the next one's products go into the other half of the
+ * accumulators.
+ */
+template <int NT, bool PAIR, typename OUT>
+__global__ void __launch_bounds__(kI8Threads, 1)
+    i8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                      const __grid_constant__ I8Args a) {
+    constexpr int kStages = i8_stages(NT, PAIR), kStage = i8_stage_bytes(NT, PAIR), kHalf = PAIR ? NT / 2 : NT;
+    constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
+    extern __shared__ unsigned char i8_raw[];
+    __shared__ __align__(8) uint64_t s_full[kI8MaxStages], s_empty[kI8MaxStages], s_done[2], s_free[2];
+    __shared__ uint32_t s_tmem;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t rank = 0;
+    if (PAIR) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const uint32_t ring = (i8_addr(i8_raw) + 1023u) & ~1023u;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) i8_bar_init(i8_addr(&s_full[i]), 1), i8_bar_init(i8_addr(&s_empty[i]), 1);
+        for (int i = 0; i < 2; ++i) i8_bar_init(i8_addr(&s_done[i]), 1), i8_bar_init(i8_addr(&s_free[i]), PAIR ? 8 : 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(i8_addr(&s_tmem)), "r"(kCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(i8_addr(&s_tmem)), "r"(kCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    if (PAIR) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    const int chunks = (a.cols + kI8Chunk - 1) / kI8Chunk;
+
+    if (warp == 0 && lane == 0 && !a.stall) {
+        /* ------------------------------------------------------- copies */
+        auto boxes = [](const I8Tiles<NT, PAIR> &t, int r) {  // copies of w for CTA r of the group
+            const int n = min(t.row_end - t.row - r * kI8RowsCta, kI8RowsCta);
+            return n <= 0 ? 0 : (n + kI8Box - 1) / kI8Box;
+        };
+        auto copy_w = [&](const I8Tiles<NT, PAIR> &t, int chunk, int stage) {
+            const uint32_t bar = i8_addr(&s_full[stage]);
+            if (rank == 0) {
+                int n = boxes(t, 0) * kI8Box + kHalf;
+                if (PAIR) n += boxes(t, 1) * kI8Box + kHalf;
+                i8_bar_expect(bar, (uint32_t)n * kI8Chunk);
+            }
+            const uint32_t to = PAIR ? i8_peer(bar, 0) : bar;
+            const int n = boxes(t, rank);
+            for (int i = 0; i < n; ++i)
+                i8_copy<PAIR>(&map_w, ring + stage * kStage + i * kI8Box * kI8Chunk, to, chunk * kI8Chunk,
+                              t.row + (int)rank * kI8RowsCta + i * kI8Box);
+        };
+        auto copy_a = [&](const I8Tiles<NT, PAIR> &t, int chunk, int stage) {
+            const uint32_t bar = i8_addr(&s_full[stage]);
+            i8_copy<PAIR>(&map_a, ring + stage * kStage + kI8RowsCta * kI8Chunk, PAIR ? i8_peer(bar, 0) : bar,
+                          chunk * kI8Chunk, t.t0 + (int)rank * kHalf);
+        };
+        /* the weights of the first stages do not wait for the cast of the tokens */
+        I8Tiles<NT, PAIR> early(a);
+        int c = 0, n = 0;
+        for (; n < kStages && early.more(); ++n) {
+            copy_w(early, c, n);
+            if (++c == chunks) c = 0, early.next();
+        }
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        bool good = true;
+        int i = 0, stage = 0;
+        uint32_t phase = 0;
+        for (I8Tiles<NT, PAIR> t(a); good && t.more(); t.next())
+            for (int k = 0; k < chunks; ++k, ++i) {
+                if (i >= n) {
+                    good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns);
+                    if (!good) break;
+                    copy_w(t, k, stage);
+                }
+                copy_a(t, k, stage);
+                if (++stage == kStages) stage = 0, phase ^= 1;
+            }
+        if (!good) {
+            *a.failed = 1;
+            /* what is still on its way into this CTA's memory lands before it ends */
+            if (rank == 0)
+                for (int s = 0; s < kStages; ++s) {
+                    const int latest = s < stage ? (int)phase : (int)(phase ^ 1);
+                    i8_wait(i8_addr(&s_full[s]), latest, a.wait_ns);
+                }
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        /* ----------------------------------------------------- products */
+        /* 32-bit sums of signed bytes, N and M of the tile */
+        constexpr uint32_t kIdesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(NT / 8) << 17 |
+                                    (uint32_t)((PAIR ? 256 : 128) / 16) << 24;
+        int stage = 0, tile = 0;
+        uint32_t phase = 0;
+        bool good = true;
+        for (I8Tiles<NT, PAIR> t(a); good && t.more(); t.next(), ++tile) {
+            const int half = tile & 1;
+            good = i8_wait(i8_addr(&s_free[half]), ((tile >> 1) & 1) ^ 1, a.wait_ns);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int k = 0; good && k < chunks; ++k) {
+                good = i8_wait(i8_addr(&s_full[stage]), phase, a.wait_ns);
+                if (!good) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t dw = i8_desc(ring + stage * kStage), da = i8_desc(ring + stage * kStage + kI8RowsCta * kI8Chunk);
+#pragma unroll
+                for (int j = 0; j < kI8Chunk / 32; ++j)
+                    i8_mma<PAIR>(tmem + half * NT, dw + 2 * j, da + 2 * j, kIdesc, k > 0 || j > 0);
+                i8_commit<PAIR>(i8_addr(&s_empty[stage]));
+                if (++stage == kStages) stage = 0, phase ^= 1;
+            }
+            if (good) i8_commit<PAIR>(i8_addr(&s_done[half]));
+        }
+        if (!good) *a.failed = 1;
+    } else if (warp >= 2) {
+        /* ------------------------------------------------------ results */
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        const int quarter = warp & 3;  // the lanes of the tensor memory that this warp may read
+        int tile = 0;
+        for (I8Tiles<NT, PAIR> t(a); t.more(); t.next(), ++tile) {
+            const int half = tile & 1;
+            const int r = t.row + (int)rank * kI8RowsCta + quarter * 32 + lane;
+            const bool mine = r < t.row_end;
+            const float ws = mine ? a.w_scale[r] : 0.0f;
+            const int nt = min(NT, a.tokens - t.t0);
+            OUT *y = static_cast<OUT *>(a.y) + (int64_t)t.t0 * a.ldy + r;
+            const float *as = a.a_scale + t.t0;
+            if (!__all_sync(0xFFFFFFFFu, i8_wait(i8_addr(&s_done[half]), (tile >> 1) & 1, a.wait_ns))) {
+                if (lane == 0) *a.failed = 1;
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int c = 0; c < NT; c += 16) {
+                if (c >= nt) break;
+                uint32_t v[16];
+                asm volatile(
+                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                    : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                      "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                    : "r"(tmem + ((uint32_t)(quarter * 32) << 16) + half * NT + c));
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (mine) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (c + j < nt) i8_store(y + (int64_t)(c + j) * a.ldy, __int2float_rn((int)v[j]) * ws * as[c + j]);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) i8_bar_arrive(i8_peer(i8_addr(&s_free[half]), 0));
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+    }
+}
+
+}  // namespace noel

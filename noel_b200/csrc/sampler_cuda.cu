@@ -28,6 +28,7 @@
 #include "noel_postreq.h"
 #include "noel_router.h"
 #include "noel_sampler_cuda.h"
+#include "host.h"
 #include "lmhead.cuh"
 #include "logits.cuh"
 #include "lora.cuh"
@@ -45,8 +46,9 @@ namespace {
 /* ------------------------------------------------------------------ errors */
 thread_local int t_status = NOEL_OK;
 thread_local char t_msg[512] = "";
+}  // namespace
 
-int fail(int code, const char *fmt, ...) {
+int noel::fail(int code, const char *fmt, ...) {
     t_status = code;
     va_list ap;
     va_start(ap, fmt);
@@ -54,18 +56,13 @@ int fail(int code, const char *fmt, ...) {
     va_end(ap);
     return code;
 }
-int ok() {
+int noel::ok() {
     t_status = NOEL_OK;
     t_msg[0] = '\0';
     return NOEL_OK;
 }
 
-#define CUDA_TRY(call)                                                                     \
-    do {                                                                                   \
-        cudaError_t e_ = (call);                                                           \
-        if (e_ != cudaSuccess) return fail(NOEL_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); \
-    } while (0)
-
+namespace {
 /* -------------------------------------------------------- device context */
 struct Workspace {
     int32_t *counters = nullptr;  // 4 ints
@@ -180,6 +177,30 @@ int set_smem(DeviceCtx *c, const void *kernel, size_t bytes) {
     return NOEL_OK;
 }
 
+}  // namespace
+
+int noel::device_sms(int *sms) {
+    DeviceCtx *c = nullptr;
+    const int r = device_ctx(&c);
+    if (!r) *sms = c->sms;
+    return r;
+}
+
+int noel::dynamic_smem(const void *kernel, size_t bytes) {
+    DeviceCtx *c = nullptr;
+    const int r = device_ctx(&c);
+    return r ? r : set_smem(c, kernel, bytes);
+}
+
+unsigned long long noel::wait_limit_ns() { return t_wait_ns; }
+
+bool noel::take_stall() {
+    const bool stall = t_stall_next != 0;
+    t_stall_next = 0;
+    return stall;
+}
+
+namespace {
 int pow2_at_least(int x) {
     int p = 1;
     while (p < x) p <<= 1;
@@ -1602,17 +1623,19 @@ extern "C" int noel_sampler_cuda_sync_check(void *stream) {
     DeviceCtx *c = nullptr;
     int r = device_ctx(&c);
     if (r) return r;
+    bool product = false;
+    r = i8_wait_failed(&product);
+    if (r) return r;
     int32_t *flag = nullptr;
     {
         std::lock_guard<std::mutex> lk(g_mu);
         auto it = c->ws.find(s);
         if (it != c->ws.end()) flag = it->second.counters + 3;
     }
-    if (!flag) return ok();
     int32_t v = 0;
-    CUDA_TRY(cudaMemcpy(&v, flag, sizeof(v), cudaMemcpyDeviceToHost));
-    if (v) {
-        CUDA_TRY(cudaMemset(flag, 0, sizeof(v)));
+    if (flag) CUDA_TRY(cudaMemcpy(&v, flag, sizeof(v), cudaMemcpyDeviceToHost));
+    if (v || product) {
+        if (v) CUDA_TRY(cudaMemset(flag, 0, sizeof(v)));
         return fail(NOEL_ERR_DEVICE_WAIT, "a device-side wait ran out of its limit");
     }
     return ok();

@@ -144,6 +144,17 @@ def lib() -> C.CDLL:
     L.noel_lora_apply.restype = C.c_int
     L.noel_lora_apply.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_int,
                                   C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p]
+    L.noel_i8_cast.restype = C.c_int
+    L.noel_i8_cast.argtypes = [C.c_void_p, C.c_int, C.c_size_t, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p,
+                               C.c_void_p]
+    L.noel_i8_product.restype = C.c_int
+    L.noel_i8_product.argtypes = [C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p,
+                                  C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p]
+    L.noel_i8_linear_workspace_bytes.restype = C.c_size_t
+    L.noel_i8_linear_workspace_bytes.argtypes = [C.c_int, C.c_int]
+    L.noel_i8_linear.restype = C.c_int
+    L.noel_i8_linear.argtypes = [C.c_void_p, C.c_int, C.c_size_t, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p, C.c_int,
+                                 C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p]
     L.noel_moe_route_top_k.restype = C.c_int
     L.noel_moe_route_top_k.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p]
     L.noel_sampler_cuda_last_error.restype = C.c_int
@@ -695,3 +706,128 @@ def lmhead_sample(weight, hidden, rng, cfg: SamplerConfig, history=None, probs: 
         process.ref if process is not None else None, hp, H, hld, gp, ids.data_ptr(),
         pr.data_ptr() if pr is not None else None, logits.data_ptr(), work.data_ptr() if size else None, size, s))
     return ids, logits, pr
+
+
+def _row_pitch(tensor, name: str) -> int:
+    """_pitch of rows that have to lie in order and apart."""
+    pitch = _pitch(tensor)
+    if pitch < tensor.shape[1]:
+        _refuse(f"{name}: rows {pitch} elements apart hold {tensor.shape[1]}")
+    return pitch
+
+
+def _byte_rows(q, name: str, device):
+    """Address and pitch of rows of 8-bit integers as the product reads them."""
+    import torch
+
+    ptr = _on(q, torch.int8, (None, None), name, device)
+    rows, cols = q.shape
+    pitch = _row_pitch(q, name) if rows > 1 else (cols + 15) // 16 * 16  # what a single row's stride is does not matter
+    if pitch % 16 or ptr % 16:
+        _refuse(f"{name}: rows must start on 16 bytes (a pitch of {pitch})")
+    return ptr, pitch
+
+
+class Int8Rows:
+    """A matrix in 8-bit integers with a scale for each row (include/noel_int8.h):
+    row r is scale[r] * q[r].  q [R, C] CUDA int8 with unit column stride, whose
+    rows start on 16 bytes (``int8_cast`` makes it so); scale [R] float32.
+    Weights have an output channel to a row, tokens a token.  Holds the
+    tensors themselves."""
+
+    def __init__(self, q, scale):
+        import torch
+
+        self.q, self.scale, self.device = q, scale, q.device
+        self.ptr, self.pitch = _byte_rows(q, "q", q.device)
+        self.rows, self.cols = q.shape
+        self.scale_ptr = _row_values(scale, torch.float32, self.rows, "scale", q.device)
+        self.sizes = {}
+
+    def scratch(self, tokens: int):
+        """Scratch of an int8_linear of so many tokens, and its bytes."""
+        import torch
+
+        size = self.sizes.get(tokens)
+        if size is None:
+            size = self.sizes[tokens] = lib().noel_i8_linear_workspace_bytes(tokens, self.cols)
+        return (torch.empty(size, dtype=torch.uint8, device=self.device) if size else None), size
+
+
+def _float_rows(x, name: str, device, cols=None):
+    """Type, address and pitch of rows of floating numbers."""
+    import torch
+
+    kind = {torch.float32: HEAD_F32, torch.float16: HEAD_F16, torch.bfloat16: HEAD_BF16}.get(x.dtype)
+    if kind is None:
+        _refuse(f"{name}: float32, float16 or bfloat16 wanted, got {x.dtype}")
+    return kind, _on(x, x.dtype, (None, cols), name, device), _row_pitch(x, name)
+
+
+def _on_stream(stream, make):
+    """make() with stream (if any) the current one: its tensors are then that stream's."""
+    import torch
+
+    if stream is None:
+        return make()
+    with torch.cuda.stream(stream):
+        return make()
+
+
+def int8_cast(x, stream=None) -> Int8Rows:
+    """x [R, C] (CUDA float32, float16 or bfloat16, unit column stride) in 8-bit
+    integers with a scale for each row (include/noel_int8.h): scale[r] = max |x[r]| / 127,
+    q = x / scale to the nearest integer; a row with an infinity or a NaN gets the scale NaN."""
+    import torch
+
+    dev = x.device
+    kind, xp, ldx = _float_rows(x, "x", dev)
+    R, cols = x.shape
+    pitch = (cols + 15) // 16 * 16
+    q, scale = _on_stream(stream, lambda: (torch.empty(R, pitch, dtype=torch.int8, device=dev)[:, :cols],
+                                           torch.empty(R, dtype=torch.float32, device=dev)))
+    _call(dev, stream, lambda s: lib().noel_i8_cast(xp, kind, ldx, R, cols, q.data_ptr(), pitch, scale.data_ptr(), s))
+    return Int8Rows(q, scale)
+
+
+def _int8_out(out, tokens: int, rows: int, dtype, device, stream):
+    """The result's tensor, its type and its pitch."""
+    import torch
+
+    if out is None:
+        out = _on_stream(stream, lambda: torch.empty(tokens, rows, dtype=dtype, device=device))
+    kind = {torch.float32: F32, torch.bfloat16: BF16}.get(out.dtype)
+    if kind is None:
+        _refuse(f"results: float32 or bfloat16 wanted, got {out.dtype}")
+    return out, kind, _on(out, out.dtype, (tokens, rows), "out", device), _row_pitch(out, "out")
+
+
+def int8_product(a: Int8Rows, w: Int8Rows, dtype=None, out=None, stream=None):
+    """y [T, V] = a @ w^T of tokens a [T, C] and weights w [V, C], sums exact
+    (include/noel_int8.h).  y is out, or a new tensor of dtype (float32, the
+    default, or bfloat16)."""
+    import torch
+
+    if a.device != w.device or a.cols != w.cols:
+        _refuse(f"tokens of {a.cols} columns on {a.device}, weights of {w.cols} on {w.device}")
+    y, kind, yp, ldy = _int8_out(out, a.rows, w.rows, dtype or torch.float32, w.device, stream)
+    _call(w.device, stream, lambda s: lib().noel_i8_product(a.ptr, a.pitch, a.scale_ptr, a.rows, w.ptr, w.pitch, w.scale_ptr,
+                                                            w.rows, w.cols, yp, kind, ldy, s))
+    return y
+
+
+def int8_linear(x, weight: Int8Rows, dtype=None, out=None, stream=None):
+    """y [T, V] = x @ weight^T with the tokens x [T, C] (CUDA float32, float16 or
+    bfloat16, unit column stride) cast to 8 bits as ``int8_cast`` does, in one
+    call (include/noel_int8.h).  y is out, or a new tensor of dtype (float32,
+    the default, or bfloat16)."""
+    import torch
+
+    dev = weight.device
+    kind, xp, ldx = _float_rows(x, "x", dev, weight.cols)
+    T = x.shape[0]
+    y, out_kind, yp, ldy = _int8_out(out, T, weight.rows, dtype or torch.float32, dev, stream)
+    work, size = _on_stream(stream, lambda: weight.scratch(T))
+    _call(dev, stream, lambda s: lib().noel_i8_linear(xp, kind, ldx, T, weight.ptr, weight.pitch, weight.scale_ptr, weight.rows,
+                                                      weight.cols, yp, out_kind, ldy, work.data_ptr() if size else None, size, s))
+    return y
