@@ -32,7 +32,7 @@ NVCC_FLAGS = [
     "-Xptxas", "-warn-spills",
 ]
 # the library's translation units, and the headers of csrc that the smaller ones take
-UNITS = {"sampler_cuda": None, "int8": ("host.h", "int8.cuh")}
+UNITS = {"sampler_cuda": None, "int8": ("host.h", "int8.cuh"), "requests": ("host.h", "requests.cuh")}
 
 
 def _nvcc() -> str:

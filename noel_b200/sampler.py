@@ -155,6 +155,11 @@ def lib() -> C.CDLL:
     L.noel_i8_linear.restype = C.c_int
     L.noel_i8_linear.argtypes = [C.c_void_p, C.c_int, C.c_size_t, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p, C.c_int,
                                  C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p]
+    L.noel_sample_requests_workspace_bytes.restype = C.c_size_t
+    L.noel_sample_requests_workspace_bytes.argtypes = [C.c_int, C.c_int]
+    L.noel_sample_requests.restype = C.c_int
+    L.noel_sample_requests.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_size_t, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
     L.noel_moe_route_top_k.restype = C.c_int
     L.noel_moe_route_top_k.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p]
     L.noel_sampler_cuda_last_error.restype = C.c_int
@@ -831,3 +836,79 @@ def int8_linear(x, weight: Int8Rows, dtype=None, out=None, stream=None):
     _call(dev, stream, lambda s: lib().noel_i8_linear(xp, kind, ldx, T, weight.ptr, weight.pitch, weight.scale_ptr, weight.rows,
                                                       weight.cols, yp, out_kind, ldy, work.data_ptr() if size else None, size, s))
     return y
+
+
+class RequestParamsStruct(C.Structure):
+    """noel_request_params_t (include/noel_requests.h)."""
+
+    _fields_ = [("d_temperature", C.c_void_p), ("d_top_k", C.c_void_p), ("d_top_p", C.c_void_p), ("d_min_p", C.c_void_p)]
+
+
+class SampleParams:
+    """What ``sample_requests`` samples each row of a batch of B rows with
+    (include/noel_requests.h): temperature [B] float32 (left out: 1; <= 0: the
+    largest logit), top_k [B] int32 (<= 0: off), top_p [B] float32 (>= 1: off)
+    and min_p [B] float32 (<= 0: off); each may be left out.
+
+    The object holds the tensors themselves: a serving loop makes it once over
+    its buffers and writes the next step's values into them.
+    """
+
+    def __init__(self, temperature=None, top_k=None, top_p=None, min_p=None):
+        import torch
+
+        self.tensors = [t for t in (temperature, top_k, top_p, min_p) if t is not None]
+        self.device = self.tensors[0].device if self.tensors else None
+        self.batch = self.tensors[0].shape[0] if self.tensors and self.tensors[0].dim() else None
+        B, dev = self.batch, self.device
+        s = self.s = RequestParamsStruct()
+        s.d_temperature = _row_values(temperature, torch.float32, B, "temperature", dev)
+        s.d_top_k = _row_values(top_k, torch.int32, B, "top_k", dev)
+        s.d_top_p = _row_values(top_p, torch.float32, B, "top_p", dev)
+        s.d_min_p = _row_values(min_p, torch.float32, B, "min_p", dev)
+        self.ref, self.sizes = C.byref(s), {}
+
+    def check(self, logits) -> None:
+        """Whether these parameters fit the rows of logits."""
+        if self.tensors and self.device != logits.device:
+            _refuse(f"parameters on {self.device}, logits on {logits.device}")
+        if self.batch is not None and self.batch != logits.shape[0]:
+            _refuse(f"parameters for {self.batch} rows, logits of {logits.shape[0]}")
+
+    def scratch(self, batch: int, vocab: int, device):
+        """Scratch of one call (None where it needs none) and its bytes."""
+        import torch
+
+        size = self.sizes.get((batch, vocab))
+        if size is None:
+            size = self.sizes[batch, vocab] = lib().noel_sample_requests_workspace_bytes(batch, vocab)
+        return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+
+
+def sample_requests(logits, uniforms, params: SampleParams, vocab: int | None = None, counts: bool = False, stream=None):
+    """One id from every row of logits with the row's own settings and random
+    number (include/noel_requests.h): logits [B, ld] CUDA float32 or bfloat16
+    with unit column stride, of which the first vocab columns (default: all)
+    are used; uniforms [B] float32 in [0, 1).  Returns (ids [B] int32, probs
+    [B] float32, the drawn id's share of what the settings left), and with
+    counts also how many ids they left [B] int32."""
+    import torch
+
+    dtype = {torch.float32: F32, torch.bfloat16: BF16}.get(logits.dtype)
+    if dtype is None:
+        _refuse(f"logits: float32 or bfloat16 wanted, got {logits.dtype}")
+    dev = logits.device
+    ptr = _on(logits, logits.dtype, (None, None), "logits", dev)
+    B, cols = logits.shape
+    V = cols if vocab is None else vocab
+    if not 0 < V <= cols:
+        _refuse(f"vocab {V} of {cols} columns")
+    up = _row_values(uniforms, torch.float32, B, "uniforms", dev)
+    params.check(logits)
+    ids, probs, left, (work, size) = _on_stream(stream, lambda: (
+        torch.empty(B, dtype=torch.int32, device=dev), torch.empty(B, dtype=torch.float32, device=dev),
+        torch.empty(B, dtype=torch.int32, device=dev) if counts else None, params.scratch(B, V, dev)))
+    _call(dev, stream, lambda s: lib().noel_sample_requests(
+        params.ref, ptr, dtype, B, V, _pitch(logits), up, ids.data_ptr(), probs.data_ptr(),
+        left.data_ptr() if counts else None, work.data_ptr() if size else None, size, s))
+    return (ids, probs, left) if counts else (ids, probs)
