@@ -35,39 +35,74 @@ int request_args(const noel_request_params_t *p, const void *logits, int dtype, 
     a.logits = logits, a.ld = (int64_t)ld, a.batch = batch, a.vocab = vocab;
     a.temperature = p->d_temperature, a.top_k = p->d_top_k, a.top_p = p->d_top_p, a.min_p = p->d_min_p;
     a.u = u, a.ids = ids, a.probs = probs, a.counts = counts;
+    a.status = static_cast<int32_t *>(const_cast<void *>(work));
     *out = a;
     return NOEL_OK;
 }
 
+/* a kernel over grid CTAs in clusters, after the one before it or (dependent) once that allows it */
+template <typename... A>
+cudaError_t launch(void (*kernel)(A...), int grid, int threads, size_t smem, int cluster, bool dependent, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)grid);
+    lc.blockDim = dim3((unsigned)threads);
+    lc.dynamicSmemBytes = smem;
+    lc.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at;
+    lc.numAttrs = dependent ? 2 : 1;
+    return cudaLaunchKernelEx(&lc, kernel, args...);
+}
+
 template <typename T>
-int request_launch(RequestArgs a, cudaStream_t s) {
+int request_launch(RequestArgs a, int sms, cudaStream_t s) {
     constexpr int kCluster = kReqMaxCluster, kMost = 190 * 1024;
+    /* the pass */
+    PassArgs p{};
+    p.r = a;
+    int parts = 8;
+    while (parts > 1 && (int64_t)a.batch * parts > 3 * sms) parts /= 2;
+    const int per_vec = 16 / (int)sizeof(T), per_turn = kPassTurn / per_vec;
+    const int vecs = (a.vocab / per_vec + parts - 1) / parts;
+    p.turns = (vecs + per_turn - 1) / per_turn;
+    if (p.turns < 1) p.turns = 1;
+    auto divisor = [](int x, int y) {
+        while (y) {
+            const int z = x % y;
+            x = y, y = z;
+        }
+        return x;
+    };
+    p.step = (int)(p.turns * 0.618);
+    while (p.step > 1 && divisor(p.turns, p.step) != 1) --p.step;
+    if (p.step < 1) p.step = 1;
+    int r = dynamic_smem((const void *)sample_pass_kernel<T>, kPassKeep * sizeof(uint64_t));
+    if (r) return r;
+    CUDA_TRY(launch(sample_pass_kernel<T>, a.batch * parts, kPassThreads, kPassKeep * sizeof(uint64_t), parts, false, s, p));
+    /* the rows that it leaves */
     const int unit = kReqThreads;  // every warp's region in whole turns
     a.per = ((a.vocab + kCluster - 1) / kCluster + unit - 1) / unit * unit;
     size_t smem = (size_t)a.per * sizeof(T);
     a.resident = smem <= kMost;
     if (!a.resident) smem = 0;
-    const int r = dynamic_smem((const void *)sample_requests_kernel<T>, smem);
+    r = dynamic_smem((const void *)sample_requests_kernel<T>, smem);
     if (r) return r;
-    cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)a.batch * kCluster);
-    lc.blockDim = dim3(kReqThreads);
-    lc.dynamicSmemBytes = smem;
-    lc.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = kCluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    lc.attrs = at;
-    lc.numAttrs = 1;
-    CUDA_TRY(cudaLaunchKernelEx(&lc, sample_requests_kernel<T>, a));
-    CUDA_TRY(cudaGetLastError());
+    int clusters = sms / 4;
+    if (clusters > a.batch) clusters = a.batch;
+    CUDA_TRY(launch(sample_requests_kernel<T>, clusters * kCluster, kReqThreads, smem, kCluster, true, s, a));
     return NOEL_OK;
 }
 
 }  // namespace
 
-extern "C" size_t noel_sample_requests_workspace_bytes(int, int) { return 0; }
+extern "C" size_t noel_sample_requests_workspace_bytes(int batch, int vocab) {
+    return batch > 0 && vocab > 0 ? (size_t)batch * sizeof(int32_t) : 0;  // whether a row is settled
+}
 
 extern "C" int noel_sample_requests(const noel_request_params_t *params, const void *d_logits, int dtype, int batch,
                                     int vocab, size_t ld, const float *d_uniforms, int32_t *d_ids, float *d_probs,
@@ -79,7 +114,7 @@ extern "C" int noel_sample_requests(const noel_request_params_t *params, const v
     int sms = 0;
     r = device_sms(&sms);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (!r) r = dtype == NOEL_DTYPE_F32 ? request_launch<float>(a, s) : request_launch<__nv_bfloat16>(a, s);
+    if (!r) r = dtype == NOEL_DTYPE_F32 ? request_launch<float>(a, sms, s) : request_launch<__nv_bfloat16>(a, sms, s);
     return r ? r : ok();
 } catch (...) {
     return fail(NOEL_ERR_CUDA, "host memory");

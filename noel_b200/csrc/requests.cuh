@@ -29,6 +29,7 @@ struct RequestArgs {
     const float *u;
     int32_t *ids, *counts;
     float *probs;
+    int32_t *status;     // [batch]: the rows that are not 0 are this kernel's
     int per;             // elements of a row to a CTA of its cluster
     bool resident;       // they fit the shared memory
 };
@@ -263,16 +264,10 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
  * from global memory each time where it does not fit).
  */
 template <typename T>
-__global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __grid_constant__ RequestArgs a) {
-    extern __shared__ __align__(16) unsigned char req_raw[];
-    __shared__ ReqShared s;
+__device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char *req_raw, int b, int &turn) {
     cg::cluster_group cluster = cg::this_cluster();
     const int me = cluster.block_rank(), nc = cluster.num_blocks();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int b = blockIdx.x / nc;
-    int turn = 0;
-    /* every CTA of the cluster is there before one writes into another's memory: see the wait below */
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
     ReqSlice<T> sl;
     sl.first = me * a.per;
@@ -295,7 +290,6 @@ __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __gr
     __syncthreads();
     uint32_t key = 0;
     for (int w = 0; w < kReqWarps; ++w) key = max(key, s.red[w]);
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     const uint64_t(*all)[2] = req_exchange(s, turn, key, 0);
     for (int c = 0; c < nc; ++c) key = max(key, (uint32_t)all[c][0]);
     const float m = req_unkey(key);
@@ -422,6 +416,559 @@ __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __gr
                 }
             }
             before += __shfl_sync(0xFFFFFFFFu, run, 31);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __grid_constant__ RequestArgs a) {
+    extern __shared__ __align__(16) unsigned char req_raw[];
+    __shared__ ReqShared s;
+    cg::cluster_group cluster = cg::this_cluster();
+    int turn = 0;
+    cluster.sync();  // every CTA of the cluster is there before one writes into another's memory
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int n = cluster.num_blocks();
+    for (int b = blockIdx.x / n; b < a.batch; b += gridDim.x / n) {
+        if (a.status[b] == 0) continue;
+        req_sample_row<T>(a, s, req_raw, b, turn);
+        __syncthreads();
+    }
+}
+
+/* ----------------------------------------------------- one pass over a row */
+
+/*
+ * The rows of a batch in one pass each.  A CTA (or each CTA of a cluster, a
+ * part of the row each) reads its elements once and keeps those that may
+ * still be left by the row's settings, from a filter that rises as more of
+ * the row has been seen:
+ *   top-k: the k-th largest so far;
+ *   min-p: the largest so far + T ln(min_p);
+ *   top-p: what has been dropped weighs at most a share of 1 - top_p of all
+ *     that has been seen.  That is a bet on the rest of the row, and the row's
+ *     end checks it: dropped ids are not left if they weigh at most 1 - top_p
+ *     of the whole row together.
+ * Then what was kept is sorted and the settings are applied to it with the
+ * same whole-number weights as above.  Of what top-p rows dropped only the sum
+ * of weights is needed, from fp32 exponentials; its error is bounded, and
+ * where the bound leaves the cut open, as where a bet is lost or too much would have
+ * to be kept, the row is marked for the kernel above.
+ */
+constexpr int kPassThreads = 256;
+constexpr int kPassWarps = kPassThreads / 32;
+constexpr int kPassEach = 16;                          // elements of a thread's turn
+constexpr int kPassTurn = kPassThreads * kPassEach;    // and of the CTA's
+constexpr int kPassKeep = 2 * kPassTurn;               // kept at most: a turn always has room
+constexpr int kPassBins = 1024;
+constexpr int kPassSort = 2048;                        // of those, at the end
+constexpr int kPassTopK = 1024;                        // largest top_k
+
+struct PassArgs {
+    RequestArgs r;    // r.status gets 1 where the row is left to sample_requests_kernel, else 0
+    int turns, step;  // turns of a CTA's part of a row, taken in steps of step (no common divisor)
+};
+
+enum PassKind { kPassGreedy, kPassCount, kPassLeast, kPassShare, kPassNot };
+
+struct PassShared {
+    uint32_t n[kPassBins];
+    uint64_t warp[kPassWarps];
+    double warp_d[kPassWarps];
+    float warp_f[kPassWarps];
+    uint32_t count, found, found_high;
+    int lost, left;
+    double part_rest[kReqMaxCluster];  // of the cluster's parts: weights dropped,
+    float part_rc[kReqMaxCluster];     // their reference,
+    float part_f[kReqMaxCluster];      // and the filter
+};
+
+/* kept elements: key, then the lower id first */
+__device__ __forceinline__ uint64_t pass_pack(float x, int id) {
+    return (uint64_t)req_key(x + 0.0f) << 32 | (0xFFFFFFFFu - (uint32_t)id);
+}
+__device__ __forceinline__ float pass_x(uint64_t e) { return req_unkey((uint32_t)(e >> 32)); }
+__device__ __forceinline__ int pass_id(uint64_t e) { return (int)(0xFFFFFFFFu - (uint32_t)e); }
+
+__device__ __forceinline__ float pass_exp2(float t) {
+    float w;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(t));
+    return w;
+}
+
+/* 16 bytes of a row as values */
+template <typename T>
+struct PassVec;
+template <>
+struct PassVec<float> {
+    static constexpr int kPer = 4;
+    static __device__ __forceinline__ void get(uint4 u, float *v) {
+        v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y), v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u); }
+};
+template <>
+struct PassVec<__nv_bfloat16> {
+    static constexpr int kPer = 8;
+    static __device__ __forceinline__ void get(uint4 u, float *v) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }
+};
+__device__ __forceinline__ uint4 pass_load(const uint4 *p) {
+    uint4 u;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+    return u;
+}
+
+__device__ __forceinline__ float pass_max(PassShared &s, float v) {  // over the CTA's threads
+    for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s.warp_f[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = s.warp_f[0];
+#pragma unroll
+    for (int w = 1; w < kPassWarps; ++w) v = fmaxf(v, s.warp_f[w]);
+    return v;
+}
+__device__ __forceinline__ double pass_sum(PassShared &s, double v) {
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s.warp_d[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < kPassWarps; ++w) v += s.warp_d[w];
+    return v;
+}
+/* inclusive running sum over the CTA's threads, the CTA's sum in all */
+__device__ __forceinline__ uint64_t pass_scan(PassShared &s, uint64_t v, uint64_t &all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint64_t o = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) s.warp[warp] = v;
+    __syncthreads();
+    uint64_t before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kPassWarps; ++w) {
+        if (w < warp) before += s.warp[w];
+        all += s.warp[w];
+    }
+    return before + v;
+}
+
+/* What a row's settings come to before its largest logit is known. */
+struct PassRow {
+    PassKind kind;
+    int k;
+    float t, p, floor_t;  // floor = largest + floor_t (a little below, so that nothing is dropped too early)
+    float c;              // log2(e) / T
+};
+
+__device__ __forceinline__ PassRow pass_row(const RequestArgs &a, int b) {
+    PassRow r;
+    const float t = a.temperature ? a.temperature[b] : 1.0f;
+    const float least = a.min_p ? a.min_p[b] : 0.0f;
+    r.p = a.top_p ? a.top_p[b] : 1.0f;
+    r.k = a.top_k ? a.top_k[b] : 0;
+    r.t = t;
+    r.c = (float)(1.4426950408889634 / (double)t);
+    r.floor_t = -30.0f * t;
+    if (least > 0.0f) r.floor_t = fmaxf(r.floor_t, t * logf(fminf(least, 1.0f)) * 1.0001f);
+    const bool plain = t >= 1e-3f && t <= 1e4f;  // what fp32 bounds below are made for
+    if (!(t > 0.0f)) r.kind = kPassGreedy, r.k = 1, r.floor_t = 0.0f;
+    else if (!plain) r.kind = kPassNot;
+    else if (r.k > 0 && r.k <= kPassTopK) r.kind = kPassCount;
+    else if (least > 0.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassLeast;
+    else if (r.p < 1.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassShare;
+    else r.kind = kPassNot;
+    return r;
+}
+/* a value that is not above the smallest that the temperature and min-p leave beside a largest logit of m */
+__device__ __forceinline__ float pass_floor(const PassRow &r, float m) {
+    const float f = m + r.floor_t;
+    return fmaxf(f - fabsf(f) * 2e-7f - fabsf(m) * 2e-7f - 1e-37f, -3.402823466e38f);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __grid_constant__ PassArgs a) {
+    extern __shared__ __align__(16) unsigned char req_raw[];
+    uint64_t *keep = reinterpret_cast<uint64_t *>(req_raw);
+    __shared__ PassShared s;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int me = cluster.block_rank(), nc = cluster.num_blocks();
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int b = blockIdx.x / nc;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const PassRow row = pass_row(a.r, b);
+    if (row.kind == kPassNot) {
+        if (me == 0 && tid == 0) a.r.status[b] = 1;
+        return;  // the whole cluster
+    }
+    using V = PassVec<T>;
+    constexpr int kVecs = kPassEach / V::kPer;
+    const T *base = static_cast<const T *>(a.r.logits) + (int64_t)b * a.r.ld;
+    const int vocab = a.r.vocab;
+    const int head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / (int)sizeof(T));
+    const int vecs = (vocab - head) / V::kPer;
+    const uint4 *body = reinterpret_cast<const uint4 *>(base + head);
+    const int first = (int)((int64_t)vecs * me / nc), last = (int)((int64_t)vecs * (me + 1) / nc);
+
+    if (tid == 0) s.count = 0, s.lost = 0;
+    __syncthreads();
+
+    float f = -3.402823466e38f;  // elements from f on are kept
+    float rc = 0.0f;             // weights of what is dropped are 2^(x c - rc)
+    bool weigh = false;
+    double rest = 0.0;           // and their sum, of this thread
+    bool full = false;
+
+    auto put = [&](float x, int id) {
+        const uint32_t at = atomicAdd(&s.count, 1u);
+        keep[at] = pass_pack(x, id);
+        full |= at >= kPassTurn;
+    };
+
+    /* Raise the filter and drop what it drops. */
+    auto raise = [&]() {
+        const int n = (int)s.count;
+        float hi = -INFINITY, lo = INFINITY;
+        for (int i = tid; i < n; i += kPassThreads) {
+            const float x = pass_x(keep[i]);
+            hi = fmaxf(hi, x), lo = fminf(lo, x);
+        }
+        hi = pass_max(s, hi);
+        lo = -pass_max(s, -lo);
+        if (n == 0) return;
+        if (!(hi < INFINITY)) {  // the kernel for every row
+            s.lost = 1;
+            return;
+        }
+        if (row.kind == kPassShare && !weigh) weigh = true, rc = hi * row.c;
+        float f_new = fmaxf(pass_floor(row, hi), f);
+        if (row.kind == kPassCount || row.kind == kPassShare) {
+            const float low = fmaxf(f_new, lo), scale = hi > low ? ((float)kPassBins - 0.5f) / (hi - low) : 0.0f;
+            for (int i = tid; i < kPassBins; i += kPassThreads) s.n[i] = 0;
+            if (tid == 0) s.found = kPassBins;
+            const double dropped = row.kind == kPassShare ? pass_sum(s, rest) : 0.0;
+            __syncthreads();
+            for (int i = tid; i < n; i += kPassThreads) {
+                const float x = pass_x(keep[i]);
+                if (x >= low) atomicAdd(&s.n[min((int)((hi - x) * scale), kPassBins - 1)], 1u);
+            }
+            __syncthreads();
+            /* counts, or weights of the bins in 2^-40 (of their upper ends) */
+            constexpr int kEach = kPassBins / kPassThreads;
+            uint64_t in[kEach], mine = 0, all;
+            for (int i = 0; i < kEach; ++i) {
+                const int bin = tid * kEach + i;
+                in[i] = s.n[bin];
+                if (row.kind == kPassShare && in[i])
+                    in[i] = (uint64_t)((float)in[i] * pass_exp2(-(float)bin / scale * row.c) * 1.0995116e12f);
+                mine += in[i];
+            }
+            uint64_t run = pass_scan(s, mine, all) - mine;
+            uint64_t want = (uint64_t)row.k;
+            if (row.kind == kPassShare) {
+                /* keep until what is below weighs 3/4 of what it may */
+                const double gone = dropped * exp2((double)rc - (double)hi * (double)row.c) * 1.0995116e12;
+                const double may = 0.75 * (1.0 - (double)row.p) * ((double)all + gone) - gone;
+                want = may > 0.0 && may < (double)all ? all - (uint64_t)may : all;
+            }
+            for (int i = 0; i < kEach; ++i) {
+                if (run < want && run + in[i] >= want) s.found = tid * kEach + i;
+                run += in[i];
+            }
+            __syncthreads();
+            if (s.found < kPassBins - 1 && scale > 0.0f) {
+                const float edge = hi - (float)(s.found + 1) / scale;
+                f_new = fmaxf(f_new, edge - fabsf(edge) * 2e-7f - (hi - low) * 4e-7f);
+            }
+        }
+        f = f_new;
+        /* the kept ones move up; a turn's places are read before any of them is written */
+        __syncthreads();
+        if (tid == 0) s.count = 0;
+        for (int at = 0; at < n; at += 4 * kPassThreads) {
+            uint64_t e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = at + j * kPassThreads + tid;
+                e[j] = i < n ? keep[i] : 0;  // 0 is below every key
+            }
+            __syncthreads();
+            int mine = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = pass_x(e[j]);
+                if (e[j] && x >= f) ++mine;
+                else if (e[j] && weigh) rest += (double)pass_exp2(fmaf(x, row.c, -rc)), e[j] = 0;
+                else e[j] = 0;
+            }
+            uint32_t to = mine ? atomicAdd(&s.count, (uint32_t)mine) : 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (e[j]) keep[to++] = e[j];
+        }
+        __syncthreads();
+        if (tid == 0 && s.count > kPassTurn) s.lost = 1;
+        full = false;
+        __syncthreads();
+    };
+
+    if (me == 0) {
+        const int tail = head + vecs * V::kPer;
+        if (tid < head) {
+            const float x = req_value(base[tid]);
+            if (x >= f) put(x, tid);
+        }
+        if (tid < vocab - tail) {
+            const float x = req_value(base[tail + tid]);
+            if (x >= f) put(x, tail + tid);
+        }
+    }
+    uint4 next[kVecs];
+    auto load = [&](int turn) {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            const int v = first + turn * (kPassThreads * kVecs) + j * kPassThreads + tid;
+            next[j] = v < last ? pass_load(body + v) : V::none();
+        }
+    };
+    int turn = 0;
+    load(0);
+    for (int i = 0; i < a.turns; ++i) {
+        float x[kPassEach];
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) V::get(next[j], x + j * V::kPer);
+        const int here = turn;
+        turn += a.step;
+        if (turn >= a.turns) turn -= a.turns;
+        if (i + 1 < a.turns) load(turn);
+        float most = x[0];
+#pragma unroll
+        for (int j = 1; j < kPassEach; ++j) most = fmaxf(most, x[j]);
+        if (__any_sync(0xFFFFFFFFu, most >= f)) {
+#pragma unroll
+            for (int j = 0; j < kPassEach; ++j) {
+                if (x[j] >= f) {
+                    const int v = first + here * (kPassThreads * kVecs) + (j / V::kPer) * kPassThreads + tid;
+                    put(x[j], head + v * V::kPer + j % V::kPer);
+                    x[j] = -INFINITY;
+                }
+            }
+        }
+        if (weigh) {
+            float w[kPassEach];
+#pragma unroll
+            for (int j = 0; j < kPassEach; ++j) w[j] = x[j] == x[j] ? pass_exp2(fmaf(x[j], row.c, -rc)) : 0.0f;
+#pragma unroll
+            for (int d = kPassEach / 2; d; d >>= 1)
+#pragma unroll
+                for (int j = 0; j < d; ++j) w[j] += w[j + d];
+            rest += (double)w[0];
+        }
+        if (__syncthreads_or(full || i == 0)) {
+            raise();
+            if (s.lost) break;
+        }
+    }
+    __syncthreads();
+
+    /* the cluster's parts come together in the first one's memory, after a last rise so that little moves */
+    if (nc > 1 && !s.lost) raise();
+    const double dropped = weigh ? pass_sum(s, rest) : 0.0;
+    if (nc > 1) {
+        __syncthreads();
+        cluster.sync();  // every CTA of the cluster is there, and the first one has its own
+        PassShared *to = cluster.map_shared_rank(&s, 0);
+        uint64_t *to_keep = cluster.map_shared_rank(keep, 0);
+        if (me != 0) {
+            const int n = s.lost ? 0 : (int)s.count;
+            if (tid == 0) {
+                to->part_rest[me] = dropped;
+                to->part_rc[me] = rc;
+                to->part_f[me] = f;
+                const uint32_t at = atomicAdd(&to->count, (uint32_t)n);
+                s.left = (int)at;
+                if (s.lost || at + n > kPassKeep) s.left = -1, to->lost = 1;
+            }
+            __syncthreads();
+            if (s.left >= 0)
+                for (int i = tid; i < n; i += kPassThreads) to_keep[s.left + i] = keep[i];
+        }
+        cluster.sync();
+        if (me != 0) return;
+    }
+    if (s.lost) {
+        if (tid == 0) a.r.status[b] = 1;
+        return;
+    }
+    if (tid == 0) s.part_rest[0] = dropped, s.part_rc[0] = rc;
+    __syncthreads();
+    for (int c = 1; c < nc; ++c) f = fmaxf(f, s.part_f[c]);  // from here on every element of the row is kept
+    int n = (int)s.count;
+    if (n == 0) {
+        if (tid == 0) {
+            a.r.status[b] = 0;
+            a.r.ids[b] = -1;
+            if (a.r.probs) a.r.probs[b] = 0.0f;
+            if (a.r.counts) a.r.counts[b] = 0;
+        }
+        return;
+    }
+    /* the parts' dropped weights, as of the row's largest logit */
+    float hi = -INFINITY;
+    for (int i = tid; i < n; i += kPassThreads) hi = fmaxf(hi, pass_x(keep[i]));
+    hi = pass_max(s, hi);
+    double gone = 0.0, gone_error = 0.0;
+    if (row.kind == kPassShare) {
+        double apart = 0.0;
+        for (int c = 0; c < nc; ++c) {
+            const double up = (double)s.part_rc[c] - (double)hi * (double)row.c;
+            if (s.part_rest[c] > 0.0) gone += s.part_rest[c] * exp2(up), apart = fmax(apart, fabs(up));
+        }
+        /*
+         * Against the sum of the definition's weights: an exponential is off by 2^-22 of itself, four additions by
+         * 2^-24 each; the exponent's rounding by 2^-24 of it and that of log2(e) / T by as much (of the exponent from
+         * the largest logit on, from which that of the part's reference lies apart).  Weights W over N ids have sum
+         * W log2(1 / W) <= sum log2(N / sum).  Ids under the floor of 30 T are in it, at e^-30 each, weights below
+         * 2^-126 of the reference's are not, and the definition's weights are rounded to 2^-43.
+         */
+        const double ids = (double)vocab;
+        const double spread = gone > 0.0 ? log2(fmax(ids / gone, 2.0)) : 0.0;
+        gone_error = gone * (ldexp(1.0, -21) + 0.6932 * (spread * 2.0 + apart) * ldexp(1.0, -24)) * 1.01 +
+                     ids * (1e-13 + ldexp(1.0, -43));
+        if (!(gone < 1e7)) {  // the reference was too far below
+            if (tid == 0) a.r.status[b] = 1;
+            return;
+        }
+    }
+    if (!(hi < INFINITY)) {
+        if (tid == 0) a.r.status[b] = 1;
+        return;
+    }
+    /* one more rise for a shorter sort */
+    if (n > 512) {
+        const double other = gone;
+        if (row.kind == kPassShare) {
+            /* the parts' weights as one thread's, of one reference */
+            weigh = true;
+            rc = hi * row.c;
+            rest = tid == 0 ? gone * exp2((double)hi * (double)row.c - (double)rc) : 0.0;
+        }
+        raise();
+        n = (int)s.count;
+        if (row.kind == kPassShare) {
+            gone = pass_sum(s, rest) * exp2((double)rc - (double)hi * (double)row.c);
+            /* exponents of 44 at most: ids are above the floor of 30 T */
+            gone_error += fmax(gone - other, 0.0) * (ldexp(1.0, -21) + 0.6932 * 2.0 * 44.0 * ldexp(1.0, -24)) * 1.01 + gone * 1e-14;
+        }
+        __syncthreads();
+    }
+    if (s.lost || n > kPassSort) {
+        if (tid == 0) a.r.status[b] = 1;
+        return;
+    }
+    int size = 32;
+    while (size < n) size <<= 1;
+    auto sort = [&]() {  // largest first
+        for (int width = 2; width <= size; width <<= 1)
+            for (int d = width >> 1; d; d >>= 1) {
+                for (int i = tid; i < size / 2; i += kPassThreads) {
+                    const int lo = 2 * i - (i & (d - 1)), up = lo + d;
+                    const uint64_t x = keep[lo], y = keep[up];
+                    if ((x < y) == ((lo & width) == 0)) keep[lo] = y, keep[up] = x;
+                }
+                __syncthreads();
+            }
+    };
+    for (int i = n + tid; i < size; i += kPassThreads) keep[i] = 0;
+    __syncthreads();
+    sort();
+    const ReqRow r = req_row(a.r, b, hi);
+    if (r.greedy) {
+        if (tid == 0) {
+            a.r.status[b] = 0;
+            a.r.ids[b] = pass_id(keep[0]);
+            if (a.r.probs) a.r.probs[b] = 1.0f;
+            if (a.r.counts) a.r.counts[b] = 1;
+        }
+        return;
+    }
+    /* what is left by the temperature, min-p and top-k is a beginning of the order */
+    if (tid == 0) s.left = 0;
+    __syncthreads();
+    const int most = r.k ? min(n, r.k) : n;
+    for (int i = tid; i < most; i += kPassThreads)
+        if ((uint32_t)(keep[i] >> 32) >= r.floor && (i + 1 == most || (uint32_t)(keep[i + 1] >> 32) < r.floor)) s.left = i + 1;
+    __syncthreads();
+    int left = s.left;
+    const int each = (size + kPassThreads - 1) / kPassThreads;
+    auto weight = [&](int i) -> uint64_t { return i < left ? req_weight(r, pass_x(keep[i])) : 0; };
+    if (r.p < 1.0) {
+        uint64_t mine = 0, all;
+        for (int i = tid * each; i < tid * each + each && i < size; ++i) mine += weight(i);
+        const uint64_t end = pass_scan(s, mine, all);
+        uint64_t want[2];
+        for (int side = 0; side < 2; ++side) {
+            const double d = side ? gone + gone_error : fmax(gone - gone_error, 0.0);
+            const uint64_t total = all + (row.kind == kPassShare ? (uint64_t)(d * (double)(1ull << kReqFraction)) + side : 0);
+            const uint64_t share = (uint64_t)(r.p * 18446744073709551616.0);
+            want[side] = __umul64hi(share, total) + (share * total != 0);
+            if (want[side] == 0) want[side] = 1;
+        }
+        if (tid == 0) s.found = s.found_high = 0;
+        __syncthreads();
+        uint64_t run = end - mine;
+        for (int i = tid * each; i < tid * each + each && i < left; ++i) {
+            const uint64_t after = run + weight(i);
+            if (run < want[0] && after >= want[0]) s.found = (uint32_t)i + 1;
+            if (run < want[1] && after >= want[1]) s.found_high = (uint32_t)i + 1;
+            run = after;
+        }
+        __syncthreads();
+        left = (int)s.found;
+        /* open within the error, or a lost bet: the row's other ids weigh too much, or some come before the cut */
+        if (s.found != s.found_high || left == 0 || (row.kind == kPassShare && !(pass_x(keep[left - 1]) >= f))) {
+            if (tid == 0) a.r.status[b] = 1;
+            return;
+        }
+    }
+    /* the walk in the order of ids */
+    for (int i = tid; i < size; i += kPassThreads) {
+        const uint64_t e = keep[i];
+        keep[i] = i < left ? e << 32 | e >> 32 : 0;  // the lower id is the larger number
+    }
+    __syncthreads();
+    size = 32;
+    while (size < left) size <<= 1;
+    sort();
+    const int per = (size + kPassThreads - 1) / kPassThreads;
+    uint64_t mine = 0, total;
+    for (int i = tid * per; i < tid * per + per && i < left; ++i) mine += req_weight(r, req_unkey((uint32_t)keep[i]));
+    const uint64_t end = pass_scan(s, mine, total);
+    uint64_t target = r.u >= 1.0f ? total : __umul64hi((uint64_t)((double)r.u * 18446744073709551616.0), total);
+    if (target >= total) target = total - 1;
+    uint64_t run = end - mine;
+    if (run <= target && target < end) {
+        for (int i = tid * per; i < tid * per + per && i < left; ++i) {
+            const float x = req_unkey((uint32_t)keep[i]);
+            run += req_weight(r, x);
+            if (run > target) {
+                a.r.status[b] = 0;
+                a.r.ids[b] = (int)(0xFFFFFFFFu - (uint32_t)(keep[i] >> 32));
+                if (a.r.probs) a.r.probs[b] = (float)(req_exp(r, x) * (double)(1ull << kReqFraction) / (double)total);
+                if (a.r.counts) a.r.counts[b] = left;
+                break;
+            }
         }
     }
 }
