@@ -67,9 +67,8 @@ int request_launch(RequestArgs a, int sms, cudaStream_t s) {
     p.r = a;
     int parts = 8;
     while (parts > 1 && (int64_t)a.batch * parts > 3 * sms) parts /= 2;
-    const int per_vec = 16 / (int)sizeof(T), per_turn = kPassTurn / per_vec;
-    const int vecs = (a.vocab / per_vec + parts - 1) / parts;
-    p.turns = (vecs + per_turn - 1) / per_turn;
+    const int per_vec = 16 / (int)sizeof(T), per_turn = parts * kPassThreads * kPassEach / per_vec;
+    p.turns = (a.vocab / per_vec + per_turn - 1) / per_turn;
     if (p.turns < 1) p.turns = 1;
     auto divisor = [](int x, int y) {
         while (y) {

@@ -457,16 +457,16 @@ __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __gr
  */
 constexpr int kPassThreads = 256;
 constexpr int kPassWarps = kPassThreads / 32;
-constexpr int kPassEach = 16;                          // elements of a thread's turn
-constexpr int kPassTurn = kPassThreads * kPassEach;    // and of the CTA's
-constexpr int kPassKeep = 2 * kPassTurn;               // kept at most: a turn always has room
+constexpr int kPassEach = 16;     // elements of a thread's turn
+constexpr int kPassKeep = 4096;   // kept at most
+constexpr int kPassFull = 3072;   // and at most after the filter has risen
 constexpr int kPassBins = 1024;
-constexpr int kPassSort = 2048;                        // of those, at the end
-constexpr int kPassTopK = 1024;                        // largest top_k
+constexpr int kPassSort = 2048;   // of those, at the end
+constexpr int kPassTopK = 1024;   // largest top_k
 
 struct PassArgs {
     RequestArgs r;    // r.status gets 1 where the row is left to sample_requests_kernel, else 0
-    int turns, step;  // turns of a CTA's part of a row, taken in steps of step (no common divisor)
+    int turns, step;  // turns of a warp's part of a row, taken in steps of step (no common divisor)
 };
 
 enum PassKind { kPassGreedy, kPassCount, kPassLeast, kPassShare, kPassNot };
@@ -476,8 +476,11 @@ struct PassShared {
     uint64_t warp[kPassWarps];
     double warp_d[kPassWarps];
     float warp_f[kPassWarps];
-    uint32_t count, found, found_high;
-    int lost, left;
+    uint32_t count;       // places taken in the list of what is kept
+    uint32_t valid;       // and those that were filled, where it ran over
+    uint32_t found, found_high;
+    int full, lost, left;
+    double top;
     double part_rest[kReqMaxCluster];  // of the cluster's parts: weights dropped,
     float part_rc[kReqMaxCluster];     // their reference,
     float part_f[kReqMaxCluster];      // and the filter
@@ -604,7 +607,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
     __shared__ PassShared s;
     cg::cluster_group cluster = cg::this_cluster();
     const int me = cluster.block_rank(), nc = cluster.num_blocks();
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = blockIdx.x / nc;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const PassRow row = pass_row(a.r, b);
@@ -619,33 +622,121 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
     const int head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / (int)sizeof(T));
     const int vecs = (vocab - head) / V::kPer;
     const uint4 *body = reinterpret_cast<const uint4 *>(base + head);
-    const int first = (int)((int64_t)vecs * me / nc), last = (int)((int64_t)vecs * (me + 1) / nc);
+    /* a warp's part of the row: whole turns, so that a turn of the CTA is spread over the row */
+    const int first = min((int64_t)vecs, (int64_t)(me * kPassWarps + warp) * a.turns * (32 * kVecs));
+    const int last = min((int64_t)vecs, (int64_t)first + a.turns * (32 * kVecs));
 
-    if (tid == 0) s.count = 0, s.lost = 0;
-    __syncthreads();
+    uint4 next[kVecs];
+    auto load = [&](int turn) {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            const int v = first + turn * (32 * kVecs) + j * 32 + lane;
+            next[j] = v < last ? pass_load(body + v) : V::none();
+        }
+    };
+    int turn = 0, ahead = a.step < a.turns ? a.step : 0;  // the turn in x, and the one on its way
+    load(0);
+
+    if (tid == 0) s.count = 0, s.valid = kPassKeep, s.lost = s.full = 0;
+    for (int i = tid; i < kPassBins; i += kPassThreads) s.n[i] = 0;
 
     float f = -3.402823466e38f;  // elements from f on are kept
     float rc = 0.0f;             // weights of what is dropped are 2^(x c - rc)
     bool weigh = false;
     double rest = 0.0;           // and their sum, of this thread
-    bool full = false;
+    float x[kPassEach];
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) V::get(next[j], x + j * V::kPer);
+    if (a.turns > 1) load(ahead);
 
-    auto put = [&](float x, int id) {
-        const uint32_t at = atomicAdd(&s.count, 1u);
-        keep[at] = pass_pack(x, id);
-        full |= at >= kPassTurn;
+    /*
+     * The filter that the histogram in s.n of elements from low to hi gives:
+     * 1 / grow of the part has been seen, and dropped is what has been dropped
+     * weighs (as of hi).
+     */
+    auto edge = [&](float hi, float low, float scale, double dropped, double grow) -> float {
+        /* counts in the low 14 bits, above them the weights of the bins (of their upper ends) in 2^-36 */
+        constexpr int kEach = kPassBins / kPassThreads;
+        uint64_t in[kEach], mine = 0, all;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int bin = tid * kEach + i;
+            const uint32_t n = s.n[bin];
+            in[i] = n;
+            if (row.kind == kPassShare && n)
+                in[i] += (uint64_t)((float)n * pass_exp2(-(float)bin / scale * row.c) * 6.8719477e10f) << 14;
+            mine += in[i];
+        }
+        const uint64_t begin = pass_scan(s, mine, all) - mine;
+        if (tid == 0) s.found = kPassBins, s.top = (double)(all >> 14);
+        __syncthreads();
+        const uint32_t need = row.kind == kPassCount ? (uint32_t)row.k : 16u;
+        uint64_t run = begin;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint64_t after = run + in[i];
+            if ((uint32_t)(run & 16383) < need && (uint32_t)(after & 16383) >= need) {
+                if (row.kind == kPassCount) s.found = tid * kEach + i;
+                else s.top = (double)(after >> 14);
+            }
+            run = after;
+        }
+        __syncthreads();
+        if (row.kind == kPassShare) {
+            /*
+             * What will have been dropped in the end, as of the part seen so far, may be 3/4 of 1 - top_p of the row's
+             * weight; for that the 16 largest so far count once and the others for as much as the part has seen.
+             */
+            const double weight = (double)(all >> 14), gone = dropped * 6.8719477e10, seen = weight + gone;
+            const double row_weight = seen + (grow - 1.0) * (seen - s.top);
+            const double may = 0.75 * (1.0 - (double)row.p) * row_weight / grow - gone;
+            const uint64_t want = may > 0.0 && may < weight ? (all >> 14) - (uint64_t)may : all >> 14;
+            run = begin;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const uint64_t after = run + in[i];
+                if (run >> 14 < want && after >> 14 >= want) s.found = tid * kEach + i;
+                run = after;
+            }
+            __syncthreads();
+        }
+        if (s.found >= kPassBins - 1 || !(scale > 0.0f)) return -INFINITY;
+        const float e = hi - (float)(s.found + 1) / scale;
+        return e - fabsf(e) * 2e-7f - (hi - low) * 4e-7f;
     };
 
-    /* Raise the filter and drop what it drops. */
-    auto raise = [&]() {
-        const int n = (int)s.count;
-        float hi = -INFINITY, lo = INFINITY;
-        for (int i = tid; i < n; i += kPassThreads) {
-            const float x = pass_x(keep[i]);
-            hi = fmaxf(hi, x), lo = fminf(lo, x);
+    /* the first filter, from the first turn */
+    float lo;  // the smallest of that turn
+    {
+        float hi = -INFINITY;
+        lo = INFINITY;
+#pragma unroll
+        for (int j = 0; j < kPassEach; ++j) {
+            hi = fmaxf(hi, x[j]);
+            lo = fminf(lo, x[j] > -INFINITY ? x[j] : INFINITY);
         }
         hi = pass_max(s, hi);
-        lo = -pass_max(s, -lo);
+        if (hi > -INFINITY && hi < INFINITY) {
+            f = pass_floor(row, hi);
+            if (row.kind == kPassShare) weigh = true, rc = hi * row.c;
+            if (row.kind == kPassCount || row.kind == kPassShare) {
+                lo = -pass_max(s, -lo);
+                const float low = fmaxf(f, lo), scale = hi > low ? ((float)kPassBins - 0.5f) / (hi - low) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < kPassEach; ++j)
+                    if (x[j] >= low) atomicAdd(&s.n[min((int)((hi - x[j]) * scale), kPassBins - 1)], 1u);
+                __syncthreads();
+                f = fmaxf(f, edge(hi, low, scale, 0.0, (double)a.turns));
+            }
+        }
+    }
+
+    /* Raise the filter and drop what it drops. */
+    auto raise = [&](double grow) {
+        const int n = (int)min(s.count, s.valid);
+        float hi = -INFINITY;
+        for (int i = tid; i < n; i += kPassThreads) hi = fmaxf(hi, pass_x(keep[i]));
+        hi = pass_max(s, hi);
         if (n == 0) return;
         if (!(hi < INFINITY)) {  // the kernel for every row
             s.lost = 1;
@@ -654,48 +745,22 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         if (row.kind == kPassShare && !weigh) weigh = true, rc = hi * row.c;
         float f_new = fmaxf(pass_floor(row, hi), f);
         if (row.kind == kPassCount || row.kind == kPassShare) {
-            const float low = fmaxf(f_new, lo), scale = hi > low ? ((float)kPassBins - 0.5f) / (hi - low) : 0.0f;
+            const float low = lo < hi ? fmaxf(f_new, lo) : f_new, scale = hi > low ? ((float)kPassBins - 0.5f) / (hi - low) : 0.0f;
             for (int i = tid; i < kPassBins; i += kPassThreads) s.n[i] = 0;
-            if (tid == 0) s.found = kPassBins;
-            const double dropped = row.kind == kPassShare ? pass_sum(s, rest) : 0.0;
+            const double dropped =
+                row.kind == kPassShare ? pass_sum(s, rest) * exp2((double)rc - (double)hi * (double)row.c) : 0.0;
             __syncthreads();
             for (int i = tid; i < n; i += kPassThreads) {
-                const float x = pass_x(keep[i]);
-                if (x >= low) atomicAdd(&s.n[min((int)((hi - x) * scale), kPassBins - 1)], 1u);
+                const float v = pass_x(keep[i]);
+                if (v >= low) atomicAdd(&s.n[min((int)((hi - v) * scale), kPassBins - 1)], 1u);
             }
             __syncthreads();
-            /* counts, or weights of the bins in 2^-40 (of their upper ends) */
-            constexpr int kEach = kPassBins / kPassThreads;
-            uint64_t in[kEach], mine = 0, all;
-            for (int i = 0; i < kEach; ++i) {
-                const int bin = tid * kEach + i;
-                in[i] = s.n[bin];
-                if (row.kind == kPassShare && in[i])
-                    in[i] = (uint64_t)((float)in[i] * pass_exp2(-(float)bin / scale * row.c) * 1.0995116e12f);
-                mine += in[i];
-            }
-            uint64_t run = pass_scan(s, mine, all) - mine;
-            uint64_t want = (uint64_t)row.k;
-            if (row.kind == kPassShare) {
-                /* keep until what is below weighs 3/4 of what it may */
-                const double gone = dropped * exp2((double)rc - (double)hi * (double)row.c) * 1.0995116e12;
-                const double may = 0.75 * (1.0 - (double)row.p) * ((double)all + gone) - gone;
-                want = may > 0.0 && may < (double)all ? all - (uint64_t)may : all;
-            }
-            for (int i = 0; i < kEach; ++i) {
-                if (run < want && run + in[i] >= want) s.found = tid * kEach + i;
-                run += in[i];
-            }
-            __syncthreads();
-            if (s.found < kPassBins - 1 && scale > 0.0f) {
-                const float edge = hi - (float)(s.found + 1) / scale;
-                f_new = fmaxf(f_new, edge - fabsf(edge) * 2e-7f - (hi - low) * 4e-7f);
-            }
+            f_new = fmaxf(f_new, edge(hi, low, scale, dropped, grow));
         }
         f = f_new;
         /* the kept ones move up; a turn's places are read before any of them is written */
         __syncthreads();
-        if (tid == 0) s.count = 0;
+        if (tid == 0) s.count = 0, s.valid = kPassKeep, s.full = 0;
         for (int at = 0; at < n; at += 4 * kPassThreads) {
             uint64_t e[4];
 #pragma unroll
@@ -707,9 +772,9 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
             int mine = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float x = pass_x(e[j]);
-                if (e[j] && x >= f) ++mine;
-                else if (e[j] && weigh) rest += (double)pass_exp2(fmaf(x, row.c, -rc)), e[j] = 0;
+                const float v = pass_x(e[j]);
+                if (e[j] && v >= f) ++mine;
+                else if (e[j] && weigh) rest += (double)pass_exp2(fmaf(v, row.c, -rc)), e[j] = 0;
                 else e[j] = 0;
             }
             uint32_t to = mine ? atomicAdd(&s.count, (uint32_t)mine) : 0;
@@ -718,72 +783,85 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
                 if (e[j]) keep[to++] = e[j];
         }
         __syncthreads();
-        if (tid == 0 && s.count > kPassTurn) s.lost = 1;
-        full = false;
+        if (tid == 0 && s.count > kPassFull) s.lost = 1;
         __syncthreads();
     };
 
     if (me == 0) {
+        /* the row's ends beside whole vectors: at most 14 elements */
         const int tail = head + vecs * V::kPer;
-        if (tid < head) {
-            const float x = req_value(base[tid]);
-            if (x >= f) put(x, tid);
-        }
-        if (tid < vocab - tail) {
-            const float x = req_value(base[tail + tid]);
-            if (x >= f) put(x, tail + tid);
-        }
+        const int id = tid < head ? tid : tail + tid - head;
+        const float v = id < vocab ? req_value(base[id]) : -INFINITY;
+        if (tid < 16 && v >= f) keep[atomicAdd(&s.count, 1u)] = pass_pack(v, id);
+        else if (weigh && tid < 16) rest += (double)pass_exp2(fmaf(v, row.c, -rc));
     }
-    uint4 next[kVecs];
-    auto load = [&](int turn) {
+    __syncthreads();
+
+    /*
+     * The row.  Warps go on by themselves; where the list runs over, all of
+     * them meet to raise the filter, and those whose elements found no place
+     * try again.
+     */
+    int done = 0;  // turns of this warp
+    for (;;) {
+        while (done < a.turns) {
+            const int full = *(volatile int *)&s.full;
+            float most = x[0];
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j) {
-            const int v = first + turn * (kPassThreads * kVecs) + j * kPassThreads + tid;
-            next[j] = v < last ? pass_load(body + v) : V::none();
-        }
-    };
-    int turn = 0;
-    load(0);
-    for (int i = 0; i < a.turns; ++i) {
-        float x[kPassEach];
+            for (int j = 1; j < kPassEach; ++j) most = fmaxf(most, x[j]);
+            if (__any_sync(0xFFFFFFFFu, most >= f)) {
+                uint32_t mask = 0;
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j) V::get(next[j], x + j * V::kPer);
-        const int here = turn;
-        turn += a.step;
-        if (turn >= a.turns) turn -= a.turns;
-        if (i + 1 < a.turns) load(turn);
-        float most = x[0];
+                for (int j = 0; j < kPassEach; ++j) mask |= x[j] >= f ? 1u << j : 0u;
+                bool again = false;
+                if (mask) {
+                    const uint32_t n = __popc(mask);
+                    uint32_t at = atomicAdd(&s.count, n);
+                    if (at + n <= kPassKeep) {
 #pragma unroll
-        for (int j = 1; j < kPassEach; ++j) most = fmaxf(most, x[j]);
-        if (__any_sync(0xFFFFFFFFu, most >= f)) {
-#pragma unroll
-            for (int j = 0; j < kPassEach; ++j) {
-                if (x[j] >= f) {
-                    const int v = first + here * (kPassThreads * kVecs) + (j / V::kPer) * kPassThreads + tid;
-                    put(x[j], head + v * V::kPer + j % V::kPer);
-                    x[j] = -INFINITY;
+                        for (int j = 0; j < kPassEach; ++j)
+                            if (mask >> j & 1) {
+                                const int v = first + turn * (32 * kVecs) + (j / V::kPer) * 32 + lane;
+                                keep[at++] = pass_pack(x[j], head + v * V::kPer + j % V::kPer);
+                                x[j] = -INFINITY;
+                            }
+                    } else {  // from the first place that ran over on, none is filled
+                        atomicMin(&s.valid, at);
+                        s.full = 1;
+                        again = true;
+                    }
                 }
+                if (__any_sync(0xFFFFFFFFu, again)) break;
             }
-        }
-        if (weigh) {
-            float w[kPassEach];
+            if (weigh) {
+                float w[kPassEach];
 #pragma unroll
-            for (int j = 0; j < kPassEach; ++j) w[j] = x[j] == x[j] ? pass_exp2(fmaf(x[j], row.c, -rc)) : 0.0f;
+                for (int j = 0; j < kPassEach; ++j) w[j] = pass_exp2(fmaf(x[j], row.c, -rc));  // a NaN stays in the sum
 #pragma unroll
-            for (int d = kPassEach / 2; d; d >>= 1)
+                for (int d = kPassEach / 2; d; d >>= 1)
 #pragma unroll
-                for (int j = 0; j < d; ++j) w[j] += w[j + d];
-            rest += (double)w[0];
+                    for (int j = 0; j < d; ++j) w[j] += w[j + d];
+                rest += (double)w[0];
+            }
+            if (++done < a.turns) {
+                turn = ahead;
+#pragma unroll
+                for (int j = 0; j < kVecs; ++j) V::get(next[j], x + j * V::kPer);
+                ahead += a.step;
+                if (ahead >= a.turns) ahead -= a.turns;
+                if (done + 1 < a.turns) load(ahead);
+            }
+            if (full) break;
         }
-        if (__syncthreads_or(full || i == 0)) {
-            raise();
-            if (s.lost) break;
-        }
+        __syncthreads();
+        if (!s.full) break;  // every warp is through
+        raise(row.kind == kPassShare ? (double)a.turns * kPassThreads / fmax(pass_sum(s, (double)done), 1.0) : 1.0);
+        if (s.lost) break;
     }
     __syncthreads();
 
     /* the cluster's parts come together in the first one's memory, after a last rise so that little moves */
-    if (nc > 1 && !s.lost) raise();
+    if (nc > 1 && !s.lost) raise(1.0);
     const double dropped = weigh ? pass_sum(s, rest) : 0.0;
     if (nc > 1) {
         __syncthreads();
@@ -833,7 +911,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         double apart = 0.0;
         for (int c = 0; c < nc; ++c) {
             const double up = (double)s.part_rc[c] - (double)hi * (double)row.c;
-            if (s.part_rest[c] > 0.0) gone += s.part_rest[c] * exp2(up), apart = fmax(apart, fabs(up));
+            if (s.part_rest[c] != 0.0) gone += s.part_rest[c] * exp2(up), apart = fmax(apart, fabs(up));  // NaN too
         }
         /*
          * Against the sum of the definition's weights: an exponential is off by 2^-22 of itself, four additions by
@@ -846,7 +924,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         const double spread = gone > 0.0 ? log2(fmax(ids / gone, 2.0)) : 0.0;
         gone_error = gone * (ldexp(1.0, -21) + 0.6932 * (spread * 2.0 + apart) * ldexp(1.0, -24)) * 1.01 +
                      ids * (1e-13 + ldexp(1.0, -43));
-        if (!(gone < 1e7)) {  // the reference was too far below
+        if (!(gone < 1e7)) {  // the reference was too far below, or there is a NaN
             if (tid == 0) a.r.status[b] = 1;
             return;
         }
@@ -864,7 +942,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
             rc = hi * row.c;
             rest = tid == 0 ? gone * exp2((double)hi * (double)row.c - (double)rc) : 0.0;
         }
-        raise();
+        raise(1.0);
         n = (int)s.count;
         if (row.kind == kPassShare) {
             gone = pass_sum(s, rest) * exp2((double)rc - (double)hi * (double)row.c);
