@@ -115,6 +115,10 @@ struct ReqShared {
     uint32_t warp_n[kReqWarps];
     uint32_t red[kReqWarps];
     int32_t cut_id;
+    uint32_t ends[2];
+    uint64_t before;
+    uint32_t region;
+    uint32_t rows[kReqWarps];
 };
 
 template <typename T>
@@ -185,6 +189,13 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
     };
     if (by_weight && all_weight) want_w = share(*all_weight);
     bool first = true;
+    /*
+     * The first histogram of a wide range goes by values, evenly between its ends: by keys, which are denser near
+     * zero, most elements would meet in a few bins.
+     */
+    const float top = req_unkey(hi), scale = ((float)kReqBins - 0.5f) / (top - req_unkey(lo + 1));
+    bool even = hi - lo > 64 * kReqBins && scale > 0.0f && scale < 3e38f;
+    auto even_bin = [&](uint32_t key) { return min((uint32_t)((top - req_unkey(key)) * scale), (uint32_t)kReqBins - 1); };
     for (;;) {
         const uint32_t span = hi - lo;
         const int shift = span <= kReqBins ? 0 : 32 - __clz((span - 1) / kReqBins);
@@ -194,7 +205,7 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
             const float x = sl.at(i);
             const uint32_t key = req_key(x);
             if (key > lo && key <= hi) {
-                const uint32_t bin = (hi - key) >> shift;
+                const uint32_t bin = even ? even_bin(key) : (hi - key) >> shift;
                 const uint64_t w = req_weight(r, x);
                 atomicAdd(&s.n[bin], 1u);
                 const uint32_t wl = (uint32_t)w, old = atomicAdd(&s.lo[bin], wl);
@@ -241,6 +252,24 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
         const uint32_t bin = s.found_bin;
         if (bin == kReqBins) return {lo, 0, above + s.total, false};
         above = s.found_above;
+        if (even) {
+            /* the bin's keys: bins fall as keys rise, so both ends are found by halving */
+            if (tid < 2) {
+                uint32_t in = lo, out = hi;  // the largest key whose bin is bin (thread 0) or the next one (thread 1) at least
+                if (even_bin(out) >= bin + tid) in = out;
+                while (out - in > 1) {
+                    const uint32_t mid = in + (out - in) / 2;
+                    if (even_bin(mid) >= bin + tid) in = mid;
+                    else out = mid;
+                }
+                s.ends[tid] = in;
+            }
+            __syncthreads();
+            hi = s.ends[0], lo = s.ends[1];
+            even = false;
+            __syncthreads();
+            continue;
+        }
         if (shift == 0) {
             const uint32_t key = hi - bin, n = s.all_n[bin];
             __syncthreads();
@@ -279,7 +308,7 @@ __device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char
     /* the row's largest logit */
     float top = -INFINITY;
     T *keep = reinterpret_cast<T *>(req_raw);
-#pragma unroll 8
+#pragma unroll 16
     for (int i = tid; i < sl.n; i += kReqThreads) {
         const T raw = sl.global[i];
         if (a.resident) keep[i] = raw;
@@ -392,47 +421,94 @@ __device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char
         total += all[c][0];
         count += (uint32_t)all[c][1];
     }
-    for (int w = 0; w < warp; ++w) before += s.warp[w].w;
     uint64_t target = r.u >= 1.0f ? total : __umul64hi((uint64_t)((double)r.u * 18446744073709551616.0), total);
     if (target >= total) target = total - 1;
-    if (before <= target && target < before + sum.w) {
-        bool found = false;
-        for (int i = begin; i < end && !found; i += 32) {
-            const uint64_t w = i + lane < end ? weight(i + lane) : 0;
-            uint64_t run = w;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint64_t o = __shfl_up_sync(0xFFFFFFFFu, run, d);
-                if (lane >= d) run += o;
-            }
-            const uint32_t over = __ballot_sync(0xFFFFFFFFu, before + run > target);
-            if (over) {
-                found = true;
-                if (lane == __ffs(over) - 1) {
-                    a.ids[b] = sl.first + i + lane;
-                    if (a.probs)
-                        a.probs[b] = (float)(req_exp(r, sl.at(i + lane)) * (double)(1ull << kReqFraction) / (double)total);
-                    if (a.counts) a.counts[b] = (int32_t)count;
-                }
-            }
-            before += __shfl_sync(0xFFFFFFFFu, run, 31);
+    if (target < before || target - before >= cta.w) return;  // in another CTA's part
+    for (int w = 0; w < warp; ++w) before += s.warp[w].w;
+    if (lane == 0 && before <= target && target - before < sum.w) s.region = warp, s.before = before;
+    __syncthreads();
+    /* the region that it ends in, some neighbouring elements to a thread */
+    const int each = (region + kReqThreads - 1) / kReqThreads;
+    const int from = s.region * region + tid * each, to = min(min(sl.n, (int)(s.region + 1) * region), from + each);
+    uint64_t mine = 0;
+    before = s.before;
+    for (int i = from; i < to; ++i) mine += weight(i);
+    before += req_scan(s, {0, mine}).w - mine;
+    for (int i = from; i < to; ++i) {
+        const uint64_t w = weight(i);
+        if (before <= target && target < before + w) {
+            a.ids[b] = sl.first + i;
+            if (a.probs) a.probs[b] = (float)(req_exp(r, sl.at(i)) * (double)(1ull << kReqFraction) / (double)total);
+            if (a.counts) a.counts[b] = (int32_t)count;
         }
+        before += w;
     }
 }
 
+enum PassKind { kPassGreedy, kPassCount, kPassLeast, kPassShare, kPassNot };
+constexpr int kPassTopK = 1024;  // largest top_k of sample_pass_kernel
+
+/* What a row's settings come to before its largest logit is known. */
+struct PassRow {
+    PassKind kind;
+    int k;
+    float t, p, floor_t;  // floor = largest + floor_t (a little below, so that nothing is dropped too early)
+    float c;              // log2(e) / T
+};
+
+__device__ __forceinline__ PassRow pass_row(const RequestArgs &a, int b) {
+    PassRow r;
+    const float t = a.temperature ? a.temperature[b] : 1.0f;
+    const float least = a.min_p ? a.min_p[b] : 0.0f;
+    r.p = a.top_p ? a.top_p[b] : 1.0f;
+    r.k = a.top_k ? a.top_k[b] : 0;
+    r.t = t;
+    r.c = (float)(1.4426950408889634 / (double)t);
+    r.floor_t = -30.0f * t;
+    if (least > 0.0f) r.floor_t = fmaxf(r.floor_t, t * logf(fminf(least, 1.0f)) * 1.0001f);
+    const bool plain = t >= 1e-3f && t <= 1e4f;  // what fp32 bounds below are made for
+    if (!(t > 0.0f)) r.kind = kPassGreedy, r.k = 1, r.floor_t = 0.0f;
+    else if (!plain) r.kind = kPassNot;
+    else if (r.k > 0 && r.k <= kPassTopK) r.kind = kPassCount;
+    else if (least > 0.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassLeast;
+    else if (r.p < 1.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassShare;
+    else r.kind = kPassNot;
+    return r;
+}
+/*
+ * The rows that sample_pass_kernel does not take, by their settings, while it
+ * runs, and those that it could not settle, after it.  The clusters take them
+ * in turn.
+ */
 template <typename T>
 __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __grid_constant__ RequestArgs a) {
     extern __shared__ __align__(16) unsigned char req_raw[];
     __shared__ ReqShared s;
     cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, n = cluster.num_blocks();
+    const uint32_t me = blockIdx.x / n, clusters = gridDim.x / n;
     int turn = 0;
     cluster.sync();  // every CTA of the cluster is there before one writes into another's memory
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int n = cluster.num_blocks();
-    for (int b = blockIdx.x / n; b < a.batch; b += gridDim.x / n) {
-        if (a.status[b] == 0) continue;
-        req_sample_row<T>(a, s, req_raw, b, turn);
-        __syncthreads();
+    for (int after = 0; after < 2; ++after) {
+        if (after) asm volatile("griddepcontrol.wait;" ::: "memory");
+        uint32_t rank = 0;
+        for (int at = 0; at < a.batch; at += kReqThreads) {
+            bool mine = false;
+            if (at + tid < a.batch) {
+                const bool not_passed = pass_row(a, at + tid).kind == kPassNot;
+                mine = after ? !not_passed && a.status[at + tid] != 0 : not_passed;
+            }
+            const uint32_t bits = __ballot_sync(0xFFFFFFFFu, mine);
+            __syncthreads();
+            if ((tid & 31) == 0) s.rows[tid >> 5] = bits;
+            __syncthreads();
+            for (int w = 0; w < kReqWarps; ++w)
+                for (uint32_t left = s.rows[w]; left; left &= left - 1)
+                    if (rank++ % clusters == me) {
+                        req_sample_row<T>(a, s, req_raw, at + w * 32 + __ffs(left) - 1, turn);
+                        __syncthreads();
+                    }
+        }
     }
 }
 
@@ -462,14 +538,11 @@ constexpr int kPassKeep = 4096;   // kept at most
 constexpr int kPassFull = 3072;   // and at most after the filter has risen
 constexpr int kPassBins = 1024;
 constexpr int kPassSort = 2048;   // of those, at the end
-constexpr int kPassTopK = 1024;   // largest top_k
 
 struct PassArgs {
     RequestArgs r;    // r.status gets 1 where the row is left to sample_requests_kernel, else 0
     int turns, step;  // turns of a warp's part of a row, taken in steps of step (no common divisor)
 };
-
-enum PassKind { kPassGreedy, kPassCount, kPassLeast, kPassShare, kPassNot };
 
 struct PassShared {
     uint32_t n[kPassBins];
@@ -567,33 +640,6 @@ __device__ __forceinline__ uint64_t pass_scan(PassShared &s, uint64_t v, uint64_
     return before + v;
 }
 
-/* What a row's settings come to before its largest logit is known. */
-struct PassRow {
-    PassKind kind;
-    int k;
-    float t, p, floor_t;  // floor = largest + floor_t (a little below, so that nothing is dropped too early)
-    float c;              // log2(e) / T
-};
-
-__device__ __forceinline__ PassRow pass_row(const RequestArgs &a, int b) {
-    PassRow r;
-    const float t = a.temperature ? a.temperature[b] : 1.0f;
-    const float least = a.min_p ? a.min_p[b] : 0.0f;
-    r.p = a.top_p ? a.top_p[b] : 1.0f;
-    r.k = a.top_k ? a.top_k[b] : 0;
-    r.t = t;
-    r.c = (float)(1.4426950408889634 / (double)t);
-    r.floor_t = -30.0f * t;
-    if (least > 0.0f) r.floor_t = fmaxf(r.floor_t, t * logf(fminf(least, 1.0f)) * 1.0001f);
-    const bool plain = t >= 1e-3f && t <= 1e4f;  // what fp32 bounds below are made for
-    if (!(t > 0.0f)) r.kind = kPassGreedy, r.k = 1, r.floor_t = 0.0f;
-    else if (!plain) r.kind = kPassNot;
-    else if (r.k > 0 && r.k <= kPassTopK) r.kind = kPassCount;
-    else if (least > 0.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassLeast;
-    else if (r.p < 1.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassShare;
-    else r.kind = kPassNot;
-    return r;
-}
 /* a value that is not above the smallest that the temperature and min-p leave beside a largest logit of m */
 __device__ __forceinline__ float pass_floor(const PassRow &r, float m) {
     const float f = m + r.floor_t;
@@ -684,18 +730,22 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         __syncthreads();
         if (row.kind == kPassShare) {
             /*
-             * What will have been dropped in the end, as of the part seen so far, may be 3/4 of 1 - top_p of the row's
-             * weight; for that the 16 largest so far count once and the others for as much as the part has seen.
+             * What will have been dropped in the end, as of the part seen so far, may be 3/4 (early on, 1/2) of 1 -
+             * top_p of the row's weight; for that the 16 largest so far count once and the others for as much as the
+             * part has seen.  The 24 largest of an early part stay: what lies below them is even enough to count on.
              */
             const double weight = (double)(all >> 14), gone = dropped * 6.8719477e10, seen = weight + gone;
             const double row_weight = seen + (grow - 1.0) * (seen - s.top);
-            const double may = 0.75 * (1.0 - (double)row.p) * row_weight / grow - gone;
+            const double may = (grow > 2.0 ? 0.5 : 0.75) * (1.0 - (double)row.p) * row_weight / grow - gone;
             const uint64_t want = may > 0.0 && may < weight ? (all >> 14) - (uint64_t)may : all >> 14;
+            const uint32_t least = grow > 2.0 ? 24u : 1u;
             run = begin;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const uint64_t after = run + in[i];
-                if (run >> 14 < want && after >> 14 >= want) s.found = tid * kEach + i;
+                const bool reached = after >> 14 >= want && (uint32_t)(after & 16383) >= least;
+                const bool earlier = run >> 14 >= want && (uint32_t)(run & 16383) >= least;
+                if (reached && !earlier) s.found = tid * kEach + i;
                 run = after;
             }
             __syncthreads();
@@ -886,7 +936,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         if (me != 0) return;
     }
     if (s.lost) {
-        if (tid == 0) a.r.status[b] = 1;
+        if (tid == 0) a.r.status[b] = 2;
         return;
     }
     if (tid == 0) s.part_rest[0] = dropped, s.part_rc[0] = rc;
@@ -925,12 +975,12 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         gone_error = gone * (ldexp(1.0, -21) + 0.6932 * (spread * 2.0 + apart) * ldexp(1.0, -24)) * 1.01 +
                      ids * (1e-13 + ldexp(1.0, -43));
         if (!(gone < 1e7)) {  // the reference was too far below, or there is a NaN
-            if (tid == 0) a.r.status[b] = 1;
+            if (tid == 0) a.r.status[b] = 3;
             return;
         }
     }
     if (!(hi < INFINITY)) {
-        if (tid == 0) a.r.status[b] = 1;
+        if (tid == 0) a.r.status[b] = 4;
         return;
     }
     /* one more rise for a shorter sort */
@@ -952,7 +1002,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         __syncthreads();
     }
     if (s.lost || n > kPassSort) {
-        if (tid == 0) a.r.status[b] = 1;
+        if (tid == 0) a.r.status[b] = 5;
         return;
     }
     int size = 32;
@@ -1016,7 +1066,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         left = (int)s.found;
         /* open within the error, or a lost bet: the row's other ids weigh too much, or some come before the cut */
         if (s.found != s.found_high || left == 0 || (row.kind == kPassShare && !(pass_x(keep[left - 1]) >= f))) {
-            if (tid == 0) a.r.status[b] = 1;
+            if (tid == 0) a.r.status[b] = 6;
             return;
         }
     }
