@@ -36,7 +36,7 @@ int byte_map(CUtensorMap *m, const void *base, int rows, int cols, size_t ld, in
     const int r = encode_fn(&encode);
     if (r) return r;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
-    const cuuint32_t box[2] = {(cuuint32_t)kI8Chunk, (cuuint32_t)box_rows}, each[2] = {1, 1};
+    const cuuint32_t box[2] = {(cuuint32_t)kI8Line, (cuuint32_t)box_rows}, each[2] = {1, 1};
     const CUresult e = encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, each,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -114,8 +114,9 @@ int product_args(const int8_t *a, size_t lda, const float *a_scale, int tokens, 
 
 template <int NT, bool PAIR, typename OUT>
 int product_launch(const Product &p, const I8Args &args, int groups, bool dependent, cudaStream_t s) {
-    CUtensorMap mw, ma;
-    int r = byte_map(&mw, p.w, args.rows, args.cols, p.ldw, kI8Box);
+    CUtensorMap mw, mp, ma;
+    int r = byte_map(&mw, p.w, args.rows, args.cols, p.ldw, kI8RowsCta);
+    if (!r) r = byte_map(&mp, p.w, args.rows, args.cols, p.ldw, kI8Box);
     if (!r) r = byte_map(&ma, p.a, args.tokens, args.cols, p.lda, PAIR ? NT / 2 : NT);
     if (!r) r = dynamic_smem((const void *)i8_product_kernel<NT, PAIR, OUT>, i8_smem(NT, PAIR));
     if (r) return r;
@@ -138,7 +139,7 @@ int product_launch(const Product &p, const I8Args &args, int groups, bool depend
     }
     lc.attrs = at;
     lc.numAttrs = n;
-    CUDA_TRY(cudaLaunchKernelEx(&lc, i8_product_kernel<NT, PAIR, OUT>, mw, ma, args));
+    CUDA_TRY(cudaLaunchKernelEx(&lc, i8_product_kernel<NT, PAIR, OUT>, mw, mp, ma, args));
     CUDA_TRY(cudaGetLastError());
     return NOEL_OK;
 }
@@ -167,9 +168,9 @@ int product(const Product &p, bool dependent, cudaStream_t s) {
     const int t = p.args.tokens;
     if (t <= 16) return product_tile<16, false>(p, dependent, s);
     if (t <= 32) return product_tile<32, false>(p, dependent, s);
-    if (t <= 64) return product_tile<64, false>(p, dependent, s);
-    if (t <= 128) return product_tile<128, false>(p, dependent, s);
-    return product_tile<256, false>(p, dependent, s);
+    if (t <= 64) return product_tile<64, true>(p, dependent, s);
+    if (t <= 128) return product_tile<128, true>(p, dependent, s);
+    return product_tile<256, true>(p, dependent, s);
 }
 
 size_t cast_pitch(int cols) { return ((size_t)cols + 15) / 16 * 16; }

@@ -141,15 +141,18 @@ struct I8Args {
     int *failed;
 };
 
-constexpr int kI8Threads = 192;  // a warp of loads, one of products, four of results
+constexpr int kI8Threads = 352;  // two warps of loads, one of products, eight of results
 constexpr int kI8RowsCta = 128;  // rows of w in a CTA's tile (lanes of the tensor memory)
-constexpr int kI8Chunk = 128;    // columns (bytes) of a stage: one swizzled line of each row
-constexpr int kI8Box = 32;       // rows of w in one copy
+constexpr int kI8Line = 128;     // columns (bytes) of a copy: one swizzled line of each row
+constexpr int kI8Box = 32;       // rows of w in one copy where a tile has fewer than 128
 constexpr int kI8MaxStages = 12;
-constexpr int kI8Ring = 229376;  // bytes of the ring at most
+constexpr int kI8Ring = 225280;  // bytes of the ring at most
 
+/* lines of a row in a stage: two where tiles are narrow and the weights' stream is what counts (a stage is then 32 KB of
+ * them, and the memory is asked for 256 bytes of a row at once) */
+__host__ __device__ constexpr int i8_lines(int nt) { return nt <= 64 ? 2 : 1; }
 __host__ __device__ constexpr int i8_stage_bytes(int nt, bool pair) {
-    return (kI8RowsCta + (pair ? nt / 2 : nt)) * kI8Chunk;
+    return (kI8RowsCta + (pair ? nt / 2 : nt)) * kI8Line * i8_lines(nt);
 }
 __host__ __device__ constexpr int i8_stages(int nt, bool pair) {
     return kI8Ring / i8_stage_bytes(nt, pair) < kI8MaxStages ? kI8Ring / i8_stage_bytes(nt, pair) : kI8MaxStages;
@@ -285,19 +288,21 @@ struct I8Tiles {
  * A tile is 128 rows of w (256 of a pair of CTAs) by NT tokens: rows are
  * lanes of the tensor memory and tokens its columns, so that a warp's
  * results for a token lie side by side in y, and the few tokens of a decode
- * batch are columns of a narrow tile.  One lane copies stages of 128 columns
- * by TMA, one lane issues their products, four warps scale and store a
+ * batch are columns of a narrow tile.  Two lanes copy stages by TMA, the
+ * weights' one and the tokens' one, one lane issues their products, eight warps scale and store a
  * finished tile while the next one's products go into the other half of the
  * accumulators.
  */
 template <int NT, bool PAIR, typename OUT>
 __global__ void __launch_bounds__(kI8Threads, 1)
-    i8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
-                      const __grid_constant__ I8Args a) {
+    i8_product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_part,
+                      const __grid_constant__ CUtensorMap map_a, const __grid_constant__ I8Args a) {
     constexpr int kStages = i8_stages(NT, PAIR), kStage = i8_stage_bytes(NT, PAIR), kHalf = PAIR ? NT / 2 : NT;
+    constexpr int kLines = i8_lines(NT), kLineW = kI8RowsCta * kI8Line, kLineA = kHalf * kI8Line;  // a stage: w's lines, then a's
     constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
     extern __shared__ unsigned char i8_raw[];
     __shared__ __align__(8) uint64_t s_full[kI8MaxStages], s_empty[kI8MaxStages], s_done[2], s_free[2];
+    __shared__ float s_scale[2][NT];  // of the tile's tokens
     __shared__ uint32_t s_tmem;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t rank = 0;
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) i8_bar_init(i8_addr(&s_full[i]), 1), i8_bar_init(i8_addr(&s_empty[i]), 1);
-        for (int i = 0; i < 2; ++i) i8_bar_init(i8_addr(&s_done[i]), 1), i8_bar_init(i8_addr(&s_free[i]), PAIR ? 8 : 4);
+        for (int i = 0; i < 2; ++i) i8_bar_init(i8_addr(&s_done[i]), 1), i8_bar_init(i8_addr(&s_free[i]), PAIR ? 16 : 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -325,62 +330,64 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
-    const int chunks = (a.cols + kI8Chunk - 1) / kI8Chunk;
+    const int chunks = (a.cols + kLines * kI8Line - 1) / (kLines * kI8Line);
+    bool failed = false;  // a wait ran out
 
     if (warp == 0 && lane == 0 && !a.stall) {
-        /* ------------------------------------------------------- copies */
-        auto boxes = [](const I8Tiles<NT, PAIR> &t, int r) {  // copies of w for CTA r of the group
+        /* --------------------------------------------- copies of weights */
+        auto copies = [](const I8Tiles<NT, PAIR> &t, int r) {  // rows copied for CTA r of the group
             const int n = min(t.row_end - t.row - r * kI8RowsCta, kI8RowsCta);
-            return n <= 0 ? 0 : (n + kI8Box - 1) / kI8Box;
+            return n <= 0 ? 0 : (n + kI8Box - 1) / kI8Box * kI8Box;
         };
-        auto copy_w = [&](const I8Tiles<NT, PAIR> &t, int chunk, int stage) {
-            const uint32_t bar = i8_addr(&s_full[stage]);
-            if (rank == 0) {
-                int n = boxes(t, 0) * kI8Box + kHalf;
-                if (PAIR) n += boxes(t, 1) * kI8Box + kHalf;
-                i8_bar_expect(bar, (uint32_t)n * kI8Chunk);
-            }
-            const uint32_t to = PAIR ? i8_peer(bar, 0) : bar;
-            const int n = boxes(t, rank);
-            for (int i = 0; i < n; ++i)
-                i8_copy<PAIR>(&map_w, ring + stage * kStage + i * kI8Box * kI8Chunk, to, chunk * kI8Chunk,
-                              t.row + (int)rank * kI8RowsCta + i * kI8Box);
-        };
-        auto copy_a = [&](const I8Tiles<NT, PAIR> &t, int chunk, int stage) {
-            const uint32_t bar = i8_addr(&s_full[stage]);
-            i8_copy<PAIR>(&map_a, ring + stage * kStage + kI8RowsCta * kI8Chunk, PAIR ? i8_peer(bar, 0) : bar,
-                          chunk * kI8Chunk, t.t0 + (int)rank * kHalf);
-        };
-        /* the weights of the first stages do not wait for the cast of the tokens */
-        I8Tiles<NT, PAIR> early(a);
-        int c = 0, n = 0;
-        for (; n < kStages && early.more(); ++n) {
-            copy_w(early, c, n);
-            if (++c == chunks) c = 0, early.next();
-        }
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        bool good = true;
-        int i = 0, stage = 0;
+        I8Tiles<NT, PAIR> t(a);
+        int stage = 0;
         uint32_t phase = 0;
-        for (I8Tiles<NT, PAIR> t(a); good && t.more(); t.next())
-            for (int k = 0; k < chunks; ++k, ++i) {
-                if (i >= n) {
-                    good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns);
-                    if (!good) break;
-                    copy_w(t, k, stage);
+        bool good = true;
+        for (; good && t.more(); t.next()) {
+            const int n = copies(t, rank), row = t.row + (int)rank * kI8RowsCta;
+            int all = n + kHalf;
+            if (PAIR) all += copies(t, rank ^ 1) + kHalf;
+            for (int k = 0; k < chunks; ++k) {
+                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns);
+                if (!good) break;
+                const uint32_t bar = i8_addr(&s_full[stage]), to = PAIR ? i8_peer(bar, 0) : bar, at = ring + stage * kStage;
+                if (rank == 0) i8_bar_expect(bar, (uint32_t)all * kI8Line * kLines);
+#pragma unroll
+                for (int l = 0; l < kLines; ++l) {
+                    const int x = (k * kLines + l) * kI8Line;
+                    if (n == kI8RowsCta) {
+                        i8_copy<PAIR>(&map_w, at + l * kLineW, to, x, row);
+                    } else {
+                        for (int i = 0; i < n; i += kI8Box) i8_copy<PAIR>(&map_part, at + l * kLineW + i * kI8Line, to, x, row + i);
+                    }
                 }
-                copy_a(t, k, stage);
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
+        }
         if (!good) {
             *a.failed = 1;
             /* what is still on its way into this CTA's memory lands before it ends */
             if (rank == 0)
-                for (int s = 0; s < kStages; ++s) {
-                    const int latest = s < stage ? (int)phase : (int)(phase ^ 1);
-                    i8_wait(i8_addr(&s_full[s]), latest, a.wait_ns);
-                }
+                for (int s = 0; s < kStages; ++s) i8_wait(i8_addr(&s_full[s]), s < stage ? phase : phase ^ 1, a.wait_ns);
         }
+    } else if (warp == 10 && lane == 0 && !a.stall) {
+        /* ---------------------------------------------- copies of tokens */
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // their cast; the first weights do not wait for it
+        int stage = 0;
+        uint32_t phase = 0;
+        bool good = true;
+        for (I8Tiles<NT, PAIR> t(a); good && t.more(); t.next())
+            for (int k = 0; k < chunks; ++k) {
+                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns);
+                if (!good) break;
+                const uint32_t bar = i8_addr(&s_full[stage]), to = PAIR ? i8_peer(bar, 0) : bar;
+#pragma unroll
+                for (int l = 0; l < kLines; ++l)
+                    i8_copy<PAIR>(&map_a, ring + stage * kStage + kLines * kLineW + l * kLineA, to, (k * kLines + l) * kI8Line,
+                                  t.t0 + (int)rank * kHalf);
+                if (++stage == kStages) stage = 0, phase ^= 1;
+            }
+        if (!good) *a.failed = 1;
     } else if (warp == 1 && lane == 0 && rank == 0) {
         /* ----------------------------------------------------- products */
         /* 32-bit sums of signed bytes, N and M of the tile */
@@ -397,20 +404,24 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                 good = i8_wait(i8_addr(&s_full[stage]), phase, a.wait_ns);
                 if (!good) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t dw = i8_desc(ring + stage * kStage), da = i8_desc(ring + stage * kStage + kI8RowsCta * kI8Chunk);
+                const uint64_t dw = i8_desc(ring + stage * kStage), da = i8_desc(ring + stage * kStage + kLines * kLineW);
 #pragma unroll
-                for (int j = 0; j < kI8Chunk / 32; ++j)
-                    i8_mma<PAIR>(tmem + half * NT, dw + 2 * j, da + 2 * j, kIdesc, k > 0 || j > 0);
+                for (int l = 0; l < kLines; ++l)
+#pragma unroll
+                    for (int j = 0; j < kI8Line / 32; ++j)
+                        i8_mma<PAIR>(tmem + half * NT, dw + l * (kLineW >> 4) + 2 * j, da + l * (kLineA >> 4) + 2 * j, kIdesc,
+                                     k > 0 || l > 0 || j > 0);
                 i8_commit<PAIR>(i8_addr(&s_empty[stage]));
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
             if (good) i8_commit<PAIR>(i8_addr(&s_done[half]));
         }
         if (!good) *a.failed = 1;
-    } else if (warp >= 2) {
+    } else if (warp >= 2 && warp < 10) {
         /* ------------------------------------------------------ results */
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        const int quarter = warp & 3;  // the lanes of the tensor memory that this warp may read
+        /* a quarter of the tensor memory's lanes, which is all that a warp may read, and every other 16 tokens */
+        const int quarter = warp & 3, side = (warp - 2) >> 2;
         int tile = 0;
         for (I8Tiles<NT, PAIR> t(a); t.more(); t.next(), ++tile) {
             const int half = tile & 1;
@@ -418,16 +429,16 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             const bool mine = r < t.row_end;
             const float ws = mine ? a.w_scale[r] : 0.0f;
             const int nt = min(NT, a.tokens - t.t0);
-            OUT *y = static_cast<OUT *>(a.y) + (int64_t)t.t0 * a.ldy + r;
-            const float *as = a.a_scale + t.t0;
+            for (int i = threadIdx.x - 64; i < nt; i += 256) s_scale[half][i] = a.a_scale[t.t0 + i];
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // those of two tiles ago have been used
             if (!__all_sync(0xFFFFFFFFu, i8_wait(i8_addr(&s_done[half]), (tile >> 1) & 1, a.wait_ns))) {
                 if (lane == 0) *a.failed = 1;
-                break;
+                failed = true;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            OUT *y = static_cast<OUT *>(a.y) + (int64_t)(t.t0 + side * 16) * a.ldy + r;
 #pragma unroll 1
-            for (int c = 0; c < NT; c += 16) {
-                if (c >= nt) break;
+            for (int c = side * 16; c < nt && !failed; c += 32, y += 32 * a.ldy) {
                 uint32_t v[16];
                 asm volatile(
                     "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -436,9 +447,16 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                     : "r"(tmem + ((uint32_t)(quarter * 32) << 16) + half * NT + c));
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 if (mine) {
+                    const float *as = &s_scale[half][c];
+                    OUT *to = y;
+                    if (c + 16 <= nt) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (c + j < nt) i8_store(y + (int64_t)(c + j) * a.ldy, __int2float_rn((int)v[j]) * ws * as[c + j]);
+                        for (int j = 0; j < 16; ++j, to += a.ldy) i8_store(to, __int2float_rn((int)v[j]) * ws * as[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 15; ++j, to += a.ldy)
+                            if (c + j < nt) i8_store(to, __int2float_rn((int)v[j]) * ws * as[j]);
+                    }
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
