@@ -37,6 +37,7 @@ struct RequestArgs {
 constexpr int kReqThreads = 512;
 constexpr int kReqWarps = kReqThreads / 32;
 constexpr int kReqBins = 1024;
+constexpr int kReqList = 1024;
 constexpr int kReqMaxCluster = 8;
 constexpr int kReqFraction = 43;  // bits behind the point of a weight: 2^20 of them fit 64 bits, and e^-30 is not 0
 
@@ -55,7 +56,7 @@ __device__ __forceinline__ float req_unkey(uint32_t k) {
 /* One row's settings. */
 struct ReqRow {
     float m;          // its largest logit
-    double inv_t;
+    double c64;       // 64 log2(e) / T
     bool greedy;
     uint32_t floor;   // key of the smallest value left by the temperature and by min-p
     int k;            // 0: off
@@ -63,24 +64,48 @@ struct ReqRow {
     float u;
 };
 
-__device__ __forceinline__ double req_exp(const ReqRow &r, float x) {
-    return x == r.m ? 1.0 : exp(((double)x - (double)r.m) * r.inv_t);
-}
-__device__ __forceinline__ uint64_t req_weight(const ReqRow &r, float x) {
-    return __double2ull_rn(req_exp(r, x) * (double)(1ull << kReqFraction));
+constexpr int kReqTable = 64;  // 2^(j / 64), in shared memory
+
+__device__ __forceinline__ void req_table(double *table) {
+    if (threadIdx.x < kReqTable) table[threadIdx.x] = exp2((double)threadIdx.x / kReqTable);
 }
 
-__device__ __forceinline__ ReqRow req_row(const RequestArgs &a, int b, float m) {
+/*
+ * exp((x - m) / T) for x from the row's floor on: 2^(t / 64) with t from -2771
+ * to 0, its whole part by the table and the exponent, the rest (half of one
+ * at most, z = its natural exponent, below 0.0055) by the exponential
+ * series, whose next term z^6 / 720 is below 2^-54.
+ */
+__device__ __forceinline__ double req_exp(const ReqRow &r, float x, const double *table) {
+    if (x == r.m) return 1.0;  // infinite ones too
+    const double t = ((double)x - (double)r.m) * r.c64;
+    const double up = t + 6755399441055744.0;  // 1.5 * 2^52: its low bits are t to the nearest whole number
+    const int k = __double2loint(up);
+    const double z = (t - (up - 6755399441055744.0)) * (0.69314718055994531 / kReqTable);
+    double v = fma(1.0 / 120, z, 1.0 / 24);
+    v = fma(v, z, 1.0 / 6);
+    v = fma(v, z, 0.5);
+    v = fma(v, z, 1.0);
+    v = fma(v, z, 1.0);
+    v *= table[k & (kReqTable - 1)];
+    return __hiloint2double(__double2hiint(v) + (k >> 6 << 20), __double2loint(v));
+}
+/* in 2^-43, to the nearest */
+__device__ __forceinline__ uint64_t req_weight(const ReqRow &r, float x, const double *table) {
+    const double v = fma(req_exp(r, x, table), (double)(1ull << kReqFraction), 4503599627370496.0);  // 2^52: the number is its low bits
+    return (uint64_t)__double_as_longlong(v) & 0xFFFFFFFFFFFFFull;
+}
+
+__device__ __forceinline__ ReqRow req_row(const RequestArgs &a, int b, float m, float u) {
     ReqRow r;
     const float t = a.temperature ? a.temperature[b] : 1.0f;
     const float least = a.min_p ? a.min_p[b] : 0.0f, p = a.top_p ? a.top_p[b] : 1.0f;
     r.m = m;
     r.greedy = !(t > 0.0f);
-    r.inv_t = 1.0 / (double)t;
+    r.c64 = kReqTable * 1.4426950408889634 / (double)t;
     r.k = a.top_k ? a.top_k[b] : 0;
     if (r.k <= 0 || r.k >= a.vocab) r.k = 0;
     r.p = p < 1.0f ? fmax((double)p, 0.0) : 1.0;
-    const float u = a.u[b];
     r.u = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
     /* in 64 bits, then the smallest fp32 number that is not below */
     double floor = (double)m - 30.0 * (double)t;
@@ -119,6 +144,9 @@ struct ReqShared {
     uint64_t before;
     uint32_t region;
     uint32_t rows[kReqWarps];
+    double table[kReqTable];
+    uint64_t list[kReqList];  // the elements around a cut, of the whole row
+    uint32_t count;
 };
 
 template <typename T>
@@ -167,7 +195,72 @@ struct ReqCut {
     uint32_t ties;  // the first so many at it
     ReqSum above;   // of the ids above it
     bool some;      // false: nothing is cut
+    int32_t id;     // the last of those at it, or -1: not known
+    uint64_t kept;  // weight of all that is left
 };
+
+/* The CTA's list of size (a power of two) numbers, largest first. */
+template <int THREADS>
+__device__ __forceinline__ void req_sort(uint64_t *list, int size) {
+    for (int width = 2; width <= size; width <<= 1)
+        for (int d = width >> 1; d; d >>= 1) {
+            for (int i = threadIdx.x; i < size / 2; i += THREADS) {
+                const int lo = 2 * i - (i & (d - 1)), up = lo + d;
+                const uint64_t x = list[lo], y = list[up];
+                if ((x < y) == ((lo & width) == 0)) list[lo] = y, list[up] = x;
+            }
+            __syncthreads();
+        }
+}
+
+/* req_cut where few elements (n of the row) are in the range that holds the cut: every CTA sorts all of them. */
+template <typename T>
+__device__ ReqCut req_cut_list(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, uint32_t lo, uint32_t hi, uint32_t n,
+                               ReqSum above, bool by_weight, uint32_t want_n, uint64_t want_w, int &turn) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int me = cluster.block_rank(), nc = cluster.num_blocks(), tid = threadIdx.x;
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    uint64_t *mine = s.all_w;  // what it held has been used
+    for (int i = tid; i < sl.n; i += kReqThreads) {
+        const uint32_t key = req_key(sl.at(i));
+        if (key > lo && key <= hi) mine[atomicAdd(&s.count, 1u)] = (uint64_t)key << 32 | (0xFFFFFFFFu - (uint32_t)(sl.first + i));
+    }
+    __syncthreads();
+    const uint32_t have = s.count;
+    const uint64_t(*all)[2] = req_exchange(s, turn, have, 0);
+    uint32_t at = 0;
+    for (int c = 0; c < me; ++c) at += (uint32_t)all[c][0];
+    for (int c = 0; c < nc; ++c) {
+        uint64_t *to = cluster.map_shared_rank(&s, c)->list + at;
+        for (uint32_t i = tid; i < have; i += kReqThreads) to[i] = mine[i];
+    }
+    cluster.sync();
+    int size = 2;
+    while (size < (int)n) size <<= 1;
+    for (int i = n + tid; i < size; i += kReqThreads) s.list[i] = 0;
+    __syncthreads();
+    req_sort<kReqThreads>(s.list, size);
+    constexpr int kEach = kReqList / kReqThreads;
+    ReqSum in[kEach], sum = {0, 0};
+    for (int i = 0; i < kEach; ++i) {
+        const uint32_t j = tid * kEach + i;
+        in[i] = j < n ? ReqSum{1, req_weight(r, req_unkey((uint32_t)(s.list[j] >> 32)), s.table)} : ReqSum{0, 0};
+        sum = sum + in[i];
+    }
+    const ReqSum run = req_scan(s, sum);
+    ReqSum before = {above.n + run.n - sum.n, above.w + run.w - sum.w};
+    for (int i = 0; i < kEach; ++i) {
+        const ReqSum after = before + in[i];
+        const bool reached = by_weight ? after.w >= want_w : after.n >= want_n;
+        const bool earlier = by_weight ? before.w >= want_w : before.n >= want_n;
+        if (reached && !earlier) s.found_bin = tid * kEach + i, s.found_above = after;
+        before = after;
+    }
+    __syncthreads();
+    const uint64_t last = s.list[s.found_bin];
+    return {(uint32_t)(last >> 32), 1, s.found_above, true, (int32_t)(0xFFFFFFFFu - (uint32_t)last), s.found_above.w};
+}
 
 /*
  * The cut at which the row's ids with keys in (lo, hi], largest first, reach
@@ -177,7 +270,7 @@ struct ReqCut {
  */
 template <typename T>
 __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, uint32_t lo, uint32_t hi, bool by_weight,
-                          uint32_t want_n, double want_share, const uint64_t *all_weight) {
+                          uint32_t want_n, double want_share, const uint64_t *all_weight, int &turn) {
     cg::cluster_group cluster = cg::this_cluster();
     const int me = cluster.block_rank(), nc = cluster.num_blocks(), tid = threadIdx.x;
     ReqSum above = {0, 0};
@@ -206,7 +299,7 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
             const uint32_t key = req_key(x);
             if (key > lo && key <= hi) {
                 const uint32_t bin = even ? even_bin(key) : (hi - key) >> shift;
-                const uint64_t w = req_weight(r, x);
+                const uint64_t w = req_weight(r, x, s.table);
                 atomicAdd(&s.n[bin], 1u);
                 const uint32_t wl = (uint32_t)w, old = atomicAdd(&s.lo[bin], wl);
                 const uint32_t carry = old + wl < old;
@@ -250,7 +343,7 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
         }
         __syncthreads();
         const uint32_t bin = s.found_bin;
-        if (bin == kReqBins) return {lo, 0, above + s.total, false};
+        if (bin == kReqBins) return {lo, 0, above + s.total, false, -1, 0};
         above = s.found_above;
         if (even) {
             /* the bin's keys: bins fall as keys rise, so both ends are found by halving */
@@ -267,6 +360,8 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
             __syncthreads();
             hi = s.ends[0], lo = s.ends[1];
             even = false;
+            const uint32_t in = s.all_n[bin];
+            if (in <= kReqList) return req_cut_list(sl, s, r, lo, hi, in, above, by_weight, want_n, want_w, turn);
             __syncthreads();
             continue;
         }
@@ -275,12 +370,12 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
             __syncthreads();
             uint32_t ties = n;
             if (by_weight) {
-                const uint64_t w = req_weight(r, req_unkey(key)), need = want_w - above.w;
+                const uint64_t w = req_weight(r, req_unkey(key), s.table), need = want_w - above.w;
                 ties = (uint32_t)min((uint64_t)n, (need + w - 1) / w);
             } else {
                 ties = want_n - above.n;
             }
-            return {key, ties, above, true};
+            return {key, ties, above, true, -1, above.w + ties * req_weight(r, req_unkey(key), s.table)};
         }
         hi -= bin << shift;
         lo = hi - lo > 1u << shift ? hi - (1u << shift) : lo;
@@ -330,7 +425,7 @@ __device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char
         }
         return;
     }
-    const ReqRow r = req_row(a, b, m);
+    const ReqRow r = req_row(a, b, m, a.u[b]);
     if (r.greedy) {
         int32_t id = 0x7FFFFFFF;
         for (int i = tid; i < sl.n; i += kReqThreads)
@@ -353,19 +448,21 @@ __device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char
         return;
     }
 
-    ReqCut cut = {r.floor - 1, 0, {0, 0}, false};
-    if (r.k) cut = req_cut(sl, s, r, r.floor - 1, key, false, (uint32_t)r.k, 0.0, nullptr);
+    ReqCut cut = {r.floor - 1, 0, {0, 0}, false, -1, 0};
+    if (r.k) cut = req_cut(sl, s, r, r.floor - 1, key, false, (uint32_t)r.k, 0.0, nullptr, turn);
     if (r.p < 1.0) {
         uint64_t all_weight = cut.above.w;
-        if (cut.some) all_weight += cut.ties * req_weight(r, req_unkey(cut.key));
-        const ReqCut by_p = req_cut(sl, s, r, cut.some ? cut.key - 1 : cut.key, key, true, 0, r.p, r.k ? &all_weight : nullptr);
+        if (cut.some) all_weight = cut.kept;
+        const ReqCut by_p = req_cut(sl, s, r, cut.some ? cut.key - 1 : cut.key, key, true, 0, r.p, r.k ? &all_weight : nullptr, turn);
         if (by_p.some) cut = by_p;
     }
 
     /* of several ids at the cut, the lowest */
     int32_t cut_id = 0x7FFFFFFF;
     const int region = a.per / kReqWarps, begin = warp * region, end = min(sl.n, begin + region);
-    if (cut.some) {
+    if (cut.some && cut.id >= 0) {
+        cut_id = cut.id;
+    } else if (cut.some) {
         uint32_t n = 0;
         for (int i = begin + lane; i < end; i += 32) n += req_key(sl.at(i)) == cut.key;
         n = __reduce_add_sync(0xFFFFFFFFu, n);
@@ -396,7 +493,7 @@ __device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char
     auto weight = [&](int i) -> uint64_t {  // of element i, 0 where it is not left
         const float x = sl.at(i);
         const uint32_t k = req_key(x);
-        return k > cut.key || (cut.some && k == cut.key && sl.first + i <= cut_id) ? req_weight(r, x) : 0;
+        return k > cut.key || (cut.some && k == cut.key && sl.first + i <= cut_id) ? req_weight(r, x, s.table) : 0;
     };
 
     /* the walk: sums of regions, then the one that the draw ends in */
@@ -438,14 +535,14 @@ __device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char
         const uint64_t w = weight(i);
         if (before <= target && target < before + w) {
             a.ids[b] = sl.first + i;
-            if (a.probs) a.probs[b] = (float)(req_exp(r, sl.at(i)) * (double)(1ull << kReqFraction) / (double)total);
+            if (a.probs) a.probs[b] = (float)(req_exp(r, sl.at(i), s.table) * (double)(1ull << kReqFraction) / (double)total);
             if (a.counts) a.counts[b] = (int32_t)count;
         }
         before += w;
     }
 }
 
-enum PassKind { kPassGreedy, kPassCount, kPassLeast, kPassShare, kPassNot };
+enum PassKind { kPassGreedy, kPassCount, kPassLeast, kPassShare, kPassOpen, kPassNot };
 constexpr int kPassTopK = 1024;  // largest top_k of sample_pass_kernel
 
 /* What a row's settings come to before its largest logit is known. */
@@ -471,8 +568,8 @@ __device__ __forceinline__ PassRow pass_row(const RequestArgs &a, int b) {
     else if (!plain) r.kind = kPassNot;
     else if (r.k > 0 && r.k <= kPassTopK) r.kind = kPassCount;
     else if (least > 0.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassLeast;
-    else if (r.p < 1.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassShare;
-    else r.kind = kPassNot;
+    else if (r.k > 0 && r.k < a.vocab) r.kind = kPassNot;
+    else r.kind = r.p < 1.0f ? kPassShare : kPassOpen;
     return r;
 }
 /*
@@ -488,6 +585,7 @@ __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __gr
     const int tid = threadIdx.x, n = cluster.num_blocks();
     const uint32_t me = blockIdx.x / n, clusters = gridDim.x / n;
     int turn = 0;
+    req_table(s.table);
     cluster.sync();  // every CTA of the cluster is there before one writes into another's memory
     for (int after = 0; after < 2; ++after) {
         if (after) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -553,10 +651,14 @@ struct PassShared {
     uint32_t valid;       // and those that were filled, where it ran over
     uint32_t found, found_high;
     int full, lost, left;
+    float u;
+    uint64_t ends[2], before;
+    double table[kReqTable];
     double top;
     double part_rest[kReqMaxCluster];  // of the cluster's parts: weights dropped,
     float part_rc[kReqMaxCluster];     // their reference,
-    float part_f[kReqMaxCluster];      // and the filter
+    float part_f[kReqMaxCluster];      // and the filter (rows that keep everything: the largest logit)
+    uint64_t part_w[kReqMaxCluster], part_n[kReqMaxCluster];  // weights and ids of rows that keep everything
 };
 
 /* kept elements: key, then the lower id first */
@@ -646,8 +748,160 @@ __device__ __forceinline__ float pass_floor(const PassRow &r, float m) {
     return fmaxf(f - fabsf(f) * 2e-7f - fabsf(m) * 2e-7f - 1e-37f, -3.402823466e38f);
 }
 
+/*
+ * Rows that keep everything: once for the largest logit, once for the
+ * weights' exact sums of pieces of 512 ids, then the piece that the draw ends
+ * in.  first, last: this warp's 16-byte vectors; the ids beside whole vectors
+ * are the first and the last CTA's.
+ */
 template <typename T>
-__global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __grid_constant__ PassArgs a) {
+__device__ __noinline__ void pass_open(const PassArgs &a, PassShared &s, uint64_t *pieces, int b, int first, int last,
+                                       int head, int vecs) {
+    using V = PassVec<T>;
+    constexpr int kVecs = kPassEach / V::kPer;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int me = cluster.block_rank(), nc = cluster.num_blocks();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const T *base = static_cast<const T *>(a.r.logits) + (int64_t)b * a.r.ld;
+    const uint4 *body = reinterpret_cast<const uint4 *>(base + head);
+    const int vocab = a.r.vocab, tail = head + vecs * V::kPer;
+    uint4 next[kVecs];
+    auto load = [&](int turn) {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+            const int v = first + turn * (32 * kVecs) + j * 32 + lane;
+            next[j] = v < last ? pass_load(body + v) : V::none();
+        }
+    };
+    /* the ends: at most 7 ids each, of the first two lots of 8 threads */
+    const int end_id = tid < 8 ? (tid < head ? tid : vocab) : tail + tid - 8;
+    const bool mine = tid < 8 ? me == 0 : tid < 16 && me == nc - 1;
+    const float end_x = mine && end_id < vocab ? req_value(base[end_id]) : -INFINITY;
+    float hi = end_x;
+    load(0);
+    for (int turn = 0; turn < a.turns; ++turn) {
+        float x[kPassEach];
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) V::get(next[j], x + j * V::kPer);
+        if (turn + 1 < a.turns) load(turn + 1);
+#pragma unroll
+        for (int j = 0; j < kPassEach; ++j) hi = fmaxf(hi, x[j]);
+    }
+    hi = pass_max(s, hi);
+    if (nc > 1) {
+        cluster.sync();  // every CTA of the cluster is there
+        if (tid < nc) cluster.map_shared_rank(&s, tid)->part_f[me] = hi;
+        cluster.sync();
+        for (int c = 0; c < nc; ++c) hi = fmaxf(hi, s.part_f[c]);
+    }
+    if (!(hi > -INFINITY && hi < INFINITY)) {
+        if (me == 0 && tid == 0) {
+            a.r.status[b] = hi > 0.0f;  // several infinite ones: sample_requests_kernel
+            if (!(hi > 0.0f)) {
+                a.r.ids[b] = -1;
+                if (a.r.probs) a.r.probs[b] = 0.0f;
+                if (a.r.counts) a.r.counts[b] = 0;
+            }
+        }
+        return;
+    }
+    const ReqRow r = req_row(a.r, b, hi, s.u);
+    const float floor = req_unkey(r.floor);
+    auto weight = [&](float x) -> uint64_t { return x >= floor ? req_weight(r, x, s.table) : 0; };  // not a NaN's
+    uint32_t n = 0;
+    load(0);
+    for (int turn = 0; turn < a.turns; ++turn) {
+        float x[kPassEach];
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) V::get(next[j], x + j * V::kPer);
+        if (turn + 1 < a.turns) load(turn + 1);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int j = 0; j < kPassEach; ++j) {
+            const uint64_t w = weight(x[j]);
+            n += w != 0;
+            sum += w;
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        if (lane == 0) pieces[warp * a.turns + turn] = sum;
+    }
+    const uint64_t end_w = weight(end_x);
+    n += end_w != 0;
+    uint64_t w = end_w;  // of the 8 threads of each end
+#pragma unroll
+    for (int d = 4; d; d >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, d);
+    if (tid == 0 || tid == 8) s.ends[tid / 8] = w;
+    __syncthreads();
+    const int count = kPassWarps * a.turns, each = (count + kPassThreads - 1) / kPassThreads;
+    const int from = min(count, tid * each), to = min(count, from + each);
+    uint64_t sum = 0, all, ids;
+    for (int i = from; i < to; ++i) sum += pieces[i];
+    const uint64_t run = pass_scan(s, sum, all) - sum;
+    pass_scan(s, n, ids);
+    const uint64_t part = s.ends[0] + all + s.ends[1];
+    uint64_t total = part, before = 0;
+    if (nc > 1) {
+        if (tid < nc) {
+            PassShared *to_s = cluster.map_shared_rank(&s, tid);
+            to_s->part_w[me] = part, to_s->part_n[me] = ids;
+        }
+        cluster.sync();
+        total = ids = 0;
+        for (int c = 0; c < nc; ++c) {
+            if (c < me) before += s.part_w[c];
+            total += s.part_w[c], ids += s.part_n[c];
+        }
+    }
+    uint64_t target = r.u >= 1.0f ? total : __umul64hi((uint64_t)((double)r.u * 18446744073709551616.0), total);
+    if (target >= total) target = total - 1;
+    if (target < before || target - before >= part) return;  // in another CTA's part
+    target -= before;
+    /* the piece: 512 ids of a warp's turn, or one of the ends */
+    int begin = 0, length = head;
+    if (target >= s.ends[0]) {
+        target -= s.ends[0];
+        begin = tail, length = vocab - tail;
+        if (target >= all) {
+            target -= all;
+        } else {
+            uint64_t here = run;
+            for (int i = from; i < to; ++i) {
+                if (here <= target && target - here < pieces[i]) s.found = (uint32_t)i, s.before = here;
+                here += pieces[i];
+            }
+            __syncthreads();
+            target -= s.before;
+            const int vec = (me * kPassWarps * a.turns + (int)s.found) * (32 * kVecs);
+            begin = head + vec * V::kPer;
+            length = min(32 * kVecs, vecs - vec) * V::kPer;
+        }
+    }
+    const int i0 = tid * (32 * kPassEach / kPassThreads);
+    uint64_t own[32 * kPassEach / kPassThreads];
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < 32 * kPassEach / kPassThreads; ++i) {
+        own[i] = i0 + i < length ? weight(req_value(base[begin + i0 + i])) : 0;
+        sum += own[i];
+    }
+    uint64_t here = pass_scan(s, sum, all) - sum;
+#pragma unroll
+    for (int i = 0; i < 32 * kPassEach / kPassThreads; ++i) {
+        if (here <= target && target - here < own[i]) {
+            const int id = begin + i0 + i;
+            a.r.status[b] = 0;
+            a.r.ids[b] = id;
+            if (a.r.probs)
+                a.r.probs[b] = (float)(req_exp(r, req_value(base[id]), s.table) * (double)(1ull << kReqFraction) / (double)total);
+            if (a.r.counts) a.r.counts[b] = (int32_t)ids;
+        }
+        here += own[i];
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __grid_constant__ PassArgs a) {
     extern __shared__ __align__(16) unsigned char req_raw[];
     uint64_t *keep = reinterpret_cast<uint64_t *>(req_raw);
     __shared__ PassShared s;
@@ -656,11 +910,6 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = blockIdx.x / nc;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const PassRow row = pass_row(a.r, b);
-    if (row.kind == kPassNot) {
-        if (me == 0 && tid == 0) a.r.status[b] = 1;
-        return;  // the whole cluster
-    }
     using V = PassVec<T>;
     constexpr int kVecs = kPassEach / V::kPer;
     const T *base = static_cast<const T *>(a.r.logits) + (int64_t)b * a.r.ld;
@@ -682,6 +931,17 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
     };
     int turn = 0, ahead = a.step < a.turns ? a.step : 0;  // the turn in x, and the one on its way
     load(0);
+    const PassRow row = pass_row(a.r, b);
+    if (row.kind == kPassNot) {
+        if (me == 0 && tid == 0) a.r.status[b] = 1;
+        return;  // the whole cluster
+    }
+    if (tid == 0) s.u = a.r.u[b];
+    req_table(s.table);
+    if (row.kind == kPassOpen) {
+        pass_open<T>(a, s, keep, b, first, last, head, vecs);
+        return;
+    }
 
     if (tid == 0) s.count = 0, s.valid = kPassKeep, s.lost = s.full = 0;
     for (int i = tid; i < kPassBins; i += kPassThreads) s.n[i] = 0;
@@ -716,7 +976,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         const uint64_t begin = pass_scan(s, mine, all) - mine;
         if (tid == 0) s.found = kPassBins, s.top = (double)(all >> 14);
         __syncthreads();
-        const uint32_t need = row.kind == kPassCount ? (uint32_t)row.k : 16u;
+        const uint32_t need = row.kind == kPassCount ? (uint32_t)row.k : 4u;
         uint64_t run = begin;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
@@ -731,7 +991,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         if (row.kind == kPassShare) {
             /*
              * What will have been dropped in the end, as of the part seen so far, may be 3/4 (early on, 1/2) of 1 -
-             * top_p of the row's weight; for that the 16 largest so far count once and the others for as much as the
+             * top_p of the row's weight; for that the 4 largest so far count once and the others for as much as the
              * part has seen.  The 24 largest of an early part stay: what lies below them is even enough to count on.
              */
             const double weight = (double)(all >> 14), gone = dropped * 6.8719477e10, seen = weight + gone;
@@ -984,7 +1244,7 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         return;
     }
     /* one more rise for a shorter sort */
-    if (n > 512) {
+    if (n > kPassThreads) {
         const double other = gone;
         if (row.kind == kPassShare) {
             /* the parts' weights as one thread's, of one reference */
@@ -1005,45 +1265,51 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         if (tid == 0) a.r.status[b] = 5;
         return;
     }
-    int size = 32;
-    while (size < n) size <<= 1;
-    auto sort = [&]() {  // largest first
-        for (int width = 2; width <= size; width <<= 1)
-            for (int d = width >> 1; d; d >>= 1) {
-                for (int i = tid; i < size / 2; i += kPassThreads) {
-                    const int lo = 2 * i - (i & (d - 1)), up = lo + d;
-                    const uint64_t x = keep[lo], y = keep[up];
-                    if ((x < y) == ((lo & width) == 0)) keep[lo] = y, keep[up] = x;
-                }
-                __syncthreads();
-            }
-    };
-    for (int i = n + tid; i < size; i += kPassThreads) keep[i] = 0;
-    __syncthreads();
-    sort();
-    const ReqRow r = req_row(a.r, b, hi);
+    /*
+     * In order, largest first: each thread counts what is larger than its
+     * element, or where they are more than threads, a sort.
+     */
+    uint64_t *list = keep, *weights = keep + kPassSort;
+    if (n <= kPassThreads) {
+        list = keep + kPassSort, weights = keep;
+        if (tid < n) {
+            const uint64_t e = keep[tid];
+            int larger = 0;
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) larger += keep[i] > e;
+            list[larger] = e;
+        }
+        __syncthreads();
+    } else {
+        int size = 2 * kPassThreads;
+        while (size < n) size <<= 1;
+        for (int i = n + tid; i < size; i += kPassThreads) keep[i] = 0;
+        __syncthreads();
+        req_sort<kPassThreads>(keep, size);
+    }
+    const ReqRow r = req_row(a.r, b, hi, s.u);
     if (r.greedy) {
         if (tid == 0) {
             a.r.status[b] = 0;
-            a.r.ids[b] = pass_id(keep[0]);
+            a.r.ids[b] = pass_id(list[0]);
             if (a.r.probs) a.r.probs[b] = 1.0f;
             if (a.r.counts) a.r.counts[b] = 1;
         }
         return;
     }
     /* what is left by the temperature, min-p and top-k is a beginning of the order */
-    if (tid == 0) s.left = 0;
-    __syncthreads();
     const int most = r.k ? min(n, r.k) : n;
-    for (int i = tid; i < most; i += kPassThreads)
-        if ((uint32_t)(keep[i] >> 32) >= r.floor && (i + 1 == most || (uint32_t)(keep[i + 1] >> 32) < r.floor)) s.left = i + 1;
-    __syncthreads();
-    int left = s.left;
-    const int each = (size + kPassThreads - 1) / kPassThreads;
-    auto weight = [&](int i) -> uint64_t { return i < left ? req_weight(r, pass_x(keep[i])) : 0; };
+    int left = 0;
+    for (int at = 0; at < most; at += kPassThreads) {
+        const int i = at + tid;
+        const bool in = i < most && (uint32_t)(list[i] >> 32) >= r.floor;
+        if (in) weights[i] = req_weight(r, pass_x(list[i]), s.table);
+        left += __syncthreads_count(in);
+    }
     if (r.p < 1.0) {
+        const int each = (left + kPassThreads - 1) / kPassThreads, from = min(left, tid * each), to = min(left, from + each);
         uint64_t mine = 0, all;
-        for (int i = tid * each; i < tid * each + each && i < size; ++i) mine += weight(i);
+        for (int i = from; i < to; ++i) mine += weights[i];
         const uint64_t end = pass_scan(s, mine, all);
         uint64_t want[2];
         for (int side = 0; side < 2; ++side) {
@@ -1056,8 +1322,8 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         if (tid == 0) s.found = s.found_high = 0;
         __syncthreads();
         uint64_t run = end - mine;
-        for (int i = tid * each; i < tid * each + each && i < left; ++i) {
-            const uint64_t after = run + weight(i);
+        for (int i = from; i < to; ++i) {
+            const uint64_t after = run + weights[i];
             if (run < want[0] && after >= want[0]) s.found = (uint32_t)i + 1;
             if (run < want[1] && after >= want[1]) s.found_high = (uint32_t)i + 1;
             run = after;
@@ -1065,39 +1331,50 @@ __global__ void __launch_bounds__(kPassThreads, 3) sample_pass_kernel(const __gr
         __syncthreads();
         left = (int)s.found;
         /* open within the error, or a lost bet: the row's other ids weigh too much, or some come before the cut */
-        if (s.found != s.found_high || left == 0 || (row.kind == kPassShare && !(pass_x(keep[left - 1]) >= f))) {
+        if (s.found != s.found_high || left == 0 || (row.kind == kPassShare && !(pass_x(list[left - 1]) >= f))) {
             if (tid == 0) a.r.status[b] = 6;
             return;
         }
     }
-    /* the walk in the order of ids */
-    for (int i = tid; i < size; i += kPassThreads) {
-        const uint64_t e = keep[i];
-        keep[i] = i < left ? e << 32 | e >> 32 : 0;  // the lower id is the larger number
+    /* the walk in the order of ids: each thread adds up what lies before its element, or after a sort */
+    uint64_t before = 0, total = 0;
+    int at = tid, end = min(left, tid + 1);
+    if (left <= kPassThreads) {
+        const uint32_t id = tid < left ? (uint32_t)list[tid] : 0;  // the larger, the earlier
+#pragma unroll 4
+        for (int i = 0; i < left; ++i) {
+            const uint64_t w = weights[i];
+            total += w;
+            before += (uint32_t)list[i] > id ? w : 0;
+        }
+    } else {
+        int size = 2 * kPassThreads;
+        while (size < left) size <<= 1;
+        for (int i = tid; i < size; i += kPassThreads) list[i] = i < left ? list[i] << 32 | list[i] >> 32 : 0;
+        __syncthreads();
+        req_sort<kPassThreads>(list, size);
+        for (int i = tid; i < left; i += kPassThreads) {
+            list[i] = list[i] << 32 | list[i] >> 32;
+            weights[i] = req_weight(r, pass_x(list[i]), s.table);
+        }
+        __syncthreads();
+        const int each = (left + kPassThreads - 1) / kPassThreads;
+        at = min(left, tid * each), end = min(left, at + each);
+        uint64_t mine = 0;
+        for (int i = at; i < end; ++i) mine += weights[i];
+        before = pass_scan(s, mine, total) - mine;
     }
-    __syncthreads();
-    size = 32;
-    while (size < left) size <<= 1;
-    sort();
-    const int per = (size + kPassThreads - 1) / kPassThreads;
-    uint64_t mine = 0, total;
-    for (int i = tid * per; i < tid * per + per && i < left; ++i) mine += req_weight(r, req_unkey((uint32_t)keep[i]));
-    const uint64_t end = pass_scan(s, mine, total);
     uint64_t target = r.u >= 1.0f ? total : __umul64hi((uint64_t)((double)r.u * 18446744073709551616.0), total);
     if (target >= total) target = total - 1;
-    uint64_t run = end - mine;
-    if (run <= target && target < end) {
-        for (int i = tid * per; i < tid * per + per && i < left; ++i) {
-            const float x = req_unkey((uint32_t)keep[i]);
-            run += req_weight(r, x);
-            if (run > target) {
-                a.r.status[b] = 0;
-                a.r.ids[b] = (int)(0xFFFFFFFFu - (uint32_t)(keep[i] >> 32));
-                if (a.r.probs) a.r.probs[b] = (float)(req_exp(r, x) * (double)(1ull << kReqFraction) / (double)total);
-                if (a.r.counts) a.r.counts[b] = left;
-                break;
-            }
+    for (; at < end; ++at) {
+        if (before <= target && target - before < weights[at]) {
+            a.r.status[b] = 0;
+            a.r.ids[b] = pass_id(list[at]);
+            if (a.r.probs)
+                a.r.probs[b] = (float)(req_exp(r, pass_x(list[at]), s.table) * (double)(1ull << kReqFraction) / (double)total);
+            if (a.r.counts) a.r.counts[b] = left;
         }
+        before += weights[at];
     }
 }
 
