@@ -61,12 +61,12 @@ cudaError_t launch(void (*kernel)(A...), int grid, int threads, size_t smem, int
 
 template <typename T>
 int request_launch(RequestArgs a, int sms, cudaStream_t s) {
-    constexpr int kCluster = kReqMaxCluster, kMost = 190 * 1024;
+    constexpr int kMost = 190 * 1024;
     /* the pass */
     PassArgs p{};
     p.r = a;
     int parts = 8;
-    while (parts > 1 && (int64_t)a.batch * parts > 3 * sms) parts /= 2;
+    while (parts > 1 && (int64_t)a.batch * parts > 4 * sms) parts /= 2;
     const int per_vec = 16 / (int)sizeof(T), per_turn = parts * kPassThreads * kPassEach / per_vec;
     p.turns = (a.vocab / per_vec + per_turn - 1) / per_turn;
     if (p.turns < 1) p.turns = 1;
@@ -80,20 +80,35 @@ int request_launch(RequestArgs a, int sms, cudaStream_t s) {
     p.step = (int)(p.turns * 0.618);
     while (p.step > 1 && divisor(p.turns, p.step) != 1) --p.step;
     if (p.step < 1) p.step = 1;
-    int r = dynamic_smem((const void *)sample_pass_kernel<T>, kPassKeep * sizeof(uint64_t));
+    const size_t pass_smem = kPassKeep * sizeof(uint64_t);
+    int r = dynamic_smem((const void *)sample_pass_kernel<T>, pass_smem);
     if (r) return r;
-    CUDA_TRY(launch(sample_pass_kernel<T>, a.batch * parts, kPassThreads, kPassKeep * sizeof(uint64_t), parts, false, s, p));
-    /* the rows that it leaves */
+    /* the rows that it does not take, and those that it leaves */
+    const int64_t row = (int64_t)a.vocab * sizeof(T);
+    const int cluster = row > 262144 ? 16 : row > 131072 ? 8 : row > 65536 ? 4 : 2;
     const int unit = kReqThreads;  // every warp's region in whole turns
-    a.per = ((a.vocab + kCluster - 1) / kCluster + unit - 1) / unit * unit;
+    a.per = ((a.vocab + cluster - 1) / cluster + unit - 1) / unit * unit;
     size_t smem = (size_t)a.per * sizeof(T);
     a.resident = smem <= kMost;
     if (!a.resident) smem = 0;
     r = dynamic_smem((const void *)sample_requests_kernel<T>, smem);
     if (r) return r;
-    int clusters = sms / 4;
-    if (clusters > a.batch) clusters = a.batch;
-    CUDA_TRY(launch(sample_requests_kernel<T>, clusters * kCluster, kReqThreads, smem, kCluster, true, s, a));
+    /*
+     * The former run before the pass, which fills the SMs as they leave room
+     * (beside it they would end long after it); where every row may have a
+     * cluster of its own, beside it, in the launch for the latter.
+     */
+    if (cluster > 8)
+        CUDA_TRY(cudaFuncSetAttribute((const void *)sample_requests_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    const bool few = a.batch <= 2 * sms / cluster;
+    const int beside = few ? a.batch : sms / cluster, after = few ? a.batch : a.batch < 256 ? sms / cluster : 2 * sms / cluster;
+    if (!few) {
+        a.rows = kReqBySettings;
+        CUDA_TRY(launch(sample_requests_kernel<T>, beside * cluster, kReqThreads, smem, cluster, false, s, a));
+    }
+    CUDA_TRY(launch(sample_pass_kernel<T>, a.batch * parts, kPassThreads, pass_smem, parts, !few, s, p));
+    a.rows = few ? kReqBySettings | kReqUnsettled : kReqUnsettled;
+    CUDA_TRY(launch(sample_requests_kernel<T>, after * cluster, kReqThreads, smem, cluster, true, s, a));
     return NOEL_OK;
 }
 

@@ -29,16 +29,17 @@ struct RequestArgs {
     const float *u;
     int32_t *ids, *counts;
     float *probs;
-    int32_t *status;     // [batch]: the rows that are not 0 are this kernel's
+    int32_t *status;     // [batch] PassStatus
     int per;             // elements of a row to a CTA of its cluster
     bool resident;       // they fit the shared memory
+    int rows;            // ReqRows of this launch
 };
 
 constexpr int kReqThreads = 512;
 constexpr int kReqWarps = kReqThreads / 32;
 constexpr int kReqBins = 1024;
 constexpr int kReqList = 1024;
-constexpr int kReqMaxCluster = 8;
+constexpr int kReqMaxCluster = 16;
 constexpr int kReqFraction = 43;  // bits behind the point of a weight: 2^20 of them fit 64 bits, and e^-30 is not 0
 
 /* An element as fp32 that compares as it is drawn: NaN below everything, one zero. */
@@ -302,8 +303,8 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
                 const uint64_t w = req_weight(r, x, s.table);
                 atomicAdd(&s.n[bin], 1u);
                 const uint32_t wl = (uint32_t)w, old = atomicAdd(&s.lo[bin], wl);
-                const uint32_t carry = old + wl < old;
-                if ((uint32_t)(w >> 32) + carry) atomicAdd(&s.hi[bin], (uint32_t)(w >> 32) + carry);
+                const uint32_t wh = (uint32_t)(w >> 32) + (old + wl < old);
+                if (wh) atomicAdd(&s.hi[bin], wh);
             }
         }
         cluster.sync();
@@ -542,7 +543,8 @@ __device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char
     }
 }
 
-enum PassKind { kPassGreedy, kPassCount, kPassLeast, kPassShare, kPassOpen, kPassNot };
+enum PassStatus { kPassSettled, kPassSkipped, kPassUnsettled };
+enum PassKind { kPassGreedy, kPassCount, kPassLeast, kPassShare, kPassNot };
 constexpr int kPassTopK = 1024;  // largest top_k of sample_pass_kernel
 
 /* What a row's settings come to before its largest logit is known. */
@@ -568,15 +570,16 @@ __device__ __forceinline__ PassRow pass_row(const RequestArgs &a, int b) {
     else if (!plain) r.kind = kPassNot;
     else if (r.k > 0 && r.k <= kPassTopK) r.kind = kPassCount;
     else if (least > 0.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassLeast;
-    else if (r.k > 0 && r.k < a.vocab) r.kind = kPassNot;
-    else r.kind = r.p < 1.0f ? kPassShare : kPassOpen;
+    else if (r.p < 1.0f && !(r.k > 0 && r.k < a.vocab)) r.kind = kPassShare;
+    else r.kind = kPassNot;
     return r;
 }
 /*
- * The rows that sample_pass_kernel does not take, by their settings, while it
- * runs, and those that it could not settle, after it.  The clusters take them
- * in turn.
+ * The rows that sample_pass_kernel does not take, by their settings (rows = 1,
+ * before it or beside it), and those that it could not settle (rows = 2, after
+ * it).  The clusters take them in turn.
  */
+enum ReqRows { kReqBySettings = 1, kReqUnsettled = 2 };
 template <typename T>
 __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __grid_constant__ RequestArgs a) {
     extern __shared__ __align__(16) unsigned char req_raw[];
@@ -587,14 +590,15 @@ __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __gr
     int turn = 0;
     req_table(s.table);
     cluster.sync();  // every CTA of the cluster is there before one writes into another's memory
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     for (int after = 0; after < 2; ++after) {
+        if (!(a.rows & (after ? kReqUnsettled : kReqBySettings))) continue;
         if (after) asm volatile("griddepcontrol.wait;" ::: "memory");
         uint32_t rank = 0;
         for (int at = 0; at < a.batch; at += kReqThreads) {
             bool mine = false;
             if (at + tid < a.batch) {
-                const bool not_passed = pass_row(a, at + tid).kind == kPassNot;
-                mine = after ? !not_passed && a.status[at + tid] != 0 : not_passed;
+                mine = after ? a.status[at + tid] == kPassUnsettled : pass_row(a, at + tid).kind == kPassNot;
             }
             const uint32_t bits = __ballot_sync(0xFFFFFFFFu, mine);
             __syncthreads();
@@ -634,11 +638,12 @@ constexpr int kPassWarps = kPassThreads / 32;
 constexpr int kPassEach = 16;     // elements of a thread's turn
 constexpr int kPassKeep = 4096;   // kept at most
 constexpr int kPassFull = 3072;   // and at most after the filter has risen
+constexpr int kPassRises = 5;
 constexpr int kPassBins = 1024;
 constexpr int kPassSort = 2048;   // of those, at the end
 
 struct PassArgs {
-    RequestArgs r;    // r.status gets 1 where the row is left to sample_requests_kernel, else 0
+    RequestArgs r;
     int turns, step;  // turns of a warp's part of a row, taken in steps of step (no common divisor)
 };
 
@@ -652,13 +657,11 @@ struct PassShared {
     uint32_t found, found_high;
     int full, lost, left;
     float u;
-    uint64_t ends[2], before;
     double table[kReqTable];
     double top;
     double part_rest[kReqMaxCluster];  // of the cluster's parts: weights dropped,
     float part_rc[kReqMaxCluster];     // their reference,
-    float part_f[kReqMaxCluster];      // and the filter (rows that keep everything: the largest logit)
-    uint64_t part_w[kReqMaxCluster], part_n[kReqMaxCluster];  // weights and ids of rows that keep everything
+    float part_f[kReqMaxCluster];      // and the filter
 };
 
 /* kept elements: key, then the lower id first */
@@ -748,158 +751,6 @@ __device__ __forceinline__ float pass_floor(const PassRow &r, float m) {
     return fmaxf(f - fabsf(f) * 2e-7f - fabsf(m) * 2e-7f - 1e-37f, -3.402823466e38f);
 }
 
-/*
- * Rows that keep everything: once for the largest logit, once for the
- * weights' exact sums of pieces of 512 ids, then the piece that the draw ends
- * in.  first, last: this warp's 16-byte vectors; the ids beside whole vectors
- * are the first and the last CTA's.
- */
-template <typename T>
-__device__ __noinline__ void pass_open(const PassArgs &a, PassShared &s, uint64_t *pieces, int b, int first, int last,
-                                       int head, int vecs) {
-    using V = PassVec<T>;
-    constexpr int kVecs = kPassEach / V::kPer;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int me = cluster.block_rank(), nc = cluster.num_blocks();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const T *base = static_cast<const T *>(a.r.logits) + (int64_t)b * a.r.ld;
-    const uint4 *body = reinterpret_cast<const uint4 *>(base + head);
-    const int vocab = a.r.vocab, tail = head + vecs * V::kPer;
-    uint4 next[kVecs];
-    auto load = [&](int turn) {
-#pragma unroll
-        for (int j = 0; j < kVecs; ++j) {
-            const int v = first + turn * (32 * kVecs) + j * 32 + lane;
-            next[j] = v < last ? pass_load(body + v) : V::none();
-        }
-    };
-    /* the ends: at most 7 ids each, of the first two lots of 8 threads */
-    const int end_id = tid < 8 ? (tid < head ? tid : vocab) : tail + tid - 8;
-    const bool mine = tid < 8 ? me == 0 : tid < 16 && me == nc - 1;
-    const float end_x = mine && end_id < vocab ? req_value(base[end_id]) : -INFINITY;
-    float hi = end_x;
-    load(0);
-    for (int turn = 0; turn < a.turns; ++turn) {
-        float x[kPassEach];
-#pragma unroll
-        for (int j = 0; j < kVecs; ++j) V::get(next[j], x + j * V::kPer);
-        if (turn + 1 < a.turns) load(turn + 1);
-#pragma unroll
-        for (int j = 0; j < kPassEach; ++j) hi = fmaxf(hi, x[j]);
-    }
-    hi = pass_max(s, hi);
-    if (nc > 1) {
-        cluster.sync();  // every CTA of the cluster is there
-        if (tid < nc) cluster.map_shared_rank(&s, tid)->part_f[me] = hi;
-        cluster.sync();
-        for (int c = 0; c < nc; ++c) hi = fmaxf(hi, s.part_f[c]);
-    }
-    if (!(hi > -INFINITY && hi < INFINITY)) {
-        if (me == 0 && tid == 0) {
-            a.r.status[b] = hi > 0.0f;  // several infinite ones: sample_requests_kernel
-            if (!(hi > 0.0f)) {
-                a.r.ids[b] = -1;
-                if (a.r.probs) a.r.probs[b] = 0.0f;
-                if (a.r.counts) a.r.counts[b] = 0;
-            }
-        }
-        return;
-    }
-    const ReqRow r = req_row(a.r, b, hi, s.u);
-    const float floor = req_unkey(r.floor);
-    auto weight = [&](float x) -> uint64_t { return x >= floor ? req_weight(r, x, s.table) : 0; };  // not a NaN's
-    uint32_t n = 0;
-    load(0);
-    for (int turn = 0; turn < a.turns; ++turn) {
-        float x[kPassEach];
-#pragma unroll
-        for (int j = 0; j < kVecs; ++j) V::get(next[j], x + j * V::kPer);
-        if (turn + 1 < a.turns) load(turn + 1);
-        uint64_t sum = 0;
-#pragma unroll
-        for (int j = 0; j < kPassEach; ++j) {
-            const uint64_t w = weight(x[j]);
-            n += w != 0;
-            sum += w;
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-        if (lane == 0) pieces[warp * a.turns + turn] = sum;
-    }
-    const uint64_t end_w = weight(end_x);
-    n += end_w != 0;
-    uint64_t w = end_w;  // of the 8 threads of each end
-#pragma unroll
-    for (int d = 4; d; d >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, d);
-    if (tid == 0 || tid == 8) s.ends[tid / 8] = w;
-    __syncthreads();
-    const int count = kPassWarps * a.turns, each = (count + kPassThreads - 1) / kPassThreads;
-    const int from = min(count, tid * each), to = min(count, from + each);
-    uint64_t sum = 0, all, ids;
-    for (int i = from; i < to; ++i) sum += pieces[i];
-    const uint64_t run = pass_scan(s, sum, all) - sum;
-    pass_scan(s, n, ids);
-    const uint64_t part = s.ends[0] + all + s.ends[1];
-    uint64_t total = part, before = 0;
-    if (nc > 1) {
-        if (tid < nc) {
-            PassShared *to_s = cluster.map_shared_rank(&s, tid);
-            to_s->part_w[me] = part, to_s->part_n[me] = ids;
-        }
-        cluster.sync();
-        total = ids = 0;
-        for (int c = 0; c < nc; ++c) {
-            if (c < me) before += s.part_w[c];
-            total += s.part_w[c], ids += s.part_n[c];
-        }
-    }
-    uint64_t target = r.u >= 1.0f ? total : __umul64hi((uint64_t)((double)r.u * 18446744073709551616.0), total);
-    if (target >= total) target = total - 1;
-    if (target < before || target - before >= part) return;  // in another CTA's part
-    target -= before;
-    /* the piece: 512 ids of a warp's turn, or one of the ends */
-    int begin = 0, length = head;
-    if (target >= s.ends[0]) {
-        target -= s.ends[0];
-        begin = tail, length = vocab - tail;
-        if (target >= all) {
-            target -= all;
-        } else {
-            uint64_t here = run;
-            for (int i = from; i < to; ++i) {
-                if (here <= target && target - here < pieces[i]) s.found = (uint32_t)i, s.before = here;
-                here += pieces[i];
-            }
-            __syncthreads();
-            target -= s.before;
-            const int vec = (me * kPassWarps * a.turns + (int)s.found) * (32 * kVecs);
-            begin = head + vec * V::kPer;
-            length = min(32 * kVecs, vecs - vec) * V::kPer;
-        }
-    }
-    const int i0 = tid * (32 * kPassEach / kPassThreads);
-    uint64_t own[32 * kPassEach / kPassThreads];
-    sum = 0;
-#pragma unroll
-    for (int i = 0; i < 32 * kPassEach / kPassThreads; ++i) {
-        own[i] = i0 + i < length ? weight(req_value(base[begin + i0 + i])) : 0;
-        sum += own[i];
-    }
-    uint64_t here = pass_scan(s, sum, all) - sum;
-#pragma unroll
-    for (int i = 0; i < 32 * kPassEach / kPassThreads; ++i) {
-        if (here <= target && target - here < own[i]) {
-            const int id = begin + i0 + i;
-            a.r.status[b] = 0;
-            a.r.ids[b] = id;
-            if (a.r.probs)
-                a.r.probs[b] = (float)(req_exp(r, req_value(base[id]), s.table) * (double)(1ull << kReqFraction) / (double)total);
-            if (a.r.counts) a.r.counts[b] = (int32_t)ids;
-        }
-        here += own[i];
-    }
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __grid_constant__ PassArgs a) {
     extern __shared__ __align__(16) unsigned char req_raw[];
@@ -933,15 +784,11 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
     load(0);
     const PassRow row = pass_row(a.r, b);
     if (row.kind == kPassNot) {
-        if (me == 0 && tid == 0) a.r.status[b] = 1;
+        if (me == 0 && tid == 0) a.r.status[b] = kPassSkipped;
         return;  // the whole cluster
     }
     if (tid == 0) s.u = a.r.u[b];
     req_table(s.table);
-    if (row.kind == kPassOpen) {
-        pass_open<T>(a, s, keep, b, first, last, head, vecs);
-        return;
-    }
 
     if (tid == 0) s.count = 0, s.valid = kPassKeep, s.lost = s.full = 0;
     for (int i = tid; i < kPassBins; i += kPassThreads) s.n[i] = 0;
@@ -957,7 +804,7 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
 
     /*
      * The filter that the histogram in s.n of elements from low to hi gives:
-     * 1 / grow of the part has been seen, and dropped is what has been dropped
+     * 1 / grow of the row has been seen by this CTA, and dropped is what it has dropped
      * weighs (as of hi).
      */
     auto edge = [&](float hi, float low, float scale, double dropped, double grow) -> float {
@@ -1036,7 +883,14 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
                 for (int j = 0; j < kPassEach; ++j)
                     if (x[j] >= low) atomicAdd(&s.n[min((int)((hi - x[j]) * scale), kPassBins - 1)], 1u);
                 __syncthreads();
-                f = fmaxf(f, edge(hi, low, scale, 0.0, (double)a.turns));
+                f = fmaxf(f, edge(hi, low, scale, 0.0, (double)a.turns * nc));
+                if (row.kind == kPassShare && a.turns > 1) {
+                    int many = 0;
+#pragma unroll
+                    for (int j = 0; j < kPassEach; ++j) many += x[j] >= f;
+                    /* where a third has to be kept the list runs over again and again, and most such rows are lost in the end */
+                    if (pass_sum(s, (double)many) * 3.0 > kPassThreads * kPassEach) s.lost = 1;
+                }
             }
         }
     }
@@ -1112,8 +966,8 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
      * them meet to raise the filter, and those whose elements found no place
      * try again.
      */
-    int done = 0;  // turns of this warp
-    for (;;) {
+    int done = 0, rises = 0;  // turns of this warp, rises of the filter on the way
+    while (!s.lost) {
         while (done < a.turns) {
             const int full = *(volatile int *)&s.full;
             float most = x[0];
@@ -1165,13 +1019,15 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
         }
         __syncthreads();
         if (!s.full) break;  // every warp is through
-        raise(row.kind == kPassShare ? (double)a.turns * kPassThreads / fmax(pass_sum(s, (double)done), 1.0) : 1.0);
+        raise(row.kind == kPassShare ? (double)a.turns * nc * kPassThreads / fmax(pass_sum(s, (double)done), 1.0) : 1.0);
+        if (++rises == kPassRises && tid == 0) s.lost = 1;  // a row of many ids with some weight: not for one CTA
+        __syncthreads();
         if (s.lost) break;
     }
     __syncthreads();
 
     /* the cluster's parts come together in the first one's memory, after a last rise so that little moves */
-    if (nc > 1 && !s.lost) raise(1.0);
+    if (nc > 1 && !s.lost && s.count > kPassKeep / 2 / nc) raise((double)nc);
     const double dropped = weigh ? pass_sum(s, rest) : 0.0;
     if (nc > 1) {
         __syncthreads();
@@ -1196,7 +1052,7 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
         if (me != 0) return;
     }
     if (s.lost) {
-        if (tid == 0) a.r.status[b] = 2;
+        if (tid == 0) a.r.status[b] = kPassUnsettled;
         return;
     }
     if (tid == 0) s.part_rest[0] = dropped, s.part_rc[0] = rc;
@@ -1205,7 +1061,7 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
     int n = (int)s.count;
     if (n == 0) {
         if (tid == 0) {
-            a.r.status[b] = 0;
+            a.r.status[b] = kPassSettled;
             a.r.ids[b] = -1;
             if (a.r.probs) a.r.probs[b] = 0.0f;
             if (a.r.counts) a.r.counts[b] = 0;
@@ -1235,12 +1091,12 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
         gone_error = gone * (ldexp(1.0, -21) + 0.6932 * (spread * 2.0 + apart) * ldexp(1.0, -24)) * 1.01 +
                      ids * (1e-13 + ldexp(1.0, -43));
         if (!(gone < 1e7)) {  // the reference was too far below, or there is a NaN
-            if (tid == 0) a.r.status[b] = 3;
+            if (tid == 0) a.r.status[b] = kPassUnsettled;
             return;
         }
     }
     if (!(hi < INFINITY)) {
-        if (tid == 0) a.r.status[b] = 4;
+        if (tid == 0) a.r.status[b] = kPassUnsettled;
         return;
     }
     /* one more rise for a shorter sort */
@@ -1262,7 +1118,7 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
         __syncthreads();
     }
     if (s.lost || n > kPassSort) {
-        if (tid == 0) a.r.status[b] = 5;
+        if (tid == 0) a.r.status[b] = kPassUnsettled;
         return;
     }
     /*
@@ -1290,7 +1146,7 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
     const ReqRow r = req_row(a.r, b, hi, s.u);
     if (r.greedy) {
         if (tid == 0) {
-            a.r.status[b] = 0;
+            a.r.status[b] = kPassSettled;
             a.r.ids[b] = pass_id(list[0]);
             if (a.r.probs) a.r.probs[b] = 1.0f;
             if (a.r.counts) a.r.counts[b] = 1;
@@ -1332,7 +1188,7 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
         left = (int)s.found;
         /* open within the error, or a lost bet: the row's other ids weigh too much, or some come before the cut */
         if (s.found != s.found_high || left == 0 || (row.kind == kPassShare && !(pass_x(list[left - 1]) >= f))) {
-            if (tid == 0) a.r.status[b] = 6;
+            if (tid == 0) a.r.status[b] = kPassUnsettled;
             return;
         }
     }
@@ -1368,7 +1224,7 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
     if (target >= total) target = total - 1;
     for (; at < end; ++at) {
         if (before <= target && target - before < weights[at]) {
-            a.r.status[b] = 0;
+            a.r.status[b] = kPassSettled;
             a.r.ids[b] = pass_id(list[at]);
             if (a.r.probs)
                 a.r.probs[b] = (float)(req_exp(r, pass_x(list[at]), s.table) * (double)(1ull << kReqFraction) / (double)total);
