@@ -49,13 +49,20 @@ cudaError_t launch(void (*kernel)(A...), int grid, int threads, size_t smem, int
     lc.dynamicSmemBytes = smem;
     lc.stream = s;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
+    unsigned n = 0;
+    if (cluster > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = (unsigned)cluster;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (dependent) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
     lc.attrs = at;
-    lc.numAttrs = dependent ? 2 : 1;
+    lc.numAttrs = n;
     return cudaLaunchKernelEx(&lc, kernel, args...);
 }
 
@@ -80,12 +87,18 @@ int request_launch(RequestArgs a, int sms, cudaStream_t s) {
     p.step = (int)(p.turns * 0.618);
     while (p.step > 1 && divisor(p.turns, p.step) != 1) --p.step;
     if (p.step < 1) p.step = 1;
+    p.order = parts == 1 && a.batch > 4 * sms && a.batch <= 4096;  // more than one turn of the GPU; each CTA looks at all settings
     const size_t pass_smem = kPassKeep * sizeof(uint64_t);
     int r = dynamic_smem((const void *)sample_pass_kernel<T>, pass_smem);
     if (r) return r;
+    /* one division of the SMs' memory for both kernels, or neither starts where the other runs */
+    for (const void *kernel : {(const void *)sample_pass_kernel<T>, (const void *)sample_requests_kernel<T>})
+        CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     /* the rows that it does not take, and those that it leaves */
     const int64_t row = (int64_t)a.vocab * sizeof(T);
     const int cluster = row > 262144 ? 16 : row > 131072 ? 8 : row > 65536 ? 4 : 2;
+    if (cluster > 8)
+        CUDA_TRY(cudaFuncSetAttribute((const void *)sample_requests_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     const int unit = kReqThreads;  // every warp's region in whole turns
     a.per = ((a.vocab + cluster - 1) / cluster + unit - 1) / unit * unit;
     size_t smem = (size_t)a.per * sizeof(T);
@@ -93,22 +106,9 @@ int request_launch(RequestArgs a, int sms, cudaStream_t s) {
     if (!a.resident) smem = 0;
     r = dynamic_smem((const void *)sample_requests_kernel<T>, smem);
     if (r) return r;
-    /*
-     * The former run before the pass, which fills the SMs as they leave room
-     * (beside it they would end long after it); where every row may have a
-     * cluster of its own, beside it, in the launch for the latter.
-     */
-    if (cluster > 8)
-        CUDA_TRY(cudaFuncSetAttribute((const void *)sample_requests_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    const bool few = a.batch <= 2 * sms / cluster;
-    const int beside = few ? a.batch : sms / cluster, after = few ? a.batch : a.batch < 256 ? sms / cluster : 2 * sms / cluster;
-    if (!few) {
-        a.rows = kReqBySettings;
-        CUDA_TRY(launch(sample_requests_kernel<T>, beside * cluster, kReqThreads, smem, cluster, false, s, a));
-    }
-    CUDA_TRY(launch(sample_pass_kernel<T>, a.batch * parts, kPassThreads, pass_smem, parts, !few, s, p));
-    a.rows = few ? kReqBySettings | kReqUnsettled : kReqUnsettled;
-    CUDA_TRY(launch(sample_requests_kernel<T>, after * cluster, kReqThreads, smem, cluster, true, s, a));
+    CUDA_TRY(launch(sample_pass_kernel<T>, a.batch * parts, kPassThreads, pass_smem, parts, false, s, p));
+    const int most = a.batch < 256 ? sms / cluster : 2 * sms / cluster;
+    CUDA_TRY(launch(sample_requests_kernel<T>, (a.batch < 2 * sms / cluster ? a.batch : most) * cluster, kReqThreads, smem, cluster, true, s, a));
     return NOEL_OK;
 }
 

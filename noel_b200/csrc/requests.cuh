@@ -32,7 +32,6 @@ struct RequestArgs {
     int32_t *status;     // [batch] PassStatus
     int per;             // elements of a row to a CTA of its cluster
     bool resident;       // they fit the shared memory
-    int rows;            // ReqRows of this launch
 };
 
 constexpr int kReqThreads = 512;
@@ -575,11 +574,10 @@ __device__ __forceinline__ PassRow pass_row(const RequestArgs &a, int b) {
     return r;
 }
 /*
- * The rows that sample_pass_kernel does not take, by their settings (rows = 1,
- * before it or beside it), and those that it could not settle (rows = 2, after
- * it).  The clusters take them in turn.
+ * The rows that sample_pass_kernel does not take, by their settings, as soon
+ * as its last CTAs leave room, and then those that it could not settle.  The
+ * clusters take them in turn.
  */
-enum ReqRows { kReqBySettings = 1, kReqUnsettled = 2 };
 template <typename T>
 __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __grid_constant__ RequestArgs a) {
     extern __shared__ __align__(16) unsigned char req_raw[];
@@ -590,9 +588,7 @@ __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __gr
     int turn = 0;
     req_table(s.table);
     cluster.sync();  // every CTA of the cluster is there before one writes into another's memory
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     for (int after = 0; after < 2; ++after) {
-        if (!(a.rows & (after ? kReqUnsettled : kReqBySettings))) continue;
         if (after) asm volatile("griddepcontrol.wait;" ::: "memory");
         uint32_t rank = 0;
         for (int at = 0; at < a.batch; at += kReqThreads) {
@@ -605,11 +601,13 @@ __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __gr
             if ((tid & 31) == 0) s.rows[tid >> 5] = bits;
             __syncthreads();
             for (int w = 0; w < kReqWarps; ++w)
-                for (uint32_t left = s.rows[w]; left; left &= left - 1)
-                    if (rank++ % clusters == me) {
+                for (uint32_t left = s.rows[w]; left; left &= left - 1) {
+                    const uint32_t turn_of = rank++ % clusters;
+                    if ((after ? clusters - 1 - turn_of : turn_of) == me) {  // from the other end: those had fewer rows before
                         req_sample_row<T>(a, s, req_raw, at + w * 32 + __ffs(left) - 1, turn);
                         __syncthreads();
                     }
+                }
         }
     }
 }
@@ -645,6 +643,7 @@ constexpr int kPassSort = 2048;   // of those, at the end
 struct PassArgs {
     RequestArgs r;
     int turns, step;  // turns of a warp's part of a row, taken in steps of step (no common divisor)
+    bool order;       // the rows that take longest first
 };
 
 struct PassShared {
@@ -751,6 +750,31 @@ __device__ __forceinline__ float pass_floor(const PassRow &r, float m) {
     return fmaxf(f - fabsf(f) * 2e-7f - fabsf(m) * 2e-7f - 1e-37f, -3.402823466e38f);
 }
 
+/*
+ * The row of place at, where rows with top-p alone or a large top-k come first
+ * and the others after them: they take twice the others' time (1024 mixed
+ * rows: 100 to 140 us against 50), and the last ones to start would end alone.
+ */
+__device__ __forceinline__ int pass_order(const RequestArgs &a, PassShared &s, int at) {
+    const int each = (a.batch + kPassThreads - 1) / kPassThreads, from = threadIdx.x * each;
+    auto slow = [&](int b) {
+        const bool t = !a.temperature || a.temperature[b] > 0.0f, least = a.min_p && a.min_p[b] > 0.0f;
+        const bool p = a.top_p && a.top_p[b] < 1.0f;
+        const int k = a.top_k ? a.top_k[b] : 0;
+        return t && (k > 0 ? k > kPassThreads : p && !least);
+    };
+    uint64_t mine = 0, all;
+    for (int b = from; b < min(a.batch, from + each); ++b) mine += slow(b);
+    const int before = (int)(pass_scan(s, mine, all) - mine);
+    int place_slow = before, place = (int)all + min(from, a.batch) - before;
+    for (int b = from; b < min(a.batch, from + each); ++b)
+        if ((slow(b) ? place_slow++ : place++) == at) s.left = b;
+    __syncthreads();
+    const int b = s.left;
+    __syncthreads();
+    return b;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __grid_constant__ PassArgs a) {
     extern __shared__ __align__(16) unsigned char req_raw[];
@@ -759,7 +783,7 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
     cg::cluster_group cluster = cg::this_cluster();
     const int me = cluster.block_rank(), nc = cluster.num_blocks();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int b = blockIdx.x / nc;
+    const int b = a.order ? pass_order(a.r, s, blockIdx.x / nc) : blockIdx.x / nc;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     using V = PassVec<T>;
     constexpr int kVecs = kPassEach / V::kPer;
