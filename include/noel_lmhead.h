@@ -10,8 +10,10 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "noel_int8.h"
 #include "noel_logits.h"
 #include "noel_lora.h"
+#include "noel_requests.h"
 #include "sampler.h"
 
 #ifdef __cplusplus
@@ -53,6 +55,28 @@ int noel_lmhead_sample_ex(const noel_sampler_config_t *cfg, const void *d_weight
                           const noel_lora_t *lora, const int32_t *d_adapter, const noel_logits_params_t *process,
                           const int32_t *d_history, int history_len, size_t hld, uint64_t *d_rng, int32_t *d_ids,
                           float *d_probs, float *d_logits, void *d_work, size_t work_bytes, void *stream);
+
+/*
+ * The path of a batch whose output weights are in 8 bits and whose requests
+ * all differ: noel_i8_linear of the hidden states d_hidden [batch][ldh] (type
+ * NOEL_HEAD_F32, NOEL_HEAD_F16 or NOEL_HEAD_BF16) with d_weight [vocab][ldw]
+ * and d_weight_scale [vocab] into d_logits [batch][vocab] fp32, then each
+ * token's adapter (lora and d_adapter; fp32 hidden states only), then process
+ * (noel_logits_process), then noel_sample_requests with params and
+ * d_uniforms; all in the same stream.  lora or process may be NULL.  d_logits
+ * receives the logits that were sampled.  d_work (16-byte aligned, work_bytes
+ * >= noel_lmhead_i8_workspace_bytes(batch, hidden_dim, vocab, lora's rank, or 0
+ * without)) is scratch of this call until it has run.  Allocates nothing and
+ * may be captured into a graph.
+ */
+int noel_lmhead_i8_sample(const noel_request_params_t *params, const int8_t *d_weight, size_t ldw,
+                          const float *d_weight_scale, const void *d_hidden, int hidden_type, size_t ldh, int batch,
+                          int hidden_dim, int vocab, const noel_lora_t *lora, const int32_t *d_adapter,
+                          const noel_logits_params_t *process, const float *d_uniforms, int32_t *d_ids, float *d_probs,
+                          int32_t *d_counts, float *d_logits, void *d_work, size_t work_bytes, void *stream);
+
+/* Bytes of the scratch that noel_lmhead_i8_sample needs. */
+size_t noel_lmhead_i8_workspace_bytes(int batch, int hidden_dim, int vocab, int rank);
 
 #ifdef __cplusplus
 }

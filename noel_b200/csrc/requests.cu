@@ -1,10 +1,11 @@
 /*
  * Host side of sampling with every row's own settings
- * (include/noel_requests.h).
+ * (include/noel_requests.h), and of the path from 8-bit output weights to it.
  */
 #include "noel_requests.h"
 
 #include "host.h"
+#include "noel_lmhead.h"
 #include "requests.cuh"
 
 using namespace noel;
@@ -130,6 +131,59 @@ extern "C" int noel_sample_requests(const noel_request_params_t *params, const v
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (!r) r = dtype == NOEL_DTYPE_F32 ? request_launch<float>(a, sms, s) : request_launch<__nv_bfloat16>(a, sms, s);
     return r ? r : ok();
+} catch (...) {
+    return fail(NOEL_ERR_CUDA, "host memory");
+}
+
+/* ------------------------------- 8-bit LM head -> adapters -> processing -> sampler */
+namespace {
+/* the steps run one after the other, so they share one scratch */
+size_t head_work(int batch, int hidden_dim, int vocab, int rank) {
+    const size_t sizes[] = {noel_i8_linear_workspace_bytes(batch, hidden_dim), rank > 0 ? noel_lora_workspace_bytes(batch, rank) : 0,
+                            noel_sample_requests_workspace_bytes(batch, vocab)};
+    size_t most = 0;
+    for (const size_t n : sizes) most = n > most ? n : most;
+    return most;
+}
+}  // namespace
+
+extern "C" size_t noel_lmhead_i8_workspace_bytes(int batch, int hidden_dim, int vocab, int rank) {
+    return batch > 0 ? head_work(batch, hidden_dim, vocab, rank) : 0;
+}
+
+extern "C" int noel_lmhead_i8_sample(const noel_request_params_t *params, const int8_t *d_weight, size_t ldw,
+                                     const float *d_weight_scale, const void *d_hidden, int hidden_type, size_t ldh,
+                                     int batch, int hidden_dim, int vocab, const noel_lora_t *lora,
+                                     const int32_t *d_adapter, const noel_logits_params_t *process, const float *d_uniforms,
+                                     int32_t *d_ids, float *d_probs, int32_t *d_counts, float *d_logits, void *d_work,
+                                     size_t work_bytes, void *stream) try {
+    /* whatever a later step would refuse is refused before the first one runs */
+    RequestArgs a{};
+    int r = request_args(params, d_logits, NOEL_DTYPE_F32, batch, vocab, (size_t)(vocab > 0 ? vocab : 0), d_uniforms, d_ids,
+                         d_probs, d_counts, d_work, work_bytes, &a);
+    if (r) return r;
+    if (lora && hidden_type != NOEL_HEAD_F32) return fail(NOEL_ERR_UNSUPPORTED, "adapters need fp32 hidden states (type %d)", hidden_type);
+    if (lora && (lora->rank < 1 || lora->rank > 256)) return fail(NOEL_ERR_TOO_LARGE, "rank %d (1..256)", lora->rank);
+    const size_t need = noel_lmhead_i8_workspace_bytes(batch, hidden_dim, vocab, lora ? lora->rank : 0);
+    if (need > 0 && (!d_work || work_bytes < need))
+        return fail(NOEL_ERR_INVALID_ARG, "scratch of %zu bytes, %zu wanted", d_work ? work_bytes : 0, need);
+    if (lora || process) {
+        /* an empty batch goes through the adapters' and the processing's checks only */
+        if (lora) r = noel_lora_apply(lora, d_adapter, static_cast<const float *>(d_hidden), ldh, 0, hidden_dim, vocab, d_logits,
+                                      (size_t)vocab, d_work, work_bytes, stream);
+        if (!r && process) r = noel_logits_process(process, d_logits, NOEL_DTYPE_F32, 0, vocab, (size_t)vocab, stream);
+        if (r) return r;
+    }
+    r = noel_i8_linear(d_hidden, hidden_type, ldh, batch, d_weight, ldw, d_weight_scale, vocab, hidden_dim, d_logits,
+                       NOEL_DTYPE_F32, (size_t)vocab, d_work, work_bytes, stream);
+    if (!r && lora)
+        r = noel_lora_apply(lora, d_adapter, static_cast<const float *>(d_hidden), ldh, batch, hidden_dim, vocab, d_logits,
+                            (size_t)vocab, d_work, work_bytes, stream);
+    if (!r && process) r = noel_logits_process(process, d_logits, NOEL_DTYPE_F32, batch, vocab, (size_t)vocab, stream);
+    if (!r)
+        r = noel_sample_requests(params, d_logits, NOEL_DTYPE_F32, batch, vocab, (size_t)vocab, d_uniforms, d_ids, d_probs,
+                                 d_counts, d_work, work_bytes, stream);
+    return r;
 } catch (...) {
     return fail(NOEL_ERR_CUDA, "host memory");
 }

@@ -601,13 +601,11 @@ __global__ void __launch_bounds__(kReqThreads) sample_requests_kernel(const __gr
             if ((tid & 31) == 0) s.rows[tid >> 5] = bits;
             __syncthreads();
             for (int w = 0; w < kReqWarps; ++w)
-                for (uint32_t left = s.rows[w]; left; left &= left - 1) {
-                    const uint32_t turn_of = rank++ % clusters;
-                    if ((after ? clusters - 1 - turn_of : turn_of) == me) {  // from the other end: those had fewer rows before
+                for (uint32_t left = s.rows[w]; left; left &= left - 1)
+                    if (rank++ % clusters == me) {
                         req_sample_row<T>(a, s, req_raw, at + w * 32 + __ffs(left) - 1, turn);
                         __syncthreads();
                     }
-                }
         }
     }
 }

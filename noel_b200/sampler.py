@@ -160,6 +160,12 @@ def lib() -> C.CDLL:
     L.noel_sample_requests.restype = C.c_int
     L.noel_sample_requests.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_size_t, C.c_void_p,
                                        C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+    L.noel_lmhead_i8_workspace_bytes.restype = C.c_size_t
+    L.noel_lmhead_i8_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int]
+    L.noel_lmhead_i8_sample.restype = C.c_int
+    L.noel_lmhead_i8_sample.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_int, C.c_size_t,
+                                        C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
     L.noel_moe_route_top_k.restype = C.c_int
     L.noel_moe_route_top_k.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p]
     L.noel_sampler_cuda_last_error.restype = C.c_int
@@ -912,3 +918,45 @@ def sample_requests(logits, uniforms, params: SampleParams, vocab: int | None = 
         params.ref, ptr, dtype, B, V, _pitch(logits), up, ids.data_ptr(), probs.data_ptr(),
         left.data_ptr() if counts else None, work.data_ptr() if size else None, size, s))
     return (ids, probs, left) if counts else (ids, probs)
+
+
+def lmhead_int8_sample(weight: Int8Rows, hidden, uniforms, params: SampleParams, adapters: Adapters | None = None,
+                       adapter_ids=None, process: LogitsParams | None = None, counts: bool = False):
+    """The LM head with weights in 8 bits, then sampling with every row's own
+    settings (include/noel_lmhead.h): hidden [B, D] CUDA float32, float16 or
+    bfloat16, uniforms [B] float32.  adapters with adapter_ids [B] int32 add
+    each token's low-rank part to its logits (float32 hidden states), and
+    process is applied to them before sampling.  Returns (ids [B] int32, logits
+    [B, V] float32, probs [B] float32), and with counts also how many ids the
+    settings left [B] int32."""
+    import torch
+
+    dev, V, D = weight.device, weight.rows, weight.cols
+    kind, xp, ldx = _float_rows(hidden, "hidden", dev, D)
+    if kind == HEAD_F32:
+        ldx = _own_pitch(hidden)
+    B = hidden.shape[0]
+    up = _row_values(uniforms, torch.float32, B, "uniforms", dev)
+    if (adapters is None) != (adapter_ids is None):
+        _refuse("adapters and adapter_ids come together")
+    lora = ip = None
+    rank = 0
+    if adapters is not None:
+        if adapters.device != dev or (adapters.rows, adapters.cols) != (V, D):
+            _refuse(f"adapters of a [{adapters.rows}, {adapters.cols}] weight on {adapters.device}, "
+                    f"the head is [{V}, {D}] on {dev}")
+        lora, ip, rank = adapters.ref, _row_values(adapter_ids, torch.int32, B, "adapter_ids", dev), adapters.rank
+    logits = torch.empty(B, V, dtype=torch.float32, device=dev)
+    params.check(logits)
+    if process is not None:
+        process.check(logits, V)
+    ids = torch.empty(B, dtype=torch.int32, device=dev)
+    probs = torch.empty(B, dtype=torch.float32, device=dev)
+    left = torch.empty(B, dtype=torch.int32, device=dev) if counts else None
+    size = lib().noel_lmhead_i8_workspace_bytes(B, D, V, rank)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _call(dev, None, lambda s: lib().noel_lmhead_i8_sample(
+        params.ref, weight.ptr, weight.pitch, weight.scale_ptr, xp, kind, ldx, B, D, V, lora, ip,
+        process.ref if process is not None else None, up, ids.data_ptr(), probs.data_ptr(),
+        left.data_ptr() if counts else None, logits.data_ptr(), work.data_ptr() if size else None, size, s))
+    return (ids, logits, probs, left) if counts else (ids, logits, probs)
