@@ -164,13 +164,15 @@ int noel_sampler_sample_batch_host(const noel_sampler_config_t *cfg, const void 
  * wait of the streaming kernel (for a ring stage, a prepared row or the
  * consumers of a row) ran out of its limit; the kernel then returns instead
  * of hanging and the results of that call are invalid.  Clears the flag.
+ * Reports (and clears) the waits of the 8-bit product (noel_int8.h) on the
+ * current device as well, whichever stream they were on.
  */
 int noel_sampler_cuda_sync_check(void *stream);
 
 /*
- * Limit of every device-side wait of the batched calls this thread makes
- * next, in nanoseconds of the GPU's global timer (0 restores the default of
- * 2 s).  stall_next_call = 1 makes the next batched call's kernel issue no
+ * Limit of every device-side wait of the batched calls and of the 8-bit
+ * products (noel_int8.h) this thread makes next, in nanoseconds of the GPU's global timer (0 restores the default of
+ * 2 s).  stall_next_call = 1 makes the next such call's kernel issue no
  * row loads, so its waits run out and noel_sampler_cuda_sync_check reports
  * NOEL_ERR_DEVICE_WAIT: the failure-detection path, exercised without a GPU
  * fault.  No counterpart in the reference (its sampler never waits).

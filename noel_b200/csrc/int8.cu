@@ -3,6 +3,8 @@
  */
 #include "noel_int8.h"
 
+#include <atomic>
+
 #include "host.h"
 #include "int8.cuh"
 #include "noel_lmhead.h"
@@ -12,6 +14,7 @@ using namespace noel;
 namespace {
 
 __device__ int g_i8_failed;  // a wait of the product ran out on this device
+std::atomic<bool> g_i8_used{false};  // a product has been launched
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -139,6 +142,7 @@ int product_launch(const Product &p, const I8Args &args, int groups, bool depend
     }
     lc.attrs = at;
     lc.numAttrs = n;
+    g_i8_used = true;
     CUDA_TRY(cudaLaunchKernelEx(&lc, i8_product_kernel<NT, PAIR, OUT>, mw, mp, ma, args));
     CUDA_TRY(cudaGetLastError());
     return NOEL_OK;
@@ -178,6 +182,8 @@ size_t cast_pitch(int cols) { return ((size_t)cols + 15) / 16 * 16; }
 }  // namespace
 
 int noel::i8_wait_failed(bool *failed) {
+    *failed = false;
+    if (!g_i8_used) return NOEL_OK;  // without a copy, which a stream being captured elsewhere may not allow
     int v = 0;
     const int zero = 0;
     CUDA_TRY(cudaMemcpyFromSymbol(&v, g_i8_failed, sizeof(v)));

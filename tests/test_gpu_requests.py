@@ -184,3 +184,48 @@ def test_graphs_share_nothing(cuda):
             side.synchronize()
             for x, y in zip(out, again):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("batch", [30, 700])
+def test_odd_values_in_large_rows(cuda, dtype, batch):
+    """Infinities, NaN, masks of the type's lowest value and rows with nothing, under all kinds of settings; with 700
+    rows a CTA has a row of its own."""
+    rng = np.random.default_rng(21)
+    vocab = 20011
+    x = rows_of(rng, batch, vocab, "zipf")
+    low = np.float32(-3.3895314e38) if dtype == "bfloat16" else np.float32(-3.4028235e38)
+    kind = np.arange(batch) % 10
+    x[kind == 1, 15000:15003] = np.inf
+    x[kind == 2, ::7] = np.nan
+    x[kind == 3, :] = np.where(rng.uniform(size=vocab) < 0.999, low, x[kind == 3, :])
+    x[kind == 4, :19000] = -np.inf
+    x[kind == 5, :] = -np.inf
+    x[kind == 6, :] = low
+    x[kind == 7, 777] = np.inf
+    x[kind == 8, :] *= 1e30
+    x[kind == 9, 1:] = np.nan
+    check(x, rng.uniform(size=batch).astype(np.float32), NAMES, settings_of(rng, batch, vocab), dtype, 5, cuda)
+
+
+def test_top_p_close_to_one_and_hot_and_cold(cuda):
+    """What the one pass over a row bets on or bounds: shares near 1, temperatures far from 1, heavy and light tails."""
+    rng = np.random.default_rng(22)
+    batch, vocab = 640, 30000
+    a = np.exp(rng.uniform(np.log(0.2), np.log(8.0), (batch, 1)))
+    x = (5.0 - a * np.log(np.maximum(rng.uniform(size=(batch, vocab)), 2.0**-25) * vocab)).astype(np.float32)
+    t = np.exp(rng.uniform(np.log(0.01), np.log(50.0), batch)).astype(np.float32)
+    p = (1.0 - np.exp(rng.uniform(np.log(1e-6), np.log(0.9), batch))).astype(np.float32)
+    check(x, rng.uniform(size=batch).astype(np.float32), ("temperature", "top_p"), (t, p), dev=cuda)
+    # the largest ids of a vocabulary sorted by frequency come first, or last
+    check(np.sort(x, 1)[:, ::-1].copy(), rng.uniform(size=batch).astype(np.float32), ("temperature", "top_p"), (t, p), dev=cuda)
+    check(np.sort(x, 1), rng.uniform(size=batch).astype(np.float32), ("temperature", "top_p"), (t, p), dev=cuda)
+
+
+@pytest.mark.parametrize("k", [1, 7, 256, 257, 1000, 1024, 1025, 5000])
+def test_top_k_sizes(cuda, k):
+    rng = np.random.default_rng(23)
+    for batch in (3, 650):
+        x = rows_of(rng, batch, 12000, "normal")
+        check(x, rng.uniform(size=batch).astype(np.float32), ("top_k", "top_p"),
+              (np.full(batch, k, np.int32), np.where(np.arange(batch) % 2, 0.9, 1.0).astype(np.float32)), dev=cuda)
