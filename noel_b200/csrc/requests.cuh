@@ -1004,18 +1004,29 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
                     const uint32_t n = __popc(mask);
                     uint32_t at = atomicAdd(&s.count, n);
                     if (at + n <= kPassKeep) {
+                        /* few of a thread's elements pass: the loop takes a turn or two, each choosing one of 16 registers */
+                        for (uint32_t left = mask; left; left &= left - 1) {
+                            const int j = __ffs(left) - 1;
+                            float half[8];
 #pragma unroll
-                        for (int j = 0; j < kPassEach; ++j)
-                            if (mask >> j & 1) {
-                                const int v = first + turn * (32 * kVecs) + (j / V::kPer) * 32 + lane;
-                                keep[at++] = pass_pack(x[j], head + v * V::kPer + j % V::kPer);
-                                x[j] = -INFINITY;
-                            }
+                            for (int i = 0; i < 8; ++i) half[i] = j & 1 ? x[2 * i + 1] : x[2 * i];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) half[i] = j & 2 ? half[2 * i + 1] : half[2 * i];
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) half[i] = j & 4 ? half[2 * i + 1] : half[2 * i];
+                            const int v = first + turn * (32 * kVecs) + (j / V::kPer) * 32 + lane;
+                            keep[at++] = pass_pack(j & 8 ? half[1] : half[0], head + v * V::kPer + j % V::kPer);
+                        }
                     } else {  // from the first place that ran over on, none is filled
                         atomicMin(&s.valid, at);
                         s.full = 1;
                         again = true;
                     }
+                }
+                if (__any_sync(0xFFFFFFFFu, again) || weigh) {
+#pragma unroll
+                    for (int j = 0; j < kPassEach; ++j)
+                        if (x[j] >= f && !again) x[j] = -INFINITY;  // kept: neither tried again nor dropped
                 }
                 if (__any_sync(0xFFFFFFFFu, again)) break;
             }
