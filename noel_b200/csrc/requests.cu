@@ -102,7 +102,7 @@ int request_launch(RequestArgs a, int sms, cudaStream_t s) {
      * in clusters of 16 (two turns of the GPU), 8 and 4 */
     const int64_t row = (int64_t)a.vocab * sizeof(T);
     int cluster = row > 262144 ? 16 : row > 131072 ? 8 : row > 65536 ? 4 : 2;
-    while (cluster < 16 && (int64_t)a.batch * cluster <= sms && a.vocab / cluster >= 2048) cluster *= 2;  // SMs are free
+    while (cluster < 16 && (int64_t)a.batch * cluster <= sms / 2 && a.vocab / cluster >= 2048) cluster *= 2;  // SMs are free
     if (cluster > 8)
         CUDA_TRY(cudaFuncSetAttribute((const void *)sample_requests_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     const int unit = kReqThreads;  // every warp's region in whole turns

@@ -385,7 +385,13 @@ __device__ ReqCut req_cut(const ReqSlice<T> &sl, ReqShared &s, const ReqRow &r, 
 
 /*
  * A cluster of CTAs to a row, each with a part of it in shared memory (read
- * from global memory each time where it does not fit).
+ * from global memory each time where it does not fit): the largest logit, the
+ * cut, the exact sums of every warp's region, and the region that the draw
+ * ends in.  A row of 152,064 fp32 alone takes 14 us in a cluster of 16 where
+ * nothing is cut (3.4 to load it, 4.7 for the weights' sums; a cluster of 8:
+ * 20) and 35 where top-p cuts (5.7 for the histogram, 4 to add it up over the
+ * cluster, 2.8 and 3.9 to collect and sort what is around the cut): latency,
+ * and the issue of about 60 instructions an id.
  */
 template <typename T>
 __device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char *req_raw, int b, int &turn) {
@@ -633,7 +639,7 @@ constexpr int kPassThreads = 256;
 constexpr int kPassWarps = kPassThreads / 32;
 constexpr int kPassEach = 16;     // elements of a thread's turn
 constexpr int kPassKeep = 4096;   // kept at most
-constexpr int kPassFull = 3072;   // and at most after the filter has risen
+constexpr int kPassFull = kPassKeep / 4 * 3;  // and at most after the filter has risen
 constexpr int kPassRises = 5;
 constexpr int kPassBins = 1024;
 constexpr int kPassSort = 2048;   // of those, at the end
@@ -773,6 +779,16 @@ __device__ __forceinline__ int pass_order(const RequestArgs &a, PassShared &s, i
     return b;
 }
 
+/*
+ * Four CTAs of 64 registers to an SM.  Of 1024 mixed rows of 152,064 fp32 one
+ * takes about 53 us there: 3 for the first filter, 37 for the row (HBM, when
+ * all of them are at it), 3 for a last rise where over 256 are kept, 1.7 to rank
+ * them, 3 for weights, cuts and the walk; 8.5 for a rise on the way, which top-p
+ * rows and large top-k need several of.  Of 1024 rows of 256,000 bf16 with top-p
+ * alone one takes 97 us, 65 of them for the row, bound by instruction issue
+ * (77 % of the slots, about 22 instructions an id: an exponential each, and
+ * the kept ones).
+ */
 template <typename T>
 __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __grid_constant__ PassArgs a) {
     extern __shared__ __align__(16) unsigned char req_raw[];
