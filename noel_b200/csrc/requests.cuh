@@ -548,7 +548,9 @@ __device__ void req_sample_row(const RequestArgs &a, ReqShared &s, unsigned char
     }
 }
 
+/* what sample_pass_kernel says of a row: done, not taken (by its settings), or not settled */
 enum PassStatus { kPassSettled, kPassSkipped, kPassUnsettled };
+/* greatest logit; top-k; min-p; top-p alone; none of sample_pass_kernel's */
 enum PassKind { kPassGreedy, kPassCount, kPassLeast, kPassShare, kPassNot };
 constexpr int kPassTopK = 1024;  // largest top_k of sample_pass_kernel
 
@@ -841,9 +843,9 @@ __global__ void __launch_bounds__(kPassThreads, 4) sample_pass_kernel(const __gr
     if (a.turns > 1) load(ahead);
 
     /*
-     * The filter that the histogram in s.n of elements from low to hi gives:
-     * 1 / grow of the row has been seen by this CTA, and dropped is what it has dropped
-     * weighs (as of hi).
+     * The filter that the histogram in s.n of elements from low to hi gives.
+     * This CTA has seen 1 / grow of the row; dropped: what its dropped elements
+     * weigh, hi's weight being 1.
      */
     auto edge = [&](float hi, float low, float scale, double dropped, double grow) -> float {
         /* counts in the low 14 bits, above them the weights of the bins (of their upper ends) in 2^-36 */
