@@ -66,8 +66,9 @@ int noel_lmhead_sample_ex(const noel_sampler_config_t *cfg, const void *d_weight
  * d_uniforms; all in the same stream.  lora or process may be NULL.  d_logits
  * receives the logits that were sampled.  d_work (16-byte aligned, work_bytes
  * >= noel_lmhead_i8_workspace_bytes(batch, hidden_dim, vocab, lora's rank, or 0
- * without)) is scratch of this call until it has run.  Allocates nothing and
- * may be captured into a graph.
+ * without)) is scratch of this call until it has run.  What any step would
+ * refuse is refused before the first one runs.  Allocates nothing and may be
+ * captured into a graph.
  */
 int noel_lmhead_i8_sample(const noel_request_params_t *params, const int8_t *d_weight, size_t ldw,
                           const float *d_weight_scale, const void *d_hidden, int hidden_type, size_t ldh, int batch,

@@ -8,6 +8,8 @@
 
 #include <stddef.h>
 
+#include "noel_logits.h"
+#include "noel_lora.h"
 #include "noel_sampler_cuda.h"
 
 namespace noel {
@@ -24,6 +26,12 @@ __attribute__((visibility("hidden"))) int dynamic_smem(const void *kernel, size_
 __attribute__((visibility("hidden"))) unsigned long long wait_limit_ns();
 /* Whether the thread asked that its next call load nothing (which ends the request). */
 __attribute__((visibility("hidden"))) bool take_stall();
+/* What noel_lora_apply and noel_logits_process (of fp32 logits) refuse of these arguments; nothing is launched. */
+__attribute__((visibility("hidden"))) int lora_check(const noel_lora_t *lora, const int32_t *adapter, const float *x, size_t ldx,
+                                                     int batch, int cols, int rows, float *y, size_t ldy, void *work,
+                                                     size_t work_bytes);
+__attribute__((visibility("hidden"))) int logits_check(const noel_logits_params_t *params, float *logits, int batch, int vocab,
+                                                       size_t ld);
 /* Whether a wait of the int8 product ran out on the current device since the last call (which clears it). */
 __attribute__((visibility("hidden"))) int i8_wait_failed(bool *failed);
 

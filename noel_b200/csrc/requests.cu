@@ -162,23 +162,21 @@ extern "C" int noel_lmhead_i8_sample(const noel_request_params_t *params, const 
                                      const int32_t *d_adapter, const noel_logits_params_t *process, const float *d_uniforms,
                                      int32_t *d_ids, float *d_probs, int32_t *d_counts, float *d_logits, void *d_work,
                                      size_t work_bytes, void *stream) try {
-    /* whatever a later step would refuse is refused before the first one runs */
+    /* what a later step would refuse of the whole batch is refused before the first one runs; noel_i8_linear, the first
+     * one, checks its own arguments before it launches */
     RequestArgs a{};
     int r = request_args(params, d_logits, NOEL_DTYPE_F32, batch, vocab, (size_t)(vocab > 0 ? vocab : 0), d_uniforms, d_ids,
                          d_probs, d_counts, d_work, work_bytes, &a);
     if (r) return r;
     if (lora && hidden_type != NOEL_HEAD_F32) return fail(NOEL_ERR_UNSUPPORTED, "adapters need fp32 hidden states (type %d)", hidden_type);
-    if (lora && (lora->rank < 1 || lora->rank > 256)) return fail(NOEL_ERR_TOO_LARGE, "rank %d (1..256)", lora->rank);
+    if (lora && (r = lora_check(lora, d_adapter, static_cast<const float *>(d_hidden), ldh, batch, hidden_dim, vocab, d_logits,
+                                (size_t)vocab, d_work, work_bytes)))
+        return r;
+    /* what noel_logits_process refuses by its plan for the device are more rows and columns than request_args lets by */
+    if (process && (r = logits_check(process, d_logits, batch, vocab, (size_t)vocab))) return r;
     const size_t need = noel_lmhead_i8_workspace_bytes(batch, hidden_dim, vocab, lora ? lora->rank : 0);
     if (need > 0 && (!d_work || work_bytes < need))
         return fail(NOEL_ERR_INVALID_ARG, "scratch of %zu bytes, %zu wanted", d_work ? work_bytes : 0, need);
-    if (lora || process) {
-        /* an empty batch goes through the adapters' and the processing's checks only */
-        if (lora) r = noel_lora_apply(lora, d_adapter, static_cast<const float *>(d_hidden), ldh, 0, hidden_dim, vocab, d_logits,
-                                      (size_t)vocab, d_work, work_bytes, stream);
-        if (!r && process) r = noel_logits_process(process, d_logits, NOEL_DTYPE_F32, 0, vocab, (size_t)vocab, stream);
-        if (r) return r;
-    }
     r = noel_i8_linear(d_hidden, hidden_type, ldh, batch, d_weight, ldw, d_weight_scale, vocab, hidden_dim, d_logits,
                        NOEL_DTYPE_F32, (size_t)vocab, d_work, work_bytes, stream);
     if (!r && lora)

@@ -1155,6 +1155,11 @@ int logits_launch(DeviceCtx *c, const LogitsArgs &a, int dtype, cudaStream_t s) 
 }
 }  // namespace
 
+int noel::logits_check(const noel_logits_params_t *params, float *logits, int batch, int vocab, size_t ld) {
+    LogitsArgs a{};
+    return logits_args(params, logits, NOEL_DTYPE_F32, batch, vocab, ld, &a);
+}
+
 extern "C" int noel_logits_process(const noel_logits_params_t *params, void *d_logits, int dtype, int batch, int vocab,
                                    size_t ld, void *stream) try {
     LogitsArgs a{};
@@ -1369,6 +1374,12 @@ int lora_launch(DeviceCtx *c, const LoraArgs &a, int type, cudaStream_t s) {
                                    : lora_launch_t<kHeadBF16>(c, a, s);
 }
 }  // namespace
+
+int noel::lora_check(const noel_lora_t *lora, const int32_t *adapter, const float *x, size_t ldx, int batch, int cols, int rows,
+                     float *y, size_t ldy, void *work, size_t work_bytes) {
+    LoraArgs a{};
+    return lora_args(lora, adapter, x, ldx, batch, cols, rows, y, ldy, work, work_bytes, &a);
+}
 
 extern "C" size_t noel_lora_workspace_bytes(int batch, int rank) {
     if (batch <= 0 || rank <= 0 || rank > kLoraMaxRank) return 0;
