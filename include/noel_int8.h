@@ -40,6 +40,7 @@ int noel_i8_cast(const void *d_x, int type, size_t ldx, int rows, int cols, int8
  * < tokens, v < rows: sums exact, the sum's fp32 value times d_w_scale[v],
  * then times d_a_scale[t], each rounded to fp32, and to bf16 where d_y is.  A
  * result does not depend on the other tokens and rows of the call.
+ * tokens and rows may be 2^31 - 513 at most.
  * d_a [tokens][lda] and d_w [rows][ldw] (cols used, 1 .. NOEL_I8_MAX_COLS)
  * 16-byte aligned with lda and ldw multiples of 16; d_y [tokens][ldy] of dtype
  * NOEL_DTYPE_F32 or NOEL_DTYPE_BF16 (noel_sampler_cuda.h), aligned to the

@@ -54,6 +54,9 @@ int failed_flag(int **flag) {
     return NOEL_OK;
 }
 
+/* tokens and rows of a product: the kernel steps over both in 32 bits, by tiles of 256 */
+constexpr int kMostRows = 0x7FFFFFFF - 512;
+
 bool misaligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
 int cast_args(const void *x, int type, size_t ldx, int rows, int cols, const void *q, size_t ldq, const float *scale,
@@ -99,6 +102,8 @@ int product_args(const int8_t *a, size_t lda, const float *a_scale, int tokens, 
     if (tokens < 0 || rows < 0 || cols <= 0)
         return fail(NOEL_ERR_INVALID_ARG, "tokens %d / rows %d / cols %d", tokens, rows, cols);
     if (cols > NOEL_I8_MAX_COLS) return fail(NOEL_ERR_TOO_LARGE, "cols %d (1..%d)", cols, NOEL_I8_MAX_COLS);
+    if (tokens > kMostRows || rows > kMostRows)
+        return fail(NOEL_ERR_TOO_LARGE, "tokens %d / rows %d (up to %d)", tokens, rows, kMostRows);
     if (lda < (size_t)cols || lda % 16 || ldw < (size_t)cols || ldw % 16 || ldy < (size_t)rows)
         return fail(NOEL_ERR_INVALID_ARG, "cols %d: lda %zu / ldw %zu (multiples of 16); rows %d: ldy %zu", cols, lda, ldw, rows, ldy);
     if (misaligned(a, 16) || misaligned(w, 16)) return fail(NOEL_ERR_INVALID_ARG, "a and w must be 16-byte aligned");

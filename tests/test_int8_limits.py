@@ -56,3 +56,27 @@ def test_head_needs_the_adapters_scratch(lib):
     lora = lora_struct(ldb=256, rank=256)
     assert head(lib, lora=lora, batch=40, size=size - 1) == INVALID
     assert lib.noel_lmhead_i8_workspace_bytes(40, 64, 10, 256) == size
+
+
+MOST = 2**31 - 513  # tokens or rows of a product
+
+
+def product(lib, tokens=0, rows=0):
+    # one of the two is 0, so that what is not refused has nothing to do
+    return lib.noel_i8_product(P, 16, P, tokens, P, 16, P, rows, 16, P, 0, max(rows, 1), None)
+
+
+def test_product_sizes_that_its_tiles_would_pass(lib):
+    """Steps of whole tiles from the last row on end below 2^31."""
+    for n in (MOST + 1, 2**31 - 256, 2**31 - 1):
+        assert product(lib, tokens=n) == TOO_LARGE and product(lib, rows=n) == TOO_LARGE, n
+    assert product(lib, tokens=MOST) == OK and product(lib, rows=MOST) == OK
+
+
+def test_linear_sizes_that_its_tiles_would_pass(lib):
+    def linear(tokens=0, rows=0):
+        size = lib.noel_i8_linear_workspace_bytes(tokens, 16)
+        return lib.noel_i8_linear(P, 0, 16, tokens, P, 16, P, rows, 16, P, 0, max(rows, 1), P, size, None)
+
+    assert linear(tokens=MOST + 1) == TOO_LARGE and linear(rows=MOST + 1) == TOO_LARGE
+    assert linear(tokens=MOST) == OK and linear(rows=MOST) == OK
