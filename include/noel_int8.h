@@ -45,9 +45,11 @@ int noel_i8_cast(const void *d_x, int type, size_t ldx, int rows, int cols, int8
  * 16-byte aligned with lda and ldw multiples of 16; d_y [tokens][ldy] of dtype
  * NOEL_DTYPE_F32 or NOEL_DTYPE_BF16 (noel_sampler_cuda.h), aligned to the
  * element size, apart from the inputs; its columns from rows on are left as
- * they are.  Waits inside the kernel are limited and reported by
- * noel_sampler_cuda_sync_check, on whichever stream the call was.  Otherwise
- * as noel_i8_cast.
+ * they are.  Waits inside the kernel are limited
+ * (noel_sampler_cuda_set_wait_limit) and reported by
+ * noel_sampler_cuda_sync_check, on whichever stream the call was; once one has
+ * run out the others end as well, and the call within another limit and a
+ * millisecond.  Otherwise as noel_i8_cast.
  */
 int noel_i8_product(const int8_t *d_a, size_t lda, const float *d_a_scale, int tokens, const int8_t *d_w, size_t ldw,
                     const float *d_w_scale, int rows, int cols, void *d_y, int dtype, size_t ldy, void *stream);

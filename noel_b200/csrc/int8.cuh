@@ -147,6 +147,7 @@ constexpr int kI8Line = 128;     // columns (bytes) of a copy: one swizzled line
 constexpr int kI8Box = 32;       // rows of w in one copy where a tile has fewer than 128
 constexpr int kI8MaxStages = 12;
 constexpr int kI8Ring = 225280;  // bytes of the ring at most
+constexpr unsigned long long kI8LandNs = 1000000;  // copies and products that were issued have ended after this, by far
 
 /* lines of a row in a stage: two where tiles are narrow and the weights' stream is what counts (a stage is then 32 KB of
  * them, and the memory is asked for 256 bytes of a row at once) */
@@ -184,8 +185,8 @@ __device__ __forceinline__ unsigned long long i8_now() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-/* Wait for the phase of that parity; false where the limit ran out. */
-__device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, unsigned long long limit) {
+/* Wait for the phase of that parity; false where the limit ran out, or where stop (if any) says that another wait's has. */
+__device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, unsigned long long limit, const volatile uint32_t *stop) {
     unsigned long long begin = 0;
     for (int i = 0;; ++i) {
         uint32_t done;
@@ -198,8 +199,25 @@ __device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, unsigned 
             : "memory");
         if (done) return true;
         if (i == 0) begin = i8_now();
-        else if ((i & 15) == 0 && i8_now() - begin > limit) return false;
+        else if ((i & 15) == 0 && ((stop && *stop) || i8_now() - begin > limit)) return false;
     }
+}
+/* A wait ran out: the host is to learn of it, and the other waits of the CTA (of both CTAs of a pair) end too. */
+template <bool PAIR>
+__device__ __forceinline__ void i8_give_up(uint32_t *stop, uint32_t rank, int *failed) {
+    *failed = 1;
+    *(volatile uint32_t *)stop = 1;
+    if (PAIR) asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;" ::"r"(i8_peer(i8_addr(stop), rank ^ 1)), "r"(1u) : "memory");
+}
+/* whether it is so for any of the 256 threads of results, which meet here */
+__device__ __forceinline__ bool i8_any(bool mine) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)mine)
+        : "memory");
+    return any != 0;
 }
 template <bool PAIR>
 __device__ __forceinline__ void i8_copy(const CUtensorMap *map, uint32_t dst, uint32_t bar, int x, int y) {
@@ -310,9 +328,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     constexpr int kLines = i8_lines(NT), kLineW = kI8RowsCta * kI8Line, kLineA = kHalf * kI8Line;  // a stage: w's lines, then a's
     constexpr uint32_t kCols = 2 * NT < 32 ? 32 : 2 * NT;
     extern __shared__ unsigned char i8_raw[];
-    __shared__ __align__(8) uint64_t s_full[kI8MaxStages], s_empty[kI8MaxStages], s_done[2], s_free[2];
+    __shared__ __align__(8) uint64_t s_full[kI8MaxStages], s_empty[kI8MaxStages], s_done[2], s_free[2], s_end;
     __shared__ float s_scale[2][NT];  // of the tile's tokens
-    __shared__ uint32_t s_tmem;
+    __shared__ uint32_t s_tmem, s_stop;  // s_stop: a wait ran out
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t rank = 0;
     if (PAIR) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -321,6 +339,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) i8_bar_init(i8_addr(&s_full[i]), 1), i8_bar_init(i8_addr(&s_empty[i]), 1);
         for (int i = 0; i < 2; ++i) i8_bar_init(i8_addr(&s_done[i]), 1), i8_bar_init(i8_addr(&s_free[i]), PAIR ? 16 : 8);
+        i8_bar_init(i8_addr(&s_end), 1);
+        s_stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -340,7 +360,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
     const int chunks = (a.cols + kLines * kI8Line - 1) / (kLines * kI8Line);
-    bool failed = false;  // a wait ran out
+    int stage = 0;  // of the ring, where this warp works with it
+    uint32_t phase = 0;
 
     if (warp == 0 && lane == 0 && !a.stall) {
         /* --------------------------------------------- copies of weights */
@@ -349,15 +370,13 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             return n <= 0 ? 0 : (n + kI8Box - 1) / kI8Box * kI8Box;
         };
         I8Tiles<NT, PAIR> t(a);
-        int stage = 0;
-        uint32_t phase = 0;
         bool good = true;
         for (; good && t.more(); t.next()) {
             const int n = copies(t, rank), row = t.row + (int)rank * kI8RowsCta;
             int all = n + kHalf;
             if (PAIR) all += copies(t, rank ^ 1) + kHalf;
             for (int k = 0; k < chunks; ++k) {
-                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns);
+                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns, &s_stop);
                 if (!good) break;
                 const uint32_t bar = i8_addr(&s_full[stage]), to = PAIR ? i8_peer(bar, 0) : bar, at = ring + stage * kStage;
                 if (rank == 0) i8_bar_expect(bar, (uint32_t)all * kI8Line * kLines);
@@ -373,21 +392,14 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
         }
-        if (!good) {
-            *a.failed = 1;
-            /* what is still on its way into this CTA's memory lands before it ends */
-            if (rank == 0)
-                for (int s = 0; s < kStages; ++s) i8_wait(i8_addr(&s_full[s]), s < stage ? phase : phase ^ 1, a.wait_ns);
-        }
+        if (!good) i8_give_up<PAIR>(&s_stop, rank, a.failed);
     } else if (warp == 10 && lane == 0 && !a.stall) {
         /* ---------------------------------------------- copies of tokens */
         asm volatile("griddepcontrol.wait;" ::: "memory");  // their cast; the first weights do not wait for it
-        int stage = 0;
-        uint32_t phase = 0;
         bool good = true;
         for (I8Tiles<NT, PAIR> t(a); good && t.more(); t.next())
             for (int k = 0; k < chunks; ++k) {
-                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns);
+                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns, &s_stop);
                 if (!good) break;
                 const uint32_t bar = i8_addr(&s_full[stage]), to = PAIR ? i8_peer(bar, 0) : bar;
 #pragma unroll
@@ -396,21 +408,20 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                                   t.t0 + (int)rank * kHalf);
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
-        if (!good) *a.failed = 1;
+        if (!good) i8_give_up<PAIR>(&s_stop, rank, a.failed);
     } else if (warp == 1 && lane == 0 && rank == 0) {
         /* ----------------------------------------------------- products */
         /* 32-bit sums of signed bytes, N and M of the tile */
         constexpr uint32_t kIdesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(NT / 8) << 17 |
                                     (uint32_t)((PAIR ? 256 : 128) / 16) << 24;
-        int stage = 0, tile = 0;
-        uint32_t phase = 0;
+        int tile = 0;
         bool good = true;
         for (I8Tiles<NT, PAIR> t(a); good && t.more(); t.next(), ++tile) {
             const int half = tile & 1;
-            good = i8_wait(i8_addr(&s_free[half]), ((tile >> 1) & 1) ^ 1, a.wait_ns);
+            good = i8_wait(i8_addr(&s_free[half]), ((tile >> 1) & 1) ^ 1, a.wait_ns, &s_stop);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int k = 0; good && k < chunks; ++k) {
-                good = i8_wait(i8_addr(&s_full[stage]), phase, a.wait_ns);
+                good = i8_wait(i8_addr(&s_full[stage]), phase, a.wait_ns, &s_stop);
                 if (!good) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t dw = i8_desc(ring + stage * kStage), da = i8_desc(ring + stage * kStage + kLines * kLineW);
@@ -425,13 +436,14 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             }
             if (good) i8_commit<PAIR>(i8_addr(&s_done[half]));
         }
-        if (!good) *a.failed = 1;
+        if (!good) i8_give_up<PAIR>(&s_stop, rank, a.failed);
     } else if (warp >= 2 && warp < 10) {
         /* ------------------------------------------------------ results */
         asm volatile("griddepcontrol.wait;" ::: "memory");
         /* a quarter of the tensor memory's lanes, which is all that a warp may read, and every other 16 tokens */
         const int quarter = warp & 3, side = (warp - 2) >> 2;
         int tile = 0;
+        bool failed = false;
         for (I8Tiles<NT, PAIR> t(a); t.more(); t.next(), ++tile) {
             const int half = tile & 1;
             const int r = t.row + (int)rank * kI8RowsCta + quarter * 32 + lane;
@@ -439,9 +451,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             const float ws = mine ? a.w_scale[r] : 0.0f;
             const int nt = min(NT, a.tokens - t.t0);
             for (int i = threadIdx.x - 64; i < nt; i += 256) s_scale[half][i] = a.a_scale[t.t0 + i];
-            asm volatile("bar.sync 1, 256;" ::: "memory");  // those of two tiles ago have been used
-            if (!__all_sync(0xFFFFFFFFu, i8_wait(i8_addr(&s_done[half]), (tile >> 1) & 1, a.wait_ns))) {
-                if (lane == 0) *a.failed = 1;
+            if (i8_any(failed)) break;  // all of them or none; the scales of two tiles ago have been used
+            if (!__all_sync(0xFFFFFFFFu, i8_wait(i8_addr(&s_done[half]), (tile >> 1) & 1, a.wait_ns, &s_stop))) {
+                if (lane == 0) i8_give_up<PAIR>(&s_stop, rank, a.failed);
                 failed = true;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -477,6 +489,28 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     if (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     __syncthreads();
+    if (s_stop) {
+        /*
+         * A wait ran out, in this CTA or in its pair's other one, so copies into this memory and products of it may be
+         * on their way: they end before the CTA does.  A stage of which not all copies were issued never fills, so the
+         * time has to do as well.
+         */
+        if (warp == 1 && lane == 0 && rank == 0) {
+            i8_commit<PAIR>(i8_addr(&s_end));
+            i8_wait(i8_addr(&s_end), 0, a.wait_ns + kI8LandNs, nullptr);
+        } else if (warp == 0 && lane == 0 && !a.stall) {
+            const unsigned long long begin = i8_now();
+            for (int s = 0; rank == 0 && s < kStages; ++s) {
+                const unsigned long long spent = i8_now() - begin;
+                if (spent < a.wait_ns) i8_wait(i8_addr(&s_full[s]), s < stage ? phase : phase ^ 1, a.wait_ns - spent, nullptr);
+            }
+            while (i8_now() - begin < kI8LandNs) __nanosleep(1000);
+        }
+        __syncwarp();
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        if (PAIR) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        __syncthreads();
+    }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
