@@ -164,8 +164,11 @@ int noel_sampler_sample_batch_host(const noel_sampler_config_t *cfg, const void 
  * wait of the streaming kernel (for a ring stage, a prepared row or the
  * consumers of a row) ran out of its limit; the kernel then returns instead
  * of hanging and the results of that call are invalid.  Clears the flag.
- * Reports (and clears) the waits of the 8-bit product (noel_int8.h) on the
- * current device as well, whichever stream they were on.
+ * Reports the waits of the 8-bit products (noel_int8.h) launched on stream
+ * as well.  A product that a graph captured may be replayed on any stream, so
+ * that one of its waits ran out is reported to the next check of each stream;
+ * the same holds for streams on which a device's first product comes after
+ * those of 1023 others.
  */
 int noel_sampler_cuda_sync_check(void *stream);
 

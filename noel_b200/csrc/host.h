@@ -32,8 +32,8 @@ __attribute__((visibility("hidden"))) int lora_check(const noel_lora_t *lora, co
                                                      size_t work_bytes);
 __attribute__((visibility("hidden"))) int logits_check(const noel_logits_params_t *params, float *logits, int batch, int vocab,
                                                        size_t ld);
-/* Whether a wait of the int8 product ran out on the current device since the last call (which clears it). */
-__attribute__((visibility("hidden"))) int i8_wait_failed(bool *failed);
+/* Whether a product in 8 bits gave up since the stream's last call of this: one launched on the stream, or one of a graph. */
+__attribute__((visibility("hidden"))) int i8_wait_failed(cudaStream_t s, bool *failed);
 
 #define CUDA_TRY(call)                                                                     \
     do {                                                                                   \

@@ -3,7 +3,9 @@
  */
 #include "noel_int8.h"
 
-#include <atomic>
+#include <deque>
+#include <map>
+#include <mutex>
 
 #include "host.h"
 #include "int8.cuh"
@@ -13,8 +15,68 @@ using namespace noel;
 
 namespace {
 
-__device__ int g_i8_failed;  // a wait of the product ran out on this device
-std::atomic<bool> g_i8_used{false};  // a product has been launched
+/*
+ * Products that gave up, counted on the device and never cleared there: a
+ * count for each stream, and the first one for calls that a graph has captured
+ * (it may be replayed on any stream) and for streams that come when the others
+ * are taken.  A check compares with what its stream was last told, so that
+ * none takes another stream's report.
+ */
+constexpr int kCounts = 1024;
+__device__ unsigned g_i8_failed[kCounts];
+
+struct StreamWaits {
+    int count = 0;                  // index of its count; 0: no product yet, or the common one
+    unsigned told = 0, told_common = 0;
+};
+struct DeviceWaits {
+    unsigned *counts = nullptr;
+    int taken = 1;
+    bool common = false;            // something may be in the common count
+    std::map<const void *, StreamWaits> streams;
+};
+std::mutex g_waits_mu;
+std::deque<DeviceWaits> g_waits;
+
+/* what stands for a stream among the threads: the two names of the default one are one, the thread's own is each thread's */
+const void *stream_key(cudaStream_t s) {
+    static thread_local char mine;
+    return s == cudaStreamPerThread ? &mine : s == cudaStreamLegacy ? nullptr : static_cast<const void *>(s);
+}
+
+/* with the lock held */
+int device_waits(DeviceWaits **out) {
+    int dev = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    if ((int)g_waits.size() <= dev) g_waits.resize(dev + 1);
+    DeviceWaits &d = g_waits[dev];
+    if (!d.counts) {
+        void *p = nullptr;
+        CUDA_TRY(cudaGetSymbolAddress(&p, g_i8_failed));
+        d.counts = static_cast<unsigned *>(p);
+    }
+    *out = &d;
+    return NOEL_OK;
+}
+
+/* where a product on the stream counts that it gave up */
+int failed_count(cudaStream_t s, unsigned **count) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    CUDA_TRY(cudaStreamIsCapturing(s, &cap));
+    std::lock_guard<std::mutex> lk(g_waits_mu);
+    DeviceWaits *d = nullptr;
+    const int r = device_waits(&d);
+    if (r) return r;
+    int at = 0;
+    if (cap == cudaStreamCaptureStatusNone) {
+        StreamWaits &w = d->streams[stream_key(s)];
+        if (!w.count && d->taken < kCounts) w.count = d->taken++;
+        at = w.count;
+    }
+    if (!at) d->common = true;
+    *count = d->counts + at;
+    return NOEL_OK;
+}
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -44,13 +106,6 @@ int byte_map(CUtensorMap *m, const void *base, int rows, int cols, size_t ld, in
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (e != CUDA_SUCCESS) return fail(NOEL_ERR_CUDA, "cuTensorMapEncodeTiled: %d (%d x %d, pitch %zu)", (int)e, rows, cols, ld);
-    return NOEL_OK;
-}
-
-int failed_flag(int **flag) {
-    void *p = nullptr;
-    CUDA_TRY(cudaGetSymbolAddress(&p, g_i8_failed));
-    *flag = static_cast<int *>(p);
     return NOEL_OK;
 }
 
@@ -147,7 +202,6 @@ int product_launch(const Product &p, const I8Args &args, int groups, bool depend
     }
     lc.attrs = at;
     lc.numAttrs = n;
-    g_i8_used = true;
     CUDA_TRY(cudaLaunchKernelEx(&lc, i8_product_kernel<NT, PAIR, OUT>, mw, mp, ma, args));
     CUDA_TRY(cudaGetLastError());
     return NOEL_OK;
@@ -158,7 +212,7 @@ int product_tile(const Product &p, bool dependent, cudaStream_t s) {
     int sms = 0;
     int r = device_sms(&sms);
     I8Args args = p.args;
-    if (!r) r = failed_flag(&args.failed);
+    if (!r) r = failed_count(s, &args.failed);
     if (r) return r;
     args.wait_ns = wait_limit_ns();
     args.stall = take_stall();
@@ -186,14 +240,31 @@ size_t cast_pitch(int cols) { return ((size_t)cols + 15) / 16 * 16; }
 
 }  // namespace
 
-int noel::i8_wait_failed(bool *failed) {
+int noel::i8_wait_failed(cudaStream_t s, bool *failed) {
     *failed = false;
-    if (!g_i8_used) return NOEL_OK;  // without a copy, which a stream being captured elsewhere may not allow
-    int v = 0;
-    const int zero = 0;
-    CUDA_TRY(cudaMemcpyFromSymbol(&v, g_i8_failed, sizeof(v)));
-    if (v) CUDA_TRY(cudaMemcpyToSymbol(g_i8_failed, &zero, sizeof(zero)));
-    *failed = v != 0;
+    const unsigned *own = nullptr, *common = nullptr;
+    {
+        std::lock_guard<std::mutex> lk(g_waits_mu);
+        DeviceWaits *d = nullptr;
+        const int r = device_waits(&d);
+        if (r) return r;
+        const auto it = d->streams.find(stream_key(s));
+        if (it != d->streams.end() && it->second.count) own = d->counts + it->second.count;
+        if (d->common) common = d->counts;
+    }
+    unsigned now = 0, now_common = 0;
+    if (own) CUDA_TRY(cudaMemcpyAsync(&now, own, sizeof(now), cudaMemcpyDeviceToHost, s));
+    if (common) CUDA_TRY(cudaMemcpyAsync(&now_common, common, sizeof(now_common), cudaMemcpyDeviceToHost, s));
+    if (!own && !common) return NOEL_OK;
+    CUDA_TRY(cudaStreamSynchronize(s));
+    std::lock_guard<std::mutex> lk(g_waits_mu);
+    DeviceWaits *d = nullptr;
+    const int r = device_waits(&d);
+    if (r) return r;
+    StreamWaits &w = d->streams[stream_key(s)];
+    *failed = (own && now != w.told) || (common && now_common != w.told_common);
+    if (own) w.told = now;
+    if (common) w.told_common = now_common;
     return NOEL_OK;
 }
 

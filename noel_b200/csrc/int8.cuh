@@ -138,7 +138,7 @@ struct I8Args {
     bool ranges;           // every group one range of rows and all tokens (one tile of them)
     unsigned long long wait_ns;
     int stall;             // load nothing, so that waits run out
-    int *failed;
+    unsigned *failed;      // counts the products that gave up
 };
 
 constexpr int kI8Threads = 352;  // two warps of loads, one of products, eight of results
@@ -204,8 +204,8 @@ __device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, unsigned 
 }
 /* A wait ran out: the host is to learn of it, and the other waits of the CTA (of both CTAs of a pair) end too. */
 template <bool PAIR>
-__device__ __forceinline__ void i8_give_up(uint32_t *stop, uint32_t rank, int *failed) {
-    *failed = 1;
+__device__ __forceinline__ void i8_give_up(uint32_t *stop, uint32_t rank, unsigned *failed) {
+    atomicAdd(failed, 1u);
     *(volatile uint32_t *)stop = 1;
     if (PAIR) asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;" ::"r"(i8_peer(i8_addr(stop), rank ^ 1)), "r"(1u) : "memory");
 }

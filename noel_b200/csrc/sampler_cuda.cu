@@ -1628,14 +1628,11 @@ extern "C" int noel_sampler_sample_batch_host(const noel_sampler_config_t *cfg, 
     return ok();
 }
 
-extern "C" int noel_sampler_cuda_sync_check(void *stream) {
+extern "C" int noel_sampler_cuda_sync_check(void *stream) try {
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     CUDA_TRY(cudaStreamSynchronize(s));
     DeviceCtx *c = nullptr;
     int r = device_ctx(&c);
-    if (r) return r;
-    bool product = false;
-    r = i8_wait_failed(&product);
     if (r) return r;
     int32_t *flag = nullptr;
     {
@@ -1644,12 +1641,16 @@ extern "C" int noel_sampler_cuda_sync_check(void *stream) {
         if (it != c->ws.end()) flag = it->second.counters + 3;
     }
     int32_t v = 0;
-    if (flag) CUDA_TRY(cudaMemcpy(&v, flag, sizeof(v), cudaMemcpyDeviceToHost));
-    if (v || product) {
+    if (flag) {
+        CUDA_TRY(cudaMemcpy(&v, flag, sizeof(v), cudaMemcpyDeviceToHost));
         if (v) CUDA_TRY(cudaMemset(flag, 0, sizeof(v)));
-        return fail(NOEL_ERR_DEVICE_WAIT, "a device-side wait ran out of its limit");
     }
-    return ok();
+    bool product = false;
+    r = i8_wait_failed(s, &product);
+    if (v || product) return fail(NOEL_ERR_DEVICE_WAIT, "a device-side wait ran out of its limit");
+    return r ? r : ok();
+} catch (...) {
+    return fail(NOEL_ERR_CUDA, "host memory");
 }
 
 extern "C" int noel_sampler_cuda_set_wait_limit(long long wait_ns, int stall_next_call) {

@@ -72,3 +72,95 @@ def test_waits_that_run_out_while_copies_are_on_their_way(cuda, limits, tokens, 
     S.int8_product(x, w, out=again)
     assert S.sync_check() == 0
     assert torch.equal(again, y)
+
+
+def test_reports_go_to_their_streams(cuda, limits):
+    """A check of one stream neither takes nor clears what another stream's product has to report."""
+    import torch
+
+    from noel_b200 import sampler as S
+
+    w, x = rows(300, 256, cuda, 5), rows(4, 256, cuda, 6)
+    torch.cuda.synchronize()
+    good, bad, idle = (torch.cuda.Stream() for _ in range(3))
+    S.int8_product(x, w, stream=good)
+    assert [S.sync_check(s) for s in (good, bad, idle)] == [0, 0, 0]
+    for _ in range(3):
+        limits(2_000_000, stall_next_call=True)
+        S.int8_product(x, w, stream=bad)
+        limits(0)
+        S.int8_product(x, w, stream=good)
+        bad.synchronize()
+        assert [S.sync_check(s) for s in (idle, good, torch.cuda.current_stream())] == [0, 0, 0]
+        assert [S.sync_check(bad), S.sync_check(bad)] == [WAIT, 0]
+    # twice before a check is one report
+    for _ in range(2):
+        limits(2_000_000, stall_next_call=True)
+        S.int8_product(x, w, stream=bad)
+    assert [S.sync_check(good), S.sync_check(bad), S.sync_check(bad)] == [0, WAIT, 0]
+
+
+def test_reports_of_many_streams_and_threads(cuda):
+    """Each thread's stalled product on a stream of its own is its own report."""
+    import threading
+
+    import torch
+
+    from noel_b200 import sampler as S
+
+    w, x = rows(300, 256, cuda, 7), rows(4, 256, cuda, 8)
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(n):
+        stream = torch.cuda.Stream()
+        seen = []
+        for turn in range(6):
+            stall = (n + turn) % 3 == 0
+            S.set_wait_limit(2_000_000, stall_next_call=stall)  # of this thread
+            S.int8_product(x, w, stream=stream)
+            seen.append(S.sync_check(stream) == (WAIT if stall else 0))
+        got[n] = seen
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got == {n: [True] * 6 for n in range(6)}
+
+
+CAPTURED = """
+import torch
+from noel_b200 import sampler as S
+
+dev = torch.device("cuda:0")
+w, x = S.int8_cast(torch.randn(300, 256, device=dev)), S.int8_cast(torch.randn(4, 256, device=dev))
+S.int8_product(x, w)
+g = torch.cuda.CUDAGraph()
+S.set_wait_limit(2_000_000, stall_next_call=True)
+with torch.cuda.graph(g):
+    S.int8_product(x, w)
+S.set_wait_limit(0)
+streams = [torch.cuda.current_stream(), torch.cuda.Stream(), torch.cuda.Stream()]
+assert [S.sync_check(s) for s in streams[:2]] == [0, 0]
+for turn in range(2):
+    g.replay()
+    torch.cuda.synchronize()
+    assert [S.sync_check(s) for s in streams] == [-6, -6, -6], turn
+    assert [S.sync_check(s) for s in streams] == [0, 0, 0], turn
+S.int8_product(x, w, stream=streams[1])
+assert [S.sync_check(s) for s in streams] == [0, 0, 0]
+"""
+
+
+def test_reports_of_a_replayed_graph(cuda):
+    """It may run on any stream, so each stream's next check has it.  In a process of its own: streams that later tests make would
+    be told as well."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", CAPTURED], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
