@@ -3,6 +3,7 @@
  */
 #include "noel_int8.h"
 
+#include <atomic>
 #include <deque>
 #include <map>
 #include <mutex>
@@ -83,13 +84,15 @@ using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, vo
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 int encode_fn(EncodeFn *out) {
-    static EncodeFn fn = nullptr;  // the same for every device and thread
+    static std::atomic<EncodeFn> known{nullptr};  // the same for every device and thread
+    EncodeFn fn = known.load(std::memory_order_acquire);
     if (!fn) {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult found;
         CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found));
         if (found != cudaDriverEntryPointSuccess || !p) return fail(NOEL_ERR_CUDA, "cuTensorMapEncodeTiled is not there");
         fn = reinterpret_cast<EncodeFn>(p);
+        known.store(fn, std::memory_order_release);
     }
     *out = fn;
     return NOEL_OK;

@@ -1,11 +1,16 @@
 """Waits of the 8-bit product that run out (include/noel_sampler_cuda.h): the
 call ends soon after the first of them, is reported, and leaves the next call
 as it was."""
+import os
+import subprocess
+import sys
+
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 WAIT = -6
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture
@@ -154,13 +159,44 @@ assert [S.sync_check(s) for s in streams] == [0, 0, 0]
 """
 
 
+def in_a_process(text):
+    r = subprocess.run([sys.executable, "-c", text], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_reports_of_a_replayed_graph(cuda):
     """It may run on any stream, so each stream's next check has it.  In a process of its own: streams that later tests make would
     be told as well."""
-    import os
-    import subprocess
-    import sys
+    in_a_process(CAPTURED)
 
-    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    r = subprocess.run([sys.executable, "-c", CAPTURED], cwd=root, capture_output=True, text=True, timeout=300)
-    assert r.returncode == 0, r.stderr[-2000:]
+
+FIRST = """
+import threading
+import torch
+from noel_b200 import sampler as S
+
+dev = torch.device("cuda:0")
+q = torch.randint(-128, 128, (700, 256), dtype=torch.int8, device=dev)
+w, xs = S.Int8Rows(q, torch.ones(700, device=dev)), [S.Int8Rows(q[:n], torch.ones(n, device=dev)) for n in (3, 20, 64, 128, 300, 5)]
+wants = [(x.q.double() @ q.double().T).float() for x in xs]
+torch.cuda.synchronize()
+gate, got = threading.Barrier(len(xs)), {}
+
+def work(n):
+    stream = torch.cuda.Stream()
+    gate.wait()
+    y = S.int8_product(xs[n], w, stream=stream)
+    got[n] = S.sync_check(stream) == 0 and torch.equal(y, wants[n])
+
+threads = [threading.Thread(target=work, args=(n,)) for n in range(len(xs))]
+for t in threads:
+    t.start()
+for t in threads:
+    t.join()
+assert got == {n: True for n in range(len(xs))}, got
+"""
+
+
+def test_first_products_of_many_threads(cuda):
+    """What the library sets up on its first product is set up by several threads at once."""
+    in_a_process(FIRST)
