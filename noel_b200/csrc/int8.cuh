@@ -198,8 +198,9 @@ __device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, unsigned 
             : "r"(bar), "r"(parity)
             : "memory");
         if (done) return true;
+        if (stop && *stop) return false;
         if (i == 0) begin = i8_now();
-        else if ((i & 15) == 0 && ((stop && *stop) || i8_now() - begin > limit)) return false;
+        else if ((i & 15) == 0 && i8_now() - begin > limit) return false;
     }
 }
 /* A wait ran out: the host is to learn of it, and the other waits of the CTA (of both CTAs of a pair) end too. */
@@ -360,6 +361,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
     const int chunks = (a.cols + kLines * kI8Line - 1) / (kLines * kI8Line);
+    const volatile uint32_t *stop = &s_stop;
     int stage = 0;  // of the ring, where this warp works with it
     uint32_t phase = 0;
 
@@ -371,12 +373,12 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         };
         I8Tiles<NT, PAIR> t(a);
         bool good = true;
-        for (; good && t.more(); t.next()) {
+        for (; good && !*stop && t.more(); t.next()) {
             const int n = copies(t, rank), row = t.row + (int)rank * kI8RowsCta;
             int all = n + kHalf;
             if (PAIR) all += copies(t, rank ^ 1) + kHalf;
             for (int k = 0; k < chunks; ++k) {
-                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns, &s_stop);
+                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns, stop);
                 if (!good) break;
                 const uint32_t bar = i8_addr(&s_full[stage]), to = PAIR ? i8_peer(bar, 0) : bar, at = ring + stage * kStage;
                 if (rank == 0) i8_bar_expect(bar, (uint32_t)all * kI8Line * kLines);
@@ -397,9 +399,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         /* ---------------------------------------------- copies of tokens */
         asm volatile("griddepcontrol.wait;" ::: "memory");  // their cast; the first weights do not wait for it
         bool good = true;
-        for (I8Tiles<NT, PAIR> t(a); good && t.more(); t.next())
+        for (I8Tiles<NT, PAIR> t(a); good && !*stop && t.more(); t.next())
             for (int k = 0; k < chunks; ++k) {
-                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns, &s_stop);
+                good = i8_wait(i8_addr(&s_empty[stage]), phase ^ 1, a.wait_ns, stop);
                 if (!good) break;
                 const uint32_t bar = i8_addr(&s_full[stage]), to = PAIR ? i8_peer(bar, 0) : bar;
 #pragma unroll
@@ -416,12 +418,12 @@ __global__ void __launch_bounds__(kI8Threads, 1)
                                     (uint32_t)((PAIR ? 256 : 128) / 16) << 24;
         int tile = 0;
         bool good = true;
-        for (I8Tiles<NT, PAIR> t(a); good && t.more(); t.next(), ++tile) {
+        for (I8Tiles<NT, PAIR> t(a); good && !*stop && t.more(); t.next(), ++tile) {
             const int half = tile & 1;
-            good = i8_wait(i8_addr(&s_free[half]), ((tile >> 1) & 1) ^ 1, a.wait_ns, &s_stop);
+            good = i8_wait(i8_addr(&s_free[half]), ((tile >> 1) & 1) ^ 1, a.wait_ns, stop);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int k = 0; good && k < chunks; ++k) {
-                good = i8_wait(i8_addr(&s_full[stage]), phase, a.wait_ns, &s_stop);
+                good = i8_wait(i8_addr(&s_full[stage]), phase, a.wait_ns, stop);
                 if (!good) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t dw = i8_desc(ring + stage * kStage), da = i8_desc(ring + stage * kStage + kLines * kLineW);
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             const int nt = min(NT, a.tokens - t.t0);
             for (int i = threadIdx.x - 64; i < nt; i += 256) s_scale[half][i] = a.a_scale[t.t0 + i];
             if (i8_any(failed)) break;  // all of them or none; the scales of two tiles ago have been used
-            if (!__all_sync(0xFFFFFFFFu, i8_wait(i8_addr(&s_done[half]), (tile >> 1) & 1, a.wait_ns, &s_stop))) {
+            if (!__all_sync(0xFFFFFFFFu, i8_wait(i8_addr(&s_done[half]), (tile >> 1) & 1, a.wait_ns, stop))) {
                 if (lane == 0) i8_give_up<PAIR>(&s_stop, rank, a.failed);
                 failed = true;
             }
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) i8_bar_arrive(i8_peer(i8_addr(&s_free[half]), 0));
+            if (lane == 0 && !failed) i8_bar_arrive(i8_peer(i8_addr(&s_free[half]), 0));
         }
     }
     __syncwarp();

@@ -54,15 +54,17 @@ def test_a_stalled_product_of_many_tiles_ends_soon(cuda, limits, tokens):
     assert torch.equal(again, y)
 
 
-@pytest.mark.parametrize("tokens", [1, 17, 64, 128, 600])
-@pytest.mark.parametrize("limit", [1, 3_000, 10_000, 30_000])
-def test_waits_that_run_out_while_copies_are_on_their_way(cuda, limits, tokens, limit):
-    """A limit in the range of a copy's latency: whichever wait runs out first, the call is reported or right."""
+@pytest.mark.parametrize("tokens,cols", [(1, 2048), (17, 2048), (64, 2048), (128, 2048), (600, 2048),
+                                         (1, 131_071), (64, 131_071), (128, 131_071), (600, 131_071)])
+@pytest.mark.parametrize("limit", [1, 100_000])
+def test_waits_that_run_out_while_copies_are_on_their_way(cuda, limits, tokens, cols, limit):
+    """Limits in the range of a copy's latency, and of a tile's time where there are many columns (the results wait for
+    a whole tile): whichever wait runs out first, the call is reported or right."""
     import torch
 
     from noel_b200 import sampler as S
 
-    w, x = rows(30_000, 2048, cuda, 3), rows(tokens, 2048, cuda, 4)
+    w, x = rows(30_000 if cols == 2048 else 3_000, cols, cuda, 3), rows(tokens, cols, cuda, 4)
     y = S.int8_product(x, w)
     assert S.sync_check() == 0
     limits(limit)
