@@ -174,8 +174,8 @@ int noel_sampler_cuda_sync_check(void *stream);
 
 /*
  * Limit of every device-side wait of the batched calls and of the 8-bit
- * products (noel_int8.h) this thread makes next, in nanoseconds of the GPU's global timer (0 restores the default of
- * 2 s).  stall_next_call = 1 makes the next such call's kernel issue no
+ * products (noel_int8.h) this thread makes next, in nanoseconds of the GPU's
+ * global timer (0 restores the default of 2 s).  stall_next_call = 1 makes the next such call's kernel issue no
  * row loads, so its waits run out and noel_sampler_cuda_sync_check reports
  * NOEL_ERR_DEVICE_WAIT: the failure-detection path, exercised without a GPU
  * fault.  No counterpart in the reference (its sampler never waits).

@@ -230,6 +230,17 @@ int product_tile(const Product &p, bool dependent, cudaStream_t s) {
                                      : product_launch<NT, PAIR, __nv_bfloat16>(p, args, (int)groups, dependent, s);
 }
 
+/*
+ * Tiles by the number of tokens alone, made for matrices whose weights' stream
+ * counts.  152,064 rows of 4096, in us with tiles of 16, 32, 64, 128 and 256:
+ * 16 tokens 112 110 113 116 160; 17 tokens 128 110 113 117 172; 33 tokens 185
+ * 130 108 113 118; 65 tokens 303 186 133 117 123; 129 tokens 535 304 189 194
+ * 133; 300 tokens with 64, 128 and 256: 310 281 222; 2048 with 128 and 256: 1468
+ * 962.  Matrices of few rows would want narrower tiles, which give more groups:
+ * 4096 rows, 64 tokens 13.5 13.4 15.8 18.5 17.9, 200 tokens 28.5 21.4 15.2 17.7
+ * 20.7, 300 tokens with 64, 128 and 256: 22.3 18.6 19.9; from 768 tokens on 256
+ * is best there too (128 31.0, 256 21.9).  1024 rows: within 3 us of each other.
+ */
 int product(const Product &p, bool dependent, cudaStream_t s) {
     const int t = p.args.tokens;
     if (t <= 16) return product_tile<16, false>(p, dependent, s);

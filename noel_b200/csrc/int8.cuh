@@ -312,12 +312,13 @@ struct I8Tiles {
  * finished tile while the next one's products go into the other half of the
  * accumulators.
  *
- * 152,064 rows of 4096 columns: one token 112 us with its cast, 64 tokens 121
+ * 152,064 rows of 4096 columns: one token 112 us with its cast, 64 tokens 120
  * (HBM: 84 % of the measured copy; copies of 128 rows x 256 bytes, since a copy
  * costs its lane about 100 ns whatever its size: 32 rows at a time 124 us
- * for the copies alone, 128 rows 105).  2048 tokens 915 us in single calls (2.79
- * POPS; products alone on real data 696 us, loads and stores with a quarter
- * of the products 637) and 1070 in a loop, where power holds the clocks down.
+ * for the copies alone, 128 rows 105).  2048 tokens 870 to 915 us in a dozen
+ * single calls (2.8 to 2.9 POPS; products alone on real data 696 us, loads and
+ * stores with a quarter of the products 637) and 1050 to 1070 in a loop, where
+ * power holds the clocks down.
  * Pairs halve what a CTA needs of the tokens: 913 against 989 us; with tiles
  * of 128 tokens pairs took 1866 against 1354.
  */

@@ -344,7 +344,8 @@ def profile_events(before=None, after=None) -> None:
 
 def sync_check(stream=None) -> int:
     """Wait for ``stream`` (default: the current one) and return the status of
-    the device-side waits of the calls made on it (0, or NOEL_ERR_DEVICE_WAIT)."""
+    the device-side waits of the calls made on it (0, or NOEL_ERR_DEVICE_WAIT).
+    8-bit products that a graph captured report to every stream's next check."""
     import torch
 
     s = stream if stream is not None else torch.cuda.current_stream()
@@ -353,7 +354,7 @@ def sync_check(stream=None) -> int:
 
 def set_wait_limit(wait_ns: int = 0, stall_next_call: bool = False) -> None:
     """Limit of the device-side waits of this thread's later batched calls
-    (0: the default, 2 s); ``stall_next_call`` makes the next call's kernel
+    and 8-bit products (0: the default, 2 s); ``stall_next_call`` makes the next call's kernel
     issue no row loads so that its waits run out (failure-detection tests)."""
     _check(lib().noel_sampler_cuda_set_wait_limit(int(wait_ns), 1 if stall_next_call else 0))
 
