@@ -48,8 +48,9 @@ int noel_i8_cast(const void *d_x, int type, size_t ldx, int rows, int cols, int8
  * they are.  Waits inside the kernel are limited
  * (noel_sampler_cuda_set_wait_limit) and reported by
  * noel_sampler_cuda_sync_check of the stream (of any, for a call that a graph
- * captured); once one has run out the others end as well, and the call within
- * another limit and a millisecond.  Otherwise as noel_i8_cast.
+ * captured); once one has run out no further tile is begun, the others end as
+ * well, and the call within another limit and a millisecond.  Otherwise as
+ * noel_i8_cast.
  */
 int noel_i8_product(const int8_t *d_a, size_t lda, const float *d_a_scale, int tokens, const int8_t *d_w, size_t ldw,
                     const float *d_w_scale, int rows, int cols, void *d_y, int dtype, size_t ldy, void *stream);
